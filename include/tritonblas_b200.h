@@ -252,6 +252,43 @@ int tb_moe_plan(const void* topk_ids, int32_t ids_are_int64, int64_t n_pairs, in
                 int32_t world, int32_t rank, const int32_t* counts_all, int32_t* cursor, int64_t capacity_rows,
                 int32_t* pair_rank, int64_t* pair_row, int32_t* group_offsets, int32_t* row_token, int32_t topk, void* stream);
 
+/* Expert router (no reference counterpart): for every row of logits (tokens, num_experts; f16 / bf16 / f32, unit column stride)
+ * the topk largest entries, larger first, ties to the lowest index, as ids (tokens, topk) int32 and weights (tokens, topk)
+ * fp32. weights[t, j] is the softmax (sigmoid != 0: the sigmoid) score of the chosen expert, divided by the sum of the row's
+ * chosen scores when renormalize != 0; fp32 arithmetic. An entry of -inf or NaN is never chosen: what is left of a row with
+ * fewer than topk others has id -1 and weight 0, which the dispatch plan and tb_moe_mlp skip. +inf gives NaN weights, as the
+ * formula does. num_experts <= 1024, topk <= min(32, num_experts).
+ * tb_moe_route_backward: the gradient of the logits (tokens, num_experts) contiguous, in the logits' type, from the forward
+ * pass's weights and ids and grad_weights (tokens, topk) fp32; every element is written. */
+int tb_moe_route(const void* logits, int32_t dtype, int64_t row_stride, int64_t tokens, int32_t num_experts, int32_t topk,
+                 int32_t sigmoid, int32_t renormalize, float* weights, int32_t* ids, void* stream);
+int tb_moe_route_backward(const void* logits, int32_t dtype, int64_t row_stride, int64_t tokens, int32_t num_experts, int32_t topk,
+                          int32_t sigmoid, int32_t renormalize, const float* weights, const int32_t* ids,
+                          const float* grad_weights, void* grad_logits, void* stream);
+
+/* A whole expert layer for a few tokens in two launches (no reference counterpart):
+ *   out[t, :] = sum_j topk_weights[t, j] * W2_e ( silu(G_e x_t) * (U_e x_t) ),  e = topk_ids[t, j],  W1_e = [G_e ; U_e].
+ * x (tokens, hidden), w1 (num_experts, 2*ffn, hidden), w2 (num_experts, hidden, ffn), out (tokens, hidden), all of `dtype`
+ * (f16 or bf16), rows contiguous, x, w1 and w2 with 16-byte aligned rows and bases; topk_ids (tokens, topk) int32 or int64,
+ * topk_weights (tokens, topk) fp32, both contiguous. Sums, activation and weights are fp32, one cast at the end. An id outside
+ * [0, num_experts) adds nothing (a token with no other id gets zeros); the same id twice in a row counts twice.
+ * tokens <= 128, topk <= 32, num_experts <= 1024, hidden and ffn multiples of 8. The workspace
+ * (tb_moe_mlp_workspace_bytes, 256-byte aligned) needs no initialisation and must not be shared by calls that can overlap.
+ * Device-side waits are bounded (wait_timeout_ms, 0 = 2 s) and report through tb_device_status. */
+typedef struct tb_moe_mlp_args {
+  int32_t tokens, topk, num_experts, hidden, ffn, dtype;
+  const void* x; int64_t x_row_stride;
+  const void* w1; int64_t w1_expert_stride, w1_row_stride;
+  const void* w2; int64_t w2_expert_stride, w2_row_stride;
+  const void* topk_ids; const float* topk_weights;
+  void* out; int64_t out_row_stride;
+  void* workspace; int64_t workspace_bytes;
+  int32_t ids_are_int64;
+  int32_t wait_timeout_ms;
+} tb_moe_mlp_args;
+int64_t tb_moe_mlp_workspace_bytes(int32_t tokens, int32_t topk, int32_t num_experts, int32_t hidden, int32_t ffn);
+int tb_moe_mlp(const tb_moe_mlp_args* args, void* stream);
+
 /* Diagnostic: streams rows x row_bytes of a row-major matrix (pitch_bytes between rows) out of HBM with the access pattern
  * of the GEMM's K-major operand loader and drops the data: `programs` CTAs (one per SM), each keeping `stages` TMA boxes of
  * box_rows rows x 128 bytes in flight, row blocks dealt round-robin, K walked in 128-byte steps. Time it with events:

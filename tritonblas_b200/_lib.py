@@ -70,6 +70,18 @@ class Mxfp4Args(ctypes.Structure):
     ]
 
 
+class MoeMlpArgs(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int32) for n in ("tokens", "topk", "num_experts", "hidden", "ffn", "dtype")] + [
+        ("x", ctypes.c_void_p), ("x_row_stride", ctypes.c_int64),
+        ("w1", ctypes.c_void_p), ("w1_expert_stride", ctypes.c_int64), ("w1_row_stride", ctypes.c_int64),
+        ("w2", ctypes.c_void_p), ("w2_expert_stride", ctypes.c_int64), ("w2_row_stride", ctypes.c_int64),
+        ("topk_ids", ctypes.c_void_p), ("topk_weights", ctypes.c_void_p),
+        ("out", ctypes.c_void_p), ("out_row_stride", ctypes.c_int64),
+        ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_int64),
+        ("ids_are_int64", ctypes.c_int32), ("wait_timeout_ms", ctypes.c_int32),
+    ]
+
+
 def _load():
     if not os.path.exists(LIB_PATH):
         raise RuntimeError(
@@ -117,6 +129,15 @@ def _load():
                                          ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64, ctypes.c_int32,
                                          ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, ctypes.c_int64, ctypes.c_void_p]
     lib.tb_moe_combine_peers.restype = ctypes.c_int
+    i32, i64, ptr = ctypes.c_int32, ctypes.c_int64, ctypes.c_void_p
+    lib.tb_moe_route.argtypes = [ptr, i32, i64, i64, i32, i32, i32, i32, ptr, ptr, ptr]
+    lib.tb_moe_route.restype = ctypes.c_int
+    lib.tb_moe_route_backward.argtypes = [ptr, i32, i64, i64, i32, i32, i32, i32, ptr, ptr, ptr, ptr, ptr]
+    lib.tb_moe_route_backward.restype = ctypes.c_int
+    lib.tb_moe_mlp_workspace_bytes.argtypes = [i32] * 5
+    lib.tb_moe_mlp_workspace_bytes.restype = i64
+    lib.tb_moe_mlp.argtypes = [ctypes.POINTER(MoeMlpArgs), ptr]
+    lib.tb_moe_mlp.restype = ctypes.c_int
     lib.tb_tma_stream_probe.argtypes = [ctypes.c_void_p, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_int32,
                                         ctypes.c_int32, ctypes.c_int32, ctypes.c_void_p]
     lib.tb_tma_stream_probe.restype = ctypes.c_int32

@@ -108,6 +108,16 @@ int* device_status_word(int device) {
   return d->status;
 }
 
+int current_device_limits(int* device, int* num_sms, int* smem_optin, int** status) {
+  DeviceState* d = nullptr;
+  const int rc = current_device_state(&d, device);
+  if (rc != TB_OK) return rc;
+  *num_sms = d->num_sms;
+  *smem_optin = d->smem_optin;
+  *status = d->status;
+  return TB_OK;
+}
+
 static CUtensorMapDataType tmap_dtype(int dtype) {
   switch (dtype) {
     case TB_DTYPE_F16: return CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
@@ -130,6 +140,29 @@ int encode_2d(CUtensorMap* map, int dtype, const void* base, uint64_t inner, uin
                         swizzle == 2 ? CU_TENSOR_MAP_SWIZZLE_128B_ATOM_32B
                                      : (swizzle == 1 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE),
                         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return cu_fail(static_cast<int>(r), "cuTensorMapEncodeTiled");
+  return TB_OK;
+}
+
+int encode_nd(CUtensorMap* map, int dtype, const void* base, int rank, const uint64_t* dims, const uint64_t* strides,
+              const uint32_t* box) {
+  if (rank < 2 || rank > 5) return TB_ERR_INVALID;
+  cuuint64_t d[5], st[4];
+  cuuint32_t bx[5], estr[5];
+  bool aligned = (reinterpret_cast<uintptr_t>(base) & 15) == 0;
+  for (int i = 0; i < rank; ++i) {
+    d[i] = dims[i];
+    bx[i] = box[i];
+    estr[i] = 1;
+    if (i > 0) {
+      st[i - 1] = strides[i - 1];
+      aligned = aligned && (strides[i - 1] & 15) == 0;
+    }
+  }
+  if (!aligned) return TB_ERR_ALIGNMENT;
+  CUresult r = g_encode(map, tmap_dtype(dtype), static_cast<cuuint32_t>(rank), const_cast<void*>(base), d, st, bx, estr,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return cu_fail(static_cast<int>(r), "cuTensorMapEncodeTiled");
   return TB_OK;
 }
@@ -757,6 +790,7 @@ const char* tb_status_string(int code) {
     case tb::TB_DEV_TIMEOUT_SCALE: return "device: timed out waiting for block scales";
     case tb::TB_DEV_TIMEOUT_STORE: return "device: timed out publishing a partial tile";
     case tb::TB_DEV_TIMEOUT_TILE_QUEUE: return "device: a role timed out waiting for the next tile of the dynamic schedule";
+    case tb::TB_DEV_TIMEOUT_EXPERT_TILES: return "device: a unit of the few-token expert layer timed out waiting for the units it depends on";
     default: return "unknown status";
   }
 }

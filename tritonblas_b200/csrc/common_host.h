@@ -21,4 +21,12 @@ int* device_status_word(int device);
 int encode_2d(CUtensorMap* map, int dtype, const void* base, uint64_t inner, uint64_t outer, uint64_t outer_stride_bytes,
               uint32_t box_inner, uint32_t box_outer, int swizzle);  // swizzle: 0 none, 1 128B, 2 128B with 32-byte chunks
 
+// Tensor map of any rank up to 5 over 16-bit or wider elements, dims and box innermost first, strides in bytes of dimensions
+// 1 .. rank-1; 128-byte swizzle (box[0] elements must be 128 bytes).
+int encode_nd(CUtensorMap* map, int dtype, const void* base, int rank, const uint64_t* dims, const uint64_t* strides,
+              const uint32_t* box);
+
+// The current device: its number, SMs, shared memory a block may opt in to, and failure word.
+int current_device_limits(int* device, int* num_sms, int* smem_optin, int** status);
+
 }  // namespace tb

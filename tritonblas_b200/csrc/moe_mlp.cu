@@ -1,0 +1,813 @@
+// A whole mixture-of-experts feed-forward for a few tokens:
+//     out[t] = sum_j w[t, j] * W2_e ( silu(G_e x_t) * (U_e x_t) ),   e = ids[t, j],   W1_e = [G_e | U_e]
+//
+// With at most 128 tokens every weight of an expert meets a handful of rows, so the layer is bound by reading the chosen
+// experts' weights once: (distinct experts) * 3 * ffn * hidden * 2 bytes. Two launches:
+//   moe_mlp_plan_kernel  one CTA: the distinct (expert, token) rows in expert order, the counters of the next launch zeroed;
+//   moe_mlp_kernel       one persistent CTA per SM that works through three kinds of units, taken in order from a counter:
+//     1  (expert, tile of ffn)     D[feature, token] = W1 tile . X^T, silu(gate) * up in the epilogue, h in 16-bit pairs;
+//     2  (row group, tile of hidden) D[hidden, row]  = W2 tile . H^T, times the routing weight, fp32 to the workspace;
+//     3  (run of the output)       the sum over a token's rows in slot order, one cast.
+// The weights stand on the 64- or 128-row side of the tensor-core tile and the tokens on its narrow side, so a stage of the
+// shared-memory ring is almost only weights. A unit of the second kind waits for its expert's units of the first kind (a
+// counter per expert), one of the third kind for all units of the second. The weight loader does not: it runs ahead into the
+// second kind's weights while the first kind still drains, so HBM never pauses between the projections.
+//
+// Nothing here needs the CTAs to be resident together. Units are taken in increasing order by CTAs that run, and a unit only
+// waits for units with smaller numbers, which are then being worked on by CTAs that run.
+//
+// Rounding: sums, activation, routing weights and the sum over experts are fp32. The tensor core takes h in 16 bits, so h is
+// kept as two 16-bit halves, h = hi + lo with lo = round(h - hi), and multiplied by both: the MMAs double, the bytes do not,
+// and the result stays as close to the formula as its own rounding allows (a single 16-bit h would double the squared error).
+// No reference counterpart (the reference has no MoE path).
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <mutex>
+
+#include "common_host.h"
+#include "ptx.cuh"
+
+namespace tb {
+
+bool pdl_enabled();  // api.cu
+
+namespace {
+
+constexpr int kMlpMaxTokens = 128;
+constexpr int kMlpMaxTopk = 32;
+constexpr int kMlpMaxExperts = 1024;
+constexpr int kMlpMaxPairs = kMlpMaxTokens * kMlpMaxTopk;
+constexpr int kPlanThreads = 1024;
+constexpr int kMlpThreads = 7 * 32;  // four epilogue warps, weight loader, MMA issuer, activation loader
+constexpr int kWarpWeights = 4, kWarpMma = 5, kWarpAct = 6;
+constexpr int kQueueDepth = 4;
+constexpr int kQueueConsumers = 6;  // MMA issuer, activation loader, four epilogue warps
+constexpr int kMaxStages = 24;
+constexpr int kRowBytes = 128;      // K extent of a stage: one 128-byte swizzle row
+constexpr int kStageK = 64;         // the same in 16-bit elements
+
+// Workspace: int32 words, then h (16-bit, two planes), then the weighted rows (fp32).
+struct MlpLayout {
+  // word offsets
+  static constexpr int kNumExperts = 0;   // distinct experts
+  static constexpr int kNumRows = 1;      // distinct (expert, token) rows
+  static constexpr int kNumGroups = 2;    // row groups: at most group_cap rows of one expert
+  static constexpr int kNextUnit = 4;     // counters
+  static constexpr int kRowsDone = 5;     // units of the second kind that are complete, times the four epilogue warps
+  static constexpr int kLists = 8;
+  int pairs, experts, groups;             // capacities
+  __host__ __device__ int expert_done() const { return kLists; }                       // [experts] units of the first kind done, times four
+  __host__ __device__ int expert_id() const { return expert_done() + experts; }        // [experts] id of the i-th distinct one
+  __host__ __device__ int expert_off() const { return expert_id() + experts; }         // [experts + 1] first row
+  __host__ __device__ int group_slot() const { return expert_off() + experts + 1; }    // [groups] distinct expert of the group
+  __host__ __device__ int group_off() const { return group_slot() + groups; }          // [groups] first row
+  __host__ __device__ int group_rows() const { return group_off() + groups; }          // [groups]
+  __host__ __device__ int row_token() const { return group_rows() + groups; }          // [pairs]
+  __host__ __device__ int row_weight() const { return row_token() + pairs; }           // [pairs] fp32
+  __host__ __device__ int pair_row() const { return row_weight() + pairs; }            // [pairs] row of a (token, slot), -1 = none
+  __host__ __device__ long long words() const { return pair_row() + pairs; }
+};
+
+struct MlpParams {
+  MlpLayout lay;
+  int* ws;
+  int tokens, topk, hidden, ffn;
+  int n1;           // columns of the first kind: tokens rounded up to 16
+  int group_cap;    // rows of a group
+  int stages, stage_bytes, weight_bytes;
+  int acc_stride, tmem_cols;
+  int f_tiles, h_tiles;  // units per expert / row group
+  int items_per_thread;  // third kind: float4 runs of the output per thread
+  long long h_plane;     // rows between the hi and the lo plane of h
+  void* h;
+  float* y;
+  void* out;
+  long long out_stride;
+  int out_vec;           // rows of `out` start on 8-byte boundaries
+  int bf16;
+  uint32_t idesc;        // without the column count
+  int* status;
+  unsigned long long timeout_ns;
+};
+
+// ------------------------------------------------------------------------------------------------------------ plan
+// ids of both widths; an id outside [0, num_experts) routes nowhere. The same expert twice in one token's list is one row
+// with the weights added (in slot order). The order of an expert's rows depends on the order of atomics; every row is one
+// column of the products, computed alike wherever it stands, and the sum over a token's rows goes by slot, so no result
+// depends on it.
+__global__ void __launch_bounds__(kPlanThreads)
+moe_mlp_plan_kernel(const void* __restrict__ ids, int is64, const float* __restrict__ weights, int tokens, int topk, int num_experts,
+                    int group_cap, MlpLayout lay, int* __restrict__ ws) {
+  __shared__ int s_id[kMlpMaxPairs];
+  __shared__ int s_count[kMlpMaxExperts];
+  __shared__ int s_cursor[kMlpMaxExperts];
+  __shared__ int s_scan[3][32];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int pairs = tokens * topk;
+  griddep_wait();
+  griddep_launch_dependents();
+  s_count[tid] = 0;
+  for (int f = tid; f < pairs; f += kPlanThreads) {
+    const long long e = is64 ? static_cast<const long long*>(ids)[f] : static_cast<long long>(static_cast<const int*>(ids)[f]);
+    s_id[f] = (e >= 0 && e < num_experts) ? static_cast<int>(e) : -1;
+  }
+  __syncthreads();
+  for (int f = tid; f < pairs; f += kPlanThreads) {
+    const int e = s_id[f], first = f / topk * topk;
+    bool own = e >= 0;
+    for (int g = first; g < f; ++g) own = own && s_id[g] != e;
+    if (own) atomicAdd(&s_count[e], 1);
+  }
+  __syncthreads();
+  // exclusive sums over the experts of (is used, rows, groups)
+  const int rows = s_count[tid];
+  int v[3] = {rows > 0 ? 1 : 0, rows, (rows + group_cap - 1) / group_cap};
+  int inc[3];
+#pragma unroll
+  for (int q = 0; q < 3; ++q) {
+    int x = v[q];
+#pragma unroll
+    for (int s = 1; s < 32; s <<= 1) {
+      const int o = __shfl_up_sync(0xffffffffu, x, s);
+      if (lane >= s) x += o;
+    }
+    inc[q] = x;
+    if (lane == 31) s_scan[q][warp] = x;
+  }
+  __syncthreads();
+  if (warp == 0) {
+#pragma unroll
+    for (int q = 0; q < 3; ++q) {
+      int x = s_scan[q][lane];
+#pragma unroll
+      for (int s = 1; s < 32; s <<= 1) {
+        const int o = __shfl_up_sync(0xffffffffu, x, s);
+        if (lane >= s) x += o;
+      }
+      s_scan[q][lane] = x;
+    }
+  }
+  __syncthreads();
+  int ex[3];
+#pragma unroll
+  for (int q = 0; q < 3; ++q) ex[q] = inc[q] - v[q] + (warp > 0 ? s_scan[q][warp - 1] : 0);
+  s_cursor[tid] = ex[1];
+  if (rows > 0) {
+    ws[lay.expert_id() + ex[0]] = tid;
+    ws[lay.expert_off() + ex[0]] = ex[1];
+    for (int g = 0; g < v[2]; ++g) {
+      ws[lay.group_slot() + ex[2] + g] = ex[0];
+      ws[lay.group_off() + ex[2] + g] = ex[1] + g * group_cap;
+      ws[lay.group_rows() + ex[2] + g] = min(group_cap, rows - g * group_cap);
+    }
+  }
+  for (int i = tid; i < lay.experts; i += kPlanThreads) ws[lay.expert_done() + i] = 0;
+  if (tid == 0) {
+    ws[MlpLayout::kNumExperts] = s_scan[0][31];
+    ws[MlpLayout::kNumRows] = s_scan[1][31];
+    ws[MlpLayout::kNumGroups] = s_scan[2][31];
+    ws[lay.expert_off() + s_scan[0][31]] = s_scan[1][31];
+    ws[MlpLayout::kNextUnit] = 0;
+    ws[MlpLayout::kRowsDone] = 0;
+  }
+  __syncthreads();
+  for (int f = tid; f < pairs; f += kPlanThreads) {
+    const int e = s_id[f], t = f / topk, first = t * topk;
+    bool own = e >= 0;
+    for (int g = first; g < f; ++g) own = own && s_id[g] != e;
+    int row = -1;
+    if (own) {
+      float w = weights[f];
+      for (int g = f + 1; g < first + topk; ++g)
+        if (s_id[g] == e) w += weights[g];
+      row = atomicAdd(&s_cursor[e], 1);
+      ws[lay.row_token() + row] = t;
+      reinterpret_cast<float*>(ws)[lay.row_weight() + row] = w;
+    }
+    ws[lay.pair_row() + f] = row;
+  }
+}
+
+// ------------------------------------------------------------------------------------------------------------ layer
+__device__ __forceinline__ void tma_load_5d(void* smem_dst, const CUtensorMap* tmap, uint64_t* bar, int x, int y, int z, int w,
+                                            int v) {
+  asm volatile(
+      "cp.async.bulk.tensor.5d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6, %7}], [%2];" ::"r"(
+          smem_u32(smem_dst)),
+      "l"(tmap), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(v)
+      : "memory");
+}
+// Orders generic-proxy accesses to global memory before later accesses of the async proxy (TMA), and the other way round.
+__device__ __forceinline__ void fence_proxy_async_all() { asm volatile("fence.proxy.async;" ::: "memory"); }
+__device__ __forceinline__ int load_acquire(const int* p) {
+  int v;
+  asm volatile("ld.acquire.gpu.global.s32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
+  return v;
+}
+__device__ __forceinline__ void add_release(int* p, int v) {
+  asm volatile("red.release.gpu.global.add.s32 [%0], %1;" ::"l"(p), "r"(v) : "memory");
+}
+
+// Bounded wait until *counter reaches `want`; every lane of the warp calls it and gets the same answer.
+__device__ __forceinline__ bool counter_wait_warp(const int* counter, int want, const WaitCtx& w) {
+  bool ok = true;
+  if ((threadIdx.x & 31) == 0 && load_acquire(counter) < want) {
+    const uint64_t t0 = global_timer_ns();
+    uint32_t spins = 0;
+    while (load_acquire(counter) < want) {
+      if ((++spins & 0x3F) == 0) {
+        if (*w.abort_flag) ok = false;
+        if (ok && global_timer_ns() - t0 > w.timeout_ns) {
+          *w.abort_flag = 1;
+          atomicCAS(w.status, 0, TB_DEV_TIMEOUT_EXPERT_TILES);
+          ok = false;
+        }
+        if (!ok) break;
+      }
+      __nanosleep(spins < 8 ? 32 : 128);
+    }
+  }
+  ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
+  if (ok) load_acquire(counter);  // each lane's own acquire
+  return ok;
+}
+
+// One unit as the weight loader hands it to the other roles.
+struct Unit {
+  int kind;    // 1, 2, 3; 0 = no more units
+  int expert;  // id
+  int tile;    // tile of ffn / hidden, or the run of the output
+  int off;     // first row of the expert (kind 1) or group (kind 2)
+  int rows;
+  int slot;    // index among the distinct experts
+};
+constexpr int kUnitWords = 6;
+
+template <typename T>
+__device__ __forceinline__ unsigned short to_bits(float v);
+template <>
+__device__ __forceinline__ unsigned short to_bits<__nv_bfloat16>(float v) {
+  return __bfloat16_as_ushort(__float2bfloat16_rn(v));
+}
+template <>
+__device__ __forceinline__ unsigned short to_bits<__half>(float v) {
+  return __half_as_ushort(__float2half_rn(v));
+}
+template <typename T>
+__device__ __forceinline__ float from_bits(unsigned short v);
+template <>
+__device__ __forceinline__ float from_bits<__nv_bfloat16>(unsigned short v) {
+  return __bfloat162float(__ushort_as_bfloat16(v));
+}
+template <>
+__device__ __forceinline__ float from_bits<__half>(unsigned short v) {
+  return __half2float(__ushort_as_half(v));
+}
+
+// M: rows of the tensor-core tile. A 64-row accumulator occupies lanes 0-15 of every warp's 32 TMEM lanes, a 128-row one all.
+template <typename T, int M>
+__global__ void __launch_bounds__(kMlpThreads, 1)
+moe_mlp_kernel(const __grid_constant__ CUtensorMap tmap_w1, const __grid_constant__ CUtensorMap tmap_w2,
+               const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ CUtensorMap tmap_h, const MlpParams p) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  __shared__ uint64_t full_bar[kMaxStages], empty_bar[kMaxStages], tmem_full[2], tmem_empty[2];
+  __shared__ uint64_t queue_full[kQueueDepth], queue_empty[kQueueDepth];
+  __shared__ int queue[kQueueDepth][kUnitWords];
+  __shared__ int col_row[4][kMlpMaxTokens];  // per epilogue warp: row of a column's token, -1 = not routed here
+  __shared__ uint32_t tmem_slot;
+  __shared__ int abort_word;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  volatile int* abort_flag = &abort_word;
+  const WaitCtx wctx{abort_flag, p.status, p.timeout_ns};
+  const int stages = p.stages;
+  constexpr int kGroups = M / 64;  // eight-feature groups (16 rows: 8 gate, 8 up) per epilogue warp
+
+  if (threadIdx.x == 0) {
+    abort_word = 0;
+    for (int s = 0; s < stages; ++s) {
+      mbar_init(&full_bar[s], 2);  // weight loader and activation loader
+      mbar_init(&empty_bar[s], 1);
+    }
+    for (int a = 0; a < 2; ++a) {
+      mbar_init(&tmem_full[a], 1);
+      mbar_init(&tmem_empty[a], 4);
+    }
+    for (int i = 0; i < kQueueDepth; ++i) {
+      mbar_init(&queue_full[i], 1);
+      mbar_init(&queue_empty[i], kQueueConsumers);
+    }
+    mbar_fence_init();
+    prefetch_tmap(&tmap_w1);
+    prefetch_tmap(&tmap_w2);
+    prefetch_tmap(&tmap_x);
+    prefetch_tmap(&tmap_h);
+  }
+  if (warp == kWarpMma) {
+    tmem_alloc<1>(&tmem_slot, static_cast<uint32_t>(p.tmem_cols));
+    tmem_relinquish<1>();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = tmem_slot;
+  griddep_launch_dependents();
+  griddep_wait();
+
+  const int* ws = p.ws;
+  const int num_experts = __ldcg(ws + MlpLayout::kNumExperts), num_groups = __ldcg(ws + MlpLayout::kNumGroups);
+  const int units1 = num_experts * p.f_tiles, units2 = num_groups * p.h_tiles;
+  const long long out_items = static_cast<long long>(p.tokens) * (p.hidden / 4);
+  const int run_items = 128 * p.items_per_thread;
+  const int units3 = static_cast<int>((out_items + run_items - 1) / run_items);
+  const int kb1 = (p.hidden + kStageK - 1) / kStageK, kb2 = (p.ffn + kStageK - 1) / kStageK;
+
+  // The next unit out of the queue; every lane of a consuming warp calls it.
+  auto take = [&](int seq, bool& ok) -> Unit {
+    const int i = seq & (kQueueDepth - 1);
+    ok = mbar_wait_warp(&queue_full[i], (seq / kQueueDepth) & 1u, wctx, TB_DEV_TIMEOUT_TILE_QUEUE);
+    Unit u = {0, 0, 0, 0, 0, 0};
+    if (ok) {
+      const volatile int* q = queue[i];
+      u.kind = q[0];
+      u.expert = q[1];
+      u.tile = q[2];
+      u.off = q[3];
+      u.rows = q[4];
+      u.slot = q[5];
+    }
+    __syncwarp();
+    if (lane == 0 && ok) mbar_arrive(&queue_empty[i]);
+    return u;
+  };
+
+  if (warp == kWarpWeights) {
+    // -------------------------------------------------------------- scheduler and weight loader
+    int s = 0, seq = 0;
+    uint32_t ph = 0;
+    bool ok = true;
+    int next = 0;
+    if (lane == 0) next = atomicAdd(p.ws + MlpLayout::kNextUnit, 1);
+    while (true) {
+      const int idx = __shfl_sync(0xffffffffu, next, 0);
+      Unit u = {0, 0, 0, 0, 0, 0};
+      if (idx < units1) {
+        u.kind = 1;
+        u.slot = idx / p.f_tiles;
+        u.tile = idx - u.slot * p.f_tiles;
+        u.expert = __ldcg(ws + p.lay.expert_id() + u.slot);
+        u.off = __ldcg(ws + p.lay.expert_off() + u.slot);
+        u.rows = __ldcg(ws + p.lay.expert_off() + u.slot + 1) - u.off;
+      } else if (idx < units1 + units2) {
+        u.kind = 2;
+        const int g = (idx - units1) / p.h_tiles;
+        u.tile = idx - units1 - g * p.h_tiles;
+        u.slot = __ldcg(ws + p.lay.group_slot() + g);
+        u.off = __ldcg(ws + p.lay.group_off() + g);
+        u.rows = __ldcg(ws + p.lay.group_rows() + g);
+        u.expert = __ldcg(ws + p.lay.expert_id() + u.slot);
+      } else if (idx < units1 + units2 + units3) {
+        u.kind = 3;
+        u.tile = idx - units1 - units2;
+      }
+      const int i = seq & (kQueueDepth - 1);
+      ok = mbar_wait_warp(&queue_empty[i], ((seq / kQueueDepth) & 1u) ^ 1u, wctx, TB_DEV_TIMEOUT_TILE_QUEUE);
+      if (!ok) break;
+      if (lane == 0) {
+        volatile int* q = queue[i];
+        q[0] = u.kind;
+        q[1] = u.expert;
+        q[2] = u.tile;
+        q[3] = u.off;
+        q[4] = u.rows;
+        q[5] = u.slot;
+        mbar_arrive(&queue_full[i]);
+      }
+      __syncwarp();
+      ++seq;
+      if (u.kind == 0) break;
+      if (u.kind == 3) {
+        if (lane == 0) next = atomicAdd(p.ws + MlpLayout::kNextUnit, 1);
+        continue;
+      }
+      const int nkb = u.kind == 1 ? kb1 : kb2;
+      // The number of the next unit is asked for shortly before this one's loads end: its round trip is hidden, and the
+      // CTA does not sit on a unit that another one could have started.
+      const int ask = nkb > 8 ? nkb - 8 : 0;
+      for (int kb = 0; kb < nkb; ++kb) {
+        if (kb == ask && lane == 0) next = atomicAdd(p.ws + MlpLayout::kNextUnit, 1);
+        ok = mbar_wait_warp(&empty_bar[s], ph ^ 1, wctx, TB_DEV_TIMEOUT_SMEM_EMPTY);
+        if (!ok) break;
+        if (elect_one()) {
+          uint8_t* dst = ring + static_cast<size_t>(s) * p.stage_bytes;
+          mbar_arrive_expect_tx(&full_bar[s], static_cast<uint32_t>(p.weight_bytes));
+          if (u.kind == 1) tma_load_5d(dst, &tmap_w1, &full_bar[s], kb * kStageK, 0, 0, u.tile * (M / 16), u.expert);
+          else tma_load_3d(dst, &tmap_w2, &full_bar[s], kb * kStageK, u.tile * M, u.expert);
+        }
+        __syncwarp();
+        if (++s == stages) {
+          s = 0;
+          ph ^= 1;
+        }
+      }
+      if (!ok) break;
+    }
+  } else if (warp == kWarpAct) {
+    // -------------------------------------------------------------- activation loader
+    int s = 0, seq = 0;
+    uint32_t ph = 0;
+    bool ok = true;
+    while (true) {
+      const Unit u = take(seq++, ok);
+      if (!ok || u.kind == 0) break;
+      if (u.kind == 3) continue;
+      const int n2 = (u.rows + 15) & ~15;
+      if (u.kind == 2) {
+        ok = counter_wait_warp(p.ws + p.lay.expert_done() + u.slot, 4 * p.f_tiles, wctx);
+        if (!ok) break;
+        fence_proxy_async_all();  // h was written by ordinary stores of other SMs; it is read by TMA below
+      }
+      const int nkb = u.kind == 1 ? kb1 : kb2;
+      const uint32_t bytes = static_cast<uint32_t>(u.kind == 1 ? p.n1 : 2 * n2) * kRowBytes;
+      for (int kb = 0; kb < nkb; ++kb) {
+        ok = mbar_wait_warp(&empty_bar[s], ph ^ 1, wctx, TB_DEV_TIMEOUT_SMEM_EMPTY);
+        if (!ok) break;
+        if (elect_one()) {
+          uint8_t* dst = ring + static_cast<size_t>(s) * p.stage_bytes + p.weight_bytes;
+          mbar_arrive_expect_tx(&full_bar[s], bytes);
+          if (u.kind == 1) {
+            tma_load_2d(dst, &tmap_x, &full_bar[s], kb * kStageK, 0);
+          } else {
+            // rows behind the group's last one are other rows of h or nothing written yet: columns nobody reads
+            for (int r = 0; r < n2; r += 16) {
+              tma_load_2d(dst + r * kRowBytes, &tmap_h, &full_bar[s], kb * kStageK, u.off + r);
+              tma_load_2d(dst + (n2 + r) * kRowBytes, &tmap_h, &full_bar[s], kb * kStageK, static_cast<int>(p.h_plane) + u.off + r);
+            }
+          }
+        }
+        __syncwarp();
+        if (++s == stages) {
+          s = 0;
+          ph ^= 1;
+        }
+      }
+      if (!ok) break;
+    }
+  } else if (warp == kWarpMma) {
+    // -------------------------------------------------------------- MMA issuer
+    int s = 0, seq = 0, acc = 0;
+    uint32_t ph = 0, acc_parity = 0;
+    bool ok = true;
+    const uint32_t ring_addr = smem_u32(ring);
+    while (true) {
+      const Unit u = take(seq++, ok);
+      if (!ok || u.kind == 0) break;
+      if (u.kind == 3) continue;
+      const int n = u.kind == 1 ? p.n1 : ((u.rows + 15) & ~15);
+      const int nkb = u.kind == 1 ? kb1 : kb2;
+      const uint32_t idesc = p.idesc | (static_cast<uint32_t>(n >> 3) << 17);
+      const uint32_t d = tmem_base + static_cast<uint32_t>(acc * p.acc_stride);
+      ok = mbar_wait_warp(&tmem_empty[acc], ((acc_parity >> acc) & 1u) ^ 1u, wctx, TB_DEV_TIMEOUT_TMEM_EMPTY);
+      if (!ok) break;
+      tc_fence_after();
+      for (int kb = 0; kb < nkb; ++kb) {
+        ok = mbar_wait_warp(&full_bar[s], ph, wctx, TB_DEV_TIMEOUT_SMEM_FULL);
+        if (!ok) break;
+        if (elect_one()) {
+          const uint32_t base = ring_addr + static_cast<uint32_t>(s * p.stage_bytes);
+          const uint64_t adesc = make_smem_desc(base, 16, 1024);
+          const uint64_t bdesc = make_smem_desc(base + p.weight_bytes, 16, 1024);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) umma<0, 1>(d, adesc + 2 * k, bdesc + 2 * k, idesc, (kb > 0 || k > 0) ? 1u : 0u);
+          if (u.kind == 2) {  // the low halves of h
+            const uint64_t ldesc = bdesc + static_cast<uint64_t>((n * kRowBytes) >> 4);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) umma<0, 1>(d, adesc + 2 * k, ldesc + 2 * k, idesc, 1u);
+          }
+          umma_commit(&empty_bar[s]);
+          if (kb + 1 == nkb) umma_commit(&tmem_full[acc]);
+        }
+        __syncwarp();
+        if (++s == stages) {
+          s = 0;
+          ph ^= 1;
+        }
+      }
+      if (!ok) break;
+      acc_parity ^= 1u << acc;
+      acc ^= 1;
+    }
+  } else {
+    // -------------------------------------------------------------- epilogue (warps 0-3, one per TMEM lane quarter)
+    int seq = 0, acc = 0;
+    uint32_t parity = 0;
+    bool ok = true;
+    const float* row_weight = reinterpret_cast<const float*>(ws) + p.lay.row_weight();
+    while (true) {
+      const Unit u = take(seq++, ok);
+      if (!ok || u.kind == 0) break;
+      if (u.kind == 3) {
+        // the sum over a token's rows, in slot order
+        ok = counter_wait_warp(p.ws + MlpLayout::kRowsDone, 4 * units2, wctx);
+        if (!ok) break;
+        const int quads = p.hidden / 4;
+        for (int it = 0; it < p.items_per_thread; ++it) {
+          const long long item = static_cast<long long>(u.tile) * run_items + it * 128 + threadIdx.x;
+          if (item >= out_items) break;
+          const int t = static_cast<int>(item / quads), c = static_cast<int>(item - static_cast<long long>(t) * quads) * 4;
+          const int* rows = ws + p.lay.pair_row() + t * p.topk;
+          float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+          for (int j0 = 0; j0 < p.topk; j0 += 8) {
+            int r[8];
+            float4 v[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) r[j] = j0 + j < p.topk ? __ldcg(rows + j0 + j) : -1;
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              v[j] = r[j] >= 0 ? __ldcg(reinterpret_cast<const float4*>(p.y + static_cast<long long>(r[j]) * p.hidden + c))
+                               : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              sum.x += v[j].x;
+              sum.y += v[j].y;
+              sum.z += v[j].z;
+              sum.w += v[j].w;
+            }
+          }
+          unsigned short* o = reinterpret_cast<unsigned short*>(p.out) + t * p.out_stride + c;
+          const ushort4 b = make_ushort4(to_bits<T>(sum.x), to_bits<T>(sum.y), to_bits<T>(sum.z), to_bits<T>(sum.w));
+          if (p.out_vec) {
+            *reinterpret_cast<ushort4*>(o) = b;
+          } else {
+            o[0] = b.x;
+            o[1] = b.y;
+            o[2] = b.z;
+            o[3] = b.w;
+          }
+        }
+        continue;
+      }
+      if (u.kind == 1) {
+        // which columns are this expert's: looked up while the product is still being accumulated
+        for (int c = lane; c < p.n1; c += 32) col_row[warp][c] = -1;
+        __syncwarp();
+        for (int r = lane; r < u.rows; r += 32) col_row[warp][__ldcg(ws + p.lay.row_token() + u.off + r)] = u.off + r;
+        __syncwarp();
+      }
+      ok = __all_sync(0xffffffffu, mbar_wait(&tmem_full[acc], (parity >> acc) & 1u, wctx, TB_DEV_TIMEOUT_TMEM_FULL));
+      if (!ok) break;
+      tc_fence_after();
+      const uint32_t t_row = tmem_base + (static_cast<uint32_t>(warp * 32) << 16) + static_cast<uint32_t>(acc * p.acc_stride);
+      const int n = u.kind == 1 ? p.n1 : u.rows;
+      for (int c0 = 0; c0 < n; c0 += 32) {
+        uint32_t r[32];
+        tmem_ld_32x32(t_row + c0, r);
+        tmem_ld_wait(r);
+        if (c0 + 32 >= n) {  // the last columns sit in registers
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&tmem_empty[acc]);
+        }
+        if (u.kind == 1) {
+          // lanes 0-7 of a run of 16 hold gate features, lanes 8-15 the matching up features
+          const int f = u.tile * (M / 2) + (warp * kGroups + (lane >> 4)) * 8 + (lane & 7);
+          const bool mine = (lane & 8) == 0 && (M == 128 || lane < 16) && f < p.ffn;
+#pragma unroll
+          for (int j = 0; j < 32; ++j) {
+            const int row = c0 + j < n ? col_row[warp][c0 + j] : -1;
+            if (row >= 0) {  // the same for the whole warp
+              const float g = __uint_as_float(r[j]);
+              const float up = __shfl_xor_sync(0xffffffffu, g, 8);
+              const float h = g / (1.0f + expf(-g)) * up;
+              const unsigned short hi = to_bits<T>(h);
+              // an infinite h has no low half (inf - inf)
+              const float rest = h - from_bits<T>(hi);
+              const unsigned short lo = fabsf(rest) < __builtin_huge_valf() ? to_bits<T>(rest) : static_cast<unsigned short>(0);
+              if (mine) {
+                unsigned short* dst = reinterpret_cast<unsigned short*>(p.h) + static_cast<long long>(row) * p.ffn + f;
+                dst[0] = hi;
+                dst[p.h_plane * p.ffn] = lo;
+              }
+            }
+          }
+        } else {
+          const int hcol = u.tile * M + warp * (M / 4) + lane;
+          const bool mine = (M == 128 || lane < 16) && hcol < p.hidden;
+#pragma unroll
+          for (int j = 0; j < 32; ++j) {
+            const int row = c0 + j;
+            if (row < n && mine)
+              __stcg(p.y + static_cast<long long>(u.off + row) * p.hidden + hcol, __ldcg(row_weight + u.off + row) * __uint_as_float(r[j]));
+          }
+        }
+      }
+      parity ^= 1u << acc;
+      acc ^= 1;
+      // publish this warp's part of the unit: every epilogue warp counts for itself, so none waits for another
+      __threadfence();
+      fence_proxy_async_all();
+      __syncwarp();
+      if (lane == 0) add_release(u.kind == 1 ? p.ws + p.lay.expert_done() + u.slot : p.ws + MlpLayout::kRowsDone, 1);
+    }
+  }
+
+  // ------------------------------------------------------------------ teardown
+  __syncwarp();
+  if (*abort_flag) {
+    // A wait gave up: let copies and MMAs already in flight land before shared memory and TMEM are released.
+    for (int i = 0; i < 64; ++i) __nanosleep(2000);
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kWarpMma) {
+    tc_fence_after();
+    tmem_dealloc<1>(tmem_base, static_cast<uint32_t>(p.tmem_cols));
+  }
+}
+
+// ------------------------------------------------------------------------------------------------------------ host
+struct MlpShape {
+  MlpLayout lay;
+  int n1, group_cap;
+  long long h_offset, y_offset, bytes;  // byte offsets in the workspace
+};
+
+// Columns of the two projections and the workspace they need. The rows of an expert go in groups of at most half the token
+// columns, so that both halves of h take no more shared memory in a stage than the tokens do: an expert that more than half
+// of the tokens choose is read once per group, the second time out of L2.
+MlpShape mlp_shape(int tokens, int topk, int num_experts, int hidden, int ffn) {
+  MlpShape s;
+  s.n1 = (tokens + 15) & ~15;
+  s.group_cap = (s.n1 / 2 + 15) & ~15;
+  s.lay.pairs = tokens * topk;
+  s.lay.experts = num_experts < s.lay.pairs ? num_experts : s.lay.pairs;
+  s.lay.groups = s.lay.experts + s.lay.pairs / s.group_cap;
+  auto up = [](long long v) { return (v + 255) & ~255ll; };
+  s.h_offset = up(s.lay.words() * 4);
+  s.y_offset = s.h_offset + up(2ll * s.lay.pairs * ffn * 2);
+  s.bytes = s.y_offset + up(4ll * s.lay.pairs * hidden);
+  return s;
+}
+
+bool mlp_sizes_ok(int tokens, int topk, int num_experts, int hidden, int ffn) {
+  return tokens >= 0 && tokens <= kMlpMaxTokens && topk >= 1 && topk <= kMlpMaxTopk && num_experts >= 1 &&
+         num_experts <= kMlpMaxExperts && hidden >= 8 && ffn >= 8 && hidden % 8 == 0 && ffn % 8 == 0 &&
+         hidden <= (1 << 20) && ffn <= (1 << 20);
+}
+
+template <typename T, int M>
+int mlp_launch(const CUtensorMap& w1, const CUtensorMap& w2, const CUtensorMap& x, const CUtensorMap& h, const MlpParams& p, int grid,
+               int smem_bytes, int device, cudaStream_t stream) {
+  auto kernel = moe_mlp_kernel<T, M>;
+  // the opt-in shared-memory size is set once per instantiation and device, and again if a launch needs more
+  static int configured[64] = {};
+  static std::mutex mu;
+  {
+    std::lock_guard<std::mutex> lk(mu);
+    if (smem_bytes > configured[device & 63]) {
+      cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes);
+      if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(moe_mlp)");
+      configured[device & 63] = smem_bytes;
+    }
+  }
+  cudaLaunchConfig_t lc = {};
+  lc.gridDim = dim3(static_cast<unsigned>(grid), 1, 1);
+  lc.blockDim = dim3(kMlpThreads, 1, 1);
+  lc.dynamicSmemBytes = static_cast<size_t>(smem_bytes);
+  lc.stream = stream;
+  cudaLaunchAttribute attr[1];
+  lc.attrs = attr;
+  lc.numAttrs = 0;
+  if (pdl_enabled()) {
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    lc.numAttrs = 1;
+  }
+  cudaError_t e = cudaLaunchKernelEx(&lc, kernel, w1, w2, x, h, p);
+  if (e != cudaSuccess) return cuda_fail(e, "moe_mlp_kernel launch");
+  g_launches.fetch_add(1, std::memory_order_relaxed);
+  return TB_OK;
+}
+
+int mlp_impl(const tb_moe_mlp_args& a, cudaStream_t stream) {
+  if (!mlp_sizes_ok(a.tokens, a.topk, a.num_experts, a.hidden, a.ffn)) return TB_ERR_INVALID;
+  if (a.dtype != TB_DTYPE_BF16 && a.dtype != TB_DTYPE_F16) return TB_ERR_UNSUPPORTED;
+  if (a.tokens == 0) return TB_OK;
+  if (a.x == nullptr || a.w1 == nullptr || a.w2 == nullptr || a.topk_ids == nullptr || a.topk_weights == nullptr ||
+      a.out == nullptr)
+    return TB_ERR_INVALID;
+  if ((a.tokens > 1 && (a.x_row_stride < a.hidden || a.out_row_stride < a.hidden)) || a.w1_row_stride < a.hidden ||
+      a.w2_row_stride < a.ffn || a.w1_expert_stride < 0 || a.w2_expert_stride < 0)
+    return TB_ERR_INVALID;
+  if (reinterpret_cast<uintptr_t>(a.out) % 2 || reinterpret_cast<uintptr_t>(a.topk_weights) % 4 ||
+      reinterpret_cast<uintptr_t>(a.topk_ids) % (a.ids_are_int64 ? 8 : 4))
+    return TB_ERR_ALIGNMENT;
+  const MlpShape s = mlp_shape(a.tokens, a.topk, a.num_experts, a.hidden, a.ffn);
+  if (a.workspace == nullptr || a.workspace_bytes < s.bytes) return TB_ERR_WORKSPACE;
+  if (reinterpret_cast<uintptr_t>(a.workspace) % 256) return TB_ERR_ALIGNMENT;
+  int device = 0, num_sms = 0, smem_optin = 0;
+  int* status = nullptr;
+  int rc = current_device_limits(&device, &num_sms, &smem_optin, &status);
+  if (rc != TB_OK) return rc;
+
+  char* ws = static_cast<char*>(a.workspace);
+  MlpParams p = {};
+  p.lay = s.lay;
+  p.ws = reinterpret_cast<int*>(ws);
+  p.tokens = a.tokens;
+  p.topk = a.topk;
+  p.hidden = a.hidden;
+  p.ffn = a.ffn;
+  p.n1 = s.n1;
+  p.group_cap = s.group_cap;
+  p.h = ws + s.h_offset;
+  p.h_plane = s.lay.pairs;
+  p.y = reinterpret_cast<float*>(ws + s.y_offset);
+  p.out = a.out;
+  p.out_stride = a.out_row_stride;
+  p.out_vec = (reinterpret_cast<uintptr_t>(a.out) % 8 == 0 && (a.tokens == 1 || a.out_row_stride % 4 == 0)) ? 1 : 0;
+  p.bf16 = a.dtype == TB_DTYPE_BF16 ? 1 : 0;
+  p.status = status;
+  p.timeout_ns = a.wait_timeout_ms > 0 ? static_cast<unsigned long long>(a.wait_timeout_ms) * 1000000ull : 2000000000ull;
+
+  // Rows of the tensor-core tile. See mlp_tile_rows.
+  const int m = a.tokens * a.topk >= 64 ? 128 : 64;
+  p.weight_bytes = m * kRowBytes;
+  const int act_rows = s.n1 > 2 * s.group_cap ? s.n1 : 2 * s.group_cap;
+  p.stage_bytes = p.weight_bytes + act_rows * kRowBytes;
+  const int fixed = 8192;  // barriers, queue and column tables (static), alignment of the ring
+  p.stages = (smem_optin - fixed) / p.stage_bytes;
+  if (p.stages > kMaxStages) p.stages = kMaxStages;
+  if (p.stages < 2) return TB_ERR_UNSUPPORTED;
+  const int smem_bytes = p.stages * p.stage_bytes + 1024;
+  p.acc_stride = (s.n1 + 31) & ~31;
+  p.tmem_cols = 64;
+  while (p.tmem_cols < 2 * p.acc_stride) p.tmem_cols <<= 1;
+  p.f_tiles = (a.ffn + m / 2 - 1) / (m / 2);
+  p.h_tiles = (a.hidden + m - 1) / m;
+  const long long items = static_cast<long long>(a.tokens) * (a.hidden / 4);
+  p.items_per_thread = static_cast<int>((items + 128ll * num_sms - 1) / (128ll * num_sms));
+  // fp32 accumulators; operand format (0 = f16, 1 = bf16); the column count is added per unit
+  const uint32_t fmt = p.bf16 ? 1u : 0u;
+  p.idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | (static_cast<uint32_t>(m >> 4) << 24);
+
+  CUtensorMap tw1, tw2, tx, th;
+  const uint64_t es = 2;
+  {
+    // W1 as [expert][ffn / 8][gate, up][8][hidden]: a box of M/16 x 2 x 8 rows lands as runs of 8 gate rows and the 8 matching
+    // up rows, so gate and up of a feature end in the same warp's TMEM lanes, 8 lanes apart
+    const uint64_t row = static_cast<uint64_t>(a.w1_row_stride) * es;
+    const uint64_t dims[5] = {static_cast<uint64_t>(a.hidden), 8, 2, static_cast<uint64_t>(a.ffn / 8), static_cast<uint64_t>(a.num_experts)};
+    const uint64_t strides[4] = {row, row * a.ffn, row * 8, a.num_experts > 1 ? static_cast<uint64_t>(a.w1_expert_stride) * es : row * 2 * a.ffn};
+    const uint32_t box[5] = {kStageK, 8, 2, static_cast<uint32_t>(m / 16), 1};
+    if ((rc = encode_nd(&tw1, a.dtype, a.w1, 5, dims, strides, box)) != TB_OK) return rc;
+  }
+  {
+    const uint64_t dims[3] = {static_cast<uint64_t>(a.ffn), static_cast<uint64_t>(a.hidden), static_cast<uint64_t>(a.num_experts)};
+    const uint64_t row = static_cast<uint64_t>(a.w2_row_stride) * es;
+    const uint64_t strides[2] = {row, a.num_experts > 1 ? static_cast<uint64_t>(a.w2_expert_stride) * es : row * a.hidden};
+    const uint32_t box[3] = {kStageK, static_cast<uint32_t>(m), 1};
+    if ((rc = encode_nd(&tw2, a.dtype, a.w2, 3, dims, strides, box)) != TB_OK) return rc;
+  }
+  const uint64_t x_stride = static_cast<uint64_t>(a.tokens > 1 ? a.x_row_stride : a.hidden) * es;
+  if ((rc = encode_2d(&tx, a.dtype, a.x, a.hidden, a.tokens, x_stride, kStageK, s.n1, 1)) != TB_OK) return rc;
+  if ((rc = encode_2d(&th, a.dtype, p.h, a.ffn, 2ull * s.lay.pairs, a.ffn * es, kStageK, 16, 1)) != TB_OK) return rc;
+
+  cudaLaunchConfig_t lc = {};
+  lc.gridDim = dim3(1, 1, 1);
+  lc.blockDim = dim3(kPlanThreads, 1, 1);
+  lc.stream = stream;
+  cudaLaunchAttribute attr[1];
+  lc.attrs = attr;
+  lc.numAttrs = 0;
+  if (pdl_enabled()) {
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    lc.numAttrs = 1;
+  }
+  cudaError_t e = cudaLaunchKernelEx(&lc, moe_mlp_plan_kernel, a.topk_ids, static_cast<int>(a.ids_are_int64 != 0), a.topk_weights,
+                                     static_cast<int>(a.tokens), static_cast<int>(a.topk), static_cast<int>(a.num_experts),
+                                     s.group_cap, s.lay, p.ws);
+  if (e != cudaSuccess) return cuda_fail(e, "moe_mlp_plan_kernel launch");
+  g_launches.fetch_add(1, std::memory_order_relaxed);
+  if (p.bf16)
+    return m == 64 ? mlp_launch<__nv_bfloat16, 64>(tw1, tw2, tx, th, p, num_sms, smem_bytes, device, stream)
+                   : mlp_launch<__nv_bfloat16, 128>(tw1, tw2, tx, th, p, num_sms, smem_bytes, device, stream);
+  return m == 64 ? mlp_launch<__half, 64>(tw1, tw2, tx, th, p, num_sms, smem_bytes, device, stream)
+                 : mlp_launch<__half, 128>(tw1, tw2, tx, th, p, num_sms, smem_bytes, device, stream);
+}
+
+}  // namespace
+}  // namespace tb
+
+extern "C" int64_t tb_moe_mlp_workspace_bytes(int32_t tokens, int32_t topk, int32_t num_experts, int32_t hidden, int32_t ffn) {
+  if (!tb::mlp_sizes_ok(tokens, topk, num_experts, hidden, ffn) || tokens == 0) return 0;
+  return tb::mlp_shape(tokens, topk, num_experts, hidden, ffn).bytes;
+}
+
+extern "C" int tb_moe_mlp(const tb_moe_mlp_args* args, void* stream) {
+  if (args == nullptr) return TB_ERR_INVALID;
+  return tb::mlp_impl(*args, static_cast<cudaStream_t>(stream));
+}

@@ -18,6 +18,7 @@ enum : int {
   TB_DEV_TIMEOUT_SCALE = 106,        // block-scale copy wait
   TB_DEV_TIMEOUT_STORE = 107,
   TB_DEV_TIMEOUT_TILE_QUEUE = 108,   // a role waited for the next tile index of the dynamic schedule
+  TB_DEV_TIMEOUT_EXPERT_TILES = 109, // few-token expert layer: a unit waited for the units it depends on
 };
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) {
