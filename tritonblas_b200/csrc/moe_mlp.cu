@@ -43,9 +43,13 @@ constexpr int kMlpThreads = 7 * 32;  // four epilogue warps, weight loader, MMA 
 constexpr int kWarpWeights = 4, kWarpMma = 5, kWarpAct = 6;
 constexpr int kQueueDepth = 4;
 constexpr int kQueueConsumers = 6;  // MMA issuer, activation loader, four epilogue warps
-constexpr int kMaxStages = 24;
+constexpr int kMaxStages = 10;  // 160 KB of weights ahead: more only lengthens every other round trip to memory
 constexpr int kRowBytes = 128;      // K extent of a stage: one 128-byte swizzle row
 constexpr int kStageK = 64;         // the same in 16-bit elements
+// Slabs of 64 K elements per stage: every stage carries at least 16 KB of weights. The roles spend about 380 clocks per stage
+// on waits and branches that nothing hides; with 8 KB stages that was more than the 350 clocks HBM needs for one (measured at
+// one token, 64-row tiles: 33 GB/s per SM, 44 with 16 KB).
+__host__ __device__ constexpr int mlp_slabs(int m) { return m == 64 ? 2 : 1; }
 
 // Workspace: int32 words, then h (16-bit, two planes), then the weighted rows (fp32).
 struct MlpLayout {
@@ -61,9 +65,10 @@ struct MlpLayout {
   __host__ __device__ int expert_id() const { return expert_done() + experts; }        // [experts] id of the i-th distinct one
   __host__ __device__ int expert_off() const { return expert_id() + experts; }         // [experts + 1] first row
   __host__ __device__ int group_slot() const { return expert_off() + experts + 1; }    // [groups] distinct expert of the group
-  __host__ __device__ int group_off() const { return group_slot() + groups; }          // [groups] first row
-  __host__ __device__ int group_rows() const { return group_off() + groups; }          // [groups]
-  __host__ __device__ int row_token() const { return group_rows() + groups; }          // [pairs]
+  __host__ __device__ int group_expert() const { return group_slot() + groups; }       // [groups] its id
+  __host__ __device__ int group_off() const { return group_expert() + groups; }        // [groups] first row
+  __host__ __device__ int group_end() const { return group_off() + groups; }           // [groups] one past the last row
+  __host__ __device__ int row_token() const { return group_end() + groups; }           // [pairs]
   __host__ __device__ int row_weight() const { return row_token() + pairs; }           // [pairs] fp32
   __host__ __device__ int pair_row() const { return row_weight() + pairs; }            // [pairs] row of a (token, slot), -1 = none
   __host__ __device__ long long words() const { return pair_row() + pairs; }
@@ -73,14 +78,15 @@ struct MlpParams {
   MlpLayout lay;
   int* ws;
   int tokens, topk, hidden, ffn;
-  int n1;           // columns of the first kind: tokens rounded up to 16
+  int n1;           // columns of the first kind: tokens rounded up to the MMA's granularity
   int group_cap;    // rows of a group
-  int stages, stage_bytes, weight_bytes;
+  int stages, stage_bytes;
+  int act_bytes;    // shared memory of one slab of activations
   int acc_stride, tmem_cols;
   int f_tiles, h_tiles;  // units per expert / row group
-  int items_per_thread;  // third kind: float4 runs of the output per thread
-  long long h_plane;     // rows between the hi and the lo plane of h
-  void* h;
+  int quads_per_thread;  // third kind: float4 runs of one token's output per thread
+  int runs;              // third kind: units per token
+  void* h;               // [row][hi, lo][ffn]
   float* y;
   void* out;
   long long out_stride;
@@ -158,8 +164,9 @@ moe_mlp_plan_kernel(const void* __restrict__ ids, int is64, const float* __restr
     ws[lay.expert_off() + ex[0]] = ex[1];
     for (int g = 0; g < v[2]; ++g) {
       ws[lay.group_slot() + ex[2] + g] = ex[0];
+      ws[lay.group_expert() + ex[2] + g] = tid;
       ws[lay.group_off() + ex[2] + g] = ex[1] + g * group_cap;
-      ws[lay.group_rows() + ex[2] + g] = min(group_cap, rows - g * group_cap);
+      ws[lay.group_end() + ex[2] + g] = ex[1] + min((g + 1) * group_cap, rows);
     }
   }
   for (int i = tid; i < lay.experts; i += kPlanThreads) ws[lay.expert_done() + i] = 0;
@@ -233,6 +240,16 @@ __device__ __forceinline__ bool counter_wait_warp(const int* counter, int want, 
   return ok;
 }
 
+// mbar_wait_warp with its slow part out of line: the roles' loops are one warp each, so every taken branch in them is exposed.
+__device__ __noinline__ bool wait_slow(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* status,
+                                       unsigned long long timeout_ns, int code) {
+  return mbar_wait_warp(bar, parity, WaitCtx{abort_flag, status, timeout_ns}, code);
+}
+__device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity, const WaitCtx& w, int code) {
+  if (__builtin_expect(__all_sync(0xffffffffu, mbar_try_wait(bar, parity)), 1)) return true;
+  return wait_slow(bar, parity, w.abort_flag, w.status, w.timeout_ns, code);
+}
+
 // One unit as the weight loader hands it to the other roles.
 struct Unit {
   int kind;    // 1, 2, 3; 0 = no more units
@@ -265,11 +282,27 @@ __device__ __forceinline__ float from_bits<__half>(unsigned short v) {
   return __half2float(__ushort_as_half(v));
 }
 
-// M: rows of the tensor-core tile. A 64-row accumulator occupies lanes 0-15 of every warp's 32 TMEM lanes, a 128-row one all.
+__device__ __forceinline__ float4 add4(float4 a, float4 b) { return make_float4(a.x + b.x, a.y + b.y, a.z + b.z, a.w + b.w); }
+// Four consecutive outputs; `vec`: the address is a multiple of 8.
+template <typename T>
+__device__ __forceinline__ void store_quad(unsigned short* o, float4 v, int vec) {
+  const ushort4 b = make_ushort4(to_bits<T>(v.x), to_bits<T>(v.y), to_bits<T>(v.z), to_bits<T>(v.w));
+  if (vec) {
+    *reinterpret_cast<ushort4*>(o) = b;
+  } else {
+    o[0] = b.x;
+    o[1] = b.y;
+    o[2] = b.z;
+    o[3] = b.w;
+  }
+}
+
+// M: weight rows of a tile (256: two MMA tiles of 128). A 64-row accumulator occupies lanes 0-15 of every warp's 32 TMEM lanes, a 128-row one all.
 template <typename T, int M>
 __global__ void __launch_bounds__(kMlpThreads, 1)
 moe_mlp_kernel(const __grid_constant__ CUtensorMap tmap_w1, const __grid_constant__ CUtensorMap tmap_w2,
-               const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ CUtensorMap tmap_h, const MlpParams p) {
+               const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ CUtensorMap tmap_h2,
+               const __grid_constant__ CUtensorMap tmap_h8, const __grid_constant__ CUtensorMap tmap_h32, const MlpParams p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   __shared__ uint64_t full_bar[kMaxStages], empty_bar[kMaxStages], tmem_full[2], tmem_empty[2];
@@ -283,7 +316,12 @@ moe_mlp_kernel(const __grid_constant__ CUtensorMap tmap_w1, const __grid_constan
   volatile int* abort_flag = &abort_word;
   const WaitCtx wctx{abort_flag, p.status, p.timeout_ns};
   const int stages = p.stages;
-  constexpr int kGroups = M / 64;  // eight-feature groups (16 rows: 8 gate, 8 up) per epilogue warp
+  constexpr int kMmaRows = M < 128 ? M : 128;    // rows of one MMA
+  constexpr int kSubs = M / kMmaRows;            // MMA tiles side by side that share the activations
+  constexpr int kSlabs = mlp_slabs(M);           // 64-element slabs of K per stage
+  constexpr uint32_t kSlabBytes = M * kRowBytes; // weights of one slab
+  constexpr uint32_t kActBase = kSlabs * kSlabBytes;
+  constexpr int kGroups = kMmaRows / 64;         // eight-feature groups (16 rows: 8 gate, 8 up) per epilogue warp and MMA tile
 
   if (threadIdx.x == 0) {
     abort_word = 0;
@@ -303,7 +341,6 @@ moe_mlp_kernel(const __grid_constant__ CUtensorMap tmap_w1, const __grid_constan
     prefetch_tmap(&tmap_w1);
     prefetch_tmap(&tmap_w2);
     prefetch_tmap(&tmap_x);
-    prefetch_tmap(&tmap_h);
   }
   if (warp == kWarpMma) {
     tmem_alloc<1>(&tmem_slot, static_cast<uint32_t>(p.tmem_cols));
@@ -319,10 +356,9 @@ moe_mlp_kernel(const __grid_constant__ CUtensorMap tmap_w1, const __grid_constan
   const int* ws = p.ws;
   const int num_experts = __ldcg(ws + MlpLayout::kNumExperts), num_groups = __ldcg(ws + MlpLayout::kNumGroups);
   const int units1 = num_experts * p.f_tiles, units2 = num_groups * p.h_tiles;
-  const long long out_items = static_cast<long long>(p.tokens) * (p.hidden / 4);
-  const int run_items = 128 * p.items_per_thread;
-  const int units3 = static_cast<int>((out_items + run_items - 1) / run_items);
-  const int kb1 = (p.hidden + kStageK - 1) / kStageK, kb2 = (p.ffn + kStageK - 1) / kStageK;
+  const int units3 = p.tokens * p.runs;
+  constexpr int kColAlign = M < 128 ? 8 : 16;  // columns of an MMA come in multiples of this
+  const int kb1 = (p.hidden + kSlabs * kStageK - 1) / (kSlabs * kStageK), kb2 = (p.ffn + kSlabs * kStageK - 1) / (kSlabs * kStageK);
 
   // The next unit out of the queue; every lane of a consuming warp calls it.
   auto take = [&](int seq, bool& ok) -> Unit {
@@ -348,30 +384,41 @@ moe_mlp_kernel(const __grid_constant__ CUtensorMap tmap_w1, const __grid_constan
     int s = 0, seq = 0;
     uint32_t ph = 0;
     bool ok = true;
+    // The number of the next unit and its row of the plan are asked for while the current unit's loads go out: under load a
+    // round trip takes several microseconds, and nothing else would hide it.
     int next = 0;
-    if (lane == 0) next = atomicAdd(p.ws + MlpLayout::kNextUnit, 1);
-    while (true) {
+    Unit pending = {0, 0, 0, 0, 0, 0};
+    auto ask = [&]() {
+      if (lane == 0) next = atomicAdd(p.ws + MlpLayout::kNextUnit, 1);
+    };
+    auto look_up = [&]() {
       const int idx = __shfl_sync(0xffffffffu, next, 0);
-      Unit u = {0, 0, 0, 0, 0, 0};
+      pending = Unit{0, 0, 0, 0, 0, 0};
       if (idx < units1) {
-        u.kind = 1;
-        u.slot = idx / p.f_tiles;
-        u.tile = idx - u.slot * p.f_tiles;
-        u.expert = __ldcg(ws + p.lay.expert_id() + u.slot);
-        u.off = __ldcg(ws + p.lay.expert_off() + u.slot);
-        u.rows = __ldcg(ws + p.lay.expert_off() + u.slot + 1) - u.off;
+        pending.kind = 1;
+        pending.slot = idx / p.f_tiles;
+        pending.tile = idx - pending.slot * p.f_tiles;
+        pending.expert = __ldcg(ws + p.lay.expert_id() + pending.slot);
+        pending.off = __ldcg(ws + p.lay.expert_off() + pending.slot);
+        pending.rows = __ldcg(ws + p.lay.expert_off() + pending.slot + 1);  // one past the last row
       } else if (idx < units1 + units2) {
-        u.kind = 2;
+        pending.kind = 2;
         const int g = (idx - units1) / p.h_tiles;
-        u.tile = idx - units1 - g * p.h_tiles;
-        u.slot = __ldcg(ws + p.lay.group_slot() + g);
-        u.off = __ldcg(ws + p.lay.group_off() + g);
-        u.rows = __ldcg(ws + p.lay.group_rows() + g);
-        u.expert = __ldcg(ws + p.lay.expert_id() + u.slot);
+        pending.tile = idx - units1 - g * p.h_tiles;
+        pending.slot = __ldcg(ws + p.lay.group_slot() + g);
+        pending.expert = __ldcg(ws + p.lay.group_expert() + g);
+        pending.off = __ldcg(ws + p.lay.group_off() + g);
+        pending.rows = __ldcg(ws + p.lay.group_end() + g);
       } else if (idx < units1 + units2 + units3) {
-        u.kind = 3;
-        u.tile = idx - units1 - units2;
+        pending.kind = 3;
+        pending.tile = idx - units1 - units2;
       }
+    };
+    ask();
+    look_up();
+    while (true) {
+      Unit u = pending;
+      u.rows -= u.off;
       const int i = seq & (kQueueDepth - 1);
       ok = mbar_wait_warp(&queue_empty[i], ((seq / kQueueDepth) & 1u) ^ 1u, wctx, TB_DEV_TIMEOUT_TILE_QUEUE);
       if (!ok) break;
@@ -389,23 +436,29 @@ moe_mlp_kernel(const __grid_constant__ CUtensorMap tmap_w1, const __grid_constan
       ++seq;
       if (u.kind == 0) break;
       if (u.kind == 3) {
-        if (lane == 0) next = atomicAdd(p.ws + MlpLayout::kNextUnit, 1);
+        ask();
+        look_up();
         continue;
       }
       const int nkb = u.kind == 1 ? kb1 : kb2;
-      // The number of the next unit is asked for shortly before this one's loads end: its round trip is hidden, and the
-      // CTA does not sit on a unit that another one could have started.
-      const int ask = nkb > 8 ? nkb - 8 : 0;
-      for (int kb = 0; kb < nkb; ++kb) {
-        if (kb == ask && lane == 0) next = atomicAdd(p.ws + MlpLayout::kNextUnit, 1);
-        ok = mbar_wait_warp(&empty_bar[s], ph ^ 1, wctx, TB_DEV_TIMEOUT_SMEM_EMPTY);
-        if (!ok) break;
-        if (elect_one()) {
-          uint8_t* dst = ring + static_cast<size_t>(s) * p.stage_bytes;
-          mbar_arrive_expect_tx(&full_bar[s], static_cast<uint32_t>(p.weight_bytes));
-          if (u.kind == 1) tma_load_5d(dst, &tmap_w1, &full_bar[s], kb * kStageK, 0, 0, u.tile * (M / 16), u.expert);
-          else tma_load_3d(dst, &tmap_w2, &full_bar[s], kb * kStageK, u.tile * M, u.expert);
+      const int ask_at = nkb > 16 ? nkb - 16 : 0, look_at = nkb > 6 ? nkb - 6 : nkb - 1;
+      const CUtensorMap* map = u.kind == 1 ? &tmap_w1 : &tmap_w2;
+      auto load = [&](int kb) {
+        uint8_t* dst = ring + static_cast<size_t>(s) * p.stage_bytes;
+        mbar_arrive_expect_tx(&full_bar[s], kSlabs * kSlabBytes);
+#pragma unroll
+        for (int b = 0; b < kSlabs; ++b) {
+          const int x = (kb * kSlabs + b) * kStageK;
+          if (u.kind == 1) tma_load_5d(dst + b * kSlabBytes, map, &full_bar[s], x, 0, 0, u.tile * (M / 16), u.expert);
+          else tma_load_3d(dst + b * kSlabBytes, map, &full_bar[s], x, u.tile * M, u.expert);
         }
+      };
+      for (int kb = 0; kb < nkb; ++kb) {
+        if (kb == ask_at) ask();
+        if (kb == look_at) look_up();
+        ok = wait_warp(&empty_bar[s], ph ^ 1, wctx, TB_DEV_TIMEOUT_SMEM_EMPTY);
+        if (!ok) break;
+        if (elect_one()) load(kb);
         __syncwarp();
         if (++s == stages) {
           s = 0;
@@ -416,6 +469,8 @@ moe_mlp_kernel(const __grid_constant__ CUtensorMap tmap_w1, const __grid_constan
     }
   } else if (warp == kWarpAct) {
     // -------------------------------------------------------------- activation loader
+    // Only rows that exist are copied. What stands in the other rows of the operand (an earlier stage's values) makes columns
+    // of the product that nobody reads, and a column depends on its own row alone.
     int s = 0, seq = 0;
     uint32_t ph = 0;
     bool ok = true;
@@ -423,29 +478,28 @@ moe_mlp_kernel(const __grid_constant__ CUtensorMap tmap_w1, const __grid_constan
       const Unit u = take(seq++, ok);
       if (!ok || u.kind == 0) break;
       if (u.kind == 3) continue;
-      const int n2 = (u.rows + 15) & ~15;
+      // rows of h (hi and lo of every row of the group) come in the smallest copies that do not multiply their number
+      const int h_rows = 2 * u.rows, h_box = h_rows <= 2 ? 2 : (h_rows <= 8 ? 8 : 32);
+      const CUtensorMap* h_map = h_box == 2 ? &tmap_h2 : (h_box == 8 ? &tmap_h8 : &tmap_h32);
       if (u.kind == 2) {
         ok = counter_wait_warp(p.ws + p.lay.expert_done() + u.slot, 4 * p.f_tiles, wctx);
         if (!ok) break;
         fence_proxy_async_all();  // h was written by ordinary stores of other SMs; it is read by TMA below
       }
       const int nkb = u.kind == 1 ? kb1 : kb2;
-      const uint32_t bytes = static_cast<uint32_t>(u.kind == 1 ? p.n1 : 2 * n2) * kRowBytes;
+      const CUtensorMap* map = u.kind == 1 ? &tmap_x : h_map;
+      const int rows = u.kind == 1 ? p.tokens : (h_rows + h_box - 1) / h_box * h_box;
+      const int box = u.kind == 1 ? p.tokens : h_box, row0 = u.kind == 1 ? 0 : 2 * u.off;
       for (int kb = 0; kb < nkb; ++kb) {
-        ok = mbar_wait_warp(&empty_bar[s], ph ^ 1, wctx, TB_DEV_TIMEOUT_SMEM_EMPTY);
+        ok = wait_warp(&empty_bar[s], ph ^ 1, wctx, TB_DEV_TIMEOUT_SMEM_EMPTY);
         if (!ok) break;
         if (elect_one()) {
-          uint8_t* dst = ring + static_cast<size_t>(s) * p.stage_bytes + p.weight_bytes;
-          mbar_arrive_expect_tx(&full_bar[s], bytes);
-          if (u.kind == 1) {
-            tma_load_2d(dst, &tmap_x, &full_bar[s], kb * kStageK, 0);
-          } else {
-            // rows behind the group's last one are other rows of h or nothing written yet: columns nobody reads
-            for (int r = 0; r < n2; r += 16) {
-              tma_load_2d(dst + r * kRowBytes, &tmap_h, &full_bar[s], kb * kStageK, u.off + r);
-              tma_load_2d(dst + (n2 + r) * kRowBytes, &tmap_h, &full_bar[s], kb * kStageK, static_cast<int>(p.h_plane) + u.off + r);
-            }
-          }
+          uint8_t* dst = ring + static_cast<size_t>(s) * p.stage_bytes + kActBase;
+          mbar_arrive_expect_tx(&full_bar[s], static_cast<uint32_t>(kSlabs * rows * kRowBytes));
+#pragma unroll
+          for (int b = 0; b < kSlabs; ++b)
+            for (int r = 0; r < rows; r += box)
+              tma_load_2d(dst + b * p.act_bytes + r * kRowBytes, map, &full_bar[s], (kb * kSlabs + b) * kStageK, row0 + r);
         }
         __syncwarp();
         if (++s == stages) {
@@ -460,32 +514,31 @@ moe_mlp_kernel(const __grid_constant__ CUtensorMap tmap_w1, const __grid_constan
     int s = 0, seq = 0, acc = 0;
     uint32_t ph = 0, acc_parity = 0;
     bool ok = true;
-    const uint32_t ring_addr = smem_u32(ring);
+    const uint64_t desc0 = make_smem_desc(smem_u32(ring), 16, 1024);
     while (true) {
       const Unit u = take(seq++, ok);
       if (!ok || u.kind == 0) break;
       if (u.kind == 3) continue;
-      const int n = u.kind == 1 ? p.n1 : ((u.rows + 15) & ~15);
+      const int n = u.kind == 1 ? p.n1 : ((2 * u.rows + kColAlign - 1) & ~(kColAlign - 1));
       const int nkb = u.kind == 1 ? kb1 : kb2;
       const uint32_t idesc = p.idesc | (static_cast<uint32_t>(n >> 3) << 17);
-      const uint32_t d = tmem_base + static_cast<uint32_t>(acc * p.acc_stride);
-      ok = mbar_wait_warp(&tmem_empty[acc], ((acc_parity >> acc) & 1u) ^ 1u, wctx, TB_DEV_TIMEOUT_TMEM_EMPTY);
+      const uint32_t d = tmem_base + static_cast<uint32_t>(acc * kSubs * p.acc_stride);
+      ok = wait_warp(&tmem_empty[acc], ((acc_parity >> acc) & 1u) ^ 1u, wctx, TB_DEV_TIMEOUT_TMEM_EMPTY);
       if (!ok) break;
       tc_fence_after();
       for (int kb = 0; kb < nkb; ++kb) {
-        ok = mbar_wait_warp(&full_bar[s], ph, wctx, TB_DEV_TIMEOUT_SMEM_FULL);
+        ok = wait_warp(&full_bar[s], ph, wctx, TB_DEV_TIMEOUT_SMEM_FULL);
         if (!ok) break;
         if (elect_one()) {
-          const uint32_t base = ring_addr + static_cast<uint32_t>(s * p.stage_bytes);
-          const uint64_t adesc = make_smem_desc(base, 16, 1024);
-          const uint64_t bdesc = make_smem_desc(base + p.weight_bytes, 16, 1024);
+          const uint64_t stage = desc0 + static_cast<uint64_t>((s * p.stage_bytes) >> 4);
 #pragma unroll
-          for (int k = 0; k < 4; ++k) umma<0, 1>(d, adesc + 2 * k, bdesc + 2 * k, idesc, (kb > 0 || k > 0) ? 1u : 0u);
-          if (u.kind == 2) {  // the low halves of h
-            const uint64_t ldesc = bdesc + static_cast<uint64_t>((n * kRowBytes) >> 4);
+          for (int b = 0; b < kSlabs; ++b)
 #pragma unroll
-            for (int k = 0; k < 4; ++k) umma<0, 1>(d, adesc + 2 * k, ldesc + 2 * k, idesc, 1u);
-          }
+            for (int k = 0; k < 4; ++k)
+#pragma unroll
+              for (int j = 0; j < kSubs; ++j)
+                umma<0, 1>(d + j * p.acc_stride, stage + ((b * kSlabBytes + j * kMmaRows * kRowBytes) >> 4) + 2 * k,
+                           stage + ((kActBase + b * p.act_bytes) >> 4) + 2 * k, idesc, (b > 0 || k > 0) ? 1u : (kb > 0 ? 1u : 0u));
           umma_commit(&empty_bar[s]);
           if (kb + 1 == nkb) umma_commit(&tmem_full[acc]);
         }
@@ -512,46 +565,55 @@ moe_mlp_kernel(const __grid_constant__ CUtensorMap tmap_w1, const __grid_constan
         // the sum over a token's rows, in slot order
         ok = counter_wait_warp(p.ws + MlpLayout::kRowsDone, 4 * units2, wctx);
         if (!ok) break;
-        const int quads = p.hidden / 4;
-        for (int it = 0; it < p.items_per_thread; ++it) {
-          const long long item = static_cast<long long>(u.tile) * run_items + it * 128 + threadIdx.x;
-          if (item >= out_items) break;
-          const int t = static_cast<int>(item / quads), c = static_cast<int>(item - static_cast<long long>(t) * quads) * 4;
-          const int* rows = ws + p.lay.pair_row() + t * p.topk;
-          float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-          for (int j0 = 0; j0 < p.topk; j0 += 8) {
-            int r[8];
-            float4 v[8];
+        const int t = u.tile / p.runs, quads = p.hidden / 4;
+        const int q0 = (u.tile - t * p.runs) * p.quads_per_thread * 128 + threadIdx.x;
+        const int q1 = min(quads, q0 + p.quads_per_thread * 128);
+        const int* rows = ws + p.lay.pair_row() + t * p.topk;
+        unsigned short* o = reinterpret_cast<unsigned short*>(p.out) + t * p.out_stride;
+        if (p.topk <= 8) {
+          int r[8];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) r[j] = j0 + j < p.topk ? __ldcg(rows + j0 + j) : -1;
+          for (int j = 0; j < 8; ++j) r[j] = j < p.topk ? __ldcg(rows + j) : -1;
+          const float4* src[8];
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
-              v[j] = r[j] >= 0 ? __ldcg(reinterpret_cast<const float4*>(p.y + static_cast<long long>(r[j]) * p.hidden + c))
-                               : make_float4(0.f, 0.f, 0.f, 0.f);
+          for (int j = 0; j < 8; ++j) src[j] = reinterpret_cast<const float4*>(p.y + static_cast<long long>(max(r[j], 0)) * p.hidden);
+          // two runs of the token at a time: sixteen loads in flight, none of them conditional (a place without a row reads
+          // row 0 and drops it)
+          for (int q = q0; q < q1; q += 256) {
+            float4 a[8], b[8];
+            const int second = q + 128 < q1 ? q + 128 : q;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-              sum.x += v[j].x;
-              sum.y += v[j].y;
-              sum.z += v[j].z;
-              sum.w += v[j].w;
+              a[j] = __ldcg(src[j] + q);
+              b[j] = __ldcg(src[j] + second);
             }
+            float4 sum_a = make_float4(0.f, 0.f, 0.f, 0.f), sum_b = sum_a;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              if (r[j] >= 0) {
+                sum_a = add4(sum_a, a[j]);
+                sum_b = add4(sum_b, b[j]);
+              }
+            }
+            store_quad<T>(o + q * 4, sum_a, p.out_vec);
+            if (second != q) store_quad<T>(o + second * 4, sum_b, p.out_vec);
           }
-          unsigned short* o = reinterpret_cast<unsigned short*>(p.out) + t * p.out_stride + c;
-          const ushort4 b = make_ushort4(to_bits<T>(sum.x), to_bits<T>(sum.y), to_bits<T>(sum.z), to_bits<T>(sum.w));
-          if (p.out_vec) {
-            *reinterpret_cast<ushort4*>(o) = b;
-          } else {
-            o[0] = b.x;
-            o[1] = b.y;
-            o[2] = b.z;
-            o[3] = b.w;
+        } else {
+          for (int q = q0; q < q1; q += 128) {
+            float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+            for (int j = 0; j < p.topk; ++j) {
+              const int r = __ldcg(rows + j);
+              if (r >= 0) sum = add4(sum, __ldcg(reinterpret_cast<const float4*>(p.y + static_cast<long long>(r) * p.hidden) + q));
+            }
+            store_quad<T>(o + q * 4, sum, p.out_vec);
           }
         }
         continue;
       }
       if (u.kind == 1) {
         // which columns are this expert's: looked up while the product is still being accumulated
-        for (int c = lane; c < p.n1; c += 32) col_row[warp][c] = -1;
+        for (int c = lane; c < p.tokens; c += 32) col_row[warp][c] = -1;
         __syncwarp();
         for (int r = lane; r < u.rows; r += 32) col_row[warp][__ldcg(ws + p.lay.row_token() + u.off + r)] = u.off + r;
         __syncwarp();
@@ -559,24 +621,25 @@ moe_mlp_kernel(const __grid_constant__ CUtensorMap tmap_w1, const __grid_constan
       ok = __all_sync(0xffffffffu, mbar_wait(&tmem_full[acc], (parity >> acc) & 1u, wctx, TB_DEV_TIMEOUT_TMEM_FULL));
       if (!ok) break;
       tc_fence_after();
-      const uint32_t t_row = tmem_base + (static_cast<uint32_t>(warp * 32) << 16) + static_cast<uint32_t>(acc * p.acc_stride);
-      const int n = u.kind == 1 ? p.n1 : u.rows;
+      const uint32_t t_row = tmem_base + (static_cast<uint32_t>(warp * 32) << 16) + static_cast<uint32_t>(acc * kSubs * p.acc_stride);
+      const int n = u.kind == 1 ? p.n1 : 2 * u.rows;
+      for (int sub = 0; sub < kSubs; ++sub)
       for (int c0 = 0; c0 < n; c0 += 32) {
         uint32_t r[32];
-        tmem_ld_32x32(t_row + c0, r);
+        tmem_ld_32x32(t_row + sub * p.acc_stride + c0, r);
         tmem_ld_wait(r);
-        if (c0 + 32 >= n) {  // the last columns sit in registers
+        if (sub + 1 == kSubs && c0 + 32 >= n) {  // the last columns sit in registers
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(&tmem_empty[acc]);
         }
         if (u.kind == 1) {
           // lanes 0-7 of a run of 16 hold gate features, lanes 8-15 the matching up features
-          const int f = u.tile * (M / 2) + (warp * kGroups + (lane >> 4)) * 8 + (lane & 7);
-          const bool mine = (lane & 8) == 0 && (M == 128 || lane < 16) && f < p.ffn;
+          const int f = u.tile * (M / 2) + sub * (kMmaRows / 2) + (warp * kGroups + (lane >> 4)) * 8 + (lane & 7);
+          const bool mine = (lane & 8) == 0 && (kMmaRows == 128 || lane < 16) && f < p.ffn;
 #pragma unroll
           for (int j = 0; j < 32; ++j) {
-            const int row = c0 + j < n ? col_row[warp][c0 + j] : -1;
+            const int row = c0 + j < p.tokens ? col_row[warp][c0 + j] : -1;
             if (row >= 0) {  // the same for the whole warp
               const float g = __uint_as_float(r[j]);
               const float up = __shfl_xor_sync(0xffffffffu, g, 8);
@@ -586,28 +649,28 @@ moe_mlp_kernel(const __grid_constant__ CUtensorMap tmap_w1, const __grid_constan
               const float rest = h - from_bits<T>(hi);
               const unsigned short lo = fabsf(rest) < __builtin_huge_valf() ? to_bits<T>(rest) : static_cast<unsigned short>(0);
               if (mine) {
-                unsigned short* dst = reinterpret_cast<unsigned short*>(p.h) + static_cast<long long>(row) * p.ffn + f;
+                unsigned short* dst = reinterpret_cast<unsigned short*>(p.h) + static_cast<long long>(row) * 2 * p.ffn + f;
                 dst[0] = hi;
-                dst[p.h_plane * p.ffn] = lo;
+                dst[p.ffn] = lo;
               }
             }
           }
         } else {
-          const int hcol = u.tile * M + warp * (M / 4) + lane;
-          const bool mine = (M == 128 || lane < 16) && hcol < p.hidden;
+          const int hcol = u.tile * M + sub * kMmaRows + warp * (kMmaRows / 4) + lane;
+          const bool mine = (kMmaRows == 128 || lane < 16) && hcol < p.hidden;
 #pragma unroll
-          for (int j = 0; j < 32; ++j) {
-            const int row = c0 + j;
-            if (row < n && mine)
-              __stcg(p.y + static_cast<long long>(u.off + row) * p.hidden + hcol, __ldcg(row_weight + u.off + row) * __uint_as_float(r[j]));
+          for (int j = 0; j < 32; j += 2) {  // the products with both halves of h stand side by side
+            const int row = (c0 + j) >> 1;
+            if (row < u.rows && mine)
+              __stcg(p.y + static_cast<long long>(u.off + row) * p.hidden + hcol,
+                     __ldcg(row_weight + u.off + row) * (__uint_as_float(r[j]) + __uint_as_float(r[j + 1])));
           }
         }
       }
       parity ^= 1u << acc;
       acc ^= 1;
-      // publish this warp's part of the unit: every epilogue warp counts for itself, so none waits for another
-      __threadfence();
-      fence_proxy_async_all();
+      // publish this warp's part of the unit: every epilogue warp counts for itself, so none waits for another. The release
+      // of lane 0 covers the warp's stores (they come before the __syncwarp).
       __syncwarp();
       if (lane == 0) add_release(u.kind == 1 ? p.ws + p.lay.expert_done() + u.slot : p.ws + MlpLayout::kRowsDone, 1);
     }
@@ -630,17 +693,33 @@ moe_mlp_kernel(const __grid_constant__ CUtensorMap tmap_w1, const __grid_constan
 // ------------------------------------------------------------------------------------------------------------ host
 struct MlpShape {
   MlpLayout lay;
+  int tile_m;         // rows of the tensor-core tile
   int n1, group_cap;
+  int act_rows;       // rows of activations a stage has room for
   long long h_offset, y_offset, bytes;  // byte offsets in the workspace
 };
 
+// Weight rows of a tile. Few units (few chosen experts) are dealt more evenly in 64-row tiles, unless that makes a unit of the
+// second projection so short that its hand-overs show: measured back to back, 64 / 128 rows, 8 experts of 4096 x 1536: 61 / 68
+// us; 18 experts of 2048 x 704: 54 / 44 us. Above 64 tokens their share of a stage is as large as 128 weight rows', so a
+// tile has 256: 408 against 414 us at 128 tokens, 64 experts of 4096 x 1536.
+int mlp_tile_rows(int tokens, int topk, int ffn) {
+  if (tokens > 64) return 256;
+  return tokens * topk < 64 && ffn >= 1280 ? 64 : 128;
+}
+
 // Columns of the two projections and the workspace they need. The rows of an expert go in groups of at most half the token
-// columns, so that both halves of h take no more shared memory in a stage than the tokens do: an expert that more than half
-// of the tokens choose is read once per group, the second time out of L2.
+// columns (but 16), so that both halves of h take no more shared memory in a stage than the tokens do: an expert that more
+// than half of the tokens choose is read once per group, the second time out of L2.
 MlpShape mlp_shape(int tokens, int topk, int num_experts, int hidden, int ffn) {
   MlpShape s;
-  s.n1 = (tokens + 15) & ~15;
-  s.group_cap = (s.n1 / 2 + 15) & ~15;
+  s.tile_m = mlp_tile_rows(tokens, topk, ffn);
+  const int align = s.tile_m == 64 ? 8 : 16;
+  s.n1 = (tokens + align - 1) / align * align;
+  s.group_cap = tokens < 16 ? tokens : (s.n1 / 2 < 16 ? 16 : s.n1 / 2);
+  const int h_rows = (2 * s.group_cap + 31) / 32 * 32;
+  s.act_rows = s.group_cap <= 4 ? 8 : h_rows;
+  if (s.act_rows < s.n1) s.act_rows = s.n1;
   s.lay.pairs = tokens * topk;
   s.lay.experts = num_experts < s.lay.pairs ? num_experts : s.lay.pairs;
   s.lay.groups = s.lay.experts + s.lay.pairs / s.group_cap;
@@ -658,8 +737,8 @@ bool mlp_sizes_ok(int tokens, int topk, int num_experts, int hidden, int ffn) {
 }
 
 template <typename T, int M>
-int mlp_launch(const CUtensorMap& w1, const CUtensorMap& w2, const CUtensorMap& x, const CUtensorMap& h, const MlpParams& p, int grid,
-               int smem_bytes, int device, cudaStream_t stream) {
+int mlp_launch(const CUtensorMap& w1, const CUtensorMap& w2, const CUtensorMap& x, const CUtensorMap (&h)[3], const MlpParams& p,
+               int grid, int smem_bytes, int device, cudaStream_t stream) {
   auto kernel = moe_mlp_kernel<T, M>;
   // the opt-in shared-memory size is set once per instantiation and device, and again if a launch needs more
   static int configured[64] = {};
@@ -685,7 +764,7 @@ int mlp_launch(const CUtensorMap& w1, const CUtensorMap& w2, const CUtensorMap& 
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     lc.numAttrs = 1;
   }
-  cudaError_t e = cudaLaunchKernelEx(&lc, kernel, w1, w2, x, h, p);
+  cudaError_t e = cudaLaunchKernelEx(&lc, kernel, w1, w2, x, h[0], h[1], h[2], p);
   if (e != cudaSuccess) return cuda_fail(e, "moe_mlp_kernel launch");
   g_launches.fetch_add(1, std::memory_order_relaxed);
   return TB_OK;
@@ -723,7 +802,6 @@ int mlp_impl(const tb_moe_mlp_args& a, cudaStream_t stream) {
   p.n1 = s.n1;
   p.group_cap = s.group_cap;
   p.h = ws + s.h_offset;
-  p.h_plane = s.lay.pairs;
   p.y = reinterpret_cast<float*>(ws + s.y_offset);
   p.out = a.out;
   p.out_stride = a.out_row_stride;
@@ -732,28 +810,28 @@ int mlp_impl(const tb_moe_mlp_args& a, cudaStream_t stream) {
   p.status = status;
   p.timeout_ns = a.wait_timeout_ms > 0 ? static_cast<unsigned long long>(a.wait_timeout_ms) * 1000000ull : 2000000000ull;
 
-  // Rows of the tensor-core tile. See mlp_tile_rows.
-  const int m = a.tokens * a.topk >= 64 ? 128 : 64;
-  p.weight_bytes = m * kRowBytes;
-  const int act_rows = s.n1 > 2 * s.group_cap ? s.n1 : 2 * s.group_cap;
-  p.stage_bytes = p.weight_bytes + act_rows * kRowBytes;
-  const int fixed = 8192;  // barriers, queue and column tables (static), alignment of the ring
-  p.stages = (smem_optin - fixed) / p.stage_bytes;
+  const int m = s.tile_m;
+  p.act_bytes = s.act_rows * kRowBytes;
+  p.stage_bytes = mlp_slabs(m) * (m * kRowBytes + p.act_bytes);
+  p.stages = (smem_optin - 8192) / p.stage_bytes;  // beside the ring: barriers, queue, column tables, the ring's alignment
   if (p.stages > kMaxStages) p.stages = kMaxStages;
   if (p.stages < 2) return TB_ERR_UNSUPPORTED;
   const int smem_bytes = p.stages * p.stage_bytes + 1024;
-  p.acc_stride = (s.n1 + 31) & ~31;
+  p.acc_stride = s.act_rows < 32 ? 32 : s.act_rows;
   p.tmem_cols = 64;
-  while (p.tmem_cols < 2 * p.acc_stride) p.tmem_cols <<= 1;
+  while (p.tmem_cols < 2 * (m > 128 ? m / 128 : 1) * p.acc_stride) p.tmem_cols <<= 1;
   p.f_tiles = (a.ffn + m / 2 - 1) / (m / 2);
   p.h_tiles = (a.hidden + m - 1) / m;
-  const long long items = static_cast<long long>(a.tokens) * (a.hidden / 4);
-  p.items_per_thread = static_cast<int>((items + 128ll * num_sms - 1) / (128ll * num_sms));
+  // the sum over a token's rows: about as many units as SMs, or one per token when there are more tokens
+  const int token_runs = (a.hidden / 4 + 127) / 128;
+  p.runs = num_sms / a.tokens < 1 ? 1 : (num_sms / a.tokens > token_runs ? token_runs : num_sms / a.tokens);
+  p.quads_per_thread = (token_runs + p.runs - 1) / p.runs;
+  p.runs = (token_runs + p.quads_per_thread - 1) / p.quads_per_thread;
   // fp32 accumulators; operand format (0 = f16, 1 = bf16); the column count is added per unit
   const uint32_t fmt = p.bf16 ? 1u : 0u;
-  p.idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | (static_cast<uint32_t>(m >> 4) << 24);
+  p.idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | (static_cast<uint32_t>((m < 128 ? m : 128) >> 4) << 24);
 
-  CUtensorMap tw1, tw2, tx, th;
+  CUtensorMap tw1, tw2, tx, th[3];
   const uint64_t es = 2;
   {
     // W1 as [expert][ffn / 8][gate, up][8][hidden]: a box of M/16 x 2 x 8 rows lands as runs of 8 gate rows and the 8 matching
@@ -772,8 +850,10 @@ int mlp_impl(const tb_moe_mlp_args& a, cudaStream_t stream) {
     if ((rc = encode_nd(&tw2, a.dtype, a.w2, 3, dims, strides, box)) != TB_OK) return rc;
   }
   const uint64_t x_stride = static_cast<uint64_t>(a.tokens > 1 ? a.x_row_stride : a.hidden) * es;
-  if ((rc = encode_2d(&tx, a.dtype, a.x, a.hidden, a.tokens, x_stride, kStageK, s.n1, 1)) != TB_OK) return rc;
-  if ((rc = encode_2d(&th, a.dtype, p.h, a.ffn, 2ull * s.lay.pairs, a.ffn * es, kStageK, 16, 1)) != TB_OK) return rc;
+  if ((rc = encode_2d(&tx, a.dtype, a.x, a.hidden, a.tokens, x_stride, kStageK, a.tokens, 1)) != TB_OK) return rc;
+  const uint32_t h_box[3] = {2, 8, 32};
+  for (int i = 0; i < 3; ++i)
+    if ((rc = encode_2d(&th[i], a.dtype, p.h, a.ffn, 2ull * s.lay.pairs, a.ffn * es, kStageK, h_box[i], 1)) != TB_OK) return rc;
 
   cudaLaunchConfig_t lc = {};
   lc.gridDim = dim3(1, 1, 1);
@@ -792,11 +872,9 @@ int mlp_impl(const tb_moe_mlp_args& a, cudaStream_t stream) {
                                      s.group_cap, s.lay, p.ws);
   if (e != cudaSuccess) return cuda_fail(e, "moe_mlp_plan_kernel launch");
   g_launches.fetch_add(1, std::memory_order_relaxed);
-  if (p.bf16)
-    return m == 64 ? mlp_launch<__nv_bfloat16, 64>(tw1, tw2, tx, th, p, num_sms, smem_bytes, device, stream)
-                   : mlp_launch<__nv_bfloat16, 128>(tw1, tw2, tx, th, p, num_sms, smem_bytes, device, stream);
-  return m == 64 ? mlp_launch<__half, 64>(tw1, tw2, tx, th, p, num_sms, smem_bytes, device, stream)
-                 : mlp_launch<__half, 128>(tw1, tw2, tx, th, p, num_sms, smem_bytes, device, stream);
+  auto launch = p.bf16 ? (m == 64 ? mlp_launch<__nv_bfloat16, 64> : m == 128 ? mlp_launch<__nv_bfloat16, 128> : mlp_launch<__nv_bfloat16, 256>)
+                       : (m == 64 ? mlp_launch<__half, 64> : m == 128 ? mlp_launch<__half, 128> : mlp_launch<__half, 256>);
+  return launch(tw1, tw2, tx, th, p, num_sms, smem_bytes, device, stream);
 }
 
 }  // namespace
