@@ -289,6 +289,29 @@ typedef struct tb_moe_mlp_args {
 int64_t tb_moe_mlp_workspace_bytes(int32_t tokens, int32_t topk, int32_t num_experts, int32_t hidden, int32_t ffn);
 int tb_moe_mlp(const tb_moe_mlp_args* args, void* stream);
 
+/* A shared projection with one low-rank adapter per row, in two launches (no reference counterpart):
+ *   out[t, :] = x[t, :] W + bias + s_a (x[t, :] A_a^T) B_a^T,  a = adapter_ids[t]; no adapter when a is outside [0, num_adapters).
+ * x (m, k) rows contiguous, w (k, n) with one unit stride, lora_a (num_adapters, rank, k), lora_b (num_adapters, n, rank), out
+ * (m, n) any strides, all of `dtype` (f16 or bf16); adapter_ids (m) int32 or int64, scales (num_adapters) fp32 or NULL (1), bias
+ * (n) or NULL. k and rank multiples of 8, rank <= 128; x, w, lora_a, lora_b with 16-byte aligned bases and pitches. One fp32
+ * sum and one rounding; the rank-sized products are rounded to `dtype` in between (they are a tensor-core operand). The
+ * workspace (tb_lora_workspace_bytes of the same arguments, 256-byte aligned) needs no initialisation and must not be shared
+ * by calls that can overlap. */
+typedef struct tb_lora_args {
+  int32_t m, n, k, rank, num_adapters, dtype;
+  const void* x; int64_t x_row_stride;
+  const void* w; int64_t w_stride_k, w_stride_n;
+  const void* lora_a; int64_t lora_a_adapter_stride, lora_a_row_stride;
+  const void* lora_b; int64_t lora_b_adapter_stride, lora_b_row_stride;
+  const void* adapter_ids; const float* scales;
+  const void* bias; int64_t bias_stride;
+  void* out; int64_t out_stride_m, out_stride_n;
+  void* workspace; int64_t workspace_bytes;
+  int32_t bias_dtype, ids_are_int64, wait_timeout_ms;
+} tb_lora_args;
+int64_t tb_lora_workspace_bytes(const tb_lora_args* args);
+int tb_lora_gemm(const tb_lora_args* args, void* stream);
+
 /* Diagnostic: streams rows x row_bytes of a row-major matrix (pitch_bytes between rows) out of HBM with the access pattern
  * of the GEMM's K-major operand loader and drops the data: `programs` CTAs (one per SM), each keeping `stages` TMA boxes of
  * box_rows rows x 128 bytes in flight, row blocks dealt round-robin, K walked in 128-byte steps. Time it with events:

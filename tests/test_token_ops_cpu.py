@@ -44,6 +44,51 @@ def test_expert_layer_refusals():
             tb.moe_mlp(*case)
 
 
+def lora_case(T=4, K=64, N=40, R=8, L=3, dtype=bf):
+    return [torch.zeros(T, K, dtype=dtype), torch.zeros(N, K, dtype=dtype).T, torch.zeros(L, R, K, dtype=dtype),
+            torch.zeros(L, N, R, dtype=dtype), torch.zeros(T, dtype=torch.int32)]
+
+
+def test_adapter_projection_refusals():
+    with pytest.raises(RuntimeError, match="CUDA"):
+        tb.lora_matmul(*lora_case())
+    for kw in (dict(K=60), dict(R=4), dict(R=136), dict(R=20), dict(L=0), dict(dtype=torch.float32)):
+        with pytest.raises(ValueError):
+            tb.lora_matmul(*lora_case(**kw))
+    for i, t in ((0, torch.zeros(4, 72, dtype=bf)), (1, torch.zeros(64, 41, dtype=bf)), (1, torch.zeros(64, 40, dtype=torch.float16)),
+                 (2, torch.zeros(2, 8, 64, dtype=bf)), (3, torch.zeros(3, 40, 16, dtype=bf)), (4, torch.zeros(4)),
+                 (4, torch.zeros(5, dtype=torch.int32)), (4, torch.zeros(4, 1, dtype=torch.int32))):
+        case = lora_case()
+        case[i] = t
+        with pytest.raises(ValueError):
+            tb.lora_matmul(*case)
+    for kw in (dict(scales=torch.ones(4)), dict(scales=torch.ones(3, dtype=torch.int32)), dict(bias=torch.ones(41)),
+               dict(bias=torch.ones(40, dtype=torch.float64)), dict(out=torch.zeros(4, 41, dtype=bf)), dict(out=torch.zeros(4, 40))):
+        with pytest.raises(ValueError):
+            tb.lora_matmul(*lora_case(), **kw)
+
+
+def test_adapter_projection_c_entry_refusals():
+    lib = _lib.lib
+
+    def call(**kw):
+        a = _lib.LoraArgs(4, 40, 64, 8, 3, _lib.BF16, 256, 64, 256, 1, 64, 256, 512, 64, 256, 320, 8, 256, 0, 0, 0, 256, 40, 1, 256,
+                          1 << 30, 0, 0, 0)
+        for k, v in kw.items():
+            setattr(a, k, v)
+        return lib.tb_lora_gemm(ctypes.byref(a), None)
+
+    assert call(m=0) == 0 and call(n=0) == 0
+    for kw in (dict(m=-1), dict(k=60), dict(k=0), dict(rank=4), dict(rank=136), dict(num_adapters=0), dict(x=None), dict(w=None),
+               dict(lora_a=None), dict(lora_b=None), dict(adapter_ids=None), dict(out=None), dict(x_row_stride=56),
+               dict(lora_a_row_stride=56), dict(lora_b_row_stride=0), dict(w_stride_k=2, w_stride_n=2)):
+        assert call(**kw) == 1, kw
+    assert call(dtype=_lib.F32) == 2
+    assert call(x=264) == 3 and call(lora_a=258) == 3 and call(x_row_stride=68) == 3 and call(adapter_ids=258) == 3 and call(scales=257) == 3
+    assert call(workspace=None, x=256) in (3, 4) and call(workspace_bytes=100) == 4 and call(workspace=272) == 3
+    assert lib.tb_lora_gemm(None, None) == 1 and lib.tb_lora_workspace_bytes(None) == 0
+
+
 def test_c_entry_points_refuse_bad_arguments():
     lib = _lib.lib
     one = ctypes.c_void_p(256)      # never dereferenced: every call below is refused before a launch
@@ -83,7 +128,7 @@ def test_expert_layer_structure_matches_the_header(tmp_path):
     if cc is None:
         pytest.skip("no host C compiler")
     header = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "include", "tritonblas_b200.h")
-    for cname, mirror in (("tb_moe_mlp_args", _lib.MoeMlpArgs),):
+    for cname, mirror in (("tb_moe_mlp_args", _lib.MoeMlpArgs), ("tb_lora_args", _lib.LoraArgs)):
         names = [f[0] for f in mirror._fields_]
         lines = ["#include <stdio.h>", "#include <stddef.h>", f'#include "{header}"', "int main(void) {",
                  f'printf("%zu\\n", sizeof({cname}));'] + [f'printf("%zu\\n", offsetof({cname}, {n}));' for n in names] + ["return 0; }"]

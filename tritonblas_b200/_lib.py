@@ -82,6 +82,20 @@ class MoeMlpArgs(ctypes.Structure):
     ]
 
 
+class LoraArgs(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int32) for n in ("m", "n", "k", "rank", "num_adapters", "dtype")] + [
+        ("x", ctypes.c_void_p), ("x_row_stride", ctypes.c_int64),
+        ("w", ctypes.c_void_p), ("w_stride_k", ctypes.c_int64), ("w_stride_n", ctypes.c_int64),
+        ("lora_a", ctypes.c_void_p), ("lora_a_adapter_stride", ctypes.c_int64), ("lora_a_row_stride", ctypes.c_int64),
+        ("lora_b", ctypes.c_void_p), ("lora_b_adapter_stride", ctypes.c_int64), ("lora_b_row_stride", ctypes.c_int64),
+        ("adapter_ids", ctypes.c_void_p), ("scales", ctypes.c_void_p),
+        ("bias", ctypes.c_void_p), ("bias_stride", ctypes.c_int64),
+        ("out", ctypes.c_void_p), ("out_stride_m", ctypes.c_int64), ("out_stride_n", ctypes.c_int64),
+        ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_int64),
+        ("bias_dtype", ctypes.c_int32), ("ids_are_int64", ctypes.c_int32), ("wait_timeout_ms", ctypes.c_int32),
+    ]
+
+
 def _load():
     if not os.path.exists(LIB_PATH):
         raise RuntimeError(
@@ -138,6 +152,10 @@ def _load():
     lib.tb_moe_mlp_workspace_bytes.restype = i64
     lib.tb_moe_mlp.argtypes = [ctypes.POINTER(MoeMlpArgs), ptr]
     lib.tb_moe_mlp.restype = ctypes.c_int
+    lib.tb_lora_workspace_bytes.argtypes = [ctypes.POINTER(LoraArgs)]
+    lib.tb_lora_workspace_bytes.restype = i64
+    lib.tb_lora_gemm.argtypes = [ctypes.POINTER(LoraArgs), ptr]
+    lib.tb_lora_gemm.restype = ctypes.c_int
     lib.tb_tma_stream_probe.argtypes = [ctypes.c_void_p, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_int32,
                                         ctypes.c_int32, ctypes.c_int32, ctypes.c_void_p]
     lib.tb_tma_stream_probe.restype = ctypes.c_int32

@@ -285,7 +285,7 @@ int gemm_generic_loader(const tb_gemm_args& a, const tb_config& cfg, cudaStream_
 // `builtin`: the stream-K flags and partial tiles of this launch live in the library's own scratch array (the launch
 // takes no workspace from the caller).
 static int gemm_impl(const tb_gemm_args& a_in, const tb_config* user_cfg, cudaStream_t stream, bool grouped = false,
-                     bool swapped = false, bool builtin = false) {
+                     bool swapped = false, bool builtin = false, const LowRank* lr = nullptr) {
   const tb_gemm_args& a = a_in;
   if (a.m < 0 || a.n < 0 || a.k < 0) return TB_ERR_INVALID;
   if (grouped && (a.group_offsets == nullptr || a.num_groups <= 0 || a.num_groups > 4096 || a.streamk)) return TB_ERR_INVALID;
@@ -343,9 +343,9 @@ static int gemm_impl(const tb_gemm_args& a_in, const tb_config* user_cfg, cudaSt
     t.static_operands = ((a.static_operands & 1) << 1) | ((a.static_operands >> 1) & 1);
     tb_config c2 = cfg;
     c2.swap_ab = 0;
-    rc = gemm_impl(t, &c2, stream, false, true, builtin);
+    rc = gemm_impl(t, &c2, stream, false, true, builtin, lr);
     // Operands TMA cannot address go to the CUDA-core kernel in their original orientation (its bias is per column).
-    if (rc == TB_ERR_ALIGNMENT) return gemm_generic_loader(a, cfg, stream, dev->status);
+    if (rc == TB_ERR_ALIGNMENT && lr == nullptr) return gemm_generic_loader(a, cfg, stream, dev->status);
     return rc;
   }
   const bool glu = a.epilogue_op == TB_EPILOGUE_SWIGLU;
@@ -375,6 +375,7 @@ static int gemm_impl(const tb_gemm_args& a_in, const tb_config* user_cfg, cudaSt
   const int bk = 128 / es;
   // wide tiles (two accumulators sharing A) only for the data-parallel and grouped schedules: stream-K partials are per accumulator
   const int halves = (cfg.n_halves == 2 && !a.streamk) ? 2 : 1;
+  if (lr != nullptr && (halves != 1 || es != 2 || lr->tile_rows != (swapped ? bn : 128 * pair))) return TB_ERR_INVALID;
   int stages = cfg.stages;
   if (stages < 2) stages = 2;
   const int extra_smem = grouped ? 8 * (a.num_groups + 2) : 0;  // per-group tile prefix + copy of the row offsets
@@ -436,7 +437,7 @@ static int gemm_impl(const tb_gemm_args& a_in, const tb_config* user_cfg, cudaSt
   }
   // An operand nothing in flight writes is requested before the wait for the previous kernel (single CTAs, static
   // schedules): the larger one per stage if both are.
-  if (pair == 1 && !grouped && !gather && p.tile_counter == nullptr && pdl_enabled()) {
+  if (pair == 1 && !grouped && !gather && lr == nullptr && p.tile_counter == nullptr && pdl_enabled()) {
     if ((a.static_operands & 3) == 3) p.early_operand = bn * halves > 128 ? 2 : 1;
     else if (a.static_operands & 1) p.early_operand = 1;
     else if (a.static_operands & 2) p.early_operand = 2;
@@ -558,8 +559,30 @@ static int gemm_impl(const tb_gemm_args& a_in, const tb_config* user_cfg, cudaSt
       rc = encode_2d(&tbm, a.b_dtype, B, a.n, a.k, static_cast<uint64_t>(a.b_stride_k) * es, mn_atom, bk, mn_swz);
     }
   }
-  if (rc == TB_ERR_ALIGNMENT && !grouped && !swapped) return gemm_generic_loader(a, cfg, stream, dev->status);
+  if (rc == TB_ERR_ALIGNMENT && !grouped && !swapped && lr == nullptr) return gemm_generic_loader(a, cfg, stream, dev->status);
   if (rc != TB_OK) return rc;
+  if (lr != nullptr) {
+    p.lr_list = lr->list;
+    p.lr_list_stride = lr->list_stride;
+    p.lr_kblocks = lr->kblocks;
+    p.lr_rank = lr->rank;
+    p.lr_tile_rows = lr->tile_rows;
+    p.lr_tokens_on_b = swapped ? 1 : 0;
+    CUtensorMap tv, tlb;
+    const uint32_t token_box = swapped ? bn / pair : 128, weight_box = swapped ? 128 : bn / pair;
+    rc = encode_2d(&tv, a.a_dtype, lr->v, static_cast<uint64_t>(lr->kblocks) * bk, lr->v_rows, static_cast<uint64_t>(lr->kblocks) * 128,
+                   bk, token_box, 1);
+    if (rc != TB_OK) return rc;
+    const uint64_t dims[3] = {static_cast<uint64_t>(lr->rank), static_cast<uint64_t>(lr->n), static_cast<uint64_t>(lr->num_adapters)};
+    const uint64_t strides[2] = {static_cast<uint64_t>(lr->b_row_stride) * es,
+                                 lr->num_adapters > 1 ? static_cast<uint64_t>(lr->b_adapter_stride) * es
+                                                      : static_cast<uint64_t>(lr->b_row_stride) * es * lr->n};
+    const uint32_t box[3] = {static_cast<uint32_t>(bk), weight_box, 1};
+    if ((rc = encode_nd(&tlb, a.a_dtype, lr->b, 3, dims, strides, box)) != TB_OK) return rc;
+    const CUtensorMap *ma = swapped ? &tlb : &tv, *mb = swapped ? &tv : &tlb;
+    return pair == 1 ? launch_gemm<0, 1>(ta, tbm, p, programs, smem_bytes, stream, ma, mb)
+                     : launch_gemm<0, 2>(ta, tbm, p, programs, smem_bytes, stream, ma, mb);
+  }
 
 #define TB_LAUNCH(K, C) return launch_gemm<K, C>(ta, tbm, p, programs, smem_bytes, stream)
   if (pair == 1) {
@@ -574,6 +597,32 @@ static int gemm_impl(const tb_gemm_args& a_in, const tb_config* user_cfg, cudaSt
     TB_LAUNCH(2, 2);
   }
 #undef TB_LAUNCH
+}
+
+int low_rank_config(const tb_gemm_args& a, tb_config* cfg, int* streamk) {
+  DeviceState* dev = nullptr;
+  int device = 0;
+  // without a usable device the model falls back to the B200 constants (workspace sizes on a CPU host)
+  if (current_device_state(&dev, &device) != TB_OK) dev = nullptr;
+  tb_problem pr = {};
+  pr.m = a.m; pr.n = a.n; pr.k = a.k;
+  pr.a_dtype = a.a_dtype; pr.b_dtype = a.b_dtype; pr.c_dtype = a.c_dtype;
+  pr.b_mn_major = (a.b_stride_k != 1 && a.k != 1) ? 1 : 0;
+  pr.device = device;
+  pr.max_halves = 1;
+  tb_config dp, sk;
+  int rc = select_config(pr, machine_for(dev), &dp);
+  if (rc != TB_OK) return rc;
+  pr.streamk = 1;
+  rc = select_config(pr, machine_for(dev), &sk);
+  if (rc != TB_OK) return rc;
+  *streamk = sk.predicted_sk_us < dp.predicted_us ? 1 : 0;
+  *cfg = *streamk ? sk : dp;
+  return TB_OK;
+}
+
+int gemm_low_rank(const tb_gemm_args& a, const tb_config& cfg, const LowRank& lr, cudaStream_t stream) {
+  return gemm_impl(a, &cfg, stream, false, false, false, &lr);
 }
 
 // ---------------------------------------------------------------- MXFP4 (block-scaled e2m1 x e2m1)

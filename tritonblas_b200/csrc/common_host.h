@@ -26,6 +26,23 @@ int encode_2d(CUtensorMap* map, int dtype, const void* base, uint64_t inner, uin
 int encode_nd(CUtensorMap* map, int dtype, const void* base, int rank, const uint64_t* dims, const uint64_t* strides,
               const uint32_t* box);
 
+// Low-rank update of a dense launch (see GemmParams::lr_list): the tokens' masked projections v, one block of tile_rows rows of
+// kblocks * 64 elements per token tile and listed adapter, and lora_b (num_adapters, n, rank).
+struct LowRank {
+  const void* v;
+  int64_t v_rows;
+  int kblocks, rank, tile_rows;
+  const void* b;
+  int64_t b_adapter_stride, b_row_stride;
+  int num_adapters, n;
+  const int* list;
+  int list_stride;
+};
+// Configuration the library would pick for `a`, data-parallel or stream-K (whichever the model says is shorter; a.streamk says
+// which), narrow tiles; and the launch of `a` with that configuration and the update.
+int low_rank_config(const tb_gemm_args& a, tb_config* cfg, int* streamk);
+int gemm_low_rank(const tb_gemm_args& a, const tb_config& cfg, const LowRank& lr, cudaStream_t stream);
+
 // The current device: its number, SMs, shared memory a block may opt in to, and failure word.
 int current_device_limits(int* device, int* num_sms, int* smem_optin, int** status);
 

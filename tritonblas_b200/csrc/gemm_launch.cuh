@@ -10,7 +10,7 @@
 namespace tb {
 
 // Enqueue one launch of gemm_kernel<KIND, CTAS> with `programs` programs (CTAs, or CTA pairs when CTAS == 2).
-// tsfa / tsfb: scale-factor tensor maps of the block-scaled kind, null otherwise.
+// tsfa / tsfb: scale-factor tensor maps of the block-scaled kind, the extension operands of a low-rank update, null otherwise.
 template <int KIND, int CTAS>
 int launch_gemm(const CUtensorMap& ta, const CUtensorMap& tb_, const GemmParams& p, int programs, int smem_bytes,
                 cudaStream_t stream, const CUtensorMap* tsfa = nullptr, const CUtensorMap* tsfb = nullptr);
@@ -24,8 +24,8 @@ int launch_gemm(const CUtensorMap& ta, const CUtensorMap& tb_, const GemmParams&
                 cudaStream_t stream, const CUtensorMap* tsfa, const CUtensorMap* tsfb) {
   auto kernel = gemm_kernel<KIND, CTAS, false>;
   int variant = 0;
-  // The instantiations with per-role cycle counters (measurement runs) and with a row-gathering A loader (grouped
-  // launches whose rows are picked from another matrix by index) exist for 16-bit operands only.
+  // The instantiations with per-role cycle counters (measurement runs), with a row-gathering A loader (grouped launches whose
+  // rows are picked from another matrix by index) and with a low-rank update beside the product exist for 16-bit operands only.
   if constexpr (KIND == 0) {
     if (p.a_gather != nullptr) {
       kernel = gemm_kernel<KIND, CTAS, false, true>;
@@ -33,12 +33,15 @@ int launch_gemm(const CUtensorMap& ta, const CUtensorMap& tb_, const GemmParams&
     } else if ((p.debug_flags & 2) && p.debug_out != nullptr) {
       kernel = gemm_kernel<KIND, CTAS, true>;
       variant = 1;
+    } else if (p.lr_list != nullptr) {
+      kernel = gemm_kernel<KIND, CTAS, false, false, true>;
+      variant = 3;
     }
-  } else if (p.a_gather != nullptr) {
+  } else if (p.a_gather != nullptr || p.lr_list != nullptr) {
     return TB_ERR_UNSUPPORTED;
   }
   // The opt-in shared-memory size is set once per kernel instantiation and device (and again if a launch needs more).
-  static int configured[3][64] = {};
+  static int configured[4][64] = {};
   static std::mutex configured_mu;
   int dev_index = 0;
   cudaGetDevice(&dev_index);

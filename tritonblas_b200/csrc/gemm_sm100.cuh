@@ -101,6 +101,17 @@ struct GemmParams {
   // fills its shared-memory ring with that operand before it waits for the previous kernel (single CTAs, static
   // schedules, plain 2-D / 3-D operand copies).
   int early_operand;
+  // Low-rank update beside the product (LOWRANK instantiation, K-major 16-bit extension operands): after a tile's own K range
+  // its owner walks `lr_kblocks` further stages for every adapter that occurs among the tile's tokens. On the token side they
+  // hold the rows' rank-sized projections, zero in rows of other adapters (tensor map `sfa` / `sfb`, one block of lr_tile_rows
+  // rows per token tile and listed adapter), on the other side that adapter's rows of lora_b (the other map). All of it adds
+  // up in the same accumulator, so the sum is rounded once.
+  const int* lr_list;   // per token tile: number of adapters, then their indices; written by the kernel launched before
+  int lr_list_stride;   // words per token tile
+  int lr_kblocks;       // stages per adapter
+  int lr_rank;
+  int lr_tile_rows;     // rows of a token tile: what this launch's tile covers on the token side
+  int lr_tokens_on_b;   // 1: the tokens are the B side (transposed launch)
   // failure reporting
   int* status;
   unsigned long long timeout_ns;
@@ -559,7 +570,11 @@ static __device__ __noinline__ void park_peer_partials(const float* src, int cou
         make_float4(pre[4 * j], pre[4 * j + 1], pre[4 * j + 2], pre[4 * j + 3]);
 }
 
-template <int KIND, int CTAS, bool PROF = false, bool GATHER = false>
+// LOWRANK launches follow the kernel that projects the tokens onto the adapters' ranks and start while it still runs: that
+// kernel waits for everything before it ahead of letting this one start, so the operands of the plain product may be read at
+// once; only what it writes itself (projections, adapter lists, zeroed stream-K flags) is waited for, by each role before its
+// first use.
+template <int KIND, int CTAS, bool PROF = false, bool GATHER = false, bool LOWRANK = false>
 __global__ void __launch_bounds__(gemm_threads<KIND>(), 1)
 gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
             const __grid_constant__ CUtensorMap tmap_sfa, const __grid_constant__ CUtensorMap tmap_sfb, const GemmParams p) {
@@ -676,7 +691,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ 
         }
       }
     }
-    griddep_wait();
+    if constexpr (!LOWRANK) griddep_wait();
     if (prof && p.debug_out != nullptr) p.debug_out[blockIdx.x * 16 + 10] = static_cast<long long>(global_timer_ns());
     if (p.group_offsets != nullptr) {
       // tile_prefix[0 .. G] = tiles before each group, followed by a copy of the G + 1 row offsets. The copy is clamped to
@@ -893,6 +908,53 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ 
             ph ^= 1;
           }
         }
+        if constexpr (LOWRANK) {
+          if (!ok) break;
+          if (w.kb0 == 0) {
+            griddep_wait();
+            const int token_tile = (p.lr_tokens_on_b ? tg.n0 : tg.m0) / p.lr_tile_rows;
+            const int* list = p.lr_list + static_cast<size_t>(token_tile) * p.lr_list_stride;
+            const int adapters = __ldcg(list);
+            for (int i = 0; i < adapters && ok; ++i) {
+              const int adapter = __ldcg(list + 1 + i);
+              const int block_row = (token_tile * (p.lr_list_stride - 1) + i) * p.lr_tile_rows;
+              for (int kb = 0; kb < p.lr_kblocks; ++kb) {
+                ok = mbar_wait_warp(&empty_bar[s], ph ^ 1, wctx, TB_DEV_TIMEOUT_SMEM_EMPTY);
+                if (!ok) break;
+                uint8_t* sa = ring + static_cast<size_t>(s) * stage_bytes;
+                uint8_t* sb = sa + kATileBytes;
+                const int k0 = kb * p.k_per_stage;
+                if (elect_one()) {
+                  if constexpr (CTAS == 1) {
+                    mbar_arrive_expect_tx(&full_bar[s], expect);
+                    if (p.lr_tokens_on_b) {
+                      tma_load_3d(sa, &tmap_sfa, &full_bar[s], k0, m0, adapter);
+                      tma_load_2d(sb, &tmap_sfb, &full_bar[s], k0, block_row);
+                    } else {
+                      tma_load_2d(sa, &tmap_sfa, &full_bar[s], k0, block_row);
+                      tma_load_3d(sb, &tmap_sfb, &full_bar[s], k0, n0, adapter);
+                    }
+                  } else {
+                    const uint32_t bar = mapa_cluster(smem_u32(&full_bar[s]), 0);
+                    if (cta_rank == 0) mbar_arrive_expect_tx(&full_bar[s], expect);
+                    if (p.lr_tokens_on_b) {
+                      tma_load_3d_pair(sa, &tmap_sfa, bar, k0, m0, adapter);
+                      tma_load_2d_pair(sb, &tmap_sfb, bar, k0, block_row + static_cast<int>(cta_rank) * bn_local);
+                    } else {
+                      tma_load_2d_pair(sa, &tmap_sfa, bar, k0, block_row + static_cast<int>(cta_rank) * kTileM);
+                      tma_load_3d_pair(sb, &tmap_sfb, bar, k0, n0, adapter);
+                    }
+                  }
+                }
+                __syncwarp();
+                if (++s == stages) {
+                  s = 0;
+                  ph ^= 1;
+                }
+              }
+            }
+          }
+        }
       }
       if (prof && p.debug_out != nullptr && lane == 0) {
         p.debug_out[blockIdx.x * 16 + 0] = prof_wait;
@@ -1006,7 +1068,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ 
                 issue_stage(d0, adesc, bdesc, first);
               }
               commit(&empty_bar[s]);  // frees the stage once every MMA that reads it has finished
-              if (kb + 1 == w.kb1) commit(&tmem_full[acc0]);
+              if (kb + 1 == w.kb1 && (!LOWRANK || w.kb0 != 0)) commit(&tmem_full[acc0]);
             }
             __syncwarp();
             if (PROF) prof_issue += clock64() - pf1;
@@ -1016,6 +1078,37 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ 
             }
           }
           if (!ok) break;
+          if constexpr (LOWRANK) {
+            if (w.kb0 == 0) {
+              griddep_wait();
+              const TileGeom tg = tile_geometry(p, w.tile, kPairTileM, tile_prefix);
+              const int token_tile = (p.lr_tokens_on_b ? tg.n0 : tg.m0) / p.lr_tile_rows;
+              const int blocks = __ldcg(p.lr_list + static_cast<size_t>(token_tile) * p.lr_list_stride) * p.lr_kblocks;
+              // both extension operands are K-major whatever the product's own layouts are
+              const uint64_t xa0 = make_smem_desc(ring_addr, 16u, 1024u, 2u);
+              const uint64_t xb0 = make_smem_desc(ring_addr + kATileBytes, 16u, 1024u, 2u);
+              const uint32_t x_idesc = idesc & ~(3u << 15);
+              for (int blk = 0, kb = 0; blk < blocks; ++blk) {
+                ok = mbar_wait_warp(&full_bar[s], ph, wctx, TB_DEV_TIMEOUT_SMEM_FULL);
+                if (!ok) break;
+                if (elect_one()) {
+                  const uint64_t soff = static_cast<uint64_t>(s * stage_step);
+                  const int steps = min(4, (p.lr_rank - kb * p.k_per_stage + 15) >> 4);  // columns behind the rank are zeros
+                  for (int k = 0; k < steps; ++k) umma<KIND, CTAS>(d0, xa0 + soff + 2 * k, xb0 + soff + 2 * k, x_idesc, 1u);
+                  commit(&empty_bar[s]);
+                }
+                __syncwarp();
+                if (++kb == p.lr_kblocks) kb = 0;
+                if (++s == stages) {
+                  s = 0;
+                  ph ^= 1;
+                }
+              }
+              if (!ok) break;
+              if (elect_one()) commit(&tmem_full[acc0]);
+              __syncwarp();
+            }
+          }
           acc_parity ^= 1u << acc0;
           acc ^= 1;
         } else {
@@ -1083,6 +1176,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ 
     const uint32_t tmem_empty_remote = (CTAS == 2) ? mapa_cluster(smem_u32(&tmem_empty[0]), 0) : 0u;
     bool ok = true;
     long long prof_wait = 0, prof_t0 = clock64(), prof_drain = 0;
+    if constexpr (LOWRANK) griddep_wait();  // the stream-K flags were zeroed by the kernel before this one
     int seq = 0;
     auto next_item = [&]() -> WorkItem {
       if (!dyn) return wi.next();

@@ -4,37 +4,17 @@
 expert layer of a decode batch in two launches. Batches of more than 128 tokens go through ``distributed.PeerMemoryMoE`` /
 ``distributed.ExpertParallelMoE``, whose grouped GEMMs work on 128-row tiles. The reference has no MoE path.
 """
-import contextlib
 import ctypes
 from typing import Optional, Tuple
 
 import torch
 
 from . import _lib
+from ._checks import on_device, require, require_cuda, rows16
 
 MOE_MLP_MAX_TOKENS = 128
 _MAX_EXPERTS, _MAX_TOPK = 1024, 32
 _SCORING = {"softmax": 0, "sigmoid": 1}
-_nullcontext = contextlib.nullcontext()
-
-
-def _require(ok, message):
-    if not ok:
-        raise ValueError(message)
-
-
-def _require_cuda(first, *others):
-    if not first.is_cuda:
-        raise RuntimeError("tritonblas_b200 runs on CUDA tensors only (no CPU path)")
-    for t in others:
-        if t is not None and t.device != first.device:
-            raise RuntimeError(f"all tensors must be on one device, got {first.device} and {t.device}")
-
-
-def _on_device(device):
-    """Context that makes ``device`` current; free when it already is."""
-    return _nullcontext if device.index == torch.cuda.current_device() else torch.cuda.device(device)
-
 
 # ------------------------------------------------------------------------------------------------------------- router
 def _route_rows(logits):
@@ -49,7 +29,7 @@ def _route_forward(logits, topk, sigmoid, renormalize):
     logits = _route_rows(logits)
     weights = torch.empty(tokens, topk, dtype=torch.float32, device=logits.device)
     ids = torch.empty(tokens, topk, dtype=torch.int32, device=logits.device)
-    with _on_device(logits.device):
+    with on_device(logits.device):
         rc = _lib.lib.tb_moe_route(logits.data_ptr(), _lib.DTYPE_CODE[logits.dtype], logits.stride(0), tokens, experts, topk,
                                    sigmoid, renormalize, weights.data_ptr(), ids.data_ptr(),
                                    _lib.current_stream_ptr(logits.device))
@@ -75,7 +55,7 @@ def _moe_route_backward(logits: torch.Tensor, weights: torch.Tensor, ids: torch.
     logits = _route_rows(logits)
     weights, ids, grad = weights.contiguous(), ids.contiguous(), grad.to(torch.float32).contiguous()
     out = torch.empty(tokens, experts, dtype=logits.dtype, device=logits.device)
-    with _on_device(logits.device):
+    with on_device(logits.device):
         rc = _lib.lib.tb_moe_route_backward(logits.data_ptr(), _lib.DTYPE_CODE[logits.dtype], logits.stride(0), tokens, experts,
                                             ids.shape[1], int(sigmoid), int(renormalize), weights.data_ptr(), ids.data_ptr(),
                                             grad.data_ptr(), out.data_ptr(), _lib.current_stream_ptr(logits.device))
@@ -112,27 +92,20 @@ def moe_route(logits, topk, scoring="softmax", renormalize=True):
     never chosen; a row with fewer than ``topk`` others gets id -1 and weight 0 in the remaining places, which every expert path
     of this package skips. At most 1024 experts and ``topk`` 32. The weights are differentiable in the logits.
     """
-    _require(logits.ndim == 2, "logits must be (tokens, experts)")
-    _require(logits.dtype in (torch.float16, torch.bfloat16, torch.float32), f"logits must be float16, bfloat16 or float32, got {logits.dtype}")
-    _require(scoring in _SCORING, f"scoring must be 'softmax' or 'sigmoid', got {scoring!r}")
-    _require(1 <= logits.shape[1] <= _MAX_EXPERTS, f"between 1 and {_MAX_EXPERTS} experts, got {logits.shape[1]}")
+    require(logits.ndim == 2, "logits must be (tokens, experts)")
+    require(logits.dtype in (torch.float16, torch.bfloat16, torch.float32), f"logits must be float16, bfloat16 or float32, got {logits.dtype}")
+    require(scoring in _SCORING, f"scoring must be 'softmax' or 'sigmoid', got {scoring!r}")
+    require(1 <= logits.shape[1] <= _MAX_EXPERTS, f"between 1 and {_MAX_EXPERTS} experts, got {logits.shape[1]}")
     topk = int(topk)
-    _require(1 <= topk <= min(_MAX_TOPK, logits.shape[1]), f"topk must be between 1 and min({_MAX_TOPK}, experts), got {topk}")
+    require(1 <= topk <= min(_MAX_TOPK, logits.shape[1]), f"topk must be between 1 and min({_MAX_TOPK}, experts), got {topk}")
     sigmoid, renormalize = _SCORING[scoring], int(bool(renormalize))
     if torch.compiler.is_compiling() or (torch.is_grad_enabled() and logits.requires_grad):
         return _moe_route(logits, topk, bool(sigmoid), bool(renormalize))
-    _require_cuda(logits)
+    require_cuda(logits)
     return _route_forward(logits, topk, sigmoid, renormalize)    # no dispatcher round trip on the serving path
 
 
 # -------------------------------------------------------------------------------------------------------- expert layer
-def _rows16(t):
-    """True when the last axis is contiguous and every row starts on a 16-byte boundary (TMA reads it in place)."""
-    per16 = 16 // t.element_size()
-    return t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(
-        n == 1 or (s > 0 and s % per16 == 0) for n, s in zip(t.shape[:-1], t.stride()[:-1]))
-
-
 def moe_mlp(x, w1, w2, topk_ids, topk_weights, out: Optional[torch.Tensor] = None):
     """Expert feed-forward of up to 128 tokens in two launches:
     ``out[t] = sum_j topk_weights[t, j] * (silu(x[t] @ gate.T) * (x[t] @ up.T)) @ w2[e].T`` with ``e = topk_ids[t, j]`` and
@@ -144,32 +117,32 @@ def moe_mlp(x, w1, w2, topk_ids, topk_weights, out: Optional[torch.Tensor] = Non
     weighting are float32 with one cast at the end. ``out`` may be given: (tokens, hidden), contiguous rows, no overlap with the
     weights. Inference only. More tokens: ``distributed.PeerMemoryMoE``.
     """
-    _require(x.ndim == 2 and w1.ndim == 3 and w2.ndim == 3 and topk_ids.ndim == 2, "x (tokens, hidden), w1 and w2 3-D, topk_ids 2-D")
+    require(x.ndim == 2 and w1.ndim == 3 and w2.ndim == 3 and topk_ids.ndim == 2, "x (tokens, hidden), w1 and w2 3-D, topk_ids 2-D")
     tokens, hidden = x.shape
     experts, ffn = w1.shape[0], w2.shape[2]
-    _require(w1.shape == (experts, 2 * ffn, hidden) and w2.shape == (experts, hidden, ffn),
+    require(w1.shape == (experts, 2 * ffn, hidden) and w2.shape == (experts, hidden, ffn),
              f"Incompatible Dimensions: x {tuple(x.shape)}, w1 {tuple(w1.shape)}, w2 {tuple(w2.shape)}")
-    _require(topk_ids.shape[0] == tokens and topk_weights.shape == topk_ids.shape, "topk_ids and topk_weights must be (tokens, topk)")
-    _require(x.dtype in (torch.float16, torch.bfloat16) and w1.dtype == x.dtype and w2.dtype == x.dtype,
+    require(topk_ids.shape[0] == tokens and topk_weights.shape == topk_ids.shape, "topk_ids and topk_weights must be (tokens, topk)")
+    require(x.dtype in (torch.float16, torch.bfloat16) and w1.dtype == x.dtype and w2.dtype == x.dtype,
              f"x, w1 and w2 must all be float16 or all bfloat16, got {x.dtype}, {w1.dtype}, {w2.dtype}")
-    _require(topk_ids.dtype in (torch.int32, torch.int64), "topk_ids must be int32 or int64")
-    _require(topk_weights.is_floating_point(), "topk_weights must be floating point")
+    require(topk_ids.dtype in (torch.int32, torch.int64), "topk_ids must be int32 or int64")
+    require(topk_weights.is_floating_point(), "topk_weights must be floating point")
     topk = topk_ids.shape[1]
-    _require(tokens <= MOE_MLP_MAX_TOKENS, f"moe_mlp takes at most {MOE_MLP_MAX_TOKENS} tokens, got {tokens}; use distributed.PeerMemoryMoE for more")
-    _require(1 <= topk <= _MAX_TOPK, f"topk must be between 1 and {_MAX_TOPK}, got {topk}")
-    _require(1 <= experts <= _MAX_EXPERTS, f"between 1 and {_MAX_EXPERTS} experts, got {experts}")
-    _require(hidden >= 8 and ffn >= 8 and hidden % 8 == 0 and ffn % 8 == 0, f"hidden and ffn must be multiples of 8, got {hidden} and {ffn}")
-    _require_cuda(x, w1, w2, topk_ids, topk_weights, out)
+    require(tokens <= MOE_MLP_MAX_TOKENS, f"moe_mlp takes at most {MOE_MLP_MAX_TOKENS} tokens, got {tokens}; use distributed.PeerMemoryMoE for more")
+    require(1 <= topk <= _MAX_TOPK, f"topk must be between 1 and {_MAX_TOPK}, got {topk}")
+    require(1 <= experts <= _MAX_EXPERTS, f"between 1 and {_MAX_EXPERTS} experts, got {experts}")
+    require(hidden >= 8 and ffn >= 8 and hidden % 8 == 0 and ffn % 8 == 0, f"hidden and ffn must be multiples of 8, got {hidden} and {ffn}")
+    require_cuda(x, w1, w2, topk_ids, topk_weights, out)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, w1, w2, topk_weights, out)):
         raise RuntimeError("tritonblas.moe_mlp(): inference only, but one of the arguments requires grad.")
     if out is None:
         out = torch.empty(tokens, hidden, dtype=x.dtype, device=x.device)
     else:
-        _require(out.shape == (tokens, hidden) and out.dtype == x.dtype, f"out must be {(tokens, hidden)} of {x.dtype}")
-        _require(out.stride(1) == 1 and (tokens <= 1 or out.stride(0) >= hidden), "out must have contiguous, non-overlapping rows")
+        require(out.shape == (tokens, hidden) and out.dtype == x.dtype, f"out must be {(tokens, hidden)} of {x.dtype}")
+        require(out.stride(1) == 1 and (tokens <= 1 or out.stride(0) >= hidden), "out must have contiguous, non-overlapping rows")
     if tokens == 0:
         return out
-    x, w1, w2 = (t if _rows16(t) else t.clone(memory_format=torch.contiguous_format) for t in (x, w1, w2))
+    x, w1, w2 = (t if rows16(t) else t.clone(memory_format=torch.contiguous_format) for t in (x, w1, w2))
     ids, weights = topk_ids.contiguous(), topk_weights.to(torch.float32).contiguous()
     need = _lib.lib.tb_moe_mlp_workspace_bytes(tokens, topk, experts, hidden, ffn)
     # per call, from torch's allocator: calls on other streams and captured graphs never share it
@@ -178,7 +151,7 @@ def moe_mlp(x, w1, w2, topk_ids, topk_weights, out: Optional[torch.Tensor] = Non
                            w1.data_ptr(), w1.stride(0), w1.stride(1), w2.data_ptr(), w2.stride(0), w2.stride(1),
                            ids.data_ptr(), weights.data_ptr(), out.data_ptr(), out.stride(0), ws.data_ptr(), need,
                            int(ids.dtype == torch.int64), 0)
-    with _on_device(x.device):
+    with on_device(x.device):
         rc = _lib.lib.tb_moe_mlp(ctypes.byref(args), _lib.current_stream_ptr(x.device))
     _lib.check(rc, "tb_moe_mlp")
     return out
