@@ -144,9 +144,12 @@ int encode_2d(CUtensorMap* map, int dtype, const void* base, uint64_t inner, uin
   return TB_OK;
 }
 
+static int esize_of(int dtype);
+
 int encode_nd(CUtensorMap* map, int dtype, const void* base, int rank, const uint64_t* dims, const uint64_t* strides,
               const uint32_t* box) {
-  if (rank < 2 || rank > 5) return TB_ERR_INVALID;
+  const uint32_t width = box[0] * static_cast<uint32_t>(esize_of(dtype));
+  if (rank < 2 || rank > 5 || (width != 128 && width != 64 && width != 32)) return TB_ERR_INVALID;
   cuuint64_t d[5], st[4];
   cuuint32_t bx[5], estr[5];
   bool aligned = (reinterpret_cast<uintptr_t>(base) & 15) == 0;
@@ -161,8 +164,9 @@ int encode_nd(CUtensorMap* map, int dtype, const void* base, int rank, const uin
   }
   if (!aligned) return TB_ERR_ALIGNMENT;
   CUresult r = g_encode(map, tmap_dtype(dtype), static_cast<cuuint32_t>(rank), const_cast<void*>(base), d, st, bx, estr,
-                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                        CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        width == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : (width == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_32B),
+                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return cu_fail(static_cast<int>(r), "cuTensorMapEncodeTiled");
   return TB_OK;
 }
@@ -569,15 +573,17 @@ static int gemm_impl(const tb_gemm_args& a_in, const tb_config* user_cfg, cudaSt
     p.lr_tile_rows = lr->tile_rows;
     p.lr_tokens_on_b = swapped ? 1 : 0;
     CUtensorMap tv, tlb;
-    const uint32_t token_box = swapped ? bn / pair : 128, weight_box = swapped ? 128 : bn / pair;
-    rc = encode_2d(&tv, a.a_dtype, lr->v, static_cast<uint64_t>(lr->kblocks) * bk, lr->v_rows, static_cast<uint64_t>(lr->kblocks) * 128,
-                   bk, token_box, 1);
-    if (rc != TB_OK) return rc;
+    p.lr_pack = lr->pack;
+    const uint32_t token_box = swapped ? bn / pair : 128, weight_box = swapped ? 128 : bn / pair, inner = bk / lr->pack;
+    const uint64_t v_cols = static_cast<uint64_t>(lr->kblocks) * inner;
+    const uint64_t v_dims[2] = {v_cols, static_cast<uint64_t>(lr->v_rows)}, v_strides[1] = {v_cols * es};
+    const uint32_t v_box[2] = {inner, token_box};
+    if ((rc = encode_nd(&tv, a.a_dtype, lr->v, 2, v_dims, v_strides, v_box)) != TB_OK) return rc;
     const uint64_t dims[3] = {static_cast<uint64_t>(lr->rank), static_cast<uint64_t>(lr->n), static_cast<uint64_t>(lr->num_adapters)};
     const uint64_t strides[2] = {static_cast<uint64_t>(lr->b_row_stride) * es,
                                  lr->num_adapters > 1 ? static_cast<uint64_t>(lr->b_adapter_stride) * es
                                                       : static_cast<uint64_t>(lr->b_row_stride) * es * lr->n};
-    const uint32_t box[3] = {static_cast<uint32_t>(bk), weight_box, 1};
+    const uint32_t box[3] = {inner, weight_box, 1};
     if ((rc = encode_nd(&tlb, a.a_dtype, lr->b, 3, dims, strides, box)) != TB_OK) return rc;
     const CUtensorMap *ma = swapped ? &tlb : &tv, *mb = swapped ? &tv : &tlb;
     return pair == 1 ? launch_gemm<0, 1>(ta, tbm, p, programs, smem_bytes, stream, ma, mb)

@@ -22,16 +22,16 @@ int encode_2d(CUtensorMap* map, int dtype, const void* base, uint64_t inner, uin
               uint32_t box_inner, uint32_t box_outer, int swizzle);  // swizzle: 0 none, 1 128B, 2 128B with 32-byte chunks
 
 // Tensor map of any rank up to 5 over 16-bit or wider elements, dims and box innermost first, strides in bytes of dimensions
-// 1 .. rank-1; 128-byte swizzle (box[0] elements must be 128 bytes).
+// 1 .. rank-1; box[0] elements must be 128, 64 or 32 bytes: the swizzle has that width.
 int encode_nd(CUtensorMap* map, int dtype, const void* base, int rank, const uint64_t* dims, const uint64_t* strides,
               const uint32_t* box);
 
 // Low-rank update of a dense launch (see GemmParams::lr_list): the tokens' masked projections v, one block of tile_rows rows of
-// kblocks * 64 elements per token tile and listed adapter, and lora_b (num_adapters, n, rank).
+// kblocks * 64 / pack elements per token tile and listed adapter, and lora_b (num_adapters, n, rank).
 struct LowRank {
   const void* v;
   int64_t v_rows;
-  int kblocks, rank, tile_rows;
+  int kblocks, pack, rank, tile_rows;
   const void* b;
   int64_t b_adapter_stride, b_row_stride;
   int num_adapters, n;

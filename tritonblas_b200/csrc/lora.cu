@@ -7,16 +7,17 @@
 // blocks against the adapters' B as further K stages of the same tile, so the update costs its bytes and no pass over the
 // output, and the sum is rounded once. The GEMM starts while the projection still runs.
 //
-// The projection is bound by reading x and the used adapters' A once: every warp takes K slices, loads both operands straight
-// into the fragments of mma.sync (16 bytes per lane and row; the order of K inside a slice is the same for both, so it need
-// not be the instruction's), and the partial sums meet in shared memory and, when one block does not keep the SMs busy, across
-// a cluster. v is rounded to the operands' 16-bit type once, after the scale: it is the A operand of a tensor-core product.
+// The projection is bound by reading x and the used adapters' A once; it has a form for decode batches (up to 64 rows, mostly
+// one adapter each) and one for longer ones. v is rounded to the operands' 16-bit type once, after the scale: it is the A operand of a tensor-core product.
 // Its error is eps / 2 of each of `rank` terms of the update, next to the one rounding of the output.
 // No reference counterpart (the reference has no adapters).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <mutex>
+
 #include "common_host.h"
+#include "selector.h"
 #include "ptx.cuh"
 
 namespace tb {
@@ -28,7 +29,9 @@ namespace {
 constexpr int kWarps = 8;
 constexpr int kThreads = kWarps * 32;
 constexpr int kMaxRank = 128;
+constexpr int kMaxStages = 6;
 constexpr int kMaxTileRows = 256;
+constexpr int kTableBits = 9, kTable = 1 << kTableBits;
 constexpr long long kFlagBytes = 4096;  // stream-K flags at the start of the GEMM's workspace
 
 struct ProjectParams {
@@ -42,13 +45,19 @@ struct ProjectParams {
   int tokens, k, rank, num_adapters;
   int tile_rows;        // rows of a GEMM tile
   int max_slots;        // list entries per tile
-  int v_cols;           // columns of a block (rank rounded up to 64)
+  int v_cols;           // columns of a block (rank rounded up to 16, 32 or a multiple of 64)
   int splits;           // CTAs of a cluster that share K
   int k_chunk;          // K per CTA, a multiple of 32
   void* v;
   int* list;            // [tiles][1 + max_slots]
   unsigned* flags;      // stream-K flags to clear
   int flag_words;
+  // tensor-core form
+  int rank_pad;         // rank rounded up to 16
+  int stages, stage_bytes, tmem_cols;
+  uint32_t idesc;
+  int* status;
+  unsigned long long timeout_ns;
 };
 
 template <typename T>
@@ -74,27 +83,127 @@ __device__ __forceinline__ __nv_bfloat16 cast16<__nv_bfloat16>(float v) { return
 template <>
 __device__ __forceinline__ __half cast16<__half>(float v) { return __float2half_rn(v); }
 
-// Sum of one float per CTA of the cluster at the same shared-memory offset, in rank order.
+// Sum of one float per CTA of the cluster (at most 8) at the same shared-memory offset, in rank order.
 __device__ __forceinline__ float cluster_sum(const float* mine, int splits) {
   const uint32_t addr = smem_u32(mine);
-  float s = 0.0f;
-  for (int r = 0; r < splits; ++r) {
-    float v;
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(mapa_cluster(addr, r)) : "memory");
-    s += v;
+  float v[8];
+#pragma unroll
+  for (int r = 0; r < 8; ++r) {
+    v[r] = 0.0f;
+    if (r < splits) asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v[r]) : "r"(mapa_cluster(addr, r)) : "memory");
   }
+  float s = v[0];
+#pragma unroll
+  for (int r = 1; r < 8; ++r) s += v[r];
   return s;
 }
 
-// One cluster (of `splits` CTAs along K) per run of 16 * MT rows; blockIdx.y deals the adapters of the run. NT: n-tiles of 8
-// ranks held in registers.
-template <typename T, int NT, int MT>
-__global__ void __launch_bounds__(kThreads) lora_project_kernel(const ProjectParams p) {
-  constexpr int kRows = 16 * MT, kCols = 8 * NT;
-  __shared__ alignas(16) int s_ids[kMaxTileRows];
-  __shared__ int s_list[kMaxTileRows];
-  __shared__ int s_warp_firsts[kWarps];
-  __shared__ int s_present;
+// What a block knows about its run of kRows rows: the adapters that occur in it and where they stand in its tile's list.
+template <int kRows>
+struct RunLists {
+  int ids[kMaxTileRows];                                                       // of the tile's rows; -1 = no adapter
+  int key[kTable], first[kTable], run_first[kTable], slot[kTable];             // adapters of the tile, hashed
+  int run_ids[kRows], run_slots[kRows];                                        // adapters of the run, by their first rows
+  bool present[kMaxTileRows];                                                  // per place in the list: occurs in the run
+  int firsts[2][kWarps];
+};
+
+// Fills `l` for the run of kRows rows at row0 (all threads of a block of kThreads, ends with a barrier), writes the tile's list
+// (`writer`: the one block of the tile that does) and returns the lengths of the tile's and of the run's list. Adapters stand in
+// the order of their first rows, so every block of a tile finds the same list; equal ids meet in a small hash table that keeps
+// the lowest row.
+template <int kRows>
+__device__ __forceinline__ int2 find_adapters(const ProjectParams& p, RunLists<kRows>& l, int row0, bool writer) {
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tile = row0 / p.tile_rows, tile_row0 = tile * p.tile_rows;
+  const int run_row = tid - (row0 - tile_row0);  // row of the run this thread speaks for, if it is one
+  const bool in_run = run_row >= 0 && run_row < kRows;
+  int id = -1;
+  if (tid < p.tile_rows && tile_row0 + tid < p.tokens) {
+    const long long v = p.is64 ? static_cast<const long long*>(p.ids)[tile_row0 + tid]
+                               : static_cast<long long>(static_cast<const int*>(p.ids)[tile_row0 + tid]);
+    if (v >= 0 && v < p.num_adapters) id = static_cast<int>(v);
+  }
+  l.ids[tid] = id;
+  for (int i = tid; i < kTable; i += kThreads) {
+    l.key[i] = -1;
+    l.first[i] = l.run_first[i] = kMaxTileRows;
+  }
+  __syncthreads();
+  int entry = static_cast<int>((static_cast<unsigned>(id) * 2654435761u) >> (32 - kTableBits));
+  if (id >= 0) {
+    while (true) {  // the table has twice as many places as the tile has rows: a free one always comes
+      const int before = atomicCAS(&l.key[entry], -1, id);
+      if (before == -1 || before == id) break;
+      entry = (entry + 1) & (kTable - 1);
+    }
+    atomicMin(&l.first[entry], tid);
+    if (in_run) atomicMin(&l.run_first[entry], run_row);
+  }
+  __syncthreads();
+  const bool first = id >= 0 && l.first[entry] == tid;
+  const bool run_first = id >= 0 && in_run && l.run_first[entry] == run_row;
+  const unsigned votes = __ballot_sync(0xffffffffu, first), run_votes = __ballot_sync(0xffffffffu, run_first);
+  if (lane == 0) {
+    l.firsts[0][warp] = __popc(votes);
+    l.firsts[1][warp] = __popc(run_votes);
+  }
+  __syncthreads();
+  const unsigned below = (1u << lane) - 1u;
+  int slot_of_first = __popc(votes & below), turn_of_first = __popc(run_votes & below), count = 0, present = 0;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) {
+    if (w < warp) {
+      slot_of_first += l.firsts[0][w];
+      turn_of_first += l.firsts[1][w];
+    }
+    count += l.firsts[0][w];
+    present += l.firsts[1][w];
+  }
+  int* list = p.list + static_cast<long long>(tile) * (1 + p.max_slots);
+  if (first) {
+    l.slot[entry] = slot_of_first;
+    l.present[slot_of_first] = l.run_first[entry] < kMaxTileRows;
+    if (writer) list[1 + slot_of_first] = id;
+  }
+  if (writer && tid == 0) list[0] = count;
+  __syncthreads();
+  if (run_first) {
+    l.run_ids[turn_of_first] = id;
+    l.run_slots[turn_of_first] = l.slot[entry];
+  }
+  __syncthreads();
+  return make_int2(count, present);
+}
+
+// The run's rows in the blocks of the tile's other adapters are zeros; dealt over the blocks of the grid's y axis.
+template <int kRows, typename T>
+__device__ __forceinline__ void clear_absent(const ProjectParams& p, const RunLists<kRows>& l, T* tile_blocks, int count, int rank) {
+  const long long block_stride = static_cast<long long>(p.tile_rows) * p.v_cols;
+  for (int slot = blockIdx.y; slot < count; slot += gridDim.y) {
+    if (l.present[slot]) continue;
+    uint4* block = reinterpret_cast<uint4*>(tile_blocks + slot * block_stride);
+    for (int i = threadIdx.x + rank * kThreads; i < kRows * p.v_cols / 8; i += kThreads * p.splits) block[i] = make_uint4(0, 0, 0, 0);
+  }
+}
+
+__device__ __forceinline__ void cluster_or_block_sync(int splits) {
+  if (splits > 1) {
+    cluster_arrive();
+    cluster_wait();
+  } else {
+    __syncthreads();
+  }
+}
+
+// ------------------------------------------------------------------------------------------------------ decode batches
+// One cluster (of `splits` CTAs along K) per run of 16 rows; blockIdx.y deals the adapters of the run. Every warp takes K slices
+// and loads both operands straight into the fragments of mma.sync (16 bytes per lane and row; the order of K inside a slice is
+// the same for both, so it need not be the instruction's). NT: n-tiles of 8 ranks held in registers.
+template <typename T, int NT>
+__global__ void __launch_bounds__(kThreads, 2) lora_project_kernel(const ProjectParams p) {
+  constexpr int kRows = 16, kCols = 8 * NT;
+  __shared__ RunLists<kRows> lists;
   __shared__ float s_red[kWarps][kRows][8];
   __shared__ float s_part[kRows][kCols];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -107,105 +216,61 @@ __global__ void __launch_bounds__(kThreads) lora_project_kernel(const ProjectPar
 
   if (blockIdx.x == 0 && blockIdx.y == 0)
     for (int i = tid; i < p.flag_words; i += kThreads) p.flags[i] = 0u;
-
-  // Adapters of the tile in the order of their first rows; every block of the tile computes the same list.
-  int id = -1;
-  if (tid < p.tile_rows && tile_row0 + tid < p.tokens) {
-    const long long v = p.is64 ? static_cast<const long long*>(p.ids)[tile_row0 + tid]
-                               : static_cast<long long>(static_cast<const int*>(p.ids)[tile_row0 + tid]);
-    if (v >= 0 && v < p.num_adapters) id = static_cast<int>(v);
-  }
-  s_ids[tid] = id;
-  __syncthreads();
-  bool first = id >= 0;
-#pragma unroll 4
-  for (int j = 0; j < (warp + 1) * 32; j += 4) {
-    const int4 o = *reinterpret_cast<const int4*>(s_ids + j);
-    first = first && !(o.x == id && j < tid) && !(o.y == id && j + 1 < tid) && !(o.z == id && j + 2 < tid) && !(o.w == id && j + 3 < tid);
-  }
-  const unsigned votes = __ballot_sync(0xffffffffu, first);
-  if (lane == 0) s_warp_firsts[warp] = __popc(votes);
-  __syncthreads();
-  int before = __popc(votes & ((1u << lane) - 1u)), count = 0;
-  for (int w = 0; w < kWarps; ++w) {
-    if (w < warp) before += s_warp_firsts[w];
-    count += s_warp_firsts[w];
-  }
-  if (first) s_list[before] = id;
-  __syncthreads();
-  if (row0 == tile_row0 && blockIdx.y == 0 && rank == 0) {
-    int* list = p.list + static_cast<long long>(tile) * (1 + p.max_slots);
-    if (tid == 0) list[0] = count;
-    if (tid < count) list[1 + tid] = s_list[tid];
-  }
+  const int2 found = find_adapters<kRows>(p, lists, row0, row0 == tile_row0 && blockIdx.y == 0 && rank == 0);
+  const int* run_ids = lists.ids + (row0 - tile_row0);
+  T* tile_blocks = static_cast<T*>(p.v) + static_cast<long long>(tile) * p.max_slots * p.tile_rows * p.v_cols +
+                   static_cast<long long>(row0 - tile_row0) * p.v_cols;
+  clear_absent<kRows>(p, lists, tile_blocks, found.x, rank);
 
   const T* x = static_cast<const T*>(p.x);
   const int g = lane >> 2, q = lane & 3;
   const int k_begin = rank * p.k_chunk, k_end = min(p.k, k_begin + p.k_chunk);
-  for (int slot = blockIdx.y; slot < count; slot += gridDim.y) {
-    const int adapter = s_list[slot];
-    T* block = static_cast<T*>(p.v) + (static_cast<long long>(tile) * p.max_slots + slot) * p.tile_rows * p.v_cols +
-               static_cast<long long>(row0 - tile_row0) * p.v_cols;
-    if (tid == 0) s_present = 0;
-    __syncthreads();
-    if (tid < kRows && s_ids[row0 - tile_row0 + tid] == adapter) s_present = 1;
-    __syncthreads();
-    if (s_present == 0) {  // the same answer in every CTA of the cluster
-      if (rank == 0)
-        for (int i = tid; i < kRows * p.v_cols / 8; i += kThreads) reinterpret_cast<uint4*>(block)[i] = make_uint4(0, 0, 0, 0);
-      __syncthreads();
-      continue;
-    }
-    float acc[MT][NT][4];
+  for (int turn = blockIdx.y; turn < found.y; turn += gridDim.y) {
+    const int adapter = lists.run_ids[turn];
+    T* block = tile_blocks + lists.run_slots[turn] * static_cast<long long>(p.tile_rows) * p.v_cols;
+    const float scale = p.scales != nullptr ? __ldg(p.scales + adapter) : 1.0f;
+    // only rows with this adapter are read; the others enter the product as zeros
+    bool live[2];
 #pragma unroll
-    for (int m = 0; m < MT; ++m)
+    for (int h = 0; h < 2; ++h) live[h] = run_ids[h * 8 + g] == adapter;
+    const T* x_lane = x + (row0 + g) * p.x_stride + q * 8;
+    const T* a_lane = static_cast<const T*>(p.a) + adapter * p.a_adapter_stride + g * p.a_row_stride + q * 8;
+    float acc[NT][4];
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
+    for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) acc[m][n][i] = 0.0f;
-    const T* a = static_cast<const T*>(p.a) + adapter * p.a_adapter_stride;
-    constexpr int kUnroll = (NT * MT <= 4) ? 4 : (NT * MT <= 16 ? 2 : 1);
+      for (int i = 0; i < 4; ++i) acc[n][i] = 0.0f;
+    constexpr int kUnroll = NT <= 4 ? 4 : (NT <= 8 ? 2 : 1);
     const uint4 zero = make_uint4(0, 0, 0, 0);
     // K in steps of 32 per warp: four lanes cover 64 contiguous bytes of a row
     for (int k0 = k_begin + warp * 32; k0 < k_end; k0 += kWarps * 32 * kUnroll) {
-      uint4 xa[kUnroll][MT][2], bb[kUnroll][NT];
+      uint4 xa[kUnroll][2], bb[kUnroll][NT];
 #pragma unroll
       for (int s = 0; s < kUnroll; ++s) {
-        const int k = k0 + s * kWarps * 32 + q * 8;
-        const bool in_k = k < k_end;
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          const int r = n * 8 + g;
-          bb[s][n] = in_k && r < p.rank ? __ldg(reinterpret_cast<const uint4*>(a + r * p.a_row_stride + k)) : zero;
-        }
-#pragma unroll
-        for (int m = 0; m < MT; ++m)
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const int t = row0 + m * 16 + h * 8 + g;
-            xa[s][m][h] = in_k && t < p.tokens ? __ldg(reinterpret_cast<const uint4*>(x + t * p.x_stride + k)) : zero;
-          }
-      }
-#pragma unroll
-      for (int s = 0; s < kUnroll; ++s)
+        const int k = k0 + s * kWarps * 32;
+        const bool in_k = k + q * 8 < k_end;
 #pragma unroll
         for (int n = 0; n < NT; ++n)
+          bb[s][n] = in_k && n * 8 < p.rank ? __ldg(reinterpret_cast<const uint4*>(a_lane + n * 8 * p.a_row_stride + k)) : zero;
 #pragma unroll
-          for (int m = 0; m < MT; ++m) {
-            mma_16816<T>(acc[m][n], xa[s][m][0].x, xa[s][m][1].x, xa[s][m][0].y, xa[s][m][1].y, bb[s][n].x, bb[s][n].y);
-            mma_16816<T>(acc[m][n], xa[s][m][0].z, xa[s][m][1].z, xa[s][m][0].w, xa[s][m][1].w, bb[s][n].z, bb[s][n].w);
-          }
+        for (int h = 0; h < 2; ++h)
+          xa[s][h] = in_k && live[h] ? __ldg(reinterpret_cast<const uint4*>(x_lane + h * 8 * p.x_stride + k)) : zero;
+      }
+#pragma unroll
+      for (int s = 0; s < kUnroll; ++s) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n) mma_16816<T>(acc[n], xa[s][0].x, xa[s][1].x, xa[s][0].y, xa[s][1].y, bb[s][n].x, bb[s][n].y);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) mma_16816<T>(acc[n], xa[s][0].z, xa[s][1].z, xa[s][0].w, xa[s][1].w, bb[s][n].z, bb[s][n].w);
+      }
     }
     // the warps' sums, one n-tile at a time
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-#pragma unroll
-      for (int m = 0; m < MT; ++m) {
-        s_red[warp][m * 16 + g][2 * q] = acc[m][n][0];
-        s_red[warp][m * 16 + g][2 * q + 1] = acc[m][n][1];
-        s_red[warp][m * 16 + g + 8][2 * q] = acc[m][n][2];
-        s_red[warp][m * 16 + g + 8][2 * q + 1] = acc[m][n][3];
-      }
+      s_red[warp][g][2 * q] = acc[n][0];
+      s_red[warp][g][2 * q + 1] = acc[n][1];
+      s_red[warp][g + 8][2 * q] = acc[n][2];
+      s_red[warp][g + 8][2 * q + 1] = acc[n][3];
       __syncthreads();
       for (int i = tid; i < kRows * 8; i += kThreads) {
         float v = 0.0f;
@@ -215,33 +280,176 @@ __global__ void __launch_bounds__(kThreads) lora_project_kernel(const ProjectPar
       }
       __syncthreads();
     }
-    if (p.splits > 1) {
-      cluster_arrive();
-      cluster_wait();
-    }
-    const float scale = p.scales != nullptr ? p.scales[adapter] : 1.0f;
+    cluster_or_block_sync(p.splits);
     // the CTAs of a cluster write a share of the block each
     for (int i = tid + rank * kThreads; i < kRows * p.v_cols; i += kThreads * p.splits) {
       const int r = i / p.v_cols, c = i - r * p.v_cols;
       float v = 0.0f;
-      if (c < p.rank && s_ids[row0 - tile_row0 + r] == adapter)
+      if (c < p.rank && run_ids[r] == adapter)
         v = scale * (p.splits > 1 ? cluster_sum(&s_part[r][c], p.splits) : s_part[r][c]);
       block[i] = cast16<T>(v);
     }
-    if (p.splits > 1) {  // nobody overwrites or leaves its sums while another CTA still reads them
-      cluster_arrive();
-      cluster_wait();
-    } else {
-      __syncthreads();
-    }
+    cluster_or_block_sync(p.splits);  // nobody overwrites or leaves its sums while another CTA still reads them
   }
 }
 
-template <typename T, int NT, int MT>
-int project_launch(const ProjectParams& p, int runs, int stripes, cudaStream_t stream) {
+// ------------------------------------------------------------------------------------------------------ longer batches
+// One cluster (of `splits` CTAs along K) per run of 128 rows; blockIdx.y deals the adapters of the run. A product of the run's
+// rows with the adapter's `rank` rows on the tensor cores: TMA into a ring, one MMA warp, the accumulator read back, the CTAs'
+// partial sums joined over the cluster in rank order. Warps: 0 loads, 1 issues, 4-7 read the accumulator; all write v.
+// Every thread reaches every barrier whether its waits succeeded or not, so a wait that runs out ends the kernel.
+template <typename T>
+__global__ void __launch_bounds__(kThreads, 1)
+lora_project_tc_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ CUtensorMap tmap_a, const ProjectParams p) {
+  constexpr int kRows = 128;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  float* part = reinterpret_cast<float*>(ring);  // [rank_pad][128] partial sums, over the drained ring
+  __shared__ RunLists<kRows> lists;
+  __shared__ uint64_t full_bar[kMaxStages], empty_bar[kMaxStages], acc_bar;
+  __shared__ uint32_t tmem_slot;
+  __shared__ volatile int abort_word;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int cta = p.splits > 1 ? static_cast<int>(cluster_ctarank()) : 0;
+  const int row0 = static_cast<int>(blockIdx.x) / p.splits * kRows;
+  const int tile = row0 / p.tile_rows, tile_row0 = tile * p.tile_rows;
+  const WaitCtx wctx{&abort_word, p.status, p.timeout_ns};
+  if (tid == 0) {
+    abort_word = 0;
+    for (int s = 0; s < p.stages; ++s) {
+      mbar_init(&full_bar[s], 1);
+      mbar_init(&empty_bar[s], 1);
+    }
+    mbar_init(&acc_bar, 1);
+    mbar_fence_init();
+    prefetch_tmap(&tmap_x);
+    prefetch_tmap(&tmap_a);
+  }
+  if (warp == 1) {
+    tmem_alloc<1>(&tmem_slot, static_cast<uint32_t>(p.tmem_cols));
+    tmem_relinquish<1>();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = tmem_slot;
+  griddep_wait();
+  griddep_launch_dependents();
+
+  if (blockIdx.x == 0 && blockIdx.y == 0)
+    for (int i = tid; i < p.flag_words; i += kThreads) p.flags[i] = 0u;
+  const int2 found = find_adapters<kRows>(p, lists, row0, row0 == tile_row0 && blockIdx.y == 0 && cta == 0);
+  const int* run_ids = lists.ids + (row0 - tile_row0);
+  T* tile_blocks = static_cast<T*>(p.v) + static_cast<long long>(tile) * p.max_slots * p.tile_rows * p.v_cols +
+                   static_cast<long long>(row0 - tile_row0) * p.v_cols;
+  clear_absent<kRows>(p, lists, tile_blocks, found.x, cta);
+
+  const int kb_begin = cta * p.k_chunk / 64;
+  const int kbs = max(0, min((p.k + 63) / 64, kb_begin + p.k_chunk / 64) - kb_begin);
+  int s = 0;
+  uint32_t ph = 0, acc_ph = 0;
+  for (int turn = blockIdx.y; turn < found.y; turn += gridDim.y) {
+    const int adapter = lists.run_ids[turn];
+    T* block = tile_blocks + lists.run_slots[turn] * static_cast<long long>(p.tile_rows) * p.v_cols;
+    const float scale = p.scales != nullptr ? __ldg(p.scales + adapter) : 1.0f;
+    if (abort_word) {
+      // an earlier turn's wait ran out: nothing more is loaded or multiplied
+    } else if (warp == 0) {
+      fence_proxy_async_smem();  // the last turn's sums stood where the copies land
+      for (int kb = 0; kb < kbs; ++kb) {
+        if (!mbar_wait_warp(&empty_bar[s], ph ^ 1, wctx, TB_DEV_TIMEOUT_SMEM_EMPTY)) break;
+        if (elect_one()) {
+          uint8_t* dst = ring + static_cast<size_t>(s) * p.stage_bytes;
+          mbar_arrive_expect_tx(&full_bar[s], static_cast<uint32_t>(p.stage_bytes));
+          tma_load_2d(dst, &tmap_x, &full_bar[s], (kb_begin + kb) * 64, row0);
+          tma_load_3d(dst + kRows * 128, &tmap_a, &full_bar[s], (kb_begin + kb) * 64, 0, adapter);
+        }
+        __syncwarp();
+        if (++s == p.stages) {
+          s = 0;
+          ph ^= 1;
+        }
+      }
+    } else if (warp == 1) {
+      const uint64_t desc0 = make_smem_desc(smem_u32(ring), 16, 1024);
+      bool ok = true;
+      tc_fence_after();  // the last turn's sums have been read
+      for (int kb = 0; kb < kbs; ++kb) {
+        ok = mbar_wait_warp(&full_bar[s], ph, wctx, TB_DEV_TIMEOUT_SMEM_FULL);
+        if (!ok) break;
+        if (elect_one()) {
+          const uint64_t a = desc0 + static_cast<uint64_t>((s * p.stage_bytes) >> 4), b = a + ((kRows * 128) >> 4);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) umma<0, 1>(tmem_base, a + 2 * k, b + 2 * k, p.idesc, (kb > 0 || k > 0) ? 1u : 0u);
+          umma_commit(&empty_bar[s]);
+          if (kb + 1 == kbs) umma_commit(&acc_bar);
+        }
+        __syncwarp();
+        if (++s == p.stages) {
+          s = 0;
+          ph ^= 1;
+        }
+      }
+    } else if (warp >= 4) {
+      const int r = (warp & 3) * 32 + lane;
+      bool ok = true;
+      if (kbs > 0) ok = __all_sync(0xffffffffu, mbar_wait(&acc_bar, acc_ph, wctx, TB_DEV_TIMEOUT_TMEM_FULL));
+      tc_fence_after();
+      for (int c0 = 0; c0 < p.rank_pad; c0 += 32) {
+        uint32_t v[32];
+        if (ok && kbs > 0) {
+          tmem_ld_32x32(tmem_base + (static_cast<uint32_t>((warp & 3) * 32) << 16) + c0, v);
+          tmem_ld_wait(v);
+        }
+#pragma unroll
+        for (int j = 0; j < 32; ++j)
+          if (c0 + j < p.rank_pad) part[(c0 + j) * kRows + r] = kbs > 0 ? __uint_as_float(v[j]) : 0.0f;
+      }
+      tc_fence_before();
+    }
+    if (kbs > 0) acc_ph ^= 1;
+    cluster_or_block_sync(p.splits);
+    // the CTAs of a cluster write a share of the rows each, eight ranks per thread
+    const int share = kRows / p.splits, groups = p.v_cols / 8;
+    for (int i = tid; i < share * groups; i += kThreads) {
+      const int r = cta * share + i % share, c = i / share * 8;
+      float v[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = 0.0f;
+      if (c < p.rank && run_ids[r] == adapter) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float* mine = part + (c + j) * kRows + r;
+          v[j] = scale * (p.splits > 1 ? cluster_sum(mine, p.splits) : *mine);
+        }
+      }
+      T o[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) o[j] = cast16<T>(v[j]);
+      *reinterpret_cast<uint4*>(block + static_cast<long long>(r) * p.v_cols + c) = *reinterpret_cast<const uint4*>(o);
+    }
+    cluster_or_block_sync(p.splits);  // nobody overwrites or leaves its sums while another CTA still reads them
+  }
+  if (abort_word) {
+    // A wait gave up: let copies and MMAs already in flight land before shared memory and TMEM are released.
+    for (int i = 0; i < 64; ++i) __nanosleep(2000);
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc<1>(tmem_base, static_cast<uint32_t>(p.tmem_cols));
+  }
+}
+
+// One launch of either kernel: clusters of p.splits CTAs, programmatic dependent launch as the GEMM kernels use it.
+template <typename... Params, typename... Args>
+int project_launch(void (*kernel)(Params...), int runs, const ProjectParams& p, int stripes, int smem_bytes, cudaStream_t stream,
+                   Args... args) {
   cudaLaunchConfig_t lc = {};
   lc.gridDim = dim3(static_cast<unsigned>(runs * p.splits), static_cast<unsigned>(stripes), 1);
   lc.blockDim = dim3(kThreads, 1, 1);
+  lc.dynamicSmemBytes = static_cast<size_t>(smem_bytes);
   lc.stream = stream;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -255,35 +463,60 @@ int project_launch(const ProjectParams& p, int runs, int stripes, cudaStream_t s
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     lc.numAttrs = 2;
   }
-  cudaError_t e = cudaLaunchKernelEx(&lc, lora_project_kernel<T, NT, MT>, p);
+  cudaError_t e = cudaLaunchKernelEx(&lc, kernel, args..., p);
   if (e != cudaSuccess) return cuda_fail(e, "lora_project_kernel launch");
   g_launches.fetch_add(1, std::memory_order_relaxed);
   return TB_OK;
 }
 
-// Rows a block of the projection takes: 16 for a decode batch, 64 (32 with ranks above 64, whose sums fill the registers) for
-// longer ones, where it is the re-reading of A out of L2 that counts.
-int project_rows(int tokens, int rank) { return tokens <= 64 ? 16 : (rank > 64 ? 32 : 64); }
+template <typename T>
+int project_decode(const ProjectParams& p, int runs, int stripes, cudaStream_t stream) {
+  if (p.rank <= 16) return project_launch(lora_project_kernel<T, 2>, runs, p, stripes, 0, stream);
+  if (p.rank <= 32) return project_launch(lora_project_kernel<T, 4>, runs, p, stripes, 0, stream);
+  if (p.rank <= 64) return project_launch(lora_project_kernel<T, 8>, runs, p, stripes, 0, stream);
+  return project_launch(lora_project_kernel<T, 16>, runs, p, stripes, 0, stream);
+}
 
 template <typename T>
-int project(const ProjectParams& p, int runs, int stripes, cudaStream_t stream) {
-  if (p.tokens <= 64) {
-    if (p.rank <= 16) return project_launch<T, 2, 1>(p, runs, stripes, stream);
-    if (p.rank <= 32) return project_launch<T, 4, 1>(p, runs, stripes, stream);
-    if (p.rank <= 64) return project_launch<T, 8, 1>(p, runs, stripes, stream);
-    return project_launch<T, 16, 1>(p, runs, stripes, stream);
+int project_tc(const tb_lora_args& a, ProjectParams& p, int runs, int stripes, int device, cudaStream_t stream) {
+  p.rank_pad = (p.rank + 15) / 16 * 16;
+  p.stage_bytes = (128 + p.rank_pad) * 128;
+  p.stages = 96 * 1024 / p.stage_bytes;
+  if (p.stages > kMaxStages) p.stages = kMaxStages;
+  p.tmem_cols = 32;
+  while (p.tmem_cols < p.rank_pad) p.tmem_cols <<= 1;
+  p.idesc = (1u << 4) | ((a.dtype == TB_DTYPE_BF16 ? 1u : 0u) * ((1u << 7) | (1u << 10))) |
+            (static_cast<uint32_t>(p.rank_pad >> 3) << 17) | (static_cast<uint32_t>(128 >> 4) << 24);
+  // the ring also holds a CTA's sums once it is drained
+  const int ring = p.stages * p.stage_bytes;
+  const int smem_bytes = (ring > p.rank_pad * 512 ? ring : p.rank_pad * 512) + 1024;
+  CUtensorMap tx, ta;
+  int rc = encode_2d(&tx, a.dtype, a.x, a.k, a.m, static_cast<uint64_t>(p.x_stride) * 2, 64, 128, 1);
+  if (rc != TB_OK) return rc;
+  const uint64_t dims[3] = {static_cast<uint64_t>(a.k), static_cast<uint64_t>(a.rank), static_cast<uint64_t>(a.num_adapters)};
+  const uint64_t strides[2] = {static_cast<uint64_t>(a.lora_a_row_stride) * 2,
+                               static_cast<uint64_t>(a.num_adapters > 1 ? a.lora_a_adapter_stride : a.lora_a_row_stride * a.rank) * 2};
+  const uint32_t box[3] = {64, static_cast<uint32_t>(p.rank_pad), 1};
+  if ((rc = encode_nd(&ta, a.dtype, a.lora_a, 3, dims, strides, box)) != TB_OK) return rc;
+  auto kernel = lora_project_tc_kernel<T>;
+  static int configured[64] = {};
+  static std::mutex mu;
+  {
+    std::lock_guard<std::mutex> lk(mu);
+    if (smem_bytes > configured[device & 63]) {
+      cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes);
+      if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(lora_project_tc)");
+      configured[device & 63] = smem_bytes;
+    }
   }
-  if (p.rank <= 16) return project_launch<T, 2, 4>(p, runs, stripes, stream);
-  if (p.rank <= 32) return project_launch<T, 4, 4>(p, runs, stripes, stream);
-  if (p.rank <= 64) return project_launch<T, 8, 4>(p, runs, stripes, stream);
-  return project_launch<T, 16, 2>(p, runs, stripes, stream);
+  return project_launch(kernel, runs, p, stripes, smem_bytes, stream, tx, ta);
 }
 
 // How a call is cut and where its pieces stand in the workspace.
 struct LoraPlan {
   tb_config cfg;
   int streamk;
-  int tile_rows, tiles, max_slots, v_cols;
+  int tile_rows, tiles, max_slots, v_cols, pack;
   long long v_offset, v_rows, list_offset, gemm_offset, gemm_bytes, bytes;
 };
 
@@ -298,11 +531,15 @@ int lora_plan(const tb_lora_args& a, tb_gemm_args* g, LoraPlan* l) {
   g->wait_timeout_ms = a.wait_timeout_ms;
   const int rc = low_rank_config(*g, &l->cfg, &l->streamk);
   if (rc != TB_OK) return rc;
+  // A decode batch's projection runs beside the GEMM: leave shared memory for one of its blocks on every SM.
   const int pair = l->cfg.cta_pair == 2 ? 2 : 1;
+  while (a.m <= 64 && l->cfg.stages > 3 && smem_bytes_for(l->cfg.block_n, pair, l->cfg.stages) > 200 * 1024) --l->cfg.stages;
   l->tile_rows = l->cfg.swap_ab ? l->cfg.block_n : 128 * pair;
   l->tiles = (a.m + l->tile_rows - 1) / l->tile_rows;
   l->max_slots = l->tile_rows < a.num_adapters ? l->tile_rows : a.num_adapters;
-  l->v_cols = (a.rank + 63) / 64 * 64;
+  // small ranks share a stage of the GEMM: see GemmParams::lr_pack
+  l->pack = a.rank <= 16 ? 4 : (a.rank <= 32 ? 2 : 1);
+  l->v_cols = l->pack > 1 ? 64 / l->pack : (a.rank + 63) / 64 * 64;
   l->v_rows = static_cast<long long>(l->tiles) * l->max_slots * l->tile_rows;
   auto up = [](long long v) { return (v + 255) & ~255ll; };
   l->gemm_offset = 0;
@@ -357,18 +594,28 @@ int lora_impl(const tb_lora_args& a, cudaStream_t stream) {
   p.list = reinterpret_cast<int*>(ws + l.list_offset);
   p.flags = reinterpret_cast<unsigned*>(ws + l.gemm_offset);
   p.flag_words = l.streamk ? static_cast<int>(kFlagBytes / 4) : 0;
-  // Runs cover whole tiles: the rows behind the last token are zeros in every block. Adapters are dealt over up to two blocks
-  // per SM, and what is left of those goes along K (at least 512 elements each).
-  const int rows = project_rows(a.m, a.rank);
+  p.status = status;
+  p.timeout_ns = a.wait_timeout_ms > 0 ? static_cast<unsigned long long>(a.wait_timeout_ms) * 1000000ull : 2000000000ull;
+  // Runs cover whole tiles: the rows behind the last token are zeros in every block. A decode batch has up to one adapter per
+  // row: they are dealt over blocks first, and K is split as long as four blocks per SM are not exceeded. Longer batches have
+  // few adapters per run: K is split first, up to a block per SM, and what is left of two per SM takes the adapters.
+  const bool decode = a.m <= 64;
+  const int rows = decode ? 16 : 128;
   const int runs = l.tiles * (l.tile_rows / rows);
   const int live_runs = (a.m + rows - 1) / rows;
-  int stripes = 2 * num_sms / live_runs;
   const int most = rows < l.max_slots ? rows : l.max_slots;
-  stripes = stripes < 1 ? 1 : (stripes > most ? most : stripes);
+  const int budget = decode ? 4 * num_sms : num_sms;
+  int stripes = decode ? (most < a.m ? most : a.m) : 1;
   p.splits = 1;
-  while (p.splits < 8 && live_runs * stripes * p.splits * 2 <= 2 * num_sms && a.k / (p.splits * 2) >= 512) p.splits *= 2;
-  p.k_chunk = ((a.k + p.splits - 1) / p.splits + 31) / 32 * 32;
-  rc = a.dtype == TB_DTYPE_BF16 ? project<__nv_bfloat16>(p, runs, stripes, stream) : project<__half>(p, runs, stripes, stream);
+  while (p.splits < 8 && live_runs * stripes * p.splits * 2 <= budget && a.k / (p.splits * 2) >= 256) p.splits *= 2;
+  if (!decode) {
+    stripes = 2 * num_sms / (live_runs * p.splits);
+    stripes = stripes < 1 ? 1 : (stripes > most ? most : stripes);
+  }
+  const int k_unit = decode ? 32 : 64;
+  p.k_chunk = ((a.k + p.splits - 1) / p.splits + k_unit - 1) / k_unit * k_unit;
+  if (decode) rc = a.dtype == TB_DTYPE_BF16 ? project_decode<__nv_bfloat16>(p, runs, stripes, stream) : project_decode<__half>(p, runs, stripes, stream);
+  else rc = a.dtype == TB_DTYPE_BF16 ? project_tc<__nv_bfloat16>(a, p, runs, stripes, device, stream) : project_tc<__half>(a, p, runs, stripes, device, stream);
   if (rc != TB_OK) return rc;
 
   g.streamk = l.streamk;
@@ -378,7 +625,8 @@ int lora_impl(const tb_lora_args& a, cudaStream_t stream) {
   LowRank lr = {};
   lr.v = p.v;
   lr.v_rows = l.v_rows;
-  lr.kblocks = l.v_cols / 64;
+  lr.pack = l.pack;
+  lr.kblocks = l.pack > 1 ? 1 : l.v_cols / 64;
   lr.rank = a.rank;
   lr.tile_rows = l.tile_rows;
   lr.b = a.lora_b;
