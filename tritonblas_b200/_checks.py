@@ -1,4 +1,7 @@
-"""Argument checks and small launch helpers shared by the per-token operators."""
+"""Argument checks and small launch helpers shared by the per-token operators.
+
+These operators run in microseconds, so their argument checks are plain ``if not ...: refuse(...)`` statements: nothing is
+formatted unless a call is refused."""
 import contextlib
 
 import torch
@@ -6,17 +9,15 @@ import torch
 _nullcontext = contextlib.nullcontext()
 
 
-def require(ok, message):
-    if not ok:
-        raise ValueError(message)
+def refuse(message):
+    raise ValueError(message)
 
 
-def require_cuda(first, *others):
-    if not first.is_cuda:
+def refuse_devices(*tensors):
+    """Error for tensors that are not all on one CUDA device."""
+    if not all(t.is_cuda for t in tensors if t is not None):
         raise RuntimeError("tritonblas_b200 runs on CUDA tensors only (no CPU path)")
-    for t in others:
-        if t is not None and t.device != first.device:
-            raise RuntimeError(f"all tensors must be on one device, got {first.device} and {t.device}")
+    raise RuntimeError(f"all tensors must be on one device, got {[str(t.device) for t in tensors if t is not None]}")
 
 
 def on_device(device):
@@ -26,6 +27,11 @@ def on_device(device):
 
 def rows16(t):
     """True when the last axis is contiguous and rows start on 16-byte boundaries and do not overlap (TMA reads it in place)."""
-    per16 = 16 // t.element_size()
-    return t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(
-        n == 1 or (s >= t.shape[-1] and s % per16 == 0) for n, s in zip(t.shape[:-1], t.stride()[:-1]))
+    strides, shape = t.stride(), t.shape
+    if strides[-1] != 1 or t.data_ptr() % 16:
+        return False
+    per16, row = 16 // t.element_size(), shape[-1]
+    for n, s in zip(shape[:-1], strides[:-1]):
+        if n != 1 and (s < row or s % per16):
+            return False
+    return True

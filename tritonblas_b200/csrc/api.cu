@@ -616,6 +616,26 @@ int low_rank_config(const tb_gemm_args& a, tb_config* cfg, int* streamk) {
   pr.b_mn_major = (a.b_stride_k != 1 && a.k != 1) ? 1 : 0;
   pr.device = device;
   pr.max_halves = 1;
+  // The model only depends on the problem, and a decode step asks for the same few over and over: the last ones are kept.
+  struct Entry {
+    tb_problem pr;
+    tb_config cfg;
+    int streamk;
+    bool used;
+  };
+  static Entry cache[64];
+  static std::mutex mu;
+  const uint32_t h = (static_cast<uint32_t>(pr.m) * 2654435761u) ^ (static_cast<uint32_t>(pr.n) * 40503u) ^ (static_cast<uint32_t>(pr.k) * 97u);
+  Entry& e = cache[(h ^ (h >> 16)) & 63];
+  {
+    std::lock_guard<std::mutex> lk(mu);
+    if (e.used && std::memcmp(&e.pr, &pr, sizeof(pr)) == 0) {
+      *cfg = e.cfg;
+      *streamk = e.streamk;
+      return TB_OK;
+    }
+  }
+  const tb_problem key = pr;
   tb_config dp, sk;
   int rc = select_config(pr, machine_for(dev), &dp);
   if (rc != TB_OK) return rc;
@@ -624,6 +644,10 @@ int low_rank_config(const tb_gemm_args& a, tb_config* cfg, int* streamk) {
   if (rc != TB_OK) return rc;
   *streamk = sk.predicted_sk_us < dp.predicted_us ? 1 : 0;
   *cfg = *streamk ? sk : dp;
+  if (dev != nullptr) {
+    std::lock_guard<std::mutex> lk(mu);
+    e = {key, *cfg, *streamk, true};
+  }
   return TB_OK;
 }
 

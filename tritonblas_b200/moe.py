@@ -10,11 +10,12 @@ from typing import Optional, Tuple
 import torch
 
 from . import _lib
-from ._checks import on_device, require, require_cuda, rows16
+from ._checks import on_device, refuse, refuse_devices, rows16
 
 MOE_MLP_MAX_TOKENS = 128
 _MAX_EXPERTS, _MAX_TOPK = 1024, 32
 _SCORING = {"softmax": 0, "sigmoid": 1}
+_ROUTE_TYPES = (torch.float16, torch.bfloat16, torch.float32)
 
 # ------------------------------------------------------------------------------------------------------------- router
 def _route_rows(logits):
@@ -37,6 +38,36 @@ def _route_forward(logits, topk, sigmoid, renormalize):
     return weights, ids
 
 
+def _route_backward(logits, weights, ids, grad, sigmoid, renormalize):
+    tokens, experts = logits.shape
+    logits = _route_rows(logits)
+    weights, ids, grad = weights.contiguous(), ids.contiguous(), grad.to(torch.float32).contiguous()
+    out = torch.empty(tokens, experts, dtype=logits.dtype, device=logits.device)
+    with on_device(logits.device):
+        rc = _lib.lib.tb_moe_route_backward(logits.data_ptr(), _lib.DTYPE_CODE[logits.dtype], logits.stride(0), tokens, experts,
+                                            ids.shape[1], sigmoid, renormalize, weights.data_ptr(), ids.data_ptr(),
+                                            grad.data_ptr(), out.data_ptr(), _lib.current_stream_ptr(logits.device))
+    _lib.check(rc, "tb_moe_route_backward")
+    return out
+
+
+class _Route(torch.autograd.Function):
+    """The eager path; traced code goes through the custom operators below, which are the same two calls."""
+
+    @staticmethod
+    def forward(ctx, logits, topk, sigmoid, renormalize):
+        weights, ids = _route_forward(logits, topk, sigmoid, renormalize)
+        ctx.mark_non_differentiable(ids)
+        ctx.save_for_backward(logits, weights, ids)
+        ctx.modes = sigmoid, renormalize
+        return weights, ids
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad_weights, _grad_ids):
+        return _route_backward(*ctx.saved_tensors, grad_weights, *ctx.modes), None, None, None
+
+
 @torch.library.custom_op("tritonblas::_moe_route", mutates_args=())
 def _moe_route(logits: torch.Tensor, topk: int, sigmoid: bool, renormalize: bool) -> Tuple[torch.Tensor, torch.Tensor]:
     return _route_forward(logits, topk, int(sigmoid), int(renormalize))
@@ -51,16 +82,7 @@ def _(logits, topk, sigmoid, renormalize):
 @torch.library.custom_op("tritonblas::_moe_route_backward", mutates_args=())
 def _moe_route_backward(logits: torch.Tensor, weights: torch.Tensor, ids: torch.Tensor, grad: torch.Tensor, sigmoid: bool,
                         renormalize: bool) -> torch.Tensor:
-    tokens, experts = logits.shape
-    logits = _route_rows(logits)
-    weights, ids, grad = weights.contiguous(), ids.contiguous(), grad.to(torch.float32).contiguous()
-    out = torch.empty(tokens, experts, dtype=logits.dtype, device=logits.device)
-    with on_device(logits.device):
-        rc = _lib.lib.tb_moe_route_backward(logits.data_ptr(), _lib.DTYPE_CODE[logits.dtype], logits.stride(0), tokens, experts,
-                                            ids.shape[1], int(sigmoid), int(renormalize), weights.data_ptr(), ids.data_ptr(),
-                                            grad.data_ptr(), out.data_ptr(), _lib.current_stream_ptr(logits.device))
-    _lib.check(rc, "tb_moe_route_backward")
-    return out
+    return _route_backward(logits, weights, ids, grad, int(sigmoid), int(renormalize))
 
 
 @_moe_route_backward.register_fake
@@ -92,17 +114,26 @@ def moe_route(logits, topk, scoring="softmax", renormalize=True):
     never chosen; a row with fewer than ``topk`` others gets id -1 and weight 0 in the remaining places, which every expert path
     of this package skips. At most 1024 experts and ``topk`` 32. The weights are differentiable in the logits.
     """
-    require(logits.ndim == 2, "logits must be (tokens, experts)")
-    require(logits.dtype in (torch.float16, torch.bfloat16, torch.float32), f"logits must be float16, bfloat16 or float32, got {logits.dtype}")
-    require(scoring in _SCORING, f"scoring must be 'softmax' or 'sigmoid', got {scoring!r}")
-    require(1 <= logits.shape[1] <= _MAX_EXPERTS, f"between 1 and {_MAX_EXPERTS} experts, got {logits.shape[1]}")
+    if logits.ndim != 2:
+        refuse("logits must be (tokens, experts)")
+    if logits.dtype not in _ROUTE_TYPES:
+        refuse(f"logits must be float16, bfloat16 or float32, got {logits.dtype}")
+    if scoring not in _SCORING:
+        refuse(f"scoring must be 'softmax' or 'sigmoid', got {scoring!r}")
+    experts = logits.shape[1]
+    if not 1 <= experts <= _MAX_EXPERTS:
+        refuse(f"between 1 and {_MAX_EXPERTS} experts, got {experts}")
     topk = int(topk)
-    require(1 <= topk <= min(_MAX_TOPK, logits.shape[1]), f"topk must be between 1 and min({_MAX_TOPK}, experts), got {topk}")
-    sigmoid, renormalize = _SCORING[scoring], int(bool(renormalize))
-    if torch.compiler.is_compiling() or (torch.is_grad_enabled() and logits.requires_grad):
+    if not 1 <= topk <= min(_MAX_TOPK, experts):
+        refuse(f"topk must be between 1 and min({_MAX_TOPK}, experts), got {topk}")
+    sigmoid, renormalize = _SCORING[scoring], 1 if renormalize else 0
+    if torch.compiler.is_compiling():
         return _moe_route(logits, topk, bool(sigmoid), bool(renormalize))
-    require_cuda(logits)
-    return _route_forward(logits, topk, sigmoid, renormalize)    # no dispatcher round trip on the serving path
+    if not logits.is_cuda:
+        refuse_devices(logits)
+    if logits.requires_grad and torch.is_grad_enabled():
+        return _Route.apply(logits, topk, sigmoid, renormalize)
+    return _route_forward(logits, topk, sigmoid, renormalize)
 
 
 # -------------------------------------------------------------------------------------------------------- expert layer
@@ -117,41 +148,62 @@ def moe_mlp(x, w1, w2, topk_ids, topk_weights, out: Optional[torch.Tensor] = Non
     weighting are float32 with one cast at the end. ``out`` may be given: (tokens, hidden), contiguous rows, no overlap with the
     weights. Inference only. More tokens: ``distributed.PeerMemoryMoE``.
     """
-    require(x.ndim == 2 and w1.ndim == 3 and w2.ndim == 3 and topk_ids.ndim == 2, "x (tokens, hidden), w1 and w2 3-D, topk_ids 2-D")
+    if x.ndim != 2 or w1.ndim != 3 or w2.ndim != 3 or topk_ids.ndim != 2:
+        refuse("x must be (tokens, hidden), w1 and w2 3-D, topk_ids 2-D")
     tokens, hidden = x.shape
-    experts, ffn = w1.shape[0], w2.shape[2]
-    require(w1.shape == (experts, 2 * ffn, hidden) and w2.shape == (experts, hidden, ffn),
-             f"Incompatible Dimensions: x {tuple(x.shape)}, w1 {tuple(w1.shape)}, w2 {tuple(w2.shape)}")
-    require(topk_ids.shape[0] == tokens and topk_weights.shape == topk_ids.shape, "topk_ids and topk_weights must be (tokens, topk)")
-    require(x.dtype in (torch.float16, torch.bfloat16) and w1.dtype == x.dtype and w2.dtype == x.dtype,
-             f"x, w1 and w2 must all be float16 or all bfloat16, got {x.dtype}, {w1.dtype}, {w2.dtype}")
-    require(topk_ids.dtype in (torch.int32, torch.int64), "topk_ids must be int32 or int64")
-    require(topk_weights.is_floating_point(), "topk_weights must be floating point")
+    experts, _, ffn = w2.shape
+    dtype, device = x.dtype, x.device
+    if w1.shape != (experts, 2 * ffn, hidden) or w2.shape[1] != hidden:
+        refuse(f"Incompatible Dimensions: x {tuple(x.shape)}, w1 {tuple(w1.shape)}, w2 {tuple(w2.shape)}")
     topk = topk_ids.shape[1]
-    require(tokens <= MOE_MLP_MAX_TOKENS, f"moe_mlp takes at most {MOE_MLP_MAX_TOKENS} tokens, got {tokens}; use distributed.PeerMemoryMoE for more")
-    require(1 <= topk <= _MAX_TOPK, f"topk must be between 1 and {_MAX_TOPK}, got {topk}")
-    require(1 <= experts <= _MAX_EXPERTS, f"between 1 and {_MAX_EXPERTS} experts, got {experts}")
-    require(hidden >= 8 and ffn >= 8 and hidden % 8 == 0 and ffn % 8 == 0, f"hidden and ffn must be multiples of 8, got {hidden} and {ffn}")
-    require_cuda(x, w1, w2, topk_ids, topk_weights, out)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, w1, w2, topk_weights, out)):
+    if topk_ids.shape[0] != tokens or topk_weights.shape != topk_ids.shape:
+        refuse("topk_ids and topk_weights must be (tokens, topk)")
+    if (dtype is not torch.bfloat16 and dtype is not torch.float16) or w1.dtype is not dtype or w2.dtype is not dtype:
+        refuse(f"x, w1 and w2 must all be float16 or all bfloat16, got {x.dtype}, {w1.dtype}, {w2.dtype}")
+    if topk_ids.dtype not in (torch.int32, torch.int64):
+        refuse("topk_ids must be int32 or int64")
+    if not topk_weights.is_floating_point():
+        refuse("topk_weights must be floating point")
+    if tokens > MOE_MLP_MAX_TOKENS:
+        refuse(f"moe_mlp takes at most {MOE_MLP_MAX_TOKENS} tokens, got {tokens}; use distributed.PeerMemoryMoE for more")
+    if not 1 <= topk <= _MAX_TOPK:
+        refuse(f"topk must be between 1 and {_MAX_TOPK}, got {topk}")
+    if not 1 <= experts <= _MAX_EXPERTS:
+        refuse(f"between 1 and {_MAX_EXPERTS} experts, got {experts}")
+    if hidden < 8 or ffn < 8 or hidden % 8 or ffn % 8:
+        refuse(f"hidden and ffn must be multiples of 8, got {hidden} and {ffn}")
+    if not x.is_cuda or not device == w1.device == w2.device == topk_ids.device == topk_weights.device:
+        refuse_devices(x, w1, w2, topk_ids, topk_weights)
+    if torch.is_grad_enabled() and (x.requires_grad or w1.requires_grad or w2.requires_grad or topk_weights.requires_grad
+                                    or (out is not None and out.requires_grad)):
         raise RuntimeError("tritonblas.moe_mlp(): inference only, but one of the arguments requires grad.")
     if out is None:
-        out = torch.empty(tokens, hidden, dtype=x.dtype, device=x.device)
+        out = torch.empty(tokens, hidden, dtype=dtype, device=device)
     else:
-        require(out.shape == (tokens, hidden) and out.dtype == x.dtype, f"out must be {(tokens, hidden)} of {x.dtype}")
-        require(out.stride(1) == 1 and (tokens <= 1 or out.stride(0) >= hidden), "out must have contiguous, non-overlapping rows")
+        if out.shape != (tokens, hidden) or out.dtype is not dtype:
+            refuse(f"out must be {(tokens, hidden)} of {dtype}")
+        if out.device != device:
+            refuse_devices(x, out)
+        if out.stride(1) != 1 or (tokens > 1 and out.stride(0) < hidden):
+            refuse("out must have contiguous, non-overlapping rows")
     if tokens == 0:
         return out
-    x, w1, w2 = (t if rows16(t) else t.clone(memory_format=torch.contiguous_format) for t in (x, w1, w2))
+    if not rows16(x):
+        x = x.clone(memory_format=torch.contiguous_format)
+    if not rows16(w1):
+        w1 = w1.clone(memory_format=torch.contiguous_format)
+    if not rows16(w2):
+        w2 = w2.clone(memory_format=torch.contiguous_format)
     ids, weights = topk_ids.contiguous(), topk_weights.to(torch.float32).contiguous()
     need = _lib.lib.tb_moe_mlp_workspace_bytes(tokens, topk, experts, hidden, ffn)
     # per call, from torch's allocator: calls on other streams and captured graphs never share it
-    ws = torch.empty(need, dtype=torch.uint8, device=x.device)
-    args = _lib.MoeMlpArgs(tokens, topk, experts, hidden, ffn, _lib.DTYPE_CODE[x.dtype], x.data_ptr(), x.stride(0),
-                           w1.data_ptr(), w1.stride(0), w1.stride(1), w2.data_ptr(), w2.stride(0), w2.stride(1),
+    ws = torch.empty(need, dtype=torch.uint8, device=device)
+    w1_strides, w2_strides = w1.stride(), w2.stride()
+    args = _lib.MoeMlpArgs(tokens, topk, experts, hidden, ffn, _lib.DTYPE_CODE[dtype], x.data_ptr(), x.stride(0),
+                           w1.data_ptr(), w1_strides[0], w1_strides[1], w2.data_ptr(), w2_strides[0], w2_strides[1],
                            ids.data_ptr(), weights.data_ptr(), out.data_ptr(), out.stride(0), ws.data_ptr(), need,
-                           int(ids.dtype == torch.int64), 0)
-    with on_device(x.device):
-        rc = _lib.lib.tb_moe_mlp(ctypes.byref(args), _lib.current_stream_ptr(x.device))
+                           int(ids.dtype is torch.int64), 0)
+    with on_device(device):
+        rc = _lib.lib.tb_moe_mlp(ctypes.byref(args), _lib.current_stream_ptr(device))
     _lib.check(rc, "tb_moe_mlp")
     return out
