@@ -7,13 +7,18 @@
 //           softmax:                p_i (g~_i - sum_S g p), g~ = g on S, 0 elsewhere
 //           sigmoid:                g_j p_j (1 - p_j) on S;  renormalised: g_j replaced by (g_j - sum_S g w) / sum_S p
 //
-// One warp per row, the whole row in registers: one pass over the logits in either direction, statistics in fp32. The
-// choice is made on the logits themselves (softmax and sigmoid are increasing), so it does not depend on how an exponential
-// rounds. A round of the selection is one 32-bit warp maximum over order-preserving keys and one warp minimum over the
-// indices that hold it; only the lane that lost its best entry looks through its registers again.
+// A row is held in the registers of 4 to 32 lanes, eight logits each (16 or 32 above 256 experts), so a warp works on up to
+// eight rows at once; one pass over the logits in either direction, statistics in fp32. The choice is made on the logits
+// themselves (softmax and sigmoid are increasing), so it does not depend on how an exponential rounds: every logit becomes an
+// integer that orders like it, with the complement of its index below (16-bit logits leave 13 bits of a 32-bit word for that,
+// fp32 ones take 64 bits), so a maximum is the next choice and ties go to the lowest index by themselves. Every lane sorts its
+// eight keys once; a round is a maximum over the lanes' first keys and a shift in the lane that held it.
+// What bounds it is the number of instructions per row, then the latency of a launch: see the figures at route_kernel.
 // No reference counterpart (the reference has no MoE path).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
+
+#include <type_traits>
 
 #include "common_host.h"
 #include "ptx.cuh"
@@ -26,7 +31,7 @@ namespace {
 
 constexpr int kRouteWarps = 8;
 constexpr int kRouteMaxExperts = 1024;  // what the dispatch plan kernels take
-constexpr int kRouteMaxTopk = 32;       // one lane holds one choice
+constexpr int kRouteMaxTopk = 32;
 constexpr unsigned kFull = 0xffffffffu;
 constexpr float kNegInf = -__builtin_huge_valf();
 
@@ -38,28 +43,28 @@ __device__ __forceinline__ void from_float(float v, __half& o) { o = __float2hal
 __device__ __forceinline__ void from_float(float v, __nv_bfloat16& o) { o = __float2bfloat16_rn(v); }
 
 template <typename T, int VEC>
-struct alignas(sizeof(T) * VEC) Pack {
+struct alignas(sizeof(T) * VEC > 16 ? 16 : sizeof(T) * VEC) Pack {
   T v[VEC];
 };
 
-// Element i of a lane's registers is expert ((i / VEC) * 32 + lane) * VEC + i % VEC: every load and store instruction of a
-// warp covers one contiguous run.
-template <int VEC>
-__device__ __forceinline__ int expert_index(int i, int lane) {
-  return ((i / VEC) * 32 + lane) * VEC + (i % VEC);
+// Element i of a lane is expert ((i / VEC) * LANES + sub) * VEC + i % VEC, sub being the lane's place among the row's LANES.
+template <int LANES, int VEC>
+__device__ __forceinline__ int expert_index(int i, int sub) {
+  return ((i / VEC) * LANES + sub) * VEC + (i % VEC);
 }
 
-template <typename T, int VPT, int VEC>
-__device__ __forceinline__ void load_row(const T* __restrict__ row, int experts, int lane, float (&l)[VPT]) {
+// NaN never compares greater: it becomes -inf here, as do the places behind the last expert.
+template <typename T, int LANES, int VPT, int VEC>
+__device__ __forceinline__ void load_row(const T* __restrict__ row, int experts, int sub, bool in_range, float (&l)[VPT]) {
 #pragma unroll
   for (int i = 0; i < VPT; i += VEC) {
-    const int e = expert_index<VEC>(i, lane);
-    if (e < experts) {  // VEC divides `experts` when VEC > 1, so a run lies inside the row or outside it as a whole
+    const int e = expert_index<LANES, VEC>(i, sub);
+    if (in_range && e < experts) {  // VEC divides `experts` when VEC > 1, so a run lies inside the row or outside it as a whole
       const Pack<T, VEC> p = *reinterpret_cast<const Pack<T, VEC>*>(row + e);
 #pragma unroll
       for (int j = 0; j < VEC; ++j) {
         const float f = to_float(p.v[j]);
-        l[i + j] = f > kNegInf ? f : kNegInf;  // NaN never compares greater: it counts as -inf
+        l[i + j] = f > kNegInf ? f : kNegInf;
       }
     } else {
 #pragma unroll
@@ -68,182 +73,263 @@ __device__ __forceinline__ void load_row(const T* __restrict__ row, int experts,
   }
 }
 
-// Monotonic map of floats (no NaN) to unsigned: -inf -> 0x007fffff, so 0 marks an entry that is not there any more.
-// -0 and +0 are equal as numbers and must tie, so both take +0's key.
-__device__ __forceinline__ unsigned order_key(float f) {
-  const unsigned u = __float_as_uint(f == 0.0f ? 0.0f : f);
-  return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+// Keys: order of the value first, then the complement of the index; 0 is "nothing" (-inf, NaN, already taken).
+constexpr unsigned kIndexMask = 0x1fffu;
+__device__ __forceinline__ unsigned order_bits(float f) {  // increasing in f; -0 counts as +0
+  const int s = __float_as_int(f + 0.0f);
+  return static_cast<unsigned>(s ^ ((s >> 31) | 0x80000000));
 }
-constexpr unsigned kKeyNegInf = 0x007fffffu;
+__device__ __forceinline__ float order_value(unsigned o) {
+  return __uint_as_float((o & 0x80000000u) ? (o ^ 0x80000000u) : ~o);
+}
+template <typename T>
+struct Key {  // 16-bit logits: their fp32 images have at least 13 zero bits at the end
+  using type = unsigned;
+  static __device__ __forceinline__ type make(float f, int e) {
+    return f > kNegInf ? ((order_bits(f) & ~kIndexMask) | (kIndexMask - static_cast<unsigned>(e))) : 0u;
+  }
+  static __device__ __forceinline__ int index(type k) { return static_cast<int>(kIndexMask - (k & kIndexMask)); }
+  static __device__ __forceinline__ float value(type k) {
+    const unsigned o = k & ~kIndexMask;
+    return order_value((o & 0x80000000u) ? o : (o | kIndexMask));
+  }
+};
+template <>
+struct Key<float> {
+  using type = unsigned long long;
+  static __device__ __forceinline__ type make(float f, int e) {
+    return f > kNegInf ? ((static_cast<type>(order_bits(f)) << 32) | (kIndexMask - static_cast<unsigned>(e))) : 0ull;
+  }
+  static __device__ __forceinline__ int index(type k) { return static_cast<int>(kIndexMask - (static_cast<unsigned>(k) & kIndexMask)); }
+  static __device__ __forceinline__ float value(type k) { return order_value(static_cast<unsigned>(k >> 32)); }
+};
 
-__device__ __forceinline__ float warp_sum(float v) {
+template <int LANES>
+__device__ __forceinline__ unsigned lanes_max(unsigned v) {
+  if constexpr (LANES == 32) {
+    return __reduce_max_sync(kFull, v);
+  } else {
 #pragma unroll
-  for (int s = 16; s > 0; s >>= 1) v += __shfl_xor_sync(kFull, v, s);
+    for (int s = LANES / 2; s > 0; s >>= 1) v = max(v, __shfl_xor_sync(kFull, v, s));
+    return v;
+  }
+}
+template <int LANES>
+__device__ __forceinline__ unsigned long long lanes_max(unsigned long long v) {
+  if constexpr (LANES == 32) {
+    const unsigned hi = __reduce_max_sync(kFull, static_cast<unsigned>(v >> 32));
+    const unsigned lo = __reduce_max_sync(kFull, static_cast<unsigned>(v >> 32) == hi ? static_cast<unsigned>(v) : 0u);
+    return (static_cast<unsigned long long>(hi) << 32) | lo;
+  } else {
+#pragma unroll
+    for (int s = LANES / 2; s > 0; s >>= 1) v = max(v, __shfl_xor_sync(kFull, v, s));
+    return v;
+  }
+}
+template <int LANES>
+__device__ __forceinline__ float lanes_sum(float v) {
+#pragma unroll
+  for (int s = LANES / 2; s > 0; s >>= 1) v += __shfl_xor_sync(kFull, v, s);
   return v;
 }
-__device__ __forceinline__ float warp_max(float v) {
-#pragma unroll
-  for (int s = 16; s > 0; s >>= 1) v = fmaxf(v, __shfl_xor_sync(kFull, v, s));
-  return v;
+
+// Eight keys in descending order: odd-even merge sort, 19 exchanges.
+template <typename K>
+__device__ __forceinline__ void sort8(K (&a)[8]) {
+  auto exchange = [&](int i, int j) {
+    const K hi = max(a[i], a[j]), lo = min(a[i], a[j]);
+    a[i] = hi;
+    a[j] = lo;
+  };
+  exchange(0, 1); exchange(2, 3); exchange(4, 5); exchange(6, 7);
+  exchange(0, 2); exchange(1, 3); exchange(4, 6); exchange(5, 7);
+  exchange(1, 2); exchange(5, 6);
+  exchange(0, 4); exchange(1, 5); exchange(2, 6); exchange(3, 7);
+  exchange(2, 4); exchange(3, 5);
+  exchange(1, 2); exchange(3, 4); exchange(5, 6);
 }
 
-template <typename T, int VPT, int VEC>
+template <typename T, int LANES, int VPT, int VEC>
 __global__ void __launch_bounds__(kRouteWarps * 32) route_kernel(const T* __restrict__ logits, long long stride, long long tokens,
                                                                  int experts, int topk, int sigmoid, int renorm,
                                                                  float* __restrict__ weights, int* __restrict__ ids) {
-  const int lane = threadIdx.x & 31;
-  const long long t = static_cast<long long>(blockIdx.x) * kRouteWarps + (threadIdx.x >> 5);
+  using K = typename Key<T>::type;
+  constexpr int kRows = 32 / LANES;  // rows per warp
+  __shared__ K s_choice[kRouteWarps][kRows][kRouteMaxTopk];
+  __shared__ float s_score[kRouteWarps][kRows][kRouteMaxTopk];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = lane % LANES, group = lane / LANES;
+  const long long t = (static_cast<long long>(blockIdx.x) * kRouteWarps + warp) * kRows + group;
+  const bool live = t < tokens;  // lanes without a row go along with empty ones
   griddep_launch_dependents();
   griddep_wait();
-  if (t >= tokens) return;
   float l[VPT];
-  load_row<T, VPT, VEC>(logits + t * stride, experts, lane, l);
-
-  unsigned gone = 0;  // bit i: element i has been chosen
-  unsigned best = 0;
-  int best_e = 0;
-  auto rescan = [&]() {
-    best = 0;
-    best_e = 0x7fffffff;
+  load_row<T, LANES, VPT, VEC>(logits + (live ? t * stride : 0), experts, sub, live, l);
+  K a[VPT];
 #pragma unroll
-    for (int i = 0; i < VPT; ++i) {  // ascending experts per lane: a tie keeps the first
-      const unsigned k = ((gone >> i) & 1u) ? 0u : order_key(l[i]);
-      if (k > best) {
-        best = k;
-        best_e = expert_index<VEC>(i, lane);
+  for (int i = 0; i < VPT; ++i) a[i] = Key<T>::make(l[i], expert_index<LANES, VEC>(i, sub));
+  K* choice = s_choice[warp][group];
+  float* score = s_score[warp][group];
+  if constexpr (VPT == 8) {
+    sort8(a);
+    for (int j = 0; j < topk; ++j) {
+      const K best = lanes_max<LANES>(a[0]);
+      if (sub == 0) choice[j] = best;
+      if (a[0] == best) {
+#pragma unroll
+        for (int i = 0; i + 1 < VPT; ++i) a[i] = a[i + 1];
+        a[VPT - 1] = 0;
       }
     }
-  };
-  rescan();
-  float mine = kNegInf, top = 0.0f;
-  int mine_e = -1;
-  for (int j = 0; j < topk; ++j) {
-    const unsigned k = __reduce_max_sync(kFull, best);
-    if (k <= kKeyNegInf) break;  // only -inf left: the other choices stay empty
-    const int e = static_cast<int>(__reduce_min_sync(kFull, best == k ? static_cast<unsigned>(best_e) : 0xffffffffu));
-    const float v = __uint_as_float((k & 0x80000000u) ? (k & 0x7fffffffu) : ~k);
-    if (j == 0) top = v;
-    if (lane == j) {
-      mine = v;
-      mine_e = e;
-    }
-    if (best == k && best_e == e) {
+  } else {  // more keys per lane than rounds, mostly: look for the lane's next key when its first one is taken
+    K first = a[0];
 #pragma unroll
-      for (int i = 0; i < VPT; ++i)
-        if (expert_index<VEC>(i, lane) == e) gone |= 1u << i;
-      rescan();
+    for (int i = 1; i < VPT; ++i) first = max(first, a[i]);
+    for (int j = 0; j < topk; ++j) {
+      const K best = lanes_max<LANES>(first);
+      if (sub == 0) choice[j] = best;
+      if (first == best) {
+        first = 0;
+#pragma unroll
+        for (int i = 0; i < VPT; ++i) {
+          if (a[i] == best) a[i] = 0;
+          first = max(first, a[i]);
+        }
+      }
     }
   }
-
-  float w;
-  if (sigmoid) {
-    w = 1.0f / (1.0f + expf(-mine));  // -inf gives 0
-  } else {
-    w = expf(mine - top);
-  }
-  if (mine_e < 0) w = 0.0f;
-  if (renorm) {
-    const float s = warp_sum(w);
-    w = s > 0.0f || s != s ? w / s : 0.0f;
-  } else if (!sigmoid) {
+  __syncwarp();
+  const float top = choice[0] != 0 ? Key<T>::value(choice[0]) : 0.0f;
+  float sum = 0.0f;
+  for (int j = sub; j < topk; j += LANES) {
+    const K k = choice[j];
     float s = 0.0f;
-#pragma unroll
-    for (int i = 0; i < VPT; ++i) s += expf(l[i] - top);
-    s = warp_sum(s);
-    w = mine_e < 0 ? 0.0f : w / s;
+    if (k != 0) s = sigmoid ? 1.0f / (1.0f + expf(-Key<T>::value(k))) : expf(Key<T>::value(k) - top);
+    score[j] = s;
+    sum += s;
   }
-  if (lane < topk) {
-    weights[t * topk + lane] = w;
-    ids[t * topk + lane] = mine_e;
+  if (renorm) {
+    sum = lanes_sum<LANES>(sum);
+    if (sum == 0.0f) sum = 1.0f;  // sigmoid scores that all underflow, or nothing to choose
+  } else if (sigmoid) {
+    sum = 1.0f;
+  } else {
+    sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) sum += __expf(l[i] - top);  // 2 units in the last place more: terms below the first, which is 1
+    sum = lanes_sum<LANES>(sum);
+  }
+  if (live) {
+    for (int j = sub; j < topk; j += LANES) {
+      const K k = choice[j];
+      weights[t * topk + j] = k != 0 ? score[j] / sum : 0.0f;
+      ids[t * topk + j] = k != 0 ? Key<T>::index(k) : -1;
+    }
   }
 }
 
-// Backward: `weights` and `ids` are what the forward pass returned, `grad` the gradient of the weights. The dense modes
-// (softmax without renormalisation) read the logits again and form max and sum anew; the others only need the choice.
-template <typename T, int VPT, int VEC>
+// Backward: `weights` and `ids` are what the forward pass returned, `grad` the gradient of the weights. The dense mode (softmax
+// without renormalisation) reads the logits again: the first choice holds the row's maximum and, in its weight, the reciprocal
+// of the sum, so p_i = exp(l_i - l_first) w_first needs no reduction. The chosen places meet the dense part in shared memory.
+template <typename T, int LANES, int VPT, int VEC>
 __global__ void __launch_bounds__(kRouteWarps * 32)
 route_bwd_kernel(const T* __restrict__ logits, long long stride, long long tokens, int experts, int topk, int sigmoid, int renorm,
                  const float* __restrict__ weights, const int* __restrict__ ids, const float* __restrict__ grad,
                  T* __restrict__ dlogits) {
-  const int lane = threadIdx.x & 31;
-  const long long t = static_cast<long long>(blockIdx.x) * kRouteWarps + (threadIdx.x >> 5);
+  constexpr int kRows = 32 / LANES;
+  __shared__ alignas(16) float s_row[kRouteWarps][kRows][LANES * VPT];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = lane % LANES, group = lane / LANES;
+  const long long t = (static_cast<long long>(blockIdx.x) * kRouteWarps + warp) * kRows + group;
+  const bool live = t < tokens;
+  const bool dense = !sigmoid && !renorm;
   griddep_launch_dependents();
   griddep_wait();
-  if (t >= tokens) return;
-  const T* row = logits + t * stride;
-  float g = 0.0f, w = 0.0f;
-  int e = -1;
-  if (lane < topk) {
-    e = ids[t * topk + lane];
-    if (e >= experts) e = -1;
-    if (e >= 0) {
-      g = grad[t * topk + lane];
-      w = weights[t * topk + lane];
-    }
-  }
-  float d;  // gradient of this lane's chosen logit (softmax without renormalisation: before the dense part)
+  const T* row = logits + (live ? t * stride : 0);
+  const long long c0 = live ? t * topk : 0;
   float p[VPT];
-  float gp = 0.0f;
-  if (sigmoid) {
-    float s = w;
-    if (renorm) {
-      s = e >= 0 ? 1.0f / (1.0f + expf(-to_float(row[e]))) : 0.0f;
-      const float total = warp_sum(s), gw = warp_sum(g * w);
-      g = total > 0.0f ? (g - gw) / total : 0.0f;
+  if (dense) load_row<T, LANES, VPT, VEC>(row, experts, sub, live, p);
+  float* buf = s_row[warp][group];
+#pragma unroll
+  for (int i = 0; i < VPT; i += 4) *reinterpret_cast<float4*>(buf + (i / 4 * LANES + sub) * 4) = make_float4(0.f, 0.f, 0.f, 0.f);
+  // one of the choices: id (-1: none), gradient and weight; most rows have at most one per lane, which is read once
+  struct Choice {
+    int e;
+    float g, w;
+  };
+  auto chosen = [&](int j) {
+    Choice c = {-1, 0.0f, 0.0f};
+    if (live && j < topk) c.e = ids[c0 + j];
+    if (c.e >= experts) c.e = -1;
+    if (c.e >= 0) {
+      c.g = grad[c0 + j];
+      c.w = weights[c0 + j];
     }
-    d = e >= 0 ? g * s * (1.0f - s) : 0.0f;
-  } else if (renorm) {
-    d = w * (g - warp_sum(g * w));
-  } else {
-    load_row<T, VPT, VEC>(row, experts, lane, p);
-    float top = kNegInf, s = 0.0f;
-#pragma unroll
-    for (int i = 0; i < VPT; ++i) top = fmaxf(top, p[i]);
-    top = warp_max(top);
-    if (top == kNegInf) top = 0.0f;  // a row with nothing to choose: every p is 0
-#pragma unroll
-    for (int i = 0; i < VPT; ++i) {
-      p[i] = expf(p[i] - top);
-      s += p[i];
-    }
-    s = warp_sum(s);
-    const float inv = s > 0.0f ? 1.0f / s : 0.0f;
-#pragma unroll
-    for (int i = 0; i < VPT; ++i) p[i] *= inv;
-    d = g * w;
-    gp = warp_sum(d);
+    return c;
+  };
+  auto sigmoid_of = [&](int e) { return 1.0f / (1.0f + expf(-to_float(row[e]))); };
+  const Choice mine = chosen(sub);
+  float dot = 0.0f, total = 0.0f;  // sum of g w, and of the scores where they are needed
+  for (int j = sub; j < topk; j += LANES) {
+    const Choice c = j == sub ? mine : chosen(j);
+    dot += c.g * c.w;
+    if (sigmoid && renorm && c.e >= 0) total += sigmoid_of(c.e);
   }
-  const bool dense = !sigmoid && !renorm;
-  float out[VPT];
-#pragma unroll
-  for (int i = 0; i < VPT; ++i) out[i] = dense ? -p[i] * gp : 0.0f;
-  for (int j = 0; j < topk; ++j) {
-    const int ej = __shfl_sync(kFull, e, j);
-    const float dj = __shfl_sync(kFull, d, j);
-    if (ej >= 0 && (ej / VEC) % 32 == lane) {
-#pragma unroll
-      for (int i = 0; i < VPT; ++i)
-        if (expert_index<VEC>(i, lane) == ej) out[i] += dj;
+  dot = lanes_sum<LANES>(dot);
+  if (sigmoid && renorm) total = lanes_sum<LANES>(total);
+  __syncwarp();
+  for (int j = sub; j < topk; j += LANES) {
+    const Choice c = j == sub ? mine : chosen(j);
+    if (c.e < 0) continue;
+    float d;
+    if (sigmoid) {
+      float s = c.w, g = c.g;
+      if (renorm) {
+        s = sigmoid_of(c.e);
+        g = total > 0.0f ? (g - dot) / total : 0.0f;
+      }
+      d = g * s * (1.0f - s);
+    } else {
+      d = renorm ? c.w * (c.g - dot) : c.g * c.w;
     }
+    buf[c.e] = d;
   }
+  float first = 0.0f, inv = 0.0f;
+  if (dense) {
+    const int e = __shfl_sync(kFull, mine.e, group * LANES);
+    inv = __shfl_sync(kFull, mine.w, group * LANES) * dot;  // nothing chosen: 0
+    first = e >= 0 ? to_float(row[e]) : 0.0f;
+  }
+  __syncwarp();
+  if (!live) return;
   T* drow = dlogits + t * static_cast<long long>(experts);
 #pragma unroll
   for (int i = 0; i < VPT; i += VEC) {
-    const int c = expert_index<VEC>(i, lane);
+    const int c = expert_index<LANES, VEC>(i, sub);
     if (c < experts) {
       Pack<T, VEC> o;
+      float v[VEC];
+      if constexpr (VEC == 8) {
+        const float4 lo = *reinterpret_cast<const float4*>(buf + c), hi = *reinterpret_cast<const float4*>(buf + c + 4);
+        v[0] = lo.x; v[1] = lo.y; v[2] = lo.z; v[3] = lo.w;
+        v[4] = hi.x; v[5] = hi.y; v[6] = hi.z; v[7] = hi.w;
+      } else {
+        v[0] = buf[c];
+      }
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) from_float(out[i + j], o.v[j]);
+      for (int j = 0; j < VEC; ++j) {
+        float d = v[j];
+        if (dense) d -= __expf(p[i + j] - first) * inv;
+        from_float(d, o.v[j]);
+      }
       *reinterpret_cast<Pack<T, VEC>*>(drow + c) = o;
     }
   }
 }
 
-// One row per warp, programmatic dependent launch as the GEMM kernels use it.
+// Programmatic dependent launch as the GEMM kernels use it.
 template <typename K, typename... Args>
-int launch_rows(K kernel, long long rows, cudaStream_t st, const char* what, Args... args) {
+int launch_rows(K kernel, long long blocks, cudaStream_t st, const char* what, Args... args) {
   cudaLaunchConfig_t lc = {};
-  lc.gridDim = dim3(static_cast<unsigned>((rows + kRouteWarps - 1) / kRouteWarps), 1, 1);
+  lc.gridDim = dim3(static_cast<unsigned>(blocks), 1, 1);
   lc.blockDim = dim3(kRouteWarps * 32, 1, 1);
   lc.stream = st;
   cudaLaunchAttribute attr[1];
@@ -271,37 +357,36 @@ struct RouteCall {
   cudaStream_t stream;
 };
 
-template <typename T, int VPT, int VEC>
+template <typename T, int LANES, int VPT, int VEC>
 int route_launch(const RouteCall& c) {
+  constexpr int kPerBlock = kRouteWarps * (32 / LANES);
+  const long long blocks = (c.tokens + kPerBlock - 1) / kPerBlock;
   if (c.grad == nullptr)
-    return launch_rows(route_kernel<T, VPT, VEC>, c.tokens, c.stream, "route_kernel launch", static_cast<const T*>(c.logits),
+    return launch_rows(route_kernel<T, LANES, VPT, VEC>, blocks, c.stream, "route_kernel launch", static_cast<const T*>(c.logits),
                        c.stride, c.tokens, c.experts, c.topk, c.sigmoid, c.renorm, c.weights, c.ids);
-  return launch_rows(route_bwd_kernel<T, VPT, VEC>, c.tokens, c.stream, "route_bwd_kernel launch",
+  return launch_rows(route_bwd_kernel<T, LANES, VPT, VEC>, blocks, c.stream, "route_bwd_kernel launch",
                      static_cast<const T*>(c.logits), c.stride, c.tokens, c.experts, c.topk, c.sigmoid, c.renorm,
                      static_cast<const float*>(c.weights), static_cast<const int*>(c.ids), c.grad, static_cast<T*>(c.dlogits));
 }
 
-// Registers per lane: the smallest power of two that covers the row. Loads are as wide as rows allow: up to 16 bytes where
-// every row starts on that boundary and holds whole runs, single elements otherwise.
-template <typename T, int VPT>
+// Loads are eight elements wide where every row starts on a 16-byte boundary and holds whole runs of eight, single elements
+// otherwise.
+template <typename T, int LANES, int VPT>
 int route_vec(const RouteCall& c) {
-  constexpr int kWide = VPT < static_cast<int>(16 / sizeof(T)) ? VPT : static_cast<int>(16 / sizeof(T));
-  if constexpr (kWide > 1) {
-    const uintptr_t bits = reinterpret_cast<uintptr_t>(c.logits) | reinterpret_cast<uintptr_t>(c.dlogits) |
-                           (c.tokens > 1 ? static_cast<uintptr_t>(c.stride) * sizeof(T) : 0);
-    if (bits % (kWide * sizeof(T)) == 0 && c.experts % kWide == 0) return route_launch<T, VPT, kWide>(c);
-  }
-  return route_launch<T, VPT, 1>(c);
+  const uintptr_t bits = reinterpret_cast<uintptr_t>(c.logits) | reinterpret_cast<uintptr_t>(c.dlogits) |
+                         (c.tokens > 1 ? static_cast<uintptr_t>(c.stride) * sizeof(T) : 0);
+  if (bits % 16 == 0 && c.experts % 8 == 0) return route_launch<T, LANES, VPT, 8>(c);
+  return route_launch<T, LANES, VPT, 1>(c);
 }
 
 template <typename T>
 int route_type(const RouteCall& c) {
-  if (c.experts <= 32) return route_vec<T, 1>(c);
-  if (c.experts <= 64) return route_vec<T, 2>(c);
-  if (c.experts <= 128) return route_vec<T, 4>(c);
-  if (c.experts <= 256) return route_vec<T, 8>(c);
-  if (c.experts <= 512) return route_vec<T, 16>(c);
-  return route_vec<T, 32>(c);
+  if (c.experts <= 32) return route_vec<T, 4, 8>(c);
+  if (c.experts <= 64) return route_vec<T, 8, 8>(c);
+  if (c.experts <= 128) return route_vec<T, 16, 8>(c);
+  if (c.experts <= 256) return route_vec<T, 32, 8>(c);
+  if (c.experts <= 512) return route_vec<T, 32, 16>(c);
+  return route_vec<T, 32, 32>(c);
 }
 
 int route_call(const RouteCall& c, int dtype) {
