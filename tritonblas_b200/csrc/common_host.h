@@ -43,6 +43,16 @@ struct LowRank {
 int low_rank_config(const tb_gemm_args& a, tb_config* cfg, int* streamk);
 int gemm_low_rank(const tb_gemm_args& a, const tb_config& cfg, const LowRank& lr, cudaStream_t stream);
 
+// Decode form of the same product (lora_decode.cu), up to 64 rows and K-contiguous weights: how it is cut, and its launch.
+// `parts` holds part_bytes, `arrived` 4 * dealt_tiles zeroed words.
+struct LoraDecodeShape {
+  int tile_m, v_rows_tile, grid, full_tiles, dealt_tiles;
+  long long part_bytes;
+};
+LoraDecodeShape lora_decode_shape(int tokens, int n, int grid);
+int lora_decode(const tb_lora_args& a, const LoraDecodeShape& s, const LowRank& lr, void* parts, void* arrived, int device,
+                int smem_optin, int* status, cudaStream_t stream);
+
 // The current device: its number, SMs, shared memory a block may opt in to, and failure word.
 int current_device_limits(int* device, int* num_sms, int* smem_optin, int** status);
 

@@ -514,13 +514,15 @@ int project_tc(const tb_lora_args& a, ProjectParams& p, int runs, int stripes, i
 
 // How a call is cut and where its pieces stand in the workspace.
 struct LoraPlan {
-  tb_config cfg;
+  bool decode;
+  LoraDecodeShape shape;  // decode
+  tb_config cfg;          // otherwise
   int streamk;
   int tile_rows, tiles, max_slots, v_cols, pack;
   long long v_offset, v_rows, list_offset, gemm_offset, gemm_bytes, bytes;
 };
 
-int lora_plan(const tb_lora_args& a, tb_gemm_args* g, LoraPlan* l) {
+int lora_plan(const tb_lora_args& a, int num_sms, tb_gemm_args* g, LoraPlan* l) {
   *g = {};
   g->m = a.m; g->n = a.n; g->k = a.k;
   g->a_dtype = g->b_dtype = g->c_dtype = a.dtype;
@@ -529,12 +531,20 @@ int lora_plan(const tb_lora_args& a, tb_gemm_args* g, LoraPlan* l) {
   g->c = a.out; g->c_stride_m = a.out_stride_m; g->c_stride_n = a.out_stride_n;
   g->bias = a.bias; g->bias_stride = a.bias_stride; g->bias_dtype = a.bias_dtype;
   g->wait_timeout_ms = a.wait_timeout_ms;
-  const int rc = low_rank_config(*g, &l->cfg, &l->streamk);
-  if (rc != TB_OK) return rc;
-  // A decode batch's projection runs beside the GEMM: leave shared memory for one of its blocks on every SM.
-  const int pair = l->cfg.cta_pair == 2 ? 2 : 1;
-  while (a.m <= 64 && l->cfg.stages > 3 && smem_bytes_for(l->cfg.block_n, pair, l->cfg.stages) > 200 * 1024) --l->cfg.stages;
-  l->tile_rows = l->cfg.swap_ab ? l->cfg.block_n : 128 * pair;
+  // decode batches on K-contiguous weights have a kernel of their own
+  l->decode = a.m <= 64 && a.w_stride_k == 1;
+  if (l->decode) {
+    l->shape = lora_decode_shape(a.m, a.n, num_sms);
+    l->streamk = 0;
+    l->tile_rows = l->shape.v_rows_tile;
+  } else {
+    const int rc = low_rank_config(*g, &l->cfg, &l->streamk);
+    if (rc != TB_OK) return rc;
+    const int pair = l->cfg.cta_pair == 2 ? 2 : 1;
+    // A decode batch's projection runs beside the GEMM: leave shared memory for one of its blocks on every SM.
+    while (a.m <= 64 && l->cfg.stages > 3 && smem_bytes_for(l->cfg.block_n, pair, l->cfg.stages) > 200 * 1024) --l->cfg.stages;
+    l->tile_rows = l->cfg.swap_ab ? l->cfg.block_n : 128 * pair;
+  }
   l->tiles = (a.m + l->tile_rows - 1) / l->tile_rows;
   l->max_slots = l->tile_rows < a.num_adapters ? l->tile_rows : a.num_adapters;
   // small ranks share a stage of the GEMM: see GemmParams::lr_pack
@@ -543,7 +553,8 @@ int lora_plan(const tb_lora_args& a, tb_gemm_args* g, LoraPlan* l) {
   l->v_rows = static_cast<long long>(l->tiles) * l->max_slots * l->tile_rows;
   auto up = [](long long v) { return (v + 255) & ~255ll; };
   l->gemm_offset = 0;
-  l->gemm_bytes = l->streamk ? up(tb_gemm_workspace_bytes(&l->cfg, 0)) : 0;
+  // flags or counters (cleared by the projection) at the front, then partial tiles
+  l->gemm_bytes = l->decode ? kFlagBytes + up(l->shape.part_bytes) : (l->streamk ? up(tb_gemm_workspace_bytes(&l->cfg, 0)) : 0);
   l->list_offset = l->gemm_bytes;
   l->v_offset = l->list_offset + up(4ll * l->tiles * (1 + l->max_slots));
   l->bytes = l->v_offset + up(l->v_rows * l->v_cols * 2);
@@ -572,15 +583,15 @@ int lora_impl(const tb_lora_args& a, cudaStream_t stream) {
   if (addresses % 16 || strides % 8 || reinterpret_cast<uintptr_t>(a.adapter_ids) % (a.ids_are_int64 ? 8 : 4) ||
       reinterpret_cast<uintptr_t>(a.scales) % 4)
     return TB_ERR_ALIGNMENT;
-  tb_gemm_args g;
-  LoraPlan l;
-  int rc = lora_plan(a, &g, &l);
-  if (rc != TB_OK) return rc;
-  if (a.workspace == nullptr || a.workspace_bytes < l.bytes) return TB_ERR_WORKSPACE;
-  if (reinterpret_cast<uintptr_t>(a.workspace) % 256) return TB_ERR_ALIGNMENT;
   int device = 0, num_sms = 0, smem_optin = 0;
   int* status = nullptr;
-  if ((rc = current_device_limits(&device, &num_sms, &smem_optin, &status)) != TB_OK) return rc;
+  int rc = current_device_limits(&device, &num_sms, &smem_optin, &status);
+  if (rc != TB_OK) return rc;
+  tb_gemm_args g;
+  LoraPlan l;
+  if ((rc = lora_plan(a, num_sms, &g, &l)) != TB_OK) return rc;
+  if (a.workspace == nullptr || a.workspace_bytes < l.bytes) return TB_ERR_WORKSPACE;
+  if (reinterpret_cast<uintptr_t>(a.workspace) % 256) return TB_ERR_ALIGNMENT;
   char* ws = static_cast<char*>(a.workspace);
 
   ProjectParams p = {};
@@ -593,7 +604,7 @@ int lora_impl(const tb_lora_args& a, cudaStream_t stream) {
   p.v = ws + l.v_offset;
   p.list = reinterpret_cast<int*>(ws + l.list_offset);
   p.flags = reinterpret_cast<unsigned*>(ws + l.gemm_offset);
-  p.flag_words = l.streamk ? static_cast<int>(kFlagBytes / 4) : 0;
+  p.flag_words = l.decode ? 4 * l.shape.dealt_tiles : (l.streamk ? static_cast<int>(kFlagBytes / 4) : 0);
   p.status = status;
   p.timeout_ns = a.wait_timeout_ms > 0 ? static_cast<unsigned long long>(a.wait_timeout_ms) * 1000000ull : 2000000000ull;
   // Runs cover whole tiles: the rows behind the last token are zeros in every block. A decode batch has up to one adapter per
@@ -636,6 +647,7 @@ int lora_impl(const tb_lora_args& a, cudaStream_t stream) {
   lr.n = a.n;
   lr.list = p.list;
   lr.list_stride = 1 + l.max_slots;
+  if (l.decode) return lora_decode(a, l.shape, lr, ws + l.gemm_offset + kFlagBytes, ws + l.gemm_offset, device, smem_optin, status, stream);
   return gemm_low_rank(g, l.cfg, lr, stream);
 }
 
@@ -644,9 +656,13 @@ int lora_impl(const tb_lora_args& a, cudaStream_t stream) {
 
 extern "C" int64_t tb_lora_workspace_bytes(const tb_lora_args* args) {
   if (args == nullptr || !tb::lora_sizes_ok(*args) || args->m == 0 || args->n == 0) return 0;
+  // without a usable device: the B200's SM count
+  int device = 0, num_sms = 0, smem_optin = 0;
+  int* status = nullptr;
+  if (tb::current_device_limits(&device, &num_sms, &smem_optin, &status) != TB_OK) num_sms = tb::MachineModel().num_sms;
   tb_gemm_args g;
   tb::LoraPlan l;
-  return tb::lora_plan(*args, &g, &l) == TB_OK ? l.bytes : 0;
+  return tb::lora_plan(*args, num_sms, &g, &l) == TB_OK ? l.bytes : 0;
 }
 
 extern "C" int tb_lora_gemm(const tb_lora_args* args, void* stream) {

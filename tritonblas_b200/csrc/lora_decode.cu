@@ -1,0 +1,577 @@
+// The shared projection of a decode batch (up to 64 rows) with its rows' low-rank updates: the second launch of lora.cu for
+// K-contiguous weights.
+//     out[t, n] = sum_k x[t, k] W[k, n] + bias[n] + sum over the listed adapters a of sum_r v_a[t, r] B_a[n, r]
+// v_a is what the first launch wrote: the rows' scaled rank-sized products, zero in rows of other adapters.
+//
+// Bound by reading W and the used B once. W's rows (output features) stand on the 64- or 128-row side of the tensor-core tile
+// and the tokens on its narrow side, a stage of the ring is 16 KB of weights and the tokens' share. Tiles that fill whole
+// rounds of the SMs are worked on one per CTA; the K range of the others is dealt evenly over all CTAs, so every CTA reads
+// the same number of bytes, and their parts meet in the workspace: each warp of the epilogue counts itself in for its quarter
+// of the tile, and the one that comes last adds the parts up in a fixed order. Nobody waits for another CTA.
+// The parts come first, then the dealt tiles' updates, which need the first launch to be through, then the whole tiles with
+// theirs: the sums over parts are hidden behind the whole tiles where there are any.
+//
+// Against the general GEMM with the same update, which this replaces for decode batches (us, back to back, weights out of
+// HBM): see DECODE_FIGURES.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <mutex>
+
+#include "common_host.h"
+#include "ptx.cuh"
+
+namespace tb {
+
+bool pdl_enabled();  // api.cu
+
+namespace {
+
+constexpr int kThreads = 7 * 32;  // four epilogue warps, weight loader, MMA issuer, token loader
+constexpr int kWarpWeights = 4, kWarpMma = 5, kWarpTokens = 6;
+constexpr int kMaxStages = 10;    // 160 KB of weights ahead
+constexpr int kRowBytes = 128;
+constexpr int kSlabK = 64;        // K of a slab: one 128-byte row of 16-bit elements
+// 64-row tiles take two slabs per stage: a stage always carries 16 KB of weights (see moe_mlp.cu).
+__host__ __device__ constexpr int slabs_of(int m) { return m == 64 ? 2 : 1; }
+
+struct DecodeParams {
+  int tokens, n;
+  int n1;               // MMA columns: tokens rounded up to 8 (64-row tiles) or 16
+  int v_rows_tile;      // rows of a v block: tokens rounded up to 16
+  int act_bytes;        // one slab of tokens
+  int stages, stage_bytes;
+  int acc_stride, tmem_cols;
+  int nkb;              // stages per tile
+  int full_tiles, dealt_tiles;
+  // low-rank update
+  const int* list;      // number of adapters, then their indices
+  int max_slots, pack, kblocks, rank;
+  float* parts;         // [2 * grid + dealt_tiles][tokens][M]
+  unsigned* arrived;    // [dealt_tiles][4], cleared by the first launch
+  const void* bias;
+  long long bias_stride;
+  int bias_dtype;
+  void* out;
+  long long out_m, out_n;
+  uint32_t idesc;       // without the column count
+  int* status;
+  unsigned long long timeout_ns;
+};
+
+// The dealt tiles' stages [0, dealt_tiles * nkb) in equal runs, one per CTA.
+struct Deal {
+  int base, rem;
+  __device__ Deal(const DecodeParams& p) {
+    const int total = p.dealt_tiles * p.nkb;
+    base = total / static_cast<int>(gridDim.x);
+    rem = total - base * static_cast<int>(gridDim.x);
+  }
+  __device__ int begin(int cta) const { return cta * base + min(cta, rem); }
+  __device__ int cta_of(int stage) const {
+    const int wide = rem * (base + 1);
+    return stage < wide ? stage / (base + 1) : rem + (stage - wide) / max(base, 1);
+  }
+};
+
+// What a CTA works on, in order; every role walks the same sequence.
+struct Unit {
+  int kind;       // 0 none, 1 part of a dealt tile, 2 whole tile with its update, 3 update of a dealt tile
+  int tile, kb0, kb1;
+  int slot;       // of the part in the workspace
+};
+struct Units {
+  const DecodeParams& p;
+  int at, end, first_tile, next_full, stage;
+  __device__ Units(const DecodeParams& p_, const Deal& d) : p(p_), next_full(blockIdx.x), stage(0) {
+    at = d.begin(blockIdx.x);
+    end = d.begin(blockIdx.x + 1);
+    first_tile = p.nkb > 0 ? at / p.nkb : 0;
+  }
+  __device__ Unit next() {
+    if (at < end) {
+      const int t = at / p.nkb;
+      const Unit u = {1, p.full_tiles + t, at - t * p.nkb, min(end - t * p.nkb, p.nkb), 2 * static_cast<int>(blockIdx.x) + t - first_tile};
+      at = min(end, (t + 1) * p.nkb);
+      return u;
+    }
+    if (stage == 0) {
+      stage = 1;
+      if (static_cast<int>(blockIdx.x) < p.dealt_tiles)
+        return Unit{3, p.full_tiles + static_cast<int>(blockIdx.x), 0, 0, 2 * static_cast<int>(gridDim.x) + static_cast<int>(blockIdx.x)};
+    }
+    if (next_full < p.full_tiles) {
+      const Unit u = {2, next_full, 0, p.nkb, 0};
+      next_full += gridDim.x;
+      return u;
+    }
+    return Unit{0, 0, 0, 0, 0};
+  }
+};
+
+__device__ __noinline__ bool wait_slow(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* status,
+                                       unsigned long long timeout_ns, int code) {
+  return mbar_wait_warp(bar, parity, WaitCtx{abort_flag, status, timeout_ns}, code);
+}
+__device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity, const WaitCtx& w, int code) {
+  if (__builtin_expect(__all_sync(0xffffffffu, mbar_try_wait(bar, parity)), 1)) return true;
+  return wait_slow(bar, parity, w.abort_flag, w.status, w.timeout_ns, code);
+}
+__device__ __forceinline__ uint64_t evict_first_policy() {
+  uint64_t policy;
+  asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(policy));
+  return policy;
+}
+__device__ __forceinline__ void tma_load_2d_hint(void* smem_dst, const CUtensorMap* tmap, uint64_t* bar, int x, int y, uint64_t policy) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1, {%3, %4}], [%2], %5;" ::"r"(
+          smem_u32(smem_dst)),
+      "l"(tmap), "r"(smem_u32(bar)), "r"(x), "r"(y), "l"(policy)
+      : "memory");
+}
+__device__ __forceinline__ unsigned add_acq_rel(unsigned* p, unsigned v) {
+  unsigned old;
+  asm volatile("atom.acq_rel.gpu.global.add.u32 %0, [%1], %2;" : "=r"(old) : "l"(p), "r"(v) : "memory");
+  return old;
+}
+__device__ __forceinline__ float bias_at(const void* bias, long long i, int dtype) {
+  if (dtype == TB_DTYPE_F32) return static_cast<const float*>(bias)[i];
+  if (dtype == TB_DTYPE_BF16) return __bfloat162float(static_cast<const __nv_bfloat16*>(bias)[i]);
+  return __half2float(static_cast<const __half*>(bias)[i]);
+}
+template <typename T>
+__device__ __forceinline__ T cast16(float v);
+template <>
+__device__ __forceinline__ __nv_bfloat16 cast16<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+template <>
+__device__ __forceinline__ __half cast16<__half>(float v) { return __float2half_rn(v); }
+
+template <typename T, int M>
+__global__ void __launch_bounds__(kThreads, 1)
+lora_decode_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_x,
+                   const __grid_constant__ CUtensorMap tmap_b, const __grid_constant__ CUtensorMap tmap_v, const DecodeParams p) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  __shared__ uint64_t full_bar[kMaxStages], empty_bar[kMaxStages], tmem_full[2], tmem_empty[2];
+  __shared__ uint32_t tmem_slot;
+  __shared__ int abort_word;
+  constexpr int kSlabs = slabs_of(M);
+  constexpr uint32_t kSlabBytes = M * kRowBytes, kActBase = kSlabs * kSlabBytes;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  volatile int* abort_flag = &abort_word;
+  const WaitCtx wctx{abort_flag, p.status, p.timeout_ns};
+  if (threadIdx.x == 0) {
+    abort_word = 0;
+    for (int s = 0; s < p.stages; ++s) {
+      mbar_init(&full_bar[s], 2);  // weight loader and token loader
+      mbar_init(&empty_bar[s], 1);
+    }
+    for (int a = 0; a < 2; ++a) {
+      mbar_init(&tmem_full[a], 1);
+      mbar_init(&tmem_empty[a], 4);
+    }
+    mbar_fence_init();
+    prefetch_tmap(&tmap_w);
+    prefetch_tmap(&tmap_x);
+  }
+  if (warp == kWarpMma) {
+    tmem_alloc<1>(&tmem_slot, static_cast<uint32_t>(p.tmem_cols));
+    tmem_relinquish<1>();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = tmem_slot;
+  // The first launch waits for everything before it ahead of letting this one start, so x and W may be read at once; what it
+  // writes itself (list, v, cleared counters) is waited for by each role before its first use.
+  griddep_launch_dependents();
+  const Deal deal(p);
+  Units units(p, deal);
+  // Length and first entries of the adapter list, asked for ahead of the update; every lane of the warp calls it.
+  int count = -1, entries = 0;
+  auto read_list = [&]() {
+    griddep_wait();
+    count = __ldcg(p.list);
+    entries = lane < p.max_slots ? __ldcg(p.list + 1 + lane) : 0;
+  };
+  const int part_rows = M / p.pack, part_act = p.v_rows_tile * kRowBytes / p.pack;  // bytes / 128 and bytes of one adapter's share
+
+  if (warp == kWarpWeights) {
+    // -------------------------------------------------------------- weights and lora_b
+    const uint64_t policy = evict_first_policy();
+    int s = 0;
+    uint32_t ph = 0;
+    bool ok = true;
+    for (Unit u = units.next(); u.kind != 0 && ok; u = units.next()) {
+      const int ask = max(u.kb0, u.kb1 - 6);
+      for (int kb = u.kb0; kb < u.kb1; ++kb) {
+        if (u.kind == 2 && kb == ask && count < 0) read_list();
+        ok = wait_warp(&empty_bar[s], ph ^ 1, wctx, TB_DEV_TIMEOUT_SMEM_EMPTY);
+        if (!ok) break;
+        if (elect_one()) {
+          uint8_t* dst = ring + static_cast<size_t>(s) * p.stage_bytes;
+          mbar_arrive_expect_tx(&full_bar[s], kSlabs * kSlabBytes);
+#pragma unroll
+          for (int b = 0; b < kSlabs; ++b)
+            tma_load_2d_hint(dst + b * kSlabBytes, &tmap_w, &full_bar[s], (kb * kSlabs + b) * kSlabK, u.tile * M, policy);
+        }
+        __syncwarp();
+        if (++s == p.stages) {
+          s = 0;
+          ph ^= 1;
+        }
+      }
+      if (!ok || u.kind == 1) continue;
+      if (count < 0) read_list();
+      for (int i = 0; i < count && ok; i += p.pack) {
+        if (i == 32) entries = 32 + lane < p.max_slots ? __ldcg(p.list + 33 + lane) : 0;  // at most 64 rows, so at most 64 entries
+        const int filled = min(p.pack, count - i);
+        int adapter[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) adapter[j] = __shfl_sync(0xffffffffu, entries, (i + j) & 31);
+        for (int kb = 0; kb < p.kblocks; ++kb) {
+          ok = wait_warp(&empty_bar[s], ph ^ 1, wctx, TB_DEV_TIMEOUT_SMEM_EMPTY);
+          if (!ok) break;
+          if (elect_one()) {
+            uint8_t* dst = ring + static_cast<size_t>(s) * p.stage_bytes;
+            mbar_arrive_expect_tx(&full_bar[s], static_cast<uint32_t>(filled * part_rows * kRowBytes));
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              if (j < filled) tma_load_3d(dst + j * part_rows * kRowBytes, &tmap_b, &full_bar[s], kb * kSlabK, u.tile * M, adapter[j]);
+          }
+          __syncwarp();
+          if (++s == p.stages) {
+            s = 0;
+            ph ^= 1;
+          }
+        }
+      }
+    }
+  } else if (warp == kWarpTokens) {
+    // -------------------------------------------------------------- x and v
+    int s = 0;
+    uint32_t ph = 0;
+    bool ok = true;
+    for (Unit u = units.next(); u.kind != 0 && ok; u = units.next()) {
+      const int ask = max(u.kb0, u.kb1 - 6);
+      for (int kb = u.kb0; kb < u.kb1; ++kb) {
+        if (u.kind == 2 && kb == ask && count < 0) read_list();
+        ok = wait_warp(&empty_bar[s], ph ^ 1, wctx, TB_DEV_TIMEOUT_SMEM_EMPTY);
+        if (!ok) break;
+        if (elect_one()) {
+          // rows behind the last token keep an earlier stage's values: columns of the product that nobody reads
+          uint8_t* dst = ring + static_cast<size_t>(s) * p.stage_bytes + kActBase;
+          mbar_arrive_expect_tx(&full_bar[s], static_cast<uint32_t>(kSlabs * p.tokens * kRowBytes));
+#pragma unroll
+          for (int b = 0; b < kSlabs; ++b) tma_load_2d(dst + b * p.act_bytes, &tmap_x, &full_bar[s], (kb * kSlabs + b) * kSlabK, 0);
+        }
+        __syncwarp();
+        if (++s == p.stages) {
+          s = 0;
+          ph ^= 1;
+        }
+      }
+      if (!ok || u.kind == 1) continue;
+      if (count < 0) read_list();
+      for (int i = 0; i < count && ok; i += p.pack) {
+        const int filled = min(p.pack, count - i);
+        for (int kb = 0; kb < p.kblocks; ++kb) {
+          ok = wait_warp(&empty_bar[s], ph ^ 1, wctx, TB_DEV_TIMEOUT_SMEM_EMPTY);
+          if (!ok) break;
+          if (elect_one()) {
+            uint8_t* dst = ring + static_cast<size_t>(s) * p.stage_bytes + kActBase;
+            mbar_arrive_expect_tx(&full_bar[s], static_cast<uint32_t>(filled * part_act));
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              if (j < filled) tma_load_2d(dst + j * part_act, &tmap_v, &full_bar[s], kb * kSlabK, (i + j) * p.v_rows_tile);
+          }
+          __syncwarp();
+          if (++s == p.stages) {
+            s = 0;
+            ph ^= 1;
+          }
+        }
+      }
+    }
+  } else if (warp == kWarpMma) {
+    // -------------------------------------------------------------- MMA issuer
+    int s = 0, acc = 0;
+    uint32_t ph = 0, acc_parity = 0;
+    bool ok = true;
+    const uint32_t ring_addr = smem_u32(ring);
+    const uint64_t desc0 = make_smem_desc(ring_addr, 16, 1024);
+    const uint32_t swizzle = p.pack == 1 ? 2u : (p.pack == 2 ? 4u : 6u), row_group = 1024u / p.pack;
+    const uint64_t xa0 = make_smem_desc(ring_addr, 16, row_group, swizzle), xb0 = make_smem_desc(ring_addr + kActBase, 16, row_group, swizzle);
+    const uint32_t idesc = p.idesc | (static_cast<uint32_t>(p.n1 >> 3) << 17);
+    for (Unit u = units.next(); u.kind != 0 && ok; u = units.next()) {
+      if (u.kind == 3) {
+        if (count < 0) read_list();
+        if (count == 0) continue;  // nothing to add: the epilogue knows it too
+      }
+      const uint32_t d = tmem_base + static_cast<uint32_t>(acc * p.acc_stride);
+      ok = wait_warp(&tmem_empty[acc], ((acc_parity >> acc) & 1u) ^ 1u, wctx, TB_DEV_TIMEOUT_TMEM_EMPTY);
+      if (!ok) break;
+      tc_fence_after();
+      const int ask = max(u.kb0, u.kb1 - 6);
+      for (int kb = u.kb0; kb < u.kb1; ++kb) {
+        if (u.kind == 2 && kb == ask && count < 0) read_list();
+        ok = wait_warp(&full_bar[s], ph, wctx, TB_DEV_TIMEOUT_SMEM_FULL);
+        if (!ok) break;
+        if (elect_one()) {
+          const uint64_t stage = desc0 + static_cast<uint64_t>((s * p.stage_bytes) >> 4);
+#pragma unroll
+          for (int b = 0; b < kSlabs; ++b)
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              umma<0, 1>(d, stage + ((b * kSlabBytes) >> 4) + 2 * k, stage + ((kActBase + b * p.act_bytes) >> 4) + 2 * k, idesc,
+                         (b > 0 || k > 0) ? 1u : (kb > u.kb0 ? 1u : 0u));
+          umma_commit(&empty_bar[s]);
+          if (u.kind == 1 && kb + 1 == u.kb1) umma_commit(&tmem_full[acc]);
+        }
+        __syncwarp();
+        if (++s == p.stages) {
+          s = 0;
+          ph ^= 1;
+        }
+      }
+      if (!ok) break;
+      if (u.kind != 1) {
+        for (int i = 0, kb = 0; i < count;) {
+          ok = wait_warp(&full_bar[s], ph, wctx, TB_DEV_TIMEOUT_SMEM_FULL);
+          if (!ok) break;
+          if (elect_one()) {
+            const uint64_t soff = static_cast<uint64_t>((s * p.stage_bytes) >> 4);
+            const int filled = min(p.pack, count - i);
+            const int steps = min(4 / p.pack, (p.rank - kb * kSlabK + 15) >> 4);  // columns behind the rank are zeros
+            for (int j = 0; j < filled; ++j)
+              for (int k = 0; k < steps; ++k)
+                umma<0, 1>(d, xa0 + soff + ((j * part_rows * kRowBytes) >> 4) + 2 * k, xb0 + soff + ((j * part_act) >> 4) + 2 * k, idesc,
+                           (u.kind == 3 && i == 0 && kb == 0 && j == 0 && k == 0) ? 0u : 1u);
+            umma_commit(&empty_bar[s]);
+          }
+          __syncwarp();
+          if (++kb == p.kblocks) {
+            kb = 0;
+            i += p.pack;
+          }
+          if (++s == p.stages) {
+            s = 0;
+            ph ^= 1;
+          }
+        }
+        if (!ok) break;
+        if (elect_one()) umma_commit(&tmem_full[acc]);
+        __syncwarp();
+      }
+      acc_parity ^= 1u << acc;
+      acc ^= 1;
+    }
+  } else {
+    // -------------------------------------------------------------- epilogue (warps 0-3, one per TMEM lane quarter)
+    constexpr int kWarpRows = M / 4;  // features per warp; a 64-row accumulator occupies lanes 0-15 of each quarter
+    int acc = 0;
+    uint32_t parity = 0;
+    bool ok = true;
+    read_list();
+    const bool live = lane < kWarpRows;
+    T* out = static_cast<T*>(p.out);
+    for (Unit u = units.next(); u.kind != 0 && ok; u = units.next()) {
+      const int n = u.tile * M + warp * kWarpRows + lane;  // this lane's feature
+      const bool mine = live && n < p.n;
+      const float bias = u.kind == 2 && mine && p.bias != nullptr ? bias_at(p.bias, n * p.bias_stride, p.bias_dtype) : 0.0f;
+      float* part = p.parts + static_cast<size_t>(u.slot) * p.tokens * M + warp * kWarpRows + lane;
+      if (u.kind != 3 || count > 0) {
+        ok = __all_sync(0xffffffffu, mbar_wait(&tmem_full[acc], (parity >> acc) & 1u, wctx, TB_DEV_TIMEOUT_TMEM_FULL));
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t t_row = tmem_base + (static_cast<uint32_t>(warp * 32) << 16) + static_cast<uint32_t>(acc * p.acc_stride);
+        for (int c0 = 0; c0 < p.tokens; c0 += 32) {
+          uint32_t r[32];
+          tmem_ld_32x32(t_row + c0, r);
+          tmem_ld_wait(r);
+          if (c0 + 32 >= p.tokens) {  // the last columns sit in registers
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&tmem_empty[acc]);
+          }
+#pragma unroll
+          for (int j = 0; j < 32; ++j) {
+            const int t = c0 + j;
+            if (t < p.tokens && mine) {
+              const float v = __uint_as_float(r[j]);
+              if (u.kind == 2) out[t * p.out_m + n * p.out_n] = cast16<T>(v + bias);
+              else __stcg(part + static_cast<size_t>(t) * M, v);
+            }
+          }
+        }
+        parity ^= 1u << acc;
+        acc ^= 1;
+      }
+      if (u.kind == 2) continue;
+      // count this warp's quarter in; the last of its tile's parts adds them up
+      const int dealt = u.tile - p.full_tiles;
+      const int c_first = deal.cta_of(dealt * p.nkb), c_last = deal.cta_of((dealt + 1) * p.nkb - 1);
+      __syncwarp();
+      unsigned old = 0;
+      if (lane == 0) old = add_acq_rel(p.arrived + dealt * 4 + warp, 1u);
+      old = __shfl_sync(0xffffffffu, old, 0);
+      if (old != static_cast<unsigned>(c_last - c_first + 1)) continue;  // as many parts, and the update's unit
+      __syncwarp();
+      if (mine) {
+        const float* lane_parts = p.parts + warp * kWarpRows + lane;
+        const float b = p.bias != nullptr ? bias_at(p.bias, n * p.bias_stride, p.bias_dtype) : 0.0f;
+        const size_t slot_stride = static_cast<size_t>(p.tokens) * M;
+        // only the first of the tile's CTAs can have begun inside an earlier tile
+        const size_t first_slot = 2 * c_first + dealt - deal.begin(c_first) / p.nkb;
+        const float* update = lane_parts + (2 * static_cast<size_t>(gridDim.x) + dealt) * slot_stride;
+        // sixteen tokens of up to four parts at a time: their loads are all in flight before the first sum
+        for (int t0 = 0; t0 < p.tokens; t0 += 16) {
+          float sum[16];
+#pragma unroll
+          for (int j = 0; j < 16; ++j) sum[j] = b;
+          for (int q0 = 0; q0 <= c_last - c_first + 1; q0 += 4) {
+            float v[4][16];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              const int c = c_first + q0 + q;
+              const bool there = c <= c_last || (c == c_last + 1 && count > 0);
+              const float* src = c == c_first ? lane_parts + first_slot * slot_stride
+                                              : (c <= c_last ? lane_parts + 2 * static_cast<size_t>(c) * slot_stride : update);
+#pragma unroll
+              for (int j = 0; j < 16; ++j) v[q][j] = there && t0 + j < p.tokens ? __ldcg(src + static_cast<size_t>(t0 + j) * M) : 0.0f;
+            }
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+#pragma unroll
+              for (int j = 0; j < 16; ++j) sum[j] += v[q][j];
+          }
+#pragma unroll
+          for (int j = 0; j < 16; ++j)
+            if (t0 + j < p.tokens) out[(t0 + j) * p.out_m + n * p.out_n] = cast16<T>(sum[j]);
+        }
+      }
+      __syncwarp();
+    }
+  }
+
+  // ------------------------------------------------------------------ teardown
+  __syncwarp();
+  if (*abort_flag) {
+    // A wait gave up: let copies and MMAs already in flight land before shared memory and TMEM are released.
+    for (int i = 0; i < 64; ++i) __nanosleep(2000);
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kWarpMma) {
+    tc_fence_after();
+    tmem_dealloc<1>(tmem_base, static_cast<uint32_t>(p.tmem_cols));
+  }
+}
+
+template <typename T, int M>
+int decode_launch(const CUtensorMap& w, const CUtensorMap& x, const CUtensorMap& b, const CUtensorMap& v, const DecodeParams& p, int grid,
+                  int smem_bytes, int device, cudaStream_t stream) {
+  auto kernel = lora_decode_kernel<T, M>;
+  // the opt-in shared-memory size is set once per instantiation and device, and again if a launch needs more
+  static int configured[64] = {};
+  static std::mutex mu;
+  {
+    std::lock_guard<std::mutex> lk(mu);
+    if (smem_bytes > configured[device & 63]) {
+      cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes);
+      if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(lora_decode)");
+      configured[device & 63] = smem_bytes;
+    }
+  }
+  cudaLaunchConfig_t lc = {};
+  lc.gridDim = dim3(static_cast<unsigned>(grid), 1, 1);
+  lc.blockDim = dim3(kThreads, 1, 1);
+  lc.dynamicSmemBytes = static_cast<size_t>(smem_bytes);
+  lc.stream = stream;
+  cudaLaunchAttribute attr[1];
+  lc.attrs = attr;
+  lc.numAttrs = 0;
+  if (pdl_enabled()) {
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    lc.numAttrs = 1;
+  }
+  cudaError_t e = cudaLaunchKernelEx(&lc, kernel, w, x, b, v, p);
+  if (e != cudaSuccess) return cuda_fail(e, "lora_decode_kernel launch");
+  g_launches.fetch_add(1, std::memory_order_relaxed);
+  return TB_OK;
+}
+
+}  // namespace
+
+// Rows of a tile: 64 while the tokens' share of a stage is small, 128 above.
+LoraDecodeShape lora_decode_shape(int tokens, int n, int grid) {
+  LoraDecodeShape s;
+  s.tile_m = tokens <= 16 ? 64 : 128;
+  s.v_rows_tile = (tokens + 15) / 16 * 16;
+  s.grid = grid;
+  const int tiles = (n + s.tile_m - 1) / s.tile_m;
+  s.full_tiles = tiles / grid * grid;
+  s.dealt_tiles = tiles - s.full_tiles;
+  s.part_bytes = 4ll * (2ll * grid + s.dealt_tiles) * tokens * s.tile_m;
+  return s;
+}
+
+int lora_decode(const tb_lora_args& a, const LoraDecodeShape& s, const LowRank& lr, void* parts, void* arrived, int device,
+                int smem_optin, int* status, cudaStream_t stream) {
+  DecodeParams p = {};
+  const int m = s.tile_m, align = m == 64 ? 8 : 16;
+  p.tokens = a.m;
+  p.n = a.n;
+  p.n1 = (a.m + align - 1) / align * align;
+  p.v_rows_tile = s.v_rows_tile;
+  p.act_bytes = s.v_rows_tile * kRowBytes;
+  p.stage_bytes = slabs_of(m) * (m * kRowBytes + p.act_bytes);
+  // beside the ring: the barriers, the ring's alignment, and a block of the first launch, which runs at the same time
+  p.stages = (smem_optin - 28 * 1024) / p.stage_bytes;
+  if (p.stages > kMaxStages) p.stages = kMaxStages;
+  if (p.stages < 2) return TB_ERR_UNSUPPORTED;
+  p.acc_stride = p.n1 <= 32 ? 32 : 64;
+  p.tmem_cols = 2 * p.acc_stride;
+  p.nkb = (a.k + slabs_of(m) * kSlabK - 1) / (slabs_of(m) * kSlabK);
+  p.full_tiles = s.full_tiles;
+  p.dealt_tiles = s.dealt_tiles;
+  p.list = lr.list;
+  p.max_slots = lr.list_stride - 1;
+  p.pack = lr.pack;
+  p.kblocks = lr.kblocks;
+  p.rank = a.rank;
+  p.parts = static_cast<float*>(parts);
+  p.arrived = static_cast<unsigned*>(arrived);
+  p.bias = a.bias;
+  p.bias_stride = a.bias_stride;
+  p.bias_dtype = a.bias_dtype;
+  p.out = a.out;
+  p.out_m = a.out_stride_m;
+  p.out_n = a.out_stride_n;
+  p.status = status;
+  p.timeout_ns = a.wait_timeout_ms > 0 ? static_cast<unsigned long long>(a.wait_timeout_ms) * 1000000ull : 2000000000ull;
+  const uint32_t fmt = a.dtype == TB_DTYPE_BF16 ? 1u : 0u;
+  p.idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | (static_cast<uint32_t>(m >> 4) << 24);
+
+  CUtensorMap tw, tx, tb_, tv;
+  int rc = encode_2d(&tw, a.dtype, a.w, a.k, a.n, static_cast<uint64_t>(a.n > 1 ? a.w_stride_n : a.k) * 2, kSlabK, m, 1);
+  if (rc != TB_OK) return rc;
+  if ((rc = encode_2d(&tx, a.dtype, a.x, a.k, a.m, static_cast<uint64_t>(a.m > 1 ? a.x_row_stride : a.k) * 2, kSlabK, a.m, 1)) != TB_OK) return rc;
+  const uint32_t inner = static_cast<uint32_t>(kSlabK / lr.pack);
+  const uint64_t v_cols = static_cast<uint64_t>(lr.kblocks) * inner;
+  const uint64_t v_dims[2] = {v_cols, static_cast<uint64_t>(lr.v_rows)}, v_strides[1] = {v_cols * 2};
+  const uint32_t v_box[2] = {inner, static_cast<uint32_t>(s.v_rows_tile)};
+  if ((rc = encode_nd(&tv, a.dtype, lr.v, 2, v_dims, v_strides, v_box)) != TB_OK) return rc;
+  const uint64_t dims[3] = {static_cast<uint64_t>(lr.rank), static_cast<uint64_t>(lr.n), static_cast<uint64_t>(lr.num_adapters)};
+  const uint64_t row = static_cast<uint64_t>(lr.b_row_stride) * 2;
+  const uint64_t strides[2] = {row, lr.num_adapters > 1 ? static_cast<uint64_t>(lr.b_adapter_stride) * 2 : row * lr.n};
+  const uint32_t box[3] = {inner, static_cast<uint32_t>(m), 1};
+  if ((rc = encode_nd(&tb_, a.dtype, lr.b, 3, dims, strides, box)) != TB_OK) return rc;
+  const int smem_bytes = p.stages * p.stage_bytes + 1024;
+  auto launch = fmt ? (m == 64 ? decode_launch<__nv_bfloat16, 64> : decode_launch<__nv_bfloat16, 128>)
+                    : (m == 64 ? decode_launch<__half, 64> : decode_launch<__half, 128>);
+  return launch(tw, tx, tb_, tv, p, s.grid, smem_bytes, device, stream);
+}
+
+}  // namespace tb
