@@ -46,7 +46,7 @@ int gemm_low_rank(const tb_gemm_args& a, const tb_config& cfg, const LowRank& lr
 // Decode form of the same product (lora_decode.cu), up to 64 rows and K-contiguous weights: how it is cut, and its launch.
 // `parts` holds part_bytes, `arrived` 4 * dealt_tiles zeroed words.
 struct LoraDecodeShape {
-  int tile_m, v_rows_tile, grid, full_tiles, dealt_tiles;
+  int cols, grid, full_tiles, dealt_tiles;
   long long part_bytes;
 };
 LoraDecodeShape lora_decode_shape(int tokens, int n, int grid);

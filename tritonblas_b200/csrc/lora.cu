@@ -536,7 +536,7 @@ int lora_plan(const tb_lora_args& a, int num_sms, tb_gemm_args* g, LoraPlan* l) 
   if (l->decode) {
     l->shape = lora_decode_shape(a.m, a.n, num_sms);
     l->streamk = 0;
-    l->tile_rows = l->shape.v_rows_tile;
+    l->tile_rows = l->shape.cols;
   } else {
     const int rc = low_rank_config(*g, &l->cfg, &l->streamk);
     if (rc != TB_OK) return rc;
@@ -608,14 +608,14 @@ int lora_impl(const tb_lora_args& a, cudaStream_t stream) {
   p.status = status;
   p.timeout_ns = a.wait_timeout_ms > 0 ? static_cast<unsigned long long>(a.wait_timeout_ms) * 1000000ull : 2000000000ull;
   // Runs cover whole tiles: the rows behind the last token are zeros in every block. A decode batch has up to one adapter per
-  // row: they are dealt over blocks first, and K is split as long as four blocks per SM are not exceeded. Longer batches have
+  // row: they are dealt over blocks first, and K is split as long as the blocks fit the SMs at once, two on each. Longer batches have
   // few adapters per run: K is split first, up to a block per SM, and what is left of two per SM takes the adapters.
   const bool decode = a.m <= 64;
   const int rows = decode ? 16 : 128;
   const int runs = l.tiles * (l.tile_rows / rows);
   const int live_runs = (a.m + rows - 1) / rows;
   const int most = rows < l.max_slots ? rows : l.max_slots;
-  const int budget = decode ? 4 * num_sms : num_sms;
+  const int budget = decode ? 2 * num_sms : num_sms;
   int stripes = decode ? (most < a.m ? most : a.m) : 1;
   p.splits = 1;
   while (p.splits < 8 && live_runs * stripes * p.splits * 2 <= budget && a.k / (p.splits * 2) >= 256) p.splits *= 2;
