@@ -38,7 +38,6 @@ constexpr int kMlpMaxTokens = 128;
 constexpr int kMlpMaxTopk = 32;
 constexpr int kMlpMaxExperts = 1024;
 constexpr int kMlpMaxPairs = kMlpMaxTokens * kMlpMaxTopk;
-constexpr int kPlanThreads = 1024;
 constexpr int kMlpThreads = 7 * 32;  // four epilogue warps, weight loader, MMA issuer, activation loader
 constexpr int kWarpWeights = 4, kWarpMma = 5, kWarpAct = 6;
 constexpr int kQueueDepth = 4;
@@ -81,7 +80,7 @@ struct MlpParams {
   int n1;           // columns of the first kind: tokens rounded up to the MMA's granularity
   int group_cap;    // rows of a group
   int stages, stage_bytes;
-  int act_bytes;    // shared memory of one slab of activations
+  int act1_bytes, act2_bytes;  // shared memory of one slab of activations of either kind
   int acc_stride, tmem_cols;
   int f_tiles, h_tiles;  // units per expert / row group
   int quads_per_thread;  // third kind: float4 runs of one token's output per thread
@@ -92,7 +91,7 @@ struct MlpParams {
   long long out_stride;
   int out_vec;           // rows of `out` start on 8-byte boundaries
   int bf16;
-  uint32_t idesc;        // without the column count
+  uint32_t idesc;        // without the rows and columns
   int* status;
   unsigned long long timeout_ns;
 };
@@ -102,12 +101,16 @@ struct MlpParams {
 // with the weights added (in slot order). The order of an expert's rows depends on the order of atomics; every row is one
 // column of the products, computed alike wherever it stands, and the sum over a token's rows goes by slot, so no result
 // depends on it.
+// One thread per expert: 256 where that is enough, since the kernel is a chain of barriers and round trips on the layer's critical
+// path.
+template <int kPlanThreads>
 __global__ void __launch_bounds__(kPlanThreads)
 moe_mlp_plan_kernel(const void* __restrict__ ids, int is64, const float* __restrict__ weights, int tokens, int topk, int num_experts,
                     int group_cap, MlpLayout lay, int* __restrict__ ws) {
   __shared__ int s_id[kMlpMaxPairs];
-  __shared__ int s_count[kMlpMaxExperts];
-  __shared__ int s_cursor[kMlpMaxExperts];
+  __shared__ float s_weight[kMlpMaxPairs];
+  __shared__ int s_count[kPlanThreads];
+  __shared__ int s_cursor[kPlanThreads];
   __shared__ int s_scan[3][32];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int pairs = tokens * topk;
@@ -116,6 +119,7 @@ moe_mlp_plan_kernel(const void* __restrict__ ids, int is64, const float* __restr
   s_count[tid] = 0;
   for (int f = tid; f < pairs; f += kPlanThreads) {
     const long long e = is64 ? static_cast<const long long*>(ids)[f] : static_cast<long long>(static_cast<const int*>(ids)[f]);
+    s_weight[f] = weights[f];
     s_id[f] = (e >= 0 && e < num_experts) ? static_cast<int>(e) : -1;
   }
   __syncthreads();
@@ -145,7 +149,7 @@ moe_mlp_plan_kernel(const void* __restrict__ ids, int is64, const float* __restr
   if (warp == 0) {
 #pragma unroll
     for (int q = 0; q < 3; ++q) {
-      int x = s_scan[q][lane];
+      int x = lane < kPlanThreads / 32 ? s_scan[q][lane] : 0;
 #pragma unroll
       for (int s = 1; s < 32; s <<= 1) {
         const int o = __shfl_up_sync(0xffffffffu, x, s);
@@ -185,9 +189,9 @@ moe_mlp_plan_kernel(const void* __restrict__ ids, int is64, const float* __restr
     for (int g = first; g < f; ++g) own = own && s_id[g] != e;
     int row = -1;
     if (own) {
-      float w = weights[f];
+      float w = s_weight[f];
       for (int g = f + 1; g < first + topk; ++g)
-        if (s_id[g] == e) w += weights[g];
+        if (s_id[g] == e) w += s_weight[g];
       row = atomicAdd(&s_cursor[e], 1);
       ws[lay.row_token() + row] = t;
       reinterpret_cast<float*>(ws)[lay.row_weight() + row] = w;
@@ -313,8 +317,9 @@ __device__ __forceinline__ void store_quad(unsigned short* o, float4 v, int vec)
   }
 }
 
-// M: weight rows of a tile (256: two MMA tiles of 128). A 64-row accumulator occupies lanes 0-15 of every warp's 32 TMEM lanes, a 128-row one all.
-template <typename T, int M>
+// M1, M2: weight rows of a tile of the first and the second kind (256: two MMA tiles of 128). A 64-row accumulator occupies
+// lanes 0-15 of every warp's 32 TMEM lanes, a 128-row one all.
+template <typename T, int M1, int M2>
 __global__ void __launch_bounds__(kMlpThreads, 1)
 moe_mlp_kernel(const __grid_constant__ CUtensorMap tmap_w1, const __grid_constant__ CUtensorMap tmap_w2,
                const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ CUtensorMap tmap_h2,
@@ -332,13 +337,12 @@ moe_mlp_kernel(const __grid_constant__ CUtensorMap tmap_w1, const __grid_constan
   volatile int* abort_flag = &abort_word;
   const WaitCtx wctx{abort_flag, p.status, p.timeout_ns};
   const int stages = p.stages;
-  constexpr int kMmaRows = M < 128 ? M : 128;    // rows of one MMA
-  constexpr int kSubs = M / kMmaRows;            // MMA tiles side by side that share the activations
-  constexpr int kSlabs = mlp_slabs(M);           // 64-element slabs of K per stage
-  constexpr uint32_t kSlabBytes = M * kRowBytes; // weights of one slab
-  constexpr uint32_t kActBase = kSlabs * kSlabBytes;
-  constexpr int kGroups = kMmaRows / 64;         // eight-feature groups (16 rows: 8 gate, 8 up) per epilogue warp and MMA tile
-
+  constexpr int kRows1 = M1 < 128 ? M1 : 128, kRows2 = M2 < 128 ? M2 : 128;  // rows of one MMA
+  constexpr int kSubs = M1 / kRows1;                                         // MMA tiles side by side that share the activations
+  constexpr int kSlabs1 = mlp_slabs(M1), kSlabs2 = mlp_slabs(M2);             // 64-element slabs of K per stage
+  constexpr uint32_t kWeightBytes = kSlabs1 * M1 * kRowBytes;                 // of a stage, of either kind
+  static_assert(M2 / kRows2 == kSubs && kSlabs2 * M2 * kRowBytes == kWeightBytes, "both kinds share the ring");
+  constexpr int kGroups = kRows1 / 64;  // eight-feature groups (16 rows: 8 gate, 8 up) per epilogue warp and MMA tile
   if (threadIdx.x == 0) {
     abort_word = 0;
     for (int s = 0; s < stages; ++s) {
@@ -373,8 +377,8 @@ moe_mlp_kernel(const __grid_constant__ CUtensorMap tmap_w1, const __grid_constan
   const int num_experts = __ldcg(ws + MlpLayout::kNumExperts), num_groups = __ldcg(ws + MlpLayout::kNumGroups);
   const int units1 = num_experts * p.f_tiles, units2 = num_groups * p.h_tiles;
   const int units3 = p.tokens * p.runs;
-  constexpr int kColAlign = M < 128 ? 8 : 16;  // columns of an MMA come in multiples of this
-  const int kb1 = (p.hidden + kSlabs * kStageK - 1) / (kSlabs * kStageK), kb2 = (p.ffn + kSlabs * kStageK - 1) / (kSlabs * kStageK);
+  constexpr int kAlign2 = M2 < 128 ? 8 : 16;  // columns of an MMA come in multiples of this
+  const int kb1 = (p.hidden + kSlabs1 * kStageK - 1) / (kSlabs1 * kStageK), kb2 = (p.ffn + kSlabs2 * kStageK - 1) / (kSlabs2 * kStageK);
 
   // The next unit out of the queue; every lane of a consuming warp calls it.
   auto take = [&](int seq, bool& ok) -> Unit {
@@ -459,15 +463,17 @@ moe_mlp_kernel(const __grid_constant__ CUtensorMap tmap_w1, const __grid_constan
       }
       const int nkb = u.kind == 1 ? kb1 : kb2;
       const int ask_at = nkb > 16 ? nkb - 16 : 0, look_at = nkb > 6 ? nkb - 6 : nkb - 1;
-      const CUtensorMap* map = u.kind == 1 ? &tmap_w1 : &tmap_w2;
       auto load = [&](int kb) {
         uint8_t* dst = ring + static_cast<size_t>(s) * p.stage_bytes;
-        mbar_arrive_expect_tx(&full_bar[s], kSlabs * kSlabBytes);
+        mbar_arrive_expect_tx(&full_bar[s], kWeightBytes);
+        if (u.kind == 1) {
 #pragma unroll
-        for (int b = 0; b < kSlabs; ++b) {
-          const int x = (kb * kSlabs + b) * kStageK;
-          if (u.kind == 1) tma_load_5d_hint(dst + b * kSlabBytes, map, &full_bar[s], x, 0, 0, u.tile * (M / 16), u.expert, policy);
-          else tma_load_3d_hint(dst + b * kSlabBytes, map, &full_bar[s], x, u.tile * M, u.expert, policy);
+          for (int b = 0; b < kSlabs1; ++b)
+            tma_load_5d_hint(dst + b * M1 * kRowBytes, &tmap_w1, &full_bar[s], (kb * kSlabs1 + b) * kStageK, 0, 0, u.tile * (M1 / 16), u.expert, policy);
+        } else {
+#pragma unroll
+          for (int b = 0; b < kSlabs2; ++b)
+            tma_load_3d_hint(dst + b * M2 * kRowBytes, &tmap_w2, &full_bar[s], (kb * kSlabs2 + b) * kStageK, u.tile * M2, u.expert, policy);
         }
       };
       for (int kb = 0; kb < nkb; ++kb) {
@@ -507,16 +513,16 @@ moe_mlp_kernel(const __grid_constant__ CUtensorMap tmap_w1, const __grid_constan
       const CUtensorMap* map = u.kind == 1 ? &tmap_x : h_map;
       const int rows = u.kind == 1 ? p.tokens : (h_rows + h_box - 1) / h_box * h_box;
       const int box = u.kind == 1 ? p.tokens : h_box, row0 = u.kind == 1 ? 0 : 2 * u.off;
+      const int slabs = u.kind == 1 ? kSlabs1 : kSlabs2, act_bytes = u.kind == 1 ? p.act1_bytes : p.act2_bytes;
       for (int kb = 0; kb < nkb; ++kb) {
         ok = wait_warp(&empty_bar[s], ph ^ 1, wctx, TB_DEV_TIMEOUT_SMEM_EMPTY);
         if (!ok) break;
         if (elect_one()) {
-          uint8_t* dst = ring + static_cast<size_t>(s) * p.stage_bytes + kActBase;
-          mbar_arrive_expect_tx(&full_bar[s], static_cast<uint32_t>(kSlabs * rows * kRowBytes));
-#pragma unroll
-          for (int b = 0; b < kSlabs; ++b)
+          uint8_t* dst = ring + static_cast<size_t>(s) * p.stage_bytes + kWeightBytes;
+          mbar_arrive_expect_tx(&full_bar[s], static_cast<uint32_t>(slabs * rows * kRowBytes));
+          for (int b = 0; b < slabs; ++b)
             for (int r = 0; r < rows; r += box)
-              tma_load_2d(dst + b * p.act_bytes + r * kRowBytes, map, &full_bar[s], (kb * kSlabs + b) * kStageK, row0 + r);
+              tma_load_2d(dst + b * act_bytes + r * kRowBytes, map, &full_bar[s], (kb * slabs + b) * kStageK, row0 + r);
         }
         __syncwarp();
         if (++s == stages) {
@@ -536,9 +542,9 @@ moe_mlp_kernel(const __grid_constant__ CUtensorMap tmap_w1, const __grid_constan
       const Unit u = take(seq++, ok);
       if (!ok || u.kind == 0) break;
       if (u.kind == 3) continue;
-      const int n = u.kind == 1 ? p.n1 : ((2 * u.rows + kColAlign - 1) & ~(kColAlign - 1));
+      const int n = u.kind == 1 ? p.n1 : ((2 * u.rows + kAlign2 - 1) & ~(kAlign2 - 1));
       const int nkb = u.kind == 1 ? kb1 : kb2;
-      const uint32_t idesc = p.idesc | (static_cast<uint32_t>(n >> 3) << 17);
+      const uint32_t idesc = p.idesc | (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>((u.kind == 1 ? kRows1 : kRows2) >> 4) << 24);
       const uint32_t d = tmem_base + static_cast<uint32_t>(acc * kSubs * p.acc_stride);
       ok = wait_warp(&tmem_empty[acc], ((acc_parity >> acc) & 1u) ^ 1u, wctx, TB_DEV_TIMEOUT_TMEM_EMPTY);
       if (!ok) break;
@@ -548,14 +554,21 @@ moe_mlp_kernel(const __grid_constant__ CUtensorMap tmap_w1, const __grid_constan
         if (!ok) break;
         if (elect_one()) {
           const uint64_t stage = desc0 + static_cast<uint64_t>((s * p.stage_bytes) >> 4);
-#pragma unroll
-          for (int b = 0; b < kSlabs; ++b)
+          auto issue = [&](int b, uint32_t slab_bytes, int act_bytes, int mma_rows) {
 #pragma unroll
             for (int k = 0; k < 4; ++k)
 #pragma unroll
               for (int j = 0; j < kSubs; ++j)
-                umma<0, 1>(d + j * p.acc_stride, stage + ((b * kSlabBytes + j * kMmaRows * kRowBytes) >> 4) + 2 * k,
-                           stage + ((kActBase + b * p.act_bytes) >> 4) + 2 * k, idesc, (b > 0 || k > 0) ? 1u : (kb > 0 ? 1u : 0u));
+                umma<0, 1>(d + j * p.acc_stride, stage + ((b * slab_bytes + j * mma_rows * kRowBytes) >> 4) + 2 * k,
+                           stage + ((kWeightBytes + b * act_bytes) >> 4) + 2 * k, idesc, (b > 0 || k > 0) ? 1u : (kb > 0 ? 1u : 0u));
+          };
+          if (u.kind == 1) {
+#pragma unroll
+            for (int b = 0; b < kSlabs1; ++b) issue(b, M1 * kRowBytes, p.act1_bytes, kRows1);
+          } else {
+#pragma unroll
+            for (int b = 0; b < kSlabs2; ++b) issue(b, M2 * kRowBytes, p.act2_bytes, kRows2);
+          }
           umma_commit(&empty_bar[s]);
           if (kb + 1 == nkb) umma_commit(&tmem_full[acc]);
         }
@@ -580,17 +593,17 @@ moe_mlp_kernel(const __grid_constant__ CUtensorMap tmap_w1, const __grid_constan
       if (!ok || u.kind == 0) break;
       if (u.kind == 3) {
         // the sum over a token's rows, in slot order
-        ok = counter_wait_warp(p.ws + MlpLayout::kRowsDone, 4 * units2, wctx);
-        if (!ok) break;
         const int t = u.tile / p.runs, quads = p.hidden / 4;
         const int q0 = (u.tile - t * p.runs) * p.quads_per_thread * 128 + threadIdx.x;
         const int q1 = min(quads, q0 + p.quads_per_thread * 128);
         const int* rows = ws + p.lay.pair_row() + t * p.topk;
         unsigned short* o = reinterpret_cast<unsigned short*>(p.out) + t * p.out_stride;
-        if (p.topk <= 8) {
-          int r[8];
+        int r[8];
 #pragma unroll
-          for (int j = 0; j < 8; ++j) r[j] = j < p.topk ? __ldcg(rows + j) : -1;
+        for (int j = 0; j < 8; ++j) r[j] = j < p.topk ? __ldcg(rows + j) : -1;  // on their way while the rows are still written
+        ok = counter_wait_warp(p.ws + MlpLayout::kRowsDone, 4 * units2, wctx);
+        if (!ok) break;
+        if (p.topk <= 8) {
           const float4* src[8];
 #pragma unroll
           for (int j = 0; j < 8; ++j) src[j] = reinterpret_cast<const float4*>(p.y + static_cast<long long>(max(r[j], 0)) * p.hidden);
@@ -652,8 +665,8 @@ moe_mlp_kernel(const __grid_constant__ CUtensorMap tmap_w1, const __grid_constan
         }
         if (u.kind == 1) {
           // lanes 0-7 of a run of 16 hold gate features, lanes 8-15 the matching up features
-          const int f = u.tile * (M / 2) + sub * (kMmaRows / 2) + (warp * kGroups + (lane >> 4)) * 8 + (lane & 7);
-          const bool mine = (lane & 8) == 0 && (kMmaRows == 128 || lane < 16) && f < p.ffn;
+          const int f = u.tile * (M1 / 2) + sub * (kRows1 / 2) + (warp * kGroups + (lane >> 4)) * 8 + (lane & 7);
+          const bool mine = (lane & 8) == 0 && (kRows1 == 128 || lane < 16) && f < p.ffn;
 #pragma unroll
           for (int j = 0; j < 32; ++j) {
             const int row = c0 + j < p.tokens ? col_row[warp][c0 + j] : -1;
@@ -673,8 +686,8 @@ moe_mlp_kernel(const __grid_constant__ CUtensorMap tmap_w1, const __grid_constan
             }
           }
         } else {
-          const int hcol = u.tile * M + sub * kMmaRows + warp * (kMmaRows / 4) + lane;
-          const bool mine = (kMmaRows == 128 || lane < 16) && hcol < p.hidden;
+          const int hcol = u.tile * M2 + sub * kRows2 + warp * (kRows2 / 4) + lane;
+          const bool mine = (kRows2 == 128 || lane < 16) && hcol < p.hidden;
 #pragma unroll
           for (int j = 0; j < 32; j += 2) {  // the products with both halves of h stand side by side
             const int row = (c0 + j) >> 1;
@@ -710,19 +723,22 @@ moe_mlp_kernel(const __grid_constant__ CUtensorMap tmap_w1, const __grid_constan
 // ------------------------------------------------------------------------------------------------------------ host
 struct MlpShape {
   MlpLayout lay;
-  int tile_m;         // rows of the tensor-core tile
+  int m1, m2;         // weight rows of a tile of either projection
   int n1, group_cap;
-  int act_rows;       // rows of activations a stage has room for
+  int h_rows;         // rows of h a stage of the second projection has room for
   long long h_offset, y_offset, bytes;  // byte offsets in the workspace
 };
 
-// Weight rows of a tile. Few units (few chosen experts) are dealt more evenly in 64-row tiles, unless that makes a unit of the
-// second projection so short that its hand-overs show: measured back to back, 64 / 128 rows, 8 experts of 4096 x 1536: 61 / 68
-// us; 18 experts of 2048 x 704: 54 / 44 us. Above 64 tokens their share of a stage is as large as 128 weight rows', so a
-// tile has 256: 408 against 414 us at 128 tokens, 64 experts of 4096 x 1536.
-int mlp_tile_rows(int tokens, int topk, int ffn) {
-  if (tokens > 64) return 256;
-  return tokens * topk < 64 && ffn >= 1280 ? 64 : 128;
+// Weight rows of a tile of either projection (the second kind waits for all of an expert's units of the first, so those are
+// dealt in the smaller tiles). Measured back to back with 64 + 64 / 64 + 128 / 128 + 128 rows, tokens x chosen of hidden x ffn:
+//   1 x 8 of 4096 x 1536: 56.4 / 58.3 / 64.7 us      1 x 2 of 4096 x 4096: 48.2 / 54.8 / 53.6
+//   5 x 4 of 2048 x 704:  48.0 / 36.5 / 39.9         4 x 6 of 2048 x 1408: 65.2 / 63.4 / 64.2
+//  16 x 8 of 4096 x 1536:  313 /  306 /  310        32 x 8: 353 / 345 / 346        64 x 8: 388 / 376 / 359
+// 64 rows of the second kind pay only for single tokens, as long as a unit stays long enough (1 x 8 of 2048 x 768: 28.8 / 28.9).
+// Above 64 tokens their share of a stage is as large as 128 weight rows', so a tile has 256: 408 against 414 us at 128 tokens.
+void mlp_tile_rows(int tokens, int topk, int ffn, int* m1, int* m2) {
+  *m1 = tokens > 64 ? 256 : (tokens <= 32 ? 64 : 128);
+  *m2 = tokens > 64 ? 256 : (tokens * topk <= 8 && ffn >= 1024 ? 64 : 128);
 }
 
 // Columns of the two projections and the workspace they need. The rows of an expert go in groups of at most half the token
@@ -730,13 +746,13 @@ int mlp_tile_rows(int tokens, int topk, int ffn) {
 // than half of the tokens choose is read once per group, the second time out of L2.
 MlpShape mlp_shape(int tokens, int topk, int num_experts, int hidden, int ffn) {
   MlpShape s;
-  s.tile_m = mlp_tile_rows(tokens, topk, ffn);
-  const int align = s.tile_m == 64 ? 8 : 16;
+  mlp_tile_rows(tokens, topk, ffn, &s.m1, &s.m2);
+  const int align = s.m1 == 64 ? 8 : 16;
   s.n1 = (tokens + align - 1) / align * align;
-  s.group_cap = tokens < 16 ? tokens : (s.n1 / 2 < 16 ? 16 : s.n1 / 2);
-  const int h_rows = (2 * s.group_cap + 31) / 32 * 32;
-  s.act_rows = s.group_cap <= 4 ? 8 : h_rows;
-  if (s.act_rows < s.n1) s.act_rows = s.n1;
+  s.group_cap = tokens < 16 ? tokens : ((tokens + 15) / 16 * 8 < 16 ? 16 : (tokens + 15) / 16 * 8);
+  // rows of h arrive in copies of 2, 8 or 32
+  s.h_rows = s.group_cap <= 4 ? 8 : (2 * s.group_cap + 31) / 32 * 32;
+  if (s.h_rows < 16 && s.m2 > 64) s.h_rows = 16;
   s.lay.pairs = tokens * topk;
   s.lay.experts = num_experts < s.lay.pairs ? num_experts : s.lay.pairs;
   s.lay.groups = s.lay.experts + s.lay.pairs / s.group_cap;
@@ -753,10 +769,10 @@ bool mlp_sizes_ok(int tokens, int topk, int num_experts, int hidden, int ffn) {
          hidden <= (1 << 20) && ffn <= (1 << 20);
 }
 
-template <typename T, int M>
+template <typename T, int M1, int M2>
 int mlp_launch(const CUtensorMap& w1, const CUtensorMap& w2, const CUtensorMap& x, const CUtensorMap (&h)[3], const MlpParams& p,
                int grid, int smem_bytes, int device, cudaStream_t stream) {
-  auto kernel = moe_mlp_kernel<T, M>;
+  auto kernel = moe_mlp_kernel<T, M1, M2>;
   // the opt-in shared-memory size is set once per instantiation and device, and again if a launch needs more
   static int configured[64] = {};
   static std::mutex mu;
@@ -785,6 +801,11 @@ int mlp_launch(const CUtensorMap& w1, const CUtensorMap& w2, const CUtensorMap& 
   if (e != cudaSuccess) return cuda_fail(e, "moe_mlp_kernel launch");
   g_launches.fetch_add(1, std::memory_order_relaxed);
   return TB_OK;
+}
+
+template <typename T>
+auto mlp_variant(int m1, int m2) {
+  return m1 == 256 ? mlp_launch<T, 256, 256> : (m1 == 128 ? mlp_launch<T, 128, 128> : (m2 == 128 ? mlp_launch<T, 64, 128> : mlp_launch<T, 64, 64>));
 }
 
 int mlp_impl(const tb_moe_mlp_args& a, cudaStream_t stream) {
@@ -827,26 +848,29 @@ int mlp_impl(const tb_moe_mlp_args& a, cudaStream_t stream) {
   p.status = status;
   p.timeout_ns = a.wait_timeout_ms > 0 ? static_cast<unsigned long long>(a.wait_timeout_ms) * 1000000ull : 2000000000ull;
 
-  const int m = s.tile_m;
-  p.act_bytes = s.act_rows * kRowBytes;
-  p.stage_bytes = mlp_slabs(m) * (m * kRowBytes + p.act_bytes);
+  const int slabs1 = mlp_slabs(s.m1), slabs2 = mlp_slabs(s.m2);
+  p.act1_bytes = s.n1 * kRowBytes;
+  p.act2_bytes = s.h_rows * kRowBytes;
+  const int act = slabs1 * p.act1_bytes > slabs2 * p.act2_bytes ? slabs1 * p.act1_bytes : slabs2 * p.act2_bytes;
+  p.stage_bytes = slabs1 * s.m1 * kRowBytes + act;
   p.stages = (smem_optin - 8192) / p.stage_bytes;  // beside the ring: barriers, queue, column tables, the ring's alignment
   if (p.stages > kMaxStages) p.stages = kMaxStages;
   if (p.stages < 2) return TB_ERR_UNSUPPORTED;
   const int smem_bytes = p.stages * p.stage_bytes + 1024;
-  p.acc_stride = s.act_rows < 32 ? 32 : s.act_rows;
+  const int cols = s.n1 > s.h_rows ? s.n1 : s.h_rows;
+  p.acc_stride = cols < 32 ? 32 : (cols + 31) / 32 * 32;
   p.tmem_cols = 64;
-  while (p.tmem_cols < 2 * (m > 128 ? m / 128 : 1) * p.acc_stride) p.tmem_cols <<= 1;
-  p.f_tiles = (a.ffn + m / 2 - 1) / (m / 2);
-  p.h_tiles = (a.hidden + m - 1) / m;
+  while (p.tmem_cols < 2 * (s.m1 > 128 ? 2 : 1) * p.acc_stride) p.tmem_cols <<= 1;
+  p.f_tiles = (a.ffn + s.m1 / 2 - 1) / (s.m1 / 2);
+  p.h_tiles = (a.hidden + s.m2 - 1) / s.m2;
   // the sum over a token's rows: about as many units as SMs, or one per token when there are more tokens
   const int token_runs = (a.hidden / 4 + 127) / 128;
   p.runs = num_sms / a.tokens < 1 ? 1 : (num_sms / a.tokens > token_runs ? token_runs : num_sms / a.tokens);
   p.quads_per_thread = (token_runs + p.runs - 1) / p.runs;
   p.runs = (token_runs + p.quads_per_thread - 1) / p.quads_per_thread;
-  // fp32 accumulators; operand format (0 = f16, 1 = bf16); the column count is added per unit
+  // fp32 accumulators; operand format (0 = f16, 1 = bf16); rows and columns are added per unit
   const uint32_t fmt = p.bf16 ? 1u : 0u;
-  p.idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | (static_cast<uint32_t>((m < 128 ? m : 128) >> 4) << 24);
+  p.idesc = (1u << 4) | (fmt << 7) | (fmt << 10);
 
   CUtensorMap tw1, tw2, tx, th[3];
   const uint64_t es = 2;
@@ -856,14 +880,14 @@ int mlp_impl(const tb_moe_mlp_args& a, cudaStream_t stream) {
     const uint64_t row = static_cast<uint64_t>(a.w1_row_stride) * es;
     const uint64_t dims[5] = {static_cast<uint64_t>(a.hidden), 8, 2, static_cast<uint64_t>(a.ffn / 8), static_cast<uint64_t>(a.num_experts)};
     const uint64_t strides[4] = {row, row * a.ffn, row * 8, a.num_experts > 1 ? static_cast<uint64_t>(a.w1_expert_stride) * es : row * 2 * a.ffn};
-    const uint32_t box[5] = {kStageK, 8, 2, static_cast<uint32_t>(m / 16), 1};
+    const uint32_t box[5] = {kStageK, 8, 2, static_cast<uint32_t>(s.m1 / 16), 1};
     if ((rc = encode_nd(&tw1, a.dtype, a.w1, 5, dims, strides, box)) != TB_OK) return rc;
   }
   {
     const uint64_t dims[3] = {static_cast<uint64_t>(a.ffn), static_cast<uint64_t>(a.hidden), static_cast<uint64_t>(a.num_experts)};
     const uint64_t row = static_cast<uint64_t>(a.w2_row_stride) * es;
     const uint64_t strides[2] = {row, a.num_experts > 1 ? static_cast<uint64_t>(a.w2_expert_stride) * es : row * a.hidden};
-    const uint32_t box[3] = {kStageK, static_cast<uint32_t>(m), 1};
+    const uint32_t box[3] = {kStageK, static_cast<uint32_t>(s.m2), 1};
     if ((rc = encode_nd(&tw2, a.dtype, a.w2, 3, dims, strides, box)) != TB_OK) return rc;
   }
   const uint64_t x_stride = static_cast<uint64_t>(a.tokens > 1 ? a.x_row_stride : a.hidden) * es;
@@ -874,7 +898,8 @@ int mlp_impl(const tb_moe_mlp_args& a, cudaStream_t stream) {
 
   cudaLaunchConfig_t lc = {};
   lc.gridDim = dim3(1, 1, 1);
-  lc.blockDim = dim3(kPlanThreads, 1, 1);
+  const bool narrow = a.num_experts <= 256;
+  lc.blockDim = dim3(narrow ? 256 : kMlpMaxExperts, 1, 1);
   lc.stream = stream;
   cudaLaunchAttribute attr[1];
   lc.attrs = attr;
@@ -884,13 +909,12 @@ int mlp_impl(const tb_moe_mlp_args& a, cudaStream_t stream) {
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     lc.numAttrs = 1;
   }
-  cudaError_t e = cudaLaunchKernelEx(&lc, moe_mlp_plan_kernel, a.topk_ids, static_cast<int>(a.ids_are_int64 != 0), a.topk_weights,
+  cudaError_t e = cudaLaunchKernelEx(&lc, narrow ? moe_mlp_plan_kernel<256> : moe_mlp_plan_kernel<kMlpMaxExperts>, a.topk_ids, static_cast<int>(a.ids_are_int64 != 0), a.topk_weights,
                                      static_cast<int>(a.tokens), static_cast<int>(a.topk), static_cast<int>(a.num_experts),
                                      s.group_cap, s.lay, p.ws);
   if (e != cudaSuccess) return cuda_fail(e, "moe_mlp_plan_kernel launch");
   g_launches.fetch_add(1, std::memory_order_relaxed);
-  auto launch = p.bf16 ? (m == 64 ? mlp_launch<__nv_bfloat16, 64> : m == 128 ? mlp_launch<__nv_bfloat16, 128> : mlp_launch<__nv_bfloat16, 256>)
-                       : (m == 64 ? mlp_launch<__half, 64> : m == 128 ? mlp_launch<__half, 128> : mlp_launch<__half, 256>);
+  auto launch = p.bf16 ? mlp_variant<__nv_bfloat16>(s.m1, s.m2) : mlp_variant<__half>(s.m1, s.m2);
   return launch(tw1, tw2, tx, th, p, num_sms, smem_bytes, device, stream);
 }
 
