@@ -59,7 +59,7 @@ def check(got, *case, what="", **kw):
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("T,K,N,R,L", [(1, 64, 256, 8, 1), (1, 1024, 2048, 16, 8), (2, 72, 40, 8, 3), (5, 2056, 1000, 24, 6), (16, 512, 777, 64, 4),
                                        (33, 1024, 4096, 16, 40), (48, 520, 300, 128, 5), (64, 256, 512, 16, 64), (64, 4096, 8192, 32, 9),
-                                       (65, 512, 512, 72, 3), (130, 264, 200, 40, 200), (333, 2056, 1250, 24, 6), (700, 128, 640, 16, 2),
+                                       (65, 512, 512, 72, 3), (130, 264, 200, 40, 200), (333, 2056, 1250, 24, 6), (700, 128, 640, 16, 2), (1, 128, 64, 8, 1), (90, 192, 136, 16, 1),
                                        (1000, 512, 1536, 128, 10)])
 def test_matches_formula(T, K, N, R, L, dtype):
     case = make(T, K, N, R, L, dtype)
@@ -120,6 +120,9 @@ def test_strides_alignment_and_out():
         assert got.data_ptr() == pick(t).data_ptr() and torch.equal(got, want)
         pick(t).fill_(7.0)
         assert (t == 7.0).all()
+    square = torch.zeros(50, 256, dtype=x.dtype, device="cuda")
+    with pytest.raises(ValueError, match="out must not be x"):
+        tb.lora_matmul(square, w[:, :256], a, b[:, :256], ids, s, out=square)
     one = tb.lora_matmul(x[:1].expand(50, 256), w, a, b, ids * 0, s)                             # one row, stride 0
     assert torch.equal(one, one[:1].expand(50, 328))
     assert tb.lora_matmul(x[:0], w, a, b, ids[:0], s).shape == (0, 328)
@@ -138,6 +141,23 @@ def test_extreme_values_stay_in_their_row():
     # inside one tile a row's projection stands beside zeros of the other rows; only the row itself meets its values
     assert torch.equal(got[keep], want[keep]) and torch.isnan(got[7]).all()
     assert tb.device_status() == 0
+
+
+@pytest.mark.parametrize("T,K,N", [(5, 4096, 40000), (20, 8, 19200), (64, 64, 37888)])
+def test_decode_with_whole_and_dealt_tiles(T, K, N):
+    """More feature tiles than SMs: whole tiles, dealt ones and the update of either (the last case deals none)."""
+    case = make(T, K, N, 16, 7, torch.bfloat16)
+    check(tb.lora_matmul(*case), *case)
+    bias = torch.randn(N, device="cuda")
+    check(tb.lora_matmul(*case, bias=bias), *case[:5], scales=case[5], bias=bias)
+
+
+def test_grad_is_refused():
+    x, w, a, b, ids, s = make(4, 64, 64, 8, 2, torch.bfloat16)
+    with pytest.raises(RuntimeError, match="inference only"):
+        tb.lora_matmul(x, w, a.requires_grad_(True), b, ids, s)
+    with torch.no_grad():
+        check(tb.lora_matmul(x, w, a, b, ids, s), x, w, a.detach(), b, ids, scales=s)
 
 
 def test_large_batch_is_cut_into_pieces(monkeypatch):

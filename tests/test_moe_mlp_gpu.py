@@ -62,7 +62,8 @@ def check(got, x, w1, w2, ids, w, what=""):
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("T,E,K,H,F", [(1, 1, 1, 64, 64), (1, 8, 2, 256, 128), (2, 5, 3, 200, 72), (16, 8, 4, 512, 384), (17, 8, 8, 1024, 96),
                                        (31, 60, 4, 264, 704), (64, 16, 8, 512, 256), (100, 7, 3, 328, 200), (128, 32, 8, 512, 136),
-                                       (128, 2, 2, 256, 128), (3, 300, 10, 8, 8), (128, 1, 1, 16, 1000)])
+                                       (128, 2, 2, 256, 128), (3, 300, 10, 8, 8), (128, 1, 1, 16, 1000),
+                                       (128, 1024, 32, 64, 32), (32, 16, 9, 64, 48), (1, 2, 2, 1024, 1160)])
 def test_matches_formula(T, E, K, H, F, dtype):
     case = make(T, E, K, H, F, dtype)
     check(tb.moe_mlp(*case), *case, f"{T} {E} {K} {H} {F}")

@@ -153,6 +153,21 @@ def test_capture_and_replay_and_compile():
     rw, rids, _ = reference(logits, 8, "softmax", True)
     assert torch.equal(ids.cpu(), rids)
 
+    # forward and backward in one graph
+    leaf = logits.detach().clone().requires_grad_(True)
+    grad = torch.randn(64, 8, device="cuda")
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        w, ids = tb.moe_route(leaf, 8, scoring="sigmoid")
+        (d,) = torch.autograd.grad(w, leaf, grad)
+    with torch.no_grad():
+        leaf.copy_(make(64, 64, torch.bfloat16, seed=4, mask=False))
+    graph.replay()
+    _, rids2, rd = reference(leaf.detach(), 8, "sigmoid", True, grad)
+    assert torch.equal(ids.cpu(), rids2)
+    assert ((d.cpu().double() - rd).abs() <= 2.0 ** -8 * rd.abs() + 1e-5 * grad.abs().sum(1, keepdim=True).cpu()).all()
+    del w, d, leaf
+
     def f(x):
         w, ids = tb.moe_route(x, 8, renormalize=False)
         return (w * 2).sum(), ids

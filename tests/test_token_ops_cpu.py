@@ -22,6 +22,16 @@ def test_router_refusals():
             bad()
 
 
+def test_router_operators_refuse_host_tensors_and_shapes():
+    """Traced code reaches the router through custom operators, which check what the plain function checks."""
+    l = torch.randn(4, 8)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        torch.ops.tritonblas._moe_route(l, 2, False, True)
+    w, i = torch.zeros(4, 2), torch.zeros(4, 2, dtype=torch.int32)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        torch.ops.tritonblas._moe_route_backward(l, w, i, w, False, True)
+
+
 def mlp_case(T=4, E=4, K=2, H=64, F=32, dtype=bf):
     return [torch.zeros(T, H, dtype=dtype), torch.zeros(E, 2 * F, H, dtype=dtype), torch.zeros(E, H, F, dtype=dtype),
             torch.zeros(T, K, dtype=torch.int32), torch.zeros(T, K)]
@@ -87,6 +97,17 @@ def test_adapter_projection_c_entry_refusals():
     assert call(x=264) == 3 and call(lora_a=258) == 3 and call(x_row_stride=68) == 3 and call(adapter_ids=258) == 3 and call(scales=257) == 3
     assert call(workspace=None, x=256) in (3, 4) and call(workspace_bytes=100) == 4 and call(workspace=272) == 3
     assert lib.tb_lora_gemm(None, None) == 1 and lib.tb_lora_workspace_bytes(None) == 0
+    assert call(out=257) == 3 and call(bias=257, bias_dtype=_lib.F32) == 3 and call(bias=256, bias_dtype=_lib.E4M3) == 2
+
+    def need(**kw):
+        a = _lib.LoraArgs(4, 40, 64, 8, 3, _lib.BF16, 256, 64, 256, 1, 64, 256, 512, 64, 256, 320, 8, 256, 0, 0, 0, 256, 40, 1, 256, 0, 0, 0, 0)
+        for k, v in kw.items():
+            setattr(a, k, v)
+        return lib.tb_lora_workspace_bytes(ctypes.byref(a))
+
+    assert need() > 0 and need(m=5000) > need(m=500) > 0
+    assert need(m=1 << 26, num_adapters=1000) == 0          # more block rows than a copy's coordinate can number
+    assert need(rank=12) == 0 and need(m=0) == 0
 
 
 def test_c_entry_points_refuse_bad_arguments():

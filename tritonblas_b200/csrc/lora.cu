@@ -551,6 +551,7 @@ int lora_plan(const tb_lora_args& a, int num_sms, tb_gemm_args* g, LoraPlan* l) 
   l->pack = a.rank <= 16 ? 4 : (a.rank <= 32 ? 2 : 1);
   l->v_cols = l->pack > 1 ? 64 / l->pack : (a.rank + 63) / 64 * 64;
   l->v_rows = static_cast<long long>(l->tiles) * l->max_slots * l->tile_rows;
+  if (l->v_rows > 0x7fffffffll) return TB_ERR_UNSUPPORTED;  // a row coordinate of a copy has 32 bits; shorter batches fit
   auto up = [](long long v) { return (v + 255) & ~255ll; };
   l->gemm_offset = 0;
   // flags or counters (cleared by the projection) at the front, then partial tiles
@@ -581,17 +582,22 @@ int lora_impl(const tb_lora_args& a, cudaStream_t stream) {
                           (a.num_adapters > 1 ? a.lora_a_adapter_stride | a.lora_b_adapter_stride : 0) |
                           (a.w_stride_k == 1 ? (a.n > 1 ? a.w_stride_n : 0) : a.w_stride_k);
   if (addresses % 16 || strides % 8 || reinterpret_cast<uintptr_t>(a.adapter_ids) % (a.ids_are_int64 ? 8 : 4) ||
-      reinterpret_cast<uintptr_t>(a.scales) % 4)
+      reinterpret_cast<uintptr_t>(a.scales) % 4 || reinterpret_cast<uintptr_t>(a.out) % 2 ||
+      reinterpret_cast<uintptr_t>(a.bias) % (a.bias_dtype == TB_DTYPE_F32 ? 4 : 2))
     return TB_ERR_ALIGNMENT;
+  if (a.bias != nullptr && a.bias_dtype != TB_DTYPE_F32 && a.bias_dtype != TB_DTYPE_F16 && a.bias_dtype != TB_DTYPE_BF16)
+    return TB_ERR_UNSUPPORTED;
   int device = 0, num_sms = 0, smem_optin = 0;
   int* status = nullptr;
-  int rc = current_device_limits(&device, &num_sms, &smem_optin, &status);
-  if (rc != TB_OK) return rc;
+  const int device_rc = current_device_limits(&device, &num_sms, &smem_optin, &status);
+  if (device_rc != TB_OK) num_sms = MachineModel().num_sms;  // the other arguments are checked all the same
   tb_gemm_args g;
   LoraPlan l;
-  if ((rc = lora_plan(a, num_sms, &g, &l)) != TB_OK) return rc;
+  int rc = lora_plan(a, num_sms, &g, &l);
+  if (rc != TB_OK) return rc;
   if (a.workspace == nullptr || a.workspace_bytes < l.bytes) return TB_ERR_WORKSPACE;
   if (reinterpret_cast<uintptr_t>(a.workspace) % 256) return TB_ERR_ALIGNMENT;
+  if (device_rc != TB_OK) return device_rc;
   char* ws = static_cast<char*>(a.workspace);
 
   ProjectParams p = {};

@@ -25,6 +25,10 @@ def lora_matmul(x, w, lora_a, lora_b, adapter_ids, scales=None, bias=None, out: 
     or None for 1; bias: (n,). k and rank multiples of 8, rank up to 128. The sum is float32 and rounded once; the rank-sized
     products ``scales[a] * x[t] @ lora_a[a].T`` are rounded to the operands' type on the way. ``out`` may be given: (tokens, n),
     any strides, no overlap with the inputs. Inference only.
+
+    Values in x, lora_a and scales stay with their rows. An infinity or NaN in ``lora_b[a]`` does not: it also makes NaN of the
+    rows without that adapter that stand in the same tile (up to 256 neighbours) as a row with it, because the update is one
+    matrix product per tile in which those rows hold zeros.
     """
     if x.ndim != 2 or w.ndim != 2 or lora_a.ndim != 3 or lora_b.ndim != 3:
         refuse("x and w must be 2-D, lora_a and lora_b 3-D")
@@ -51,6 +55,8 @@ def lora_matmul(x, w, lora_a, lora_b, adapter_ids, scales=None, bias=None, out: 
         refuse("bias must be (n,) in float16, bfloat16 or float32")
     if out is not None and (out.shape != (tokens, n) or out.dtype is not dtype):
         refuse(f"out must be {(tokens, n)} of {dtype}")
+    if out is not None and tokens and n and out.data_ptr() == x.data_ptr():
+        refuse("out must not be x: other columns of its rows are still read while the first ones are written")
     if not x.is_cuda or not device == w.device == lora_a.device == lora_b.device == adapter_ids.device \
             or any(t is not None and t.device != device for t in (scales, bias, out)):
         refuse_devices(x, w, lora_a, lora_b, adapter_ids, scales, bias, out)
@@ -83,7 +89,7 @@ def lora_matmul(x, w, lora_a, lora_b, adapter_ids, scales=None, bias=None, out: 
     ref = ctypes.byref(args)
     need = _lib.lib.tb_lora_workspace_bytes(ref)
     rows = tokens
-    while need > _MAX_WORKSPACE and rows > 256:
+    while (need > _MAX_WORKSPACE or need == 0) and rows > 256:     # 0: more rows than one launch pair can number
         args.m = rows = max(256, (rows // 2 + 255) // 256 * 256)
         need = _lib.lib.tb_lora_workspace_bytes(ref)
     # per call, from torch's allocator: calls on other streams and captured graphs never share it

@@ -26,6 +26,8 @@ def _route_rows(logits):
 
 
 def _route_forward(logits, topk, sigmoid, renormalize):
+    if not logits.is_cuda:
+        refuse_devices(logits)
     tokens, experts = logits.shape
     logits = _route_rows(logits)
     weights = torch.empty(tokens, topk, dtype=torch.float32, device=logits.device)
@@ -40,6 +42,10 @@ def _route_forward(logits, topk, sigmoid, renormalize):
 
 def _route_backward(logits, weights, ids, grad, sigmoid, renormalize):
     tokens, experts = logits.shape
+    if not logits.is_cuda or not logits.device == weights.device == ids.device == grad.device:
+        refuse_devices(logits, weights, ids, grad)
+    if not (weights.shape == ids.shape == grad.shape and ids.ndim == 2 and ids.shape[0] == tokens):
+        refuse("weights, ids and their gradient must be (tokens, topk)")
     logits = _route_rows(logits)
     weights, ids, grad = weights.contiguous(), ids.contiguous(), grad.to(torch.float32).contiguous()
     out = torch.empty(tokens, experts, dtype=logits.dtype, device=logits.device)
@@ -129,8 +135,6 @@ def moe_route(logits, topk, scoring="softmax", renormalize=True):
     sigmoid, renormalize = _SCORING[scoring], 1 if renormalize else 0
     if torch.compiler.is_compiling():
         return _moe_route(logits, topk, bool(sigmoid), bool(renormalize))
-    if not logits.is_cuda:
-        refuse_devices(logits)
     if logits.requires_grad and torch.is_grad_enabled():
         return _Route.apply(logits, topk, sigmoid, renormalize)
     return _route_forward(logits, topk, sigmoid, renormalize)
