@@ -131,6 +131,12 @@ def test_layouts_strides_and_empty():
     assert ((d.cpu().double() - rd).abs() <= 1e-5).all()
 
 
+def test_second_derivative_is_refused():
+    x = make(4, 16, torch.float32, mask=False).requires_grad_(True)
+    with pytest.raises(RuntimeError, match="not differentiable again"):
+        torch.autograd.grad(tb.moe_route(x, 2, renormalize=False)[0].sum(), x, create_graph=True)
+
+
 def test_signed_zeros_tie_and_large_values():
     l = torch.tensor([[-0.0, 0.0, -1.0, 0.0], [3e38, -3e38, 1.0, 3e38]], device="cuda")
     w, ids = tb.moe_route(l, 3)

@@ -26,9 +26,14 @@ def on_device(device):
 
 
 def rows16(t):
-    """True when the last axis is contiguous and rows start on 16-byte boundaries and do not overlap (TMA reads it in place)."""
+    """True when the last axis is contiguous and rows start on 16-byte boundaries and do not overlap (TMA reads it in place).
+    For tensors whose last axis is a multiple of 16 bytes."""
+    if t.data_ptr() % 16:
+        return False
+    if t.is_contiguous():
+        return True
     strides, shape = t.stride(), t.shape
-    if strides[-1] != 1 or t.data_ptr() % 16:
+    if strides[-1] != 1:
         return False
     per16, row = 16 // t.element_size(), shape[-1]
     for n, s in zip(shape[:-1], strides[:-1]):

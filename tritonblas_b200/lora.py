@@ -72,13 +72,15 @@ def lora_matmul(x, w, lora_a, lora_b, adapter_ids, scales=None, bias=None, out: 
         lora_a = lora_a.clone(memory_format=torch.contiguous_format)
     if not rows16(lora_b):
         lora_b = lora_b.clone(memory_format=torch.contiguous_format)
-    w = _unit_stride_2d(w)
-    if not _tma_loadable(w):
-        w = _repitch(w)
+    w_k, w_n = w.stride()
+    if w_k != 1 or w_n < k or w_n % 8 or w.data_ptr() % 16:     # anything but the fast layout
+        w = _unit_stride_2d(w)
+        if not _tma_loadable(w):
+            w = _repitch(w)
+        w_k, w_n = _strides(w)
     ids = adapter_ids.contiguous()
     if scales is not None:
         scales = scales.to(torch.float32).contiguous()
-    w_k, w_n = _strides(w)
     x_row, (o_m, o_n), a_strides, b_strides = x.stride(0), out.stride(), lora_a.stride(), lora_b.stride()
     es, id_size = x.element_size(), ids.element_size()
     args = _lib.LoraArgs(tokens, n, k, rank, adapters, _lib.DTYPE_CODE[dtype], x.data_ptr(), x_row, w.data_ptr(), w_k, w_n,

@@ -69,8 +69,9 @@ class _Route(torch.autograd.Function):
         return weights, ids
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, grad_weights, _grad_ids):
+        if torch.is_grad_enabled():     # create_graph=True
+            raise RuntimeError("tritonblas.moe_route(): the gradient is not differentiable again.")
         return _route_backward(*ctx.saved_tensors, grad_weights, *ctx.modes), None, None, None
 
 
