@@ -12,7 +12,7 @@
 // theirs: the sums over parts are hidden behind the whole tiles where there are any.
 //
 // Measured back to back: 1 row of 4096 x 4096, rank 16: 15.0 us (19.5 with the general GEMM and the same update); 48 rows of 8192
-// x 28672, 28 adapters of rank 16: 88 us, 5.8 TB/s (101); 1 row of 8192 x 28672: 72.7 us, 0.99 of the copy rate.
+// x 28672, 30 adapters of rank 16: 88 us, 5.8 TB/s (101); 1 row of 8192 x 28672: 72.7 us, 0.99 of the copy rate.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
