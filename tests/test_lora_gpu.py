@@ -152,6 +152,14 @@ def test_decode_with_whole_and_dealt_tiles(T, K, N):
     check(tb.lora_matmul(*case, bias=bias), *case[:5], scales=case[5], bias=bias)
 
 
+@pytest.mark.parametrize("T,N,R", [(33, 37888, 16), (64, 37888, 16), (64, 20480, 72), (50, 56832, 32)])
+def test_more_than_32_adapters_in_every_tile_of_a_block(T, N, R):
+    """One adapter per row, and blocks that work on several tiles: each walks the whole list again."""
+    x, w, a, b, _, s = make(T, 64, N, R, T, torch.bfloat16)
+    ids = torch.randperm(T, device="cuda").int()
+    check(tb.lora_matmul(x, w, a, b, ids, s), x, w, a, b, ids, scales=s)
+
+
 def test_grad_is_refused():
     x, w, a, b, ids, s = make(4, 64, 64, 8, 2, torch.bfloat16)
     with pytest.raises(RuntimeError, match="inference only"):

@@ -183,12 +183,13 @@ lora_decode_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
   griddep_launch_dependents();
   const Deal deal(p);
   Units units(p, deal);
-  // Length and first entries of the adapter list, asked for ahead of the update; every lane of the warp calls it.
-  int count = -1, entries = 0;
+  // The adapter list, at most 64 entries for as many rows, asked for ahead of the update; every lane of the warp calls it.
+  int count = -1, entries = 0, more_entries = 0;
   auto read_list = [&]() {
     griddep_wait();
     count = __ldcg(p.list);
     entries = lane < p.max_slots ? __ldcg(p.list + 1 + lane) : 0;
+    more_entries = 32 + lane < p.max_slots ? __ldcg(p.list + 33 + lane) : 0;
   };
   const int part_w = kWeightBytes / p.pack, part_v = p.cols * kRowBytes / p.pack;  // bytes of one adapter's share of a stage
 
@@ -218,11 +219,10 @@ lora_decode_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
       if (!ok || u.kind == 1) continue;
       if (count < 0) read_list();
       for (int i = 0; i < count && ok; i += p.pack) {
-        if (i == 32) entries = 32 + lane < p.max_slots ? __ldcg(p.list + 33 + lane) : 0;  // at most 64 rows, so at most 64 entries
         const int filled = min(p.pack, count - i);
         int adapter[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) adapter[j] = __shfl_sync(0xffffffffu, entries, (i + j) & 31);
+        for (int j = 0; j < 4; ++j) adapter[j] = __shfl_sync(0xffffffffu, i < 32 ? entries : more_entries, (i + j) & 31);
         for (int kb = 0; kb < p.kblocks; ++kb) {
           ok = wait_warp(&empty_bar[s], ph ^ 1, wctx, TB_DEV_TIMEOUT_SMEM_EMPTY);
           if (!ok) break;
