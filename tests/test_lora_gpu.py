@@ -152,6 +152,38 @@ def test_decode_with_whole_and_dealt_tiles(T, K, N):
     check(tb.lora_matmul(*case, bias=bias), *case[:5], scales=case[5], bias=bias)
 
 
+@pytest.mark.parametrize("T,K,N,R,L", [(1, 64, 8, 8, 1), (1, 4096, 4096, 16, 8), (2, 72, 40, 8, 3), (17, 200, 136, 72, 5), (48, 520, 1000, 128, 40),
+                                       (5, 1024, 19200, 24, 6), (64, 64, 37888, 16, 64), (65, 512, 520, 16, 3), (333, 2056, 1256, 24, 6)])
+def test_weights_with_contiguous_outputs(T, K, N, R, L):
+    """The (k, n) layout as stored, down to one column of tiles that ends inside its first half."""
+    x, w, a, b, ids, s = make(T, K, N, R, L, torch.float16, layout="N")
+    assert w.stride() == (N, 1)
+    got = tb.lora_matmul(x, w, a, b, ids, s)
+    check(got, x, w, a, b, ids, scales=s)
+    wide = torch.full((K, N + 16), float("nan"), dtype=w.dtype, device="cuda")
+    wide[:, 8:N + 8] = w
+    assert torch.equal(tb.lora_matmul(x, wide[:, 8:N + 8], a, b, ids, s), got)
+    row = w[:1].expand(K, N)                                                                     # one row of weights, stride 0
+    check(tb.lora_matmul(x, row, a, b, ids, s), x, row, a, b, ids, scales=s)
+    column = w[:, :1].expand(K, N)
+    check(tb.lora_matmul(x, column, a, b, ids, s), x, column, a, b, ids, scales=s)
+
+
+def test_many_streams_at_once():
+    """Long batches on eight streams: more blocks than fit the device at once, none of which may hold up another's."""
+    cases = [make(T, 2056, 1000, 16, 6, torch.bfloat16, seed=T) for T in (65, 128, 200, 333, 400, 64, 500, 1)]
+    want = [tb.lora_matmul(*c) for c in cases]
+    streams = [torch.cuda.Stream() for _ in cases]
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(40):
+        for c, st in zip(cases, streams):
+            with torch.cuda.stream(st):
+                got.append(tb.lora_matmul(*c))
+    torch.cuda.synchronize()
+    assert all(torch.equal(g, want[i % len(cases)]) for i, g in enumerate(got)) and tb.device_status() == 0
+
+
 @pytest.mark.parametrize("T,N,R", [(33, 37888, 16), (64, 37888, 16), (64, 20480, 72), (50, 56832, 32)])
 def test_more_than_32_adapters_in_every_tile_of_a_block(T, N, R):
     """One adapter per row, and blocks that work on several tiles: each walks the whole list again."""

@@ -99,6 +99,11 @@ def test_adapter_projection_c_entry_refusals():
     assert lib.tb_lora_gemm(None, None) == 1 and lib.tb_lora_workspace_bytes(None) == 0
     assert call(out=257) == 3 and call(bias=257, bias_dtype=_lib.F32) == 3 and call(bias=256, bias_dtype=_lib.E4M3) == 2
 
+    # weight rows (or columns) that overlap, and sizes whose tile or stage numbers would pass 32 bits
+    assert call(w_stride_n=56) == 1 and call(w_stride_n=0) == 1 and call(w_stride_k=32, w_stride_n=1) == 1 and call(w_stride_k=0, w_stride_n=1) == 1
+    wide = dict(x_row_stride=1 << 30, w_stride_n=1 << 30, lora_a_row_stride=1 << 30)
+    assert call(k=1 << 29, **wide) == 1 and call(m=(1 << 30) + 1) == 1 and call(n=(1 << 30) + 1) == 1
+
     def need(**kw):
         a = _lib.LoraArgs(4, 40, 64, 8, 3, _lib.BF16, 256, 64, 256, 1, 64, 256, 512, 64, 256, 320, 8, 256, 0, 0, 0, 256, 40, 1, 256, 0, 0, 0, 0)
         for k, v in kw.items():

@@ -335,6 +335,7 @@ static int gemm_impl(const tb_gemm_args& a_in, const tb_config* user_cfg, cudaSt
     rc = select_config(pr, machine_for(dev), &cfg);
     if (rc != TB_OK) return rc;
   }
+  if (lr != nullptr && (cfg.swap_ab || a.streamk)) return TB_ERR_UNSUPPORTED;
   if (cfg.swap_ab && !swapped && !grouped && a.epilogue_op == TB_EPILOGUE_NONE) {
     // C^T = B^T A^T: exchange the operands' roles and transpose the output view; the per-row and per-column epilogue
     // vectors trade places and the bias becomes a per-row vector.
@@ -347,9 +348,9 @@ static int gemm_impl(const tb_gemm_args& a_in, const tb_config* user_cfg, cudaSt
     t.static_operands = ((a.static_operands & 1) << 1) | ((a.static_operands >> 1) & 1);
     tb_config c2 = cfg;
     c2.swap_ab = 0;
-    rc = gemm_impl(t, &c2, stream, false, true, builtin, lr);
+    rc = gemm_impl(t, &c2, stream, false, true, builtin);
     // Operands TMA cannot address go to the CUDA-core kernel in their original orientation (its bias is per column).
-    if (rc == TB_ERR_ALIGNMENT && lr == nullptr) return gemm_generic_loader(a, cfg, stream, dev->status);
+    if (rc == TB_ERR_ALIGNMENT) return gemm_generic_loader(a, cfg, stream, dev->status);
     return rc;
   }
   const bool glu = a.epilogue_op == TB_EPILOGUE_SWIGLU;
@@ -379,7 +380,7 @@ static int gemm_impl(const tb_gemm_args& a_in, const tb_config* user_cfg, cudaSt
   const int bk = 128 / es;
   // wide tiles (two accumulators sharing A) only for the data-parallel and grouped schedules: stream-K partials are per accumulator
   const int halves = (cfg.n_halves == 2 && !a.streamk) ? 2 : 1;
-  if (lr != nullptr && (halves != 1 || es != 2 || lr->tile_rows != (swapped ? bn : 128 * pair))) return TB_ERR_INVALID;
+  if (lr != nullptr && (halves != 1 || es != 2 || lr->tile_rows != 128 * pair)) return TB_ERR_INVALID;
   int stages = cfg.stages;
   if (stages < 2) stages = 2;
   const int extra_smem = grouped ? 8 * (a.num_groups + 2) : 0;  // per-group tile prefix + copy of the row offsets
@@ -571,23 +572,21 @@ static int gemm_impl(const tb_gemm_args& a_in, const tb_config* user_cfg, cudaSt
     p.lr_kblocks = lr->kblocks;
     p.lr_rank = lr->rank;
     p.lr_tile_rows = lr->tile_rows;
-    p.lr_tokens_on_b = swapped ? 1 : 0;
     CUtensorMap tv, tlb;
     p.lr_pack = lr->pack;
-    const uint32_t token_box = swapped ? bn / pair : 128, weight_box = swapped ? 128 : bn / pair, inner = bk / lr->pack;
+    const uint32_t inner = bk / lr->pack;
     const uint64_t v_cols = static_cast<uint64_t>(lr->kblocks) * inner;
     const uint64_t v_dims[2] = {v_cols, static_cast<uint64_t>(lr->v_rows)}, v_strides[1] = {v_cols * es};
-    const uint32_t v_box[2] = {inner, token_box};
+    const uint32_t v_box[2] = {inner, 128};
     if ((rc = encode_nd(&tv, a.a_dtype, lr->v, 2, v_dims, v_strides, v_box)) != TB_OK) return rc;
     const uint64_t dims[3] = {static_cast<uint64_t>(lr->rank), static_cast<uint64_t>(lr->n), static_cast<uint64_t>(lr->num_adapters)};
     const uint64_t strides[2] = {static_cast<uint64_t>(lr->b_row_stride) * es,
                                  lr->num_adapters > 1 ? static_cast<uint64_t>(lr->b_adapter_stride) * es
                                                       : static_cast<uint64_t>(lr->b_row_stride) * es * lr->n};
-    const uint32_t box[3] = {inner, weight_box, 1};
+    const uint32_t box[3] = {inner, static_cast<uint32_t>(bn / pair), 1};
     if ((rc = encode_nd(&tlb, a.a_dtype, lr->b, 3, dims, strides, box)) != TB_OK) return rc;
-    const CUtensorMap *ma = swapped ? &tlb : &tv, *mb = swapped ? &tv : &tlb;
-    return pair == 1 ? launch_gemm<0, 1>(ta, tbm, p, programs, smem_bytes, stream, ma, mb)
-                     : launch_gemm<0, 2>(ta, tbm, p, programs, smem_bytes, stream, ma, mb);
+    return pair == 1 ? launch_gemm<0, 1>(ta, tbm, p, programs, smem_bytes, stream, &tv, &tlb)
+                     : launch_gemm<0, 2>(ta, tbm, p, programs, smem_bytes, stream, &tv, &tlb);
   }
 
 #define TB_LAUNCH(K, C) return launch_gemm<K, C>(ta, tbm, p, programs, smem_bytes, stream)
@@ -605,7 +604,7 @@ static int gemm_impl(const tb_gemm_args& a_in, const tb_config* user_cfg, cudaSt
 #undef TB_LAUNCH
 }
 
-int low_rank_config(const tb_gemm_args& a, tb_config* cfg, int* streamk) {
+int low_rank_config(const tb_gemm_args& a, tb_config* cfg) {
   DeviceState* dev = nullptr;
   int device = 0;
   // without a usable device the model falls back to the B200 constants (workspace sizes on a CPU host)
@@ -620,7 +619,6 @@ int low_rank_config(const tb_gemm_args& a, tb_config* cfg, int* streamk) {
   struct Entry {
     tb_problem pr;
     tb_config cfg;
-    int streamk;
     bool used;
   };
   static Entry cache[64];
@@ -631,22 +629,14 @@ int low_rank_config(const tb_gemm_args& a, tb_config* cfg, int* streamk) {
     std::lock_guard<std::mutex> lk(mu);
     if (e.used && std::memcmp(&e.pr, &pr, sizeof(pr)) == 0) {
       *cfg = e.cfg;
-      *streamk = e.streamk;
       return TB_OK;
     }
   }
-  const tb_problem key = pr;
-  tb_config dp, sk;
-  int rc = select_config(pr, machine_for(dev), &dp);
+  const int rc = select_config(pr, machine_for(dev), cfg);
   if (rc != TB_OK) return rc;
-  pr.streamk = 1;
-  rc = select_config(pr, machine_for(dev), &sk);
-  if (rc != TB_OK) return rc;
-  *streamk = sk.predicted_sk_us < dp.predicted_us ? 1 : 0;
-  *cfg = *streamk ? sk : dp;
   if (dev != nullptr) {
     std::lock_guard<std::mutex> lk(mu);
-    e = {key, *cfg, *streamk, true};
+    e = {pr, *cfg, true};
   }
   return TB_OK;
 }

@@ -38,12 +38,12 @@ struct LowRank {
   const int* list;
   int list_stride;
 };
-// Configuration the library would pick for `a`, data-parallel or stream-K (whichever the model says is shorter; a.streamk says
-// which), narrow tiles; and the launch of `a` with that configuration and the update.
-int low_rank_config(const tb_gemm_args& a, tb_config* cfg, int* streamk);
+// Configuration the library would pick for `a` (more than 64 rows): data-parallel, narrow tiles; and the launch of `a` with that
+// configuration and the update.
+int low_rank_config(const tb_gemm_args& a, tb_config* cfg);
 int gemm_low_rank(const tb_gemm_args& a, const tb_config& cfg, const LowRank& lr, cudaStream_t stream);
 
-// Decode form of the same product (lora_decode.cu), up to 64 rows and K-contiguous weights: how it is cut, and its launch.
+// Decode form of the same product (lora_decode.cu), up to 64 rows: how it is cut, and its launch.
 // `parts` holds part_bytes, `arrived` 4 * dealt_tiles zeroed words.
 struct LoraDecodeShape {
   int cols, grid, full_tiles, dealt_tiles;

@@ -101,19 +101,18 @@ struct GemmParams {
   // fills its shared-memory ring with that operand before it waits for the previous kernel (single CTAs, static
   // schedules, plain 2-D / 3-D operand copies).
   int early_operand;
-  // Low-rank update beside the product (LOWRANK instantiation, K-major 16-bit extension operands): after a tile's own K range
-  // its owner walks further stages for the adapters that occur among the tile's tokens: `lr_kblocks` per adapter, or one for
-  // `lr_pack` adapters whose ranks fit side by side in a stage (each with rows of 128 / lr_pack bytes). On the token side they
-  // hold the rows' rank-sized projections, zero in rows of other adapters (tensor map `sfa` / `sfb`, one block of lr_tile_rows
-  // rows per token tile and listed adapter), on the other side that adapter's rows of lora_b (the other map). All of it adds
-  // up in the same accumulator, so the sum is rounded once.
-  const int* lr_list;   // per token tile: number of adapters, then their indices; written by the kernel launched before
-  int lr_list_stride;   // words per token tile
+  // Low-rank update beside the product (LOWRANK instantiation: data-parallel, narrow tiles, K-major 16-bit extension operands):
+  // after a tile's own K range come further stages for the adapters that occur among the tile's rows: `lr_kblocks` per adapter,
+  // or one for `lr_pack` adapters whose ranks fit side by side in a stage (each with rows of 128 / lr_pack bytes). On A's side
+  // they hold the rows' rank-sized projections, zero in rows of other adapters (tensor map `sfa`, one block of lr_tile_rows rows
+  // per tile of rows and listed adapter), on B's side that adapter's rows of lora_b (`sfb`). All of it adds up in the same
+  // accumulator, so the sum is rounded once.
+  const int* lr_list;   // per tile of rows: number of adapters, then their indices; written by the kernel launched before
+  int lr_list_stride;   // words per tile of rows
   int lr_kblocks;       // stages per adapter (1 when lr_pack > 1)
   int lr_pack;          // adapters per stage: 1 (128-byte swizzle), 2 (64-byte) or 4 (32-byte)
   int lr_rank;
-  int lr_tile_rows;     // rows of a token tile: what this launch's tile covers on the token side
-  int lr_tokens_on_b;   // 1: the tokens are the B side (transposed launch)
+  int lr_tile_rows;     // rows of a tile of this launch
   // failure reporting
   int* status;
   unsigned long long timeout_ns;
@@ -577,8 +576,7 @@ static __device__ __noinline__ void park_peer_partials(const float* src, int cou
 
 // LOWRANK launches follow the kernel that projects the tokens onto the adapters' ranks and start while it still runs: that
 // kernel waits for everything before it ahead of letting this one start, so the operands of the plain product may be read at
-// once; only what it writes itself (projections, adapter lists, zeroed stream-K flags) is waited for, by each role before its
-// first use.
+// once; only what it writes itself (projections, adapter lists) is waited for, by either role that reads it before its first use.
 template <int KIND, int CTAS, bool PROF = false, bool GATHER = false, bool LOWRANK = false>
 __global__ void __launch_bounds__(gemm_threads<KIND>(), 1)
 gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
@@ -833,16 +831,15 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ 
             if (r < tg.row_end) grow[j] = __ldg(p.a_gather + r);
           }
         }
-        // LOWRANK: length and first entries of the token tile's adapter list, asked for a few stages before they are needed (a
+        // LOWRANK: length and first entries of the tile's adapter list, asked for a few stages before they are needed (a
         // round trip to memory takes microseconds while every SM streams)
         const int* lr_entries = nullptr;
         int lr_count = 0, lr_mine = 0;
         for (int it = w.kb0; it < w.kb1; ++it) {
           if constexpr (LOWRANK) {
-            if (w.kb0 == 0 && it == max(0, w.kb1 - 8)) {
+            if (it == max(0, w.kb1 - 8)) {
               griddep_wait();
-              const int token_tile = (p.lr_tokens_on_b ? tg.n0 : tg.m0) / p.lr_tile_rows;
-              lr_entries = p.lr_list + static_cast<size_t>(token_tile) * p.lr_list_stride;
+              lr_entries = p.lr_list + static_cast<size_t>(tg.m0 / p.lr_tile_rows) * p.lr_list_stride;
               lr_count = __ldcg(lr_entries);
               lr_mine = lane + 1 < p.lr_list_stride ? __ldcg(lr_entries + 1 + lane) : 0;
             }
@@ -928,54 +925,42 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ 
         }
         if constexpr (LOWRANK) {
           if (!ok) break;
-          if (w.kb0 == 0) {
-            const int block_row0 = (p.lr_tokens_on_b ? tg.n0 : tg.m0) / p.lr_tile_rows * (p.lr_list_stride - 1) * p.lr_tile_rows;
-            const int a_part = kATileBytes / p.lr_pack, b_part = b_tile_bytes / p.lr_pack;
-            for (int i = 0; i < lr_count && ok; i += p.lr_pack) {
-              if (i > 0 && (i & 31) == 0) lr_mine = i + lane + 1 < p.lr_list_stride ? __ldcg(lr_entries + 1 + i + lane) : 0;
-              const int filled = min(p.lr_pack, lr_count - i);
-              int adapter[4];  // lr_pack divides 32: a group's entries stand in one run of the warp's lanes
+          const int block_row0 = tg.m0 / p.lr_tile_rows * (p.lr_list_stride - 1) * p.lr_tile_rows;
+          const int a_part = kATileBytes / p.lr_pack, b_part = b_tile_bytes / p.lr_pack;
+          for (int i = 0; i < lr_count && ok; i += p.lr_pack) {
+            if (i > 0 && (i & 31) == 0) lr_mine = i + lane + 1 < p.lr_list_stride ? __ldcg(lr_entries + 1 + i + lane) : 0;
+            const int filled = min(p.lr_pack, lr_count - i);
+            int adapter[4];  // lr_pack divides 32: a group's entries stand in one run of the warp's lanes
 #pragma unroll
-              for (int j = 0; j < 4; ++j) adapter[j] = __shfl_sync(0xffffffffu, lr_mine, (i + j) & 31);
-              for (int kb = 0; kb < p.lr_kblocks; ++kb) {
-                ok = mbar_wait_warp(&empty_bar[s], ph ^ 1, wctx, TB_DEV_TIMEOUT_SMEM_EMPTY);
-                if (!ok) break;
-                uint8_t* sa = ring + static_cast<size_t>(s) * stage_bytes;
-                uint8_t* sb = sa + kATileBytes;
-                const int k0 = kb * p.k_per_stage;
-                if (elect_one()) {
-                  const uint32_t bytes = static_cast<uint32_t>(filled * (a_part + b_part)) * CTAS;
-                  const uint32_t bar = (CTAS == 2) ? mapa_cluster(smem_u32(&full_bar[s]), 0) : 0u;
-                  if (CTAS == 1 || cta_rank == 0) mbar_arrive_expect_tx(&full_bar[s], bytes);
+            for (int j = 0; j < 4; ++j) adapter[j] = __shfl_sync(0xffffffffu, lr_mine, (i + j) & 31);
+            for (int kb = 0; kb < p.lr_kblocks; ++kb) {
+              ok = mbar_wait_warp(&empty_bar[s], ph ^ 1, wctx, TB_DEV_TIMEOUT_SMEM_EMPTY);
+              if (!ok) break;
+              uint8_t* sa = ring + static_cast<size_t>(s) * stage_bytes;
+              uint8_t* sb = sa + kATileBytes;
+              const int k0 = kb * p.k_per_stage;
+              if (elect_one()) {
+                const uint32_t bytes = static_cast<uint32_t>(filled * (a_part + b_part)) * CTAS;
+                const uint32_t bar = (CTAS == 2) ? mapa_cluster(smem_u32(&full_bar[s]), 0) : 0u;
+                if (CTAS == 1 || cta_rank == 0) mbar_arrive_expect_tx(&full_bar[s], bytes);
 #pragma unroll
-                  for (int j = 0; j < 4; ++j) {
-                    if (j >= filled) break;
-                    const int block_row = block_row0 + (i + j) * p.lr_tile_rows;
-                    uint8_t *da = sa + j * a_part, *db = sb + j * b_part;
-                    if constexpr (CTAS == 1) {
-                      if (p.lr_tokens_on_b) {
-                        tma_load_3d(da, &tmap_sfa, &full_bar[s], k0, m0, adapter[j]);
-                        tma_load_2d(db, &tmap_sfb, &full_bar[s], k0, block_row);
-                      } else {
-                        tma_load_2d(da, &tmap_sfa, &full_bar[s], k0, block_row);
-                        tma_load_3d(db, &tmap_sfb, &full_bar[s], k0, n0, adapter[j]);
-                      }
-                    } else {
-                      if (p.lr_tokens_on_b) {
-                        tma_load_3d_pair(da, &tmap_sfa, bar, k0, m0, adapter[j]);
-                        tma_load_2d_pair(db, &tmap_sfb, bar, k0, block_row + static_cast<int>(cta_rank) * bn_local);
-                      } else {
-                        tma_load_2d_pair(da, &tmap_sfa, bar, k0, block_row + static_cast<int>(cta_rank) * kTileM);
-                        tma_load_3d_pair(db, &tmap_sfb, bar, k0, n0, adapter[j]);
-                      }
-                    }
+                for (int j = 0; j < 4; ++j) {
+                  if (j >= filled) break;
+                  const int block_row = block_row0 + (i + j) * p.lr_tile_rows;
+                  uint8_t *da = sa + j * a_part, *db = sb + j * b_part;
+                  if constexpr (CTAS == 1) {
+                    tma_load_2d(da, &tmap_sfa, &full_bar[s], k0, block_row);
+                    tma_load_3d(db, &tmap_sfb, &full_bar[s], k0, n0, adapter[j]);
+                  } else {
+                    tma_load_2d_pair(da, &tmap_sfa, bar, k0, block_row + static_cast<int>(cta_rank) * kTileM);
+                    tma_load_3d_pair(db, &tmap_sfb, bar, k0, n0, adapter[j]);
                   }
                 }
-                __syncwarp();
-                if (++s == stages) {
-                  s = 0;
-                  ph ^= 1;
-                }
+              }
+              __syncwarp();
+              if (++s == stages) {
+                s = 0;
+                ph ^= 1;
               }
             }
           }
@@ -1054,10 +1039,10 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ 
           int lr_count = 0;
           for (int kb = w.kb0; kb < w.kb1; ++kb) {
             if constexpr (LOWRANK) {
-              if (w.kb0 == 0 && kb == max(0, w.kb1 - 8)) {
+              if (kb == max(0, w.kb1 - 8)) {
                 griddep_wait();
-                const TileGeom tg = tile_geometry(p, w.tile, kPairTileM, tile_prefix);
-                lr_count = __ldcg(p.lr_list + static_cast<size_t>((p.lr_tokens_on_b ? tg.n0 : tg.m0) / p.lr_tile_rows) * p.lr_list_stride);
+                const int row_tile = tile_geometry(p, w.tile, kPairTileM, tile_prefix).m0 / p.lr_tile_rows;
+                lr_count = __ldcg(p.lr_list + static_cast<size_t>(row_tile) * p.lr_list_stride);
               }
             }
             const long long pf0 = PROF ? clock64() : 0;
@@ -1101,7 +1086,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ 
                 issue_stage(d0, adesc, bdesc, first);
               }
               commit(&empty_bar[s]);  // frees the stage once every MMA that reads it has finished
-              if (kb + 1 == w.kb1 && (!LOWRANK || w.kb0 != 0)) commit(&tmem_full[acc0]);
+              if (!LOWRANK && kb + 1 == w.kb1) commit(&tmem_full[acc0]);
             }
             __syncwarp();
             if (PROF) prof_issue += clock64() - pf1;
@@ -1112,39 +1097,37 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ 
           }
           if (!ok) break;
           if constexpr (LOWRANK) {
-            if (w.kb0 == 0) {
-              // both extension operands are K-major whatever the product's own layouts are; rows of 128 / lr_pack bytes
-              const uint32_t swizzle = p.lr_pack == 1 ? 2u : (p.lr_pack == 2 ? 4u : 6u), row_group = 1024u / p.lr_pack;
-              const uint64_t xa0 = make_smem_desc(ring_addr, 16u, row_group, swizzle);
-              const uint64_t xb0 = make_smem_desc(ring_addr + kATileBytes, 16u, row_group, swizzle);
-              const uint64_t a_part = (kATileBytes / p.lr_pack) >> 4, b_part = (b_tile_bytes / p.lr_pack) >> 4;
-              const uint32_t x_idesc = idesc & ~(3u << 15);
-              for (int i = 0, kb = 0; i < lr_count;) {
-                ok = mbar_wait_warp(&full_bar[s], ph, wctx, TB_DEV_TIMEOUT_SMEM_FULL);
-                if (!ok) break;
-                if (elect_one()) {
-                  const uint64_t soff = static_cast<uint64_t>(s * stage_step);
-                  const int filled = min(p.lr_pack, lr_count - i);
-                  const int steps = min(4 / p.lr_pack, (p.lr_rank - kb * p.k_per_stage + 15) >> 4);  // behind the rank: zeros
-                  for (int j = 0; j < filled; ++j)
-                    for (int k = 0; k < steps; ++k)
-                      umma<KIND, CTAS>(d0, xa0 + soff + j * a_part + 2 * k, xb0 + soff + j * b_part + 2 * k, x_idesc, 1u);
-                  commit(&empty_bar[s]);
-                }
-                __syncwarp();
-                if (++kb == p.lr_kblocks) {
-                  kb = 0;
-                  i += p.lr_pack;
-                }
-                if (++s == stages) {
-                  s = 0;
-                  ph ^= 1;
-                }
-              }
+            // both extension operands are K-major whatever the product's own layouts are; rows of 128 / lr_pack bytes
+            const uint32_t swizzle = p.lr_pack == 1 ? 2u : (p.lr_pack == 2 ? 4u : 6u), row_group = 1024u / p.lr_pack;
+            const uint64_t xa0 = make_smem_desc(ring_addr, 16u, row_group, swizzle);
+            const uint64_t xb0 = make_smem_desc(ring_addr + kATileBytes, 16u, row_group, swizzle);
+            const uint64_t a_part = (kATileBytes / p.lr_pack) >> 4, b_part = (b_tile_bytes / p.lr_pack) >> 4;
+            const uint32_t x_idesc = idesc & ~(3u << 15);
+            for (int i = 0, kb = 0; i < lr_count;) {
+              ok = mbar_wait_warp(&full_bar[s], ph, wctx, TB_DEV_TIMEOUT_SMEM_FULL);
               if (!ok) break;
-              if (elect_one()) commit(&tmem_full[acc0]);
+              if (elect_one()) {
+                const uint64_t soff = static_cast<uint64_t>(s * stage_step);
+                const int filled = min(p.lr_pack, lr_count - i);
+                const int steps = min(4 / p.lr_pack, (p.lr_rank - kb * p.k_per_stage + 15) >> 4);  // behind the rank: zeros
+                for (int j = 0; j < filled; ++j)
+                  for (int k = 0; k < steps; ++k)
+                    umma<KIND, CTAS>(d0, xa0 + soff + j * a_part + 2 * k, xb0 + soff + j * b_part + 2 * k, x_idesc, 1u);
+                commit(&empty_bar[s]);
+              }
               __syncwarp();
+              if (++kb == p.lr_kblocks) {
+                kb = 0;
+                i += p.lr_pack;
+              }
+              if (++s == stages) {
+                s = 0;
+                ph ^= 1;
+              }
             }
+            if (!ok) break;
+            if (elect_one()) commit(&tmem_full[acc0]);
+            __syncwarp();
           }
           acc_parity ^= 1u << acc0;
           acc ^= 1;
@@ -1213,7 +1196,6 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ 
     const uint32_t tmem_empty_remote = (CTAS == 2) ? mapa_cluster(smem_u32(&tmem_empty[0]), 0) : 0u;
     bool ok = true;
     long long prof_wait = 0, prof_t0 = clock64(), prof_drain = 0;
-    if constexpr (LOWRANK) griddep_wait();  // the stream-K flags were zeroed by the kernel before this one
     int seq = 0;
     auto next_item = [&]() -> WorkItem {
       if (!dyn) return wi.next();

@@ -1,15 +1,16 @@
 // A shared projection with one low-rank adapter per row (the requests of a batch, each with its own):
 //     out[t] = x[t] W + bias + s_a (x[t] A_a^T) B_a^T,   a = adapter_ids[t]  (outside [0, num_adapters): no adapter)
 //
-// Two launches. lora_project_kernel forms v[t] = s_a x[t] A_a^T (rank numbers per row) and lays it out for the second one: for
-// every tile of rows that the GEMM works on, the list of the adapters that occur in it and, per listed adapter, a block of the
-// tile's rows that holds v in that adapter's rows and zeros in all others. The GEMM (gemm_kernel, LOWRANK) then walks those
-// blocks against the adapters' B as further K stages of the same tile, so the update costs its bytes and no pass over the
-// output, and the sum is rounded once. The GEMM starts while the projection still runs.
+// Two launches. The first one forms v[t] = s_a x[t] A_a^T (rank numbers per row) and lays it out for the second: for every tile of
+// rows that the product works on, the list of the adapters that occur in it and, per listed adapter, a block of the tile's rows
+// that holds v in that adapter's rows and zeros in all others. The product (lora_decode.cu up to 64 rows, gemm_kernel with
+// LOWRANK above) then walks those blocks against the adapters' B as further K stages of the same tile, so the update costs its
+// bytes and no pass over the output, and the sum is rounded once. It starts while the first launch still runs. No CTA of
+// either waits for one outside its own cluster, so calls on several streams cannot block each other.
 //
-// The projection is bound by reading x and the used adapters' A once; it has a form for decode batches (up to 64 rows, mostly
-// one adapter each) and one for longer ones. v is rounded to the operands' 16-bit type once, after the scale: it is the A operand of a tensor-core product.
-// Its error is eps / 2 of each of `rank` terms of the update, next to the one rounding of the output.
+// The projection is bound by reading x and the used adapters' A once; it has a form for decode batches (mostly one adapter per
+// row) and one for longer ones. v is rounded to the operands' 16-bit type once, after the scale: it is an operand of a tensor-core
+// product. Its error is eps / 2 of each of `rank` terms of the update, next to the one rounding of the output.
 // No reference counterpart (the reference has no adapters).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -17,7 +18,7 @@
 #include <mutex>
 
 #include "common_host.h"
-#include "selector.h"
+#include "selector.h"  // the SM count when there is no device
 #include "ptx.cuh"
 
 namespace tb {
@@ -32,7 +33,7 @@ constexpr int kMaxRank = 128;
 constexpr int kMaxStages = 6;
 constexpr int kMaxTileRows = 256;
 constexpr int kTableBits = 9, kTable = 1 << kTableBits;
-constexpr long long kFlagBytes = 4096;  // stream-K flags at the start of the GEMM's workspace
+constexpr long long kCounterBytes = 4096;  // four counters per dealt tile, of which there are fewer than SMs
 
 struct ProjectParams {
   const void* x;
@@ -50,8 +51,8 @@ struct ProjectParams {
   int k_chunk;          // K per CTA, a multiple of 32
   void* v;
   int* list;            // [tiles][1 + max_slots]
-  unsigned* flags;      // stream-K flags to clear
-  int flag_words;
+  unsigned* counters;   // of the decode kernel, to clear
+  int counter_words;
   // tensor-core form
   int rank_pad;         // rank rounded up to 16
   int stages, stage_bytes, tmem_cols;
@@ -237,7 +238,7 @@ __global__ void __launch_bounds__(kThreads, 2) lora_project_kernel(const Project
   griddep_launch_dependents();
 
   if (blockIdx.x == 0 && blockIdx.y == 0)
-    for (int i = tid; i < p.flag_words; i += kThreads) p.flags[i] = 0u;
+    for (int i = tid; i < p.counter_words; i += kThreads) p.counters[i] = 0u;
   const int2 found = find_adapters<kRows>(p, lists, row0, row0 == tile_row0 && blockIdx.y == 0 && rank == 0);
   const int* run_ids = lists.ids + (row0 - tile_row0);
   T* tile_blocks = static_cast<T*>(p.v) + static_cast<long long>(tile) * p.max_slots * p.tile_rows * p.v_cols +
@@ -358,8 +359,6 @@ lora_project_tc_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_
   griddep_wait();
   griddep_launch_dependents();
 
-  if (blockIdx.x == 0 && blockIdx.y == 0)
-    for (int i = tid; i < p.flag_words; i += kThreads) p.flags[i] = 0u;
   const int2 found = find_adapters<kRows>(p, lists, row0, row0 == tile_row0 && blockIdx.y == 0 && cta == 0);
   const int* run_ids = lists.ids + (row0 - tile_row0);
   T* tile_blocks = static_cast<T*>(p.v) + static_cast<long long>(tile) * p.max_slots * p.tile_rows * p.v_cols +
@@ -449,7 +448,7 @@ lora_project_tc_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[j] *= scale;
       }
-      T o[8];
+      alignas(16) T o[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) o[j] = cast16<T>(v[j]);
       *reinterpret_cast<uint4*>(block + static_cast<long long>(r) * p.v_cols + c) = *reinterpret_cast<const uint4*>(o);
@@ -564,7 +563,6 @@ struct LoraPlan {
   bool decode;
   LoraDecodeShape shape;  // decode
   tb_config cfg;          // otherwise
-  int streamk;
   int tile_rows, tiles, max_slots, v_cols, pack;
   long long v_offset, v_rows, list_offset, gemm_offset, gemm_bytes, bytes;
 };
@@ -578,19 +576,14 @@ int lora_plan(const tb_lora_args& a, int num_sms, tb_gemm_args* g, LoraPlan* l) 
   g->c = a.out; g->c_stride_m = a.out_stride_m; g->c_stride_n = a.out_stride_n;
   g->bias = a.bias; g->bias_stride = a.bias_stride; g->bias_dtype = a.bias_dtype;
   g->wait_timeout_ms = a.wait_timeout_ms;
-  // decode batches on K-contiguous weights have a kernel of their own
-  l->decode = a.m <= 64 && a.w_stride_k == 1;
+  l->decode = a.m <= 64;
   if (l->decode) {
     l->shape = lora_decode_shape(a.m, a.n, num_sms);
-    l->streamk = 0;
     l->tile_rows = l->shape.cols;
   } else {
-    const int rc = low_rank_config(*g, &l->cfg, &l->streamk);
+    const int rc = low_rank_config(*g, &l->cfg);
     if (rc != TB_OK) return rc;
-    const int pair = l->cfg.cta_pair == 2 ? 2 : 1;
-    // A decode batch's projection runs beside the GEMM: leave shared memory for one of its blocks on every SM.
-    while (a.m <= 64 && l->cfg.stages > 3 && smem_bytes_for(l->cfg.block_n, pair, l->cfg.stages) > 200 * 1024) --l->cfg.stages;
-    l->tile_rows = l->cfg.swap_ab ? l->cfg.block_n : 128 * pair;
+    l->tile_rows = 128 * (l->cfg.cta_pair == 2 ? 2 : 1);
   }
   l->tiles = (a.m + l->tile_rows - 1) / l->tile_rows;
   l->max_slots = l->tile_rows < a.num_adapters ? l->tile_rows : a.num_adapters;
@@ -601,8 +594,8 @@ int lora_plan(const tb_lora_args& a, int num_sms, tb_gemm_args* g, LoraPlan* l) 
   if (l->v_rows > 0x7fffffffll) return TB_ERR_UNSUPPORTED;  // a row coordinate of a copy has 32 bits; shorter batches fit
   auto up = [](long long v) { return (v + 255) & ~255ll; };
   l->gemm_offset = 0;
-  // flags or counters (cleared by the projection) at the front, then partial tiles
-  l->gemm_bytes = l->decode ? kFlagBytes + up(l->shape.part_bytes) : (l->streamk ? up(tb_gemm_workspace_bytes(&l->cfg, 0)) : 0);
+  // decode: counters (cleared by the projection) at the front, then partial tiles
+  l->gemm_bytes = l->decode ? kCounterBytes + up(l->shape.part_bytes) : 0;
   l->list_offset = l->gemm_bytes;
   l->v_offset = l->list_offset + up(4ll * l->tiles * (1 + l->max_slots));
   l->bytes = l->v_offset + up(l->v_rows * l->v_cols * 2);
@@ -610,8 +603,9 @@ int lora_plan(const tb_lora_args& a, int num_sms, tb_gemm_args* g, LoraPlan* l) 
 }
 
 bool lora_sizes_ok(const tb_lora_args& a) {
-  return a.m >= 0 && a.n >= 0 && a.k >= 8 && a.k % 8 == 0 && a.rank >= 8 && a.rank % 8 == 0 && a.rank <= kMaxRank &&
-         a.num_adapters >= 1 && (a.dtype == TB_DTYPE_BF16 || a.dtype == TB_DTYPE_F16);
+  // row, tile and stage numbers have 32 bits; so has the sum of all dealt tiles' stages, fewer tiles than SMs of k / 64 each
+  return a.m >= 0 && a.m <= (1 << 30) && a.n >= 0 && a.n <= (1 << 30) && a.k >= 8 && a.k <= (1 << 28) && a.k % 8 == 0 && a.rank >= 8 &&
+         a.rank % 8 == 0 && a.rank <= kMaxRank && a.num_adapters >= 1 && (a.dtype == TB_DTYPE_BF16 || a.dtype == TB_DTYPE_F16);
 }
 
 int lora_impl(const tb_lora_args& a, cudaStream_t stream) {
@@ -621,7 +615,7 @@ int lora_impl(const tb_lora_args& a, cudaStream_t stream) {
   if (a.x == nullptr || a.w == nullptr || a.lora_a == nullptr || a.lora_b == nullptr || a.adapter_ids == nullptr || a.out == nullptr)
     return TB_ERR_INVALID;
   if ((a.m > 1 && a.x_row_stride < a.k) || a.lora_a_row_stride < a.k || a.lora_b_row_stride < a.rank || a.lora_a_adapter_stride < 0 ||
-      a.lora_b_adapter_stride < 0 || (a.w_stride_k != 1 && a.w_stride_n != 1))
+      a.lora_b_adapter_stride < 0 || (a.w_stride_k == 1 ? a.n > 1 && a.w_stride_n < a.k : a.w_stride_n != 1 || a.w_stride_k < a.n))
     return TB_ERR_INVALID;
   const uintptr_t addresses = reinterpret_cast<uintptr_t>(a.x) | reinterpret_cast<uintptr_t>(a.w) | reinterpret_cast<uintptr_t>(a.lora_a) |
                               reinterpret_cast<uintptr_t>(a.lora_b) | reinterpret_cast<uintptr_t>(a.workspace);
@@ -656,14 +650,14 @@ int lora_impl(const tb_lora_args& a, cudaStream_t stream) {
   p.tile_rows = l.tile_rows; p.max_slots = l.max_slots; p.v_cols = l.v_cols;
   p.v = ws + l.v_offset;
   p.list = reinterpret_cast<int*>(ws + l.list_offset);
-  p.flags = reinterpret_cast<unsigned*>(ws + l.gemm_offset);
-  p.flag_words = l.decode ? 4 * l.shape.dealt_tiles : (l.streamk ? static_cast<int>(kFlagBytes / 4) : 0);
+  p.counters = reinterpret_cast<unsigned*>(ws + l.gemm_offset);
+  p.counter_words = l.decode ? 4 * l.shape.dealt_tiles : 0;
   p.status = status;
   p.timeout_ns = a.wait_timeout_ms > 0 ? static_cast<unsigned long long>(a.wait_timeout_ms) * 1000000ull : 2000000000ull;
   // Runs cover whole tiles: the rows behind the last token are zeros in every block. A decode batch has up to one adapter per
   // row: they are dealt over blocks first, and K is split as long as the blocks fit the SMs at once, two on each. Longer batches have
   // few adapters per run: K is split first, up to a block per SM, and what is left of two per SM takes the adapters.
-  const bool decode = a.m <= 64;
+  const bool decode = l.decode;
   const int rows = decode ? 16 : 128;
   const int runs = l.tiles * (l.tile_rows / rows);
   const int live_runs = (a.m + rows - 1) / rows;
@@ -682,10 +676,6 @@ int lora_impl(const tb_lora_args& a, cudaStream_t stream) {
   else rc = a.dtype == TB_DTYPE_BF16 ? project_tc<__nv_bfloat16>(a, p, runs, stripes, device, stream) : project_tc<__half>(a, p, runs, stripes, device, stream);
   if (rc != TB_OK) return rc;
 
-  g.streamk = l.streamk;
-  g.workspace = ws + l.gemm_offset;
-  g.workspace_bytes = l.gemm_bytes;
-  g.epoch = 1;  // the projection clears the flags of every call
   LowRank lr = {};
   lr.v = p.v;
   lr.v_rows = l.v_rows;
@@ -700,7 +690,7 @@ int lora_impl(const tb_lora_args& a, cudaStream_t stream) {
   lr.n = a.n;
   lr.list = p.list;
   lr.list_stride = 1 + l.max_slots;
-  if (l.decode) return lora_decode(a, l.shape, lr, ws + l.gemm_offset + kFlagBytes, ws + l.gemm_offset, device, smem_optin, status, stream);
+  if (l.decode) return lora_decode(a, l.shape, lr, ws + l.gemm_offset + kCounterBytes, ws + l.gemm_offset, device, smem_optin, status, stream);
   return gemm_low_rank(g, l.cfg, lr, stream);
 }
 

@@ -1,5 +1,4 @@
-// The shared projection of a decode batch (up to 64 rows) with its rows' low-rank updates: the second launch of lora.cu for
-// K-contiguous weights.
+// The shared projection of a decode batch (up to 64 rows) with its rows' low-rank updates: the second launch of lora.cu.
 //     out[t, n] = sum_k x[t, k] W[k, n] + bias[n] + sum over the listed adapters a of sum_r v_a[t, r] B_a[n, r]
 // v_a is what the first launch wrote: the rows' scaled rank-sized products, zero in rows of other adapters.
 //
@@ -41,6 +40,7 @@ struct DecodeParams {
   int stages, stage_bytes;
   int acc_stride, tmem_cols;
   int nkb;              // stages per tile
+  int w_mn;             // 1: W is stored with its output features contiguous
   int full_tiles, dealt_tiles;
   // low-rank update
   const int* list;      // number of adapters, then their indices
@@ -208,7 +208,12 @@ lora_decode_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
         if (elect_one()) {
           uint8_t* dst = ring + static_cast<size_t>(s) * p.stage_bytes;
           mbar_arrive_expect_tx(&full_bar[s], kWeightBytes);
-          tma_load_2d_hint(dst, &tmap_w, &full_bar[s], kb * kStageK, u.tile * kTile, policy);
+          if (p.w_mn) {  // 64 features x 64 K rows per copy, one 128-byte row per K
+            tma_load_2d_hint(dst, &tmap_w, &full_bar[s], u.tile * kTile, kb * kStageK, policy);
+            tma_load_2d_hint(dst + kWeightBytes / 2, &tmap_w, &full_bar[s], u.tile * kTile + 64, kb * kStageK, policy);
+          } else {
+            tma_load_2d_hint(dst, &tmap_w, &full_bar[s], kb * kStageK, u.tile * kTile, policy);
+          }
         }
         __syncwarp();
         if (++s == p.stages) {
@@ -292,7 +297,10 @@ lora_decode_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
     uint32_t ph = 0, acc_parity = 0;
     bool ok = true;
     const uint32_t ring_addr = smem_u32(ring);
-    const uint64_t desc0 = make_smem_desc(ring_addr, 16, 1024);
+    // W: K-contiguous rows of 128 bytes, or 64-feature columns of 64 K rows, 8 KB apart; a step of 16 K is 32 bytes or 16 rows on
+    const uint64_t w0 = make_smem_desc(ring_addr, p.w_mn ? kWeightBytes / 2 : 16u, 1024), x0 = make_smem_desc(ring_addr + kWeightBytes, 16, 1024);
+    const uint64_t w_step = p.w_mn ? 16 * kRowBytes >> 4 : 2;
+    const uint32_t idesc = p.idesc | (p.w_mn ? 1u << 15 : 0u);
     const uint32_t swizzle = p.pack == 1 ? 2u : (p.pack == 2 ? 4u : 6u), row_group = 1024u / p.pack;
     const uint64_t xa0 = make_smem_desc(ring_addr, 16, row_group, swizzle), xb0 = make_smem_desc(ring_addr + kWeightBytes, 16, row_group, swizzle);
     for (Unit u = units.next(); u.kind != 0 && ok; u = units.next()) {
@@ -310,10 +318,9 @@ lora_decode_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
         ok = wait_warp(&full_bar[s], ph, wctx, TB_DEV_TIMEOUT_SMEM_FULL);
         if (!ok) break;
         if (elect_one()) {
-          const uint64_t stage = desc0 + static_cast<uint64_t>((s * p.stage_bytes) >> 4);
+          const uint64_t soff = static_cast<uint64_t>((s * p.stage_bytes) >> 4);
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
-            umma<0, 1>(d, stage + 2 * k, stage + (kWeightBytes >> 4) + 2 * k, p.idesc, (k > 0 || kb > u.kb0) ? 1u : 0u);
+          for (int k = 0; k < 4; ++k) umma<0, 1>(d, w0 + soff + k * w_step, x0 + soff + 2 * k, idesc, (k > 0 || kb > u.kb0) ? 1u : 0u);
           umma_commit(&empty_bar[s]);
           if (u.kind == 1 && kb + 1 == u.kb1) umma_commit(&tmem_full[acc]);
         }
@@ -555,7 +562,9 @@ int lora_decode(const tb_lora_args& a, const LoraDecodeShape& s, const LowRank& 
   p.idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | (static_cast<uint32_t>(s.cols >> 3) << 17) | (static_cast<uint32_t>(kTile >> 4) << 24);
 
   CUtensorMap tw, tx, tb_, tv;
-  int rc = encode_2d(&tw, a.dtype, a.w, a.k, a.n, static_cast<uint64_t>(a.n > 1 ? a.w_stride_n : a.k) * 2, kStageK, kTile, 1);
+  p.w_mn = a.w_stride_k == 1 ? 0 : 1;
+  int rc = p.w_mn ? encode_2d(&tw, a.dtype, a.w, a.n, a.k, static_cast<uint64_t>(a.w_stride_k) * 2, 64, kStageK, 1)
+                  : encode_2d(&tw, a.dtype, a.w, a.k, a.n, static_cast<uint64_t>(a.n > 1 ? a.w_stride_n : a.k) * 2, kStageK, kTile, 1);
   if (rc != TB_OK) return rc;
   if ((rc = encode_2d(&tx, a.dtype, a.x, a.k, a.m, static_cast<uint64_t>(a.m > 1 ? a.x_row_stride : a.k) * 2, kStageK, a.m, 1)) != TB_OK) return rc;
   const uint32_t inner = static_cast<uint32_t>(kStageK / lr.pack);

@@ -75,9 +75,10 @@ def lora_matmul(x, w, lora_a, lora_b, adapter_ids, scales=None, bias=None, out: 
     w_k, w_n = w.stride()
     if w_k != 1 or w_n < k or w_n % 8 or w.data_ptr() % 16:     # anything but the fast layout
         w = _unit_stride_2d(w)
-        if not _tma_loadable(w):
-            w = _repitch(w)
         w_k, w_n = _strides(w)
+        if not _tma_loadable(w) or (w_n < k if w_k == 1 else w_k < n):     # or rows that overlap: an expanded w
+            w = _repitch(w)
+            w_k, w_n = _strides(w)
     ids = adapter_ids.contiguous()
     if scales is not None:
         scales = scales.to(torch.float32).contiguous()
