@@ -144,6 +144,22 @@ def test_signed_zeros_tie_and_large_values():
     assert torch.isfinite(w).all() and torch.allclose(w.sum(1), torch.ones(2, device="cuda"))
 
 
+def test_an_infinite_logit_stays_in_its_row():
+    """+inf: the softmax of its row is NaN by the formula, its sigmoid is 1; other rows of the same warp know nothing of it."""
+    for experts in (16, 60, 200, 600):
+        l = make(40, experts, torch.float32, mask=False)
+        l[7, 3] = float("inf")
+        keep = [t for t in range(40) if t != 7]
+        clean = l.clone()
+        clean[7, 3] = 100.0
+        for renormalize in (True, False):
+            w, ids = tb.moe_route(l, 4, renormalize=renormalize)
+            ref_w, ref_ids = tb.moe_route(clean, 4, renormalize=renormalize)
+            assert torch.isnan(w[7]).all() and torch.equal(w[keep], ref_w[keep]) and torch.equal(ids, ref_ids)
+        w, ids = tb.moe_route(l, 4, scoring="sigmoid", renormalize=False)
+        assert w[7, 0] == 1 and ids[7, 0] == 3 and torch.isfinite(w).all()
+
+
 def test_capture_and_replay_and_compile():
     logits = make(64, 64, torch.bfloat16, mask=False)
     side = torch.cuda.Stream()

@@ -672,8 +672,11 @@ int lora_impl(const tb_lora_args& a, cudaStream_t stream) {
   }
   const int k_unit = decode ? 32 : 64;
   p.k_chunk = ((a.k + p.splits - 1) / p.splits + k_unit - 1) / k_unit * k_unit;
-  if (decode) rc = a.dtype == TB_DTYPE_BF16 ? project_decode<__nv_bfloat16>(p, runs, stripes, device, stream) : project_decode<__half>(p, runs, stripes, device, stream);
-  else rc = a.dtype == TB_DTYPE_BF16 ? project_tc<__nv_bfloat16>(a, p, runs, stripes, device, stream) : project_tc<__half>(a, p, runs, stripes, device, stream);
+  const bool bf16 = a.dtype == TB_DTYPE_BF16;
+  if (decode)
+    rc = bf16 ? project_decode<__nv_bfloat16>(p, runs, stripes, device, stream) : project_decode<__half>(p, runs, stripes, device, stream);
+  else
+    rc = bf16 ? project_tc<__nv_bfloat16>(a, p, runs, stripes, device, stream) : project_tc<__half>(a, p, runs, stripes, device, stream);
   if (rc != TB_OK) return rc;
 
   LowRank lr = {};
@@ -690,7 +693,8 @@ int lora_impl(const tb_lora_args& a, cudaStream_t stream) {
   lr.n = a.n;
   lr.list = p.list;
   lr.list_stride = 1 + l.max_slots;
-  if (l.decode) return lora_decode(a, l.shape, lr, ws + l.gemm_offset + kCounterBytes, ws + l.gemm_offset, device, smem_optin, status, stream);
+  if (l.decode)
+    return lora_decode(a, l.shape, lr, ws + l.gemm_offset + kCounterBytes, ws + l.gemm_offset, device, smem_optin, status, stream);
   return gemm_low_rank(g, l.cfg, lr, stream);
 }
 

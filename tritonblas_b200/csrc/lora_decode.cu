@@ -298,11 +298,13 @@ lora_decode_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
     bool ok = true;
     const uint32_t ring_addr = smem_u32(ring);
     // W: K-contiguous rows of 128 bytes, or 64-feature columns of 64 K rows, 8 KB apart; a step of 16 K is 32 bytes or 16 rows on
-    const uint64_t w0 = make_smem_desc(ring_addr, p.w_mn ? kWeightBytes / 2 : 16u, 1024), x0 = make_smem_desc(ring_addr + kWeightBytes, 16, 1024);
+    const uint64_t w0 = make_smem_desc(ring_addr, p.w_mn ? kWeightBytes / 2 : 16u, 1024);
+    const uint64_t x0 = make_smem_desc(ring_addr + kWeightBytes, 16, 1024);
     const uint64_t w_step = p.w_mn ? 16 * kRowBytes >> 4 : 2;
     const uint32_t idesc = p.idesc | (p.w_mn ? 1u << 15 : 0u);
     const uint32_t swizzle = p.pack == 1 ? 2u : (p.pack == 2 ? 4u : 6u), row_group = 1024u / p.pack;
-    const uint64_t xa0 = make_smem_desc(ring_addr, 16, row_group, swizzle), xb0 = make_smem_desc(ring_addr + kWeightBytes, 16, row_group, swizzle);
+    const uint64_t xa0 = make_smem_desc(ring_addr, 16, row_group, swizzle);
+    const uint64_t xb0 = make_smem_desc(ring_addr + kWeightBytes, 16, row_group, swizzle);
     for (Unit u = units.next(); u.kind != 0 && ok; u = units.next()) {
       if (u.kind == 3) {
         if (count < 0) read_list();
@@ -566,7 +568,8 @@ int lora_decode(const tb_lora_args& a, const LoraDecodeShape& s, const LowRank& 
   int rc = p.w_mn ? encode_2d(&tw, a.dtype, a.w, a.n, a.k, static_cast<uint64_t>(a.w_stride_k) * 2, 64, kStageK, 1)
                   : encode_2d(&tw, a.dtype, a.w, a.k, a.n, static_cast<uint64_t>(a.n > 1 ? a.w_stride_n : a.k) * 2, kStageK, kTile, 1);
   if (rc != TB_OK) return rc;
-  if ((rc = encode_2d(&tx, a.dtype, a.x, a.k, a.m, static_cast<uint64_t>(a.m > 1 ? a.x_row_stride : a.k) * 2, kStageK, a.m, 1)) != TB_OK) return rc;
+  rc = encode_2d(&tx, a.dtype, a.x, a.k, a.m, static_cast<uint64_t>(a.m > 1 ? a.x_row_stride : a.k) * 2, kStageK, a.m, 1);
+  if (rc != TB_OK) return rc;
   const uint32_t inner = static_cast<uint32_t>(kStageK / lr.pack);
   const uint64_t v_cols = static_cast<uint64_t>(lr.kblocks) * inner;
   const uint64_t v_dims[2] = {v_cols, static_cast<uint64_t>(lr.v_rows)}, v_strides[1] = {v_cols * 2};

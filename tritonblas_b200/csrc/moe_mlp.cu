@@ -3,7 +3,8 @@
 //
 // With at most 128 tokens every weight of an expert meets a handful of rows, so the layer is bound by reading the chosen
 // experts' weights once: (distinct experts) * 3 * ffn * hidden * 2 bytes. Two launches:
-//   moe_mlp_plan_kernel  one CTA (one warp up to 32 pairs): the distinct (expert, token) rows in expert order, the counters of the next launch zeroed;
+//   moe_mlp_plan_kernel  one CTA (one warp up to 32 pairs): the distinct (expert, token) rows in expert order, the counters
+//                        of the next launch zeroed;
 //   moe_mlp_kernel       one persistent CTA per SM that works through three kinds of units, taken in order from a counter:
 //     1  (expert, tile of ffn)     D[feature, token] = W1 tile . X^T, silu(gate) * up in the epilogue, h in 16-bit pairs;
 //     2  (row group, tile of hidden) D[hidden, row]  = W2 tile . H^T, times the routing weight, fp32 to the workspace;
@@ -220,7 +221,8 @@ moe_mlp_plan_warp_kernel(const void* __restrict__ ids, int is64, const float* __
   // lanes with the same expert, and those of them in the same token; the first of the latter owns the row
   const unsigned same = __match_any_sync(kFull, e);
   const int first_lane = t * topk;
-  const unsigned token_lanes = (first_lane < 32 ? kFull << first_lane : 0u) & (first_lane + topk < 32 ? ~(kFull << (first_lane + topk)) : kFull);
+  const int last_lane = first_lane + topk;
+  const unsigned token_lanes = (first_lane < 32 ? kFull << first_lane : 0u) & (last_lane < 32 ? ~(kFull << last_lane) : kFull);
   const unsigned repeats = same & token_lanes;
   const bool own = e >= 0 && lane == __ffs(repeats) - 1;
   float sum = w;
@@ -546,7 +548,8 @@ moe_mlp_kernel(const __grid_constant__ CUtensorMap tmap_w1, const __grid_constan
         if (u.kind == 1) {
 #pragma unroll
           for (int b = 0; b < kSlabs1; ++b)
-            tma_load_5d_hint(dst + b * M1 * kRowBytes, &tmap_w1, &full_bar[s], (kb * kSlabs1 + b) * kStageK, 0, 0, u.tile * (M1 / 16), u.expert, policy);
+            tma_load_5d_hint(dst + b * M1 * kRowBytes, &tmap_w1, &full_bar[s], (kb * kSlabs1 + b) * kStageK, 0, 0, u.tile * (M1 / 16),
+                             u.expert, policy);
         } else {
 #pragma unroll
           for (int b = 0; b < kSlabs2; ++b)
@@ -986,7 +989,8 @@ int mlp_impl(const tb_moe_mlp_args& a, cudaStream_t stream) {
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     lc.numAttrs = 1;
   }
-  cudaError_t e = cudaLaunchKernelEx(&lc, one_warp ? moe_mlp_plan_warp_kernel : (narrow ? moe_mlp_plan_kernel<256> : moe_mlp_plan_kernel<kMlpMaxExperts>), a.topk_ids, static_cast<int>(a.ids_are_int64 != 0), a.topk_weights,
+  auto plan = one_warp ? moe_mlp_plan_warp_kernel : (narrow ? moe_mlp_plan_kernel<256> : moe_mlp_plan_kernel<kMlpMaxExperts>);
+  cudaError_t e = cudaLaunchKernelEx(&lc, plan, a.topk_ids, static_cast<int>(a.ids_are_int64 != 0), a.topk_weights,
                                      static_cast<int>(a.tokens), static_cast<int>(a.topk), static_cast<int>(a.num_experts),
                                      s.group_cap, s.lay, p.ws);
   if (e != cudaSuccess) return cuda_fail(e, "moe_mlp_plan_kernel launch");

@@ -119,7 +119,9 @@ def moe_route(logits, topk, scoring="softmax", renormalize=True):
     first, ties to the lowest index. A weight is the expert's softmax (``scoring="sigmoid"``: sigmoid) score, computed in
     float32; with ``renormalize`` a row's weights are divided by their sum. An expert whose logit is -inf (masked) or NaN is
     never chosen; a row with fewer than ``topk`` others gets id -1 and weight 0 in the remaining places, which every expert path
-    of this package skips. At most 1024 experts and ``topk`` 32. The weights are differentiable in the logits.
+    of this package skips. A logit of +inf makes its row's softmax weights NaN, as the formula does. At most 1024 experts and
+    ``topk`` 32. The weights are differentiable in the logits, once; a backward pass that is captured into a CUDA graph must not
+    share leaves with the autograd graph of an earlier eager pass that is still referenced, as anywhere in torch.
     """
     if logits.ndim != 2:
         refuse("logits must be (tokens, experts)")
@@ -150,7 +152,7 @@ def moe_mlp(x, w1, w2, topk_ids, topk_weights, out: Optional[torch.Tensor] = Non
     x: (tokens, hidden); w1: (experts, 2*ffn, hidden) and w2: (experts, hidden, ffn), the layout ``PeerMemoryMoE`` takes; all
     float16 or all bfloat16, hidden and ffn multiples of 8. topk_ids: (tokens, topk) int32 or int64, topk_weights: (tokens, topk),
     as ``moe_route`` returns them. An id outside [0, experts) adds nothing; the same id twice counts twice. Sums, activation and
-    weighting are float32 with one cast at the end. ``out`` may be given: (tokens, hidden), contiguous rows, no overlap with the
+    weighting are float32 with one cast at the end; silu(gate) * up itself has the operands' range (float16: infinite above 65504). ``out`` may be given: (tokens, hidden), contiguous rows, no overlap with the
     weights. Inference only. More tokens: ``distributed.PeerMemoryMoE``.
     """
     if x.ndim != 2 or w1.ndim != 3 or w2.ndim != 3 or topk_ids.ndim != 2:
