@@ -469,7 +469,7 @@ lora_project_tc_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_
 
 // One launch of either kernel: clusters of p.splits CTAs, programmatic dependent launch as the GEMM kernels use it.
 // The carve-out is asked for at its largest: an SM keeps the division between L1 and shared memory while blocks run on it, and the
-// second launch's blocks are to join these (1 row of 4096 x 4096: 15.0 -> 14.5 us).
+// second launch's blocks are to join these (1 row of 4096 x 4096: 15.0 -> 14.5 us at the time).
 template <typename K>
 int prefer_shared(K kernel, int device, bool (&done)[64]) {
   static std::mutex mu;
@@ -655,18 +655,24 @@ int lora_impl(const tb_lora_args& a, cudaStream_t stream) {
   p.status = status;
   p.timeout_ns = a.wait_timeout_ms > 0 ? static_cast<unsigned long long>(a.wait_timeout_ms) * 1000000ull : 2000000000ull;
   // Runs cover whole tiles: the rows behind the last token are zeros in every block. A decode batch has up to one adapter per
-  // row: they are dealt over blocks first, and K is split as long as the blocks fit the SMs at once, two on each. Longer batches have
-  // few adapters per run: K is split first, up to a block per SM, and what is left of two per SM takes the adapters.
+  // row: they are dealt over blocks first, and K is split as long as there is one block per SM, with an eighth to spare for where
+  // clusters do not fit: beside a second one the product's block would have no registers (64 rows of 4096 x 8192, 64 adapters of
+  // rank 16: 32.7 us, 34.5 with up to 148 blocks, 37 with 296; 32 rows: 25.2 / 26.3 / 30). Longer batches have few adapters per
+  // run: K is split first, up to a block per SM, and what is left of two per SM takes the adapters.
   const bool decode = l.decode;
   const int rows = decode ? 16 : 128;
   const int runs = l.tiles * (l.tile_rows / rows);
   const int live_runs = (a.m + rows - 1) / rows;
   const int most = rows < l.max_slots ? rows : l.max_slots;
-  const int budget = decode ? 2 * num_sms : num_sms;
-  int stripes = decode ? (most < a.m ? most : a.m) : 1;
+  int stripes = 1;
   p.splits = 1;
-  while (p.splits < 8 && live_runs * stripes * p.splits * 2 <= budget && a.k / (p.splits * 2) >= 256) p.splits *= 2;
-  if (!decode) {
+  if (decode) {
+    stripes = most < a.m ? most : a.m;
+    const int by_blocks = num_sms * 7 / 8 / (live_runs * stripes), by_k = a.k / 256;
+    p.splits = by_blocks < by_k ? by_blocks : by_k;
+    p.splits = p.splits < 1 ? 1 : (p.splits > 8 ? 8 : p.splits);
+  } else {
+    while (p.splits < 8 && live_runs * p.splits * 2 <= num_sms && a.k / (p.splits * 2) >= 256) p.splits *= 2;
     stripes = 2 * num_sms / (live_runs * p.splits);
     stripes = stripes < 1 ? 1 : (stripes > most ? most : stripes);
   }

@@ -7,15 +7,18 @@
 // rounds of the SMs are worked on one per CTA; the K range of the others is dealt evenly over all CTAs, so every CTA reads
 // the same number of bytes, and their parts meet in the workspace: each warp of the epilogue counts itself in for its quarter
 // of the tile, and the one that comes last adds the parts up in a fixed order. Nobody waits for another CTA.
-// The parts come first, then the dealt tiles' updates, which need the first launch to be through, then the whole tiles with
-// theirs: the sums over parts are hidden behind the whole tiles where there are any.
+// The parts come first, the ones that take a dealt tile's update last among them, then the whole tiles: the sums over parts are
+// hidden behind the whole tiles where there are any.
 //
-// Measured back to back: 1 row of 4096 x 4096, rank 16: 15.0 us (19.5 with the general GEMM and the same update); 48 rows of 8192
-// x 28672, 30 adapters of rank 16: 88 us, 5.8 TB/s (101); 1 row of 8192 x 28672: 72.7 us, 0.99 of the copy rate.
+// Measured back to back: 1 row of 4096 x 4096, rank 16: 12.9 us (19.5 with the general GEMM and the same update); 48 rows of 8192
+// x 28672, 30 adapters of rank 16: 89 us, 5.7 TB/s (101); 1 row of 8192 x 28672: 73-77 us, 0.95 of the copy rate; n-contiguous
+// weights within 2 %. A unit of its own for the updates instead of the last parts, and parts written only once the first launch
+// is through, took 15.0 us for 1 row of 4096 x 4096 and 37 instead of 33 for 64 rows of 4096 x 8192 with 64 adapters.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
 #include <mutex>
+#include <type_traits>
 
 #include "common_host.h"
 #include "ptx.cuh"
@@ -45,13 +48,14 @@ struct DecodeParams {
   // low-rank update
   const int* list;      // number of adapters, then their indices
   int max_slots, pack, kblocks, rank;
-  float* parts;         // [2 * grid + dealt_tiles][tokens][kTile]
+  float* parts;         // [2 * grid][tokens][kTile]
   unsigned* arrived;    // [dealt_tiles][4], cleared by the first launch
   const void* bias;
   long long bias_stride;
   int bias_dtype;
   void* out;
   long long out_m, out_n;
+  int out_vec;          // four consecutive outputs stand on an 8-byte boundary
   uint32_t idesc;
   int* status;
   unsigned long long timeout_ns;
@@ -72,31 +76,32 @@ struct Deal {
   }
 };
 
-// What a CTA works on, in order; every role walks the same sequence.
+// What a CTA works on, in order; every role walks the same sequence. Its run of dealt stages is at most one tile long, so it has
+// at most two parts: the end of a tile's K range, or a piece of it, and the beginning of the next one's. The beginning comes
+// first: the part that holds a tile's last stage also takes the tile's update, which needs the first launch to be through.
 struct Unit {
-  int kind;       // 0 none, 1 part of a dealt tile, 2 whole tile with its update, 3 update of a dealt tile
+  int kind;       // 0 none, 1 part of a dealt tile, 2 whole tile with its update, 3 last part of a dealt tile with its update
   int tile, kb0, kb1;
   int slot;       // of the part in the workspace
 };
 struct Units {
   const DecodeParams& p;
-  int at, end, first_tile, next_full, stage;
-  __device__ Units(const DecodeParams& p_, const Deal& d) : p(p_), next_full(blockIdx.x), stage(0) {
+  int at, split, end, first_tile, next_full, turn;
+  __device__ Units(const DecodeParams& p_, const Deal& d) : p(p_), next_full(blockIdx.x), turn(0) {
     at = d.begin(blockIdx.x);
     end = d.begin(blockIdx.x + 1);
-    first_tile = p.nkb > 0 ? at / p.nkb : 0;
+    first_tile = at / p.nkb;
+    split = min(end, (first_tile + 1) * p.nkb);
   }
   __device__ Unit next() {
-    if (at < end) {
-      const int t = at / p.nkb;
-      const Unit u = {1, p.full_tiles + t, at - t * p.nkb, min(end - t * p.nkb, p.nkb), 2 * static_cast<int>(blockIdx.x) + t - first_tile};
-      at = min(end, (t + 1) * p.nkb);
-      return u;
+    const int tile = p.full_tiles + first_tile, k0 = first_tile * p.nkb, slot = 2 * static_cast<int>(blockIdx.x);
+    if (turn == 0) {
+      turn = 1;
+      if (split < end) return Unit{1, tile + 1, 0, end - split, slot + 1};
     }
-    if (stage == 0) {
-      stage = 1;
-      if (static_cast<int>(blockIdx.x) < p.dealt_tiles)
-        return Unit{3, p.full_tiles + static_cast<int>(blockIdx.x), 0, 0, 2 * static_cast<int>(gridDim.x) + static_cast<int>(blockIdx.x)};
+    if (turn == 1) {
+      turn = 2;
+      if (at < split) return Unit{split - k0 == p.nkb ? 3 : 1, tile, at - k0, split - k0, slot};
     }
     if (next_full < p.full_tiles) {
       const Unit u = {2, next_full, 0, p.nkb, 0};
@@ -183,7 +188,9 @@ lora_decode_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
   griddep_launch_dependents();
   const Deal deal(p);
   Units units(p, deal);
-  // The adapter list, at most 64 entries for as many rows, asked for ahead of the update; every lane of the warp calls it.
+  // The adapter list, at most 64 entries for as many rows; every lane of the warp calls it. Whole tiles ask for it a few stages ahead
+  // of their update; the part of a dealt tile only when all of its weights are on their way, since asking means waiting for the
+  // first launch.
   int count = -1, entries = 0, more_entries = 0;
   auto read_list = [&]() {
     griddep_wait();
@@ -306,10 +313,6 @@ lora_decode_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
     const uint64_t xa0 = make_smem_desc(ring_addr, 16, row_group, swizzle);
     const uint64_t xb0 = make_smem_desc(ring_addr + kWeightBytes, 16, row_group, swizzle);
     for (Unit u = units.next(); u.kind != 0 && ok; u = units.next()) {
-      if (u.kind == 3) {
-        if (count < 0) read_list();
-        if (count == 0) continue;  // nothing to add: the epilogue knows it too
-      }
       const uint32_t d = tmem_base + static_cast<uint32_t>(acc * p.acc_stride);
       ok = wait_warp(&tmem_empty[acc], ((acc_parity >> acc) & 1u) ^ 1u, wctx, TB_DEV_TIMEOUT_TMEM_EMPTY);
       if (!ok) break;
@@ -334,6 +337,7 @@ lora_decode_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
       }
       if (!ok) break;
       if (u.kind != 1) {
+        if (count < 0) read_list();
         for (int i = 0, kb = 0; i < count;) {
           ok = wait_warp(&full_bar[s], ph, wctx, TB_DEV_TIMEOUT_SMEM_FULL);
           if (!ok) break;
@@ -343,8 +347,7 @@ lora_decode_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
             const int steps = min(4 / p.pack, (p.rank - kb * kStageK + 15) >> 4);  // columns behind the rank are zeros
             for (int j = 0; j < filled; ++j)
               for (int k = 0; k < steps; ++k)
-                umma<0, 1>(d, xa0 + soff + ((j * part_w) >> 4) + 2 * k, xb0 + soff + ((j * part_v) >> 4) + 2 * k, p.idesc,
-                           (u.kind == 3 && i == 0 && kb == 0 && j == 0 && k == 0) ? 0u : 1u);
+                umma<0, 1>(d, xa0 + soff + ((j * part_w) >> 4) + 2 * k, xb0 + soff + ((j * part_v) >> 4) + 2 * k, p.idesc, 1u);
             umma_commit(&empty_bar[s]);
           }
           __syncwarp();
@@ -369,100 +372,106 @@ lora_decode_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
     int acc = 0;
     uint32_t parity = 0;
     bool ok = true;
-    read_list();
     T* out = static_cast<T*>(p.out);
     for (Unit u = units.next(); u.kind != 0 && ok; u = units.next()) {
       const int n = u.tile * kTile + warp * 32 + lane;  // this lane's feature
       const bool mine = n < p.n;
       const float bias = u.kind == 2 && mine && p.bias != nullptr ? bias_at(p.bias, n * p.bias_stride, p.bias_dtype) : 0.0f;
       float* part = p.parts + static_cast<size_t>(u.slot) * p.tokens * kTile + warp * 32 + lane;
-      if (u.kind != 3 || count > 0) {
-        ok = __all_sync(0xffffffffu, mbar_wait(&tmem_full[acc], (parity >> acc) & 1u, wctx, TB_DEV_TIMEOUT_TMEM_FULL));
-        if (!ok) break;
-        tc_fence_after();
-        const uint32_t t_row = tmem_base + (static_cast<uint32_t>(warp * 32) << 16) + static_cast<uint32_t>(acc * p.acc_stride);
-        for (int c0 = 0; c0 < p.tokens; c0 += 32) {
-          uint32_t r[32];
-          tmem_ld_32x32(t_row + c0, r);
-          tmem_ld_wait(r);
-          if (c0 + 32 >= p.tokens) {  // the last columns sit in registers
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&tmem_empty[acc]);
-          }
+      ok = __all_sync(0xffffffffu, mbar_wait(&tmem_full[acc], (parity >> acc) & 1u, wctx, TB_DEV_TIMEOUT_TMEM_FULL));
+      if (!ok) break;
+      tc_fence_after();
+      const uint32_t t_row = tmem_base + (static_cast<uint32_t>(warp * 32) << 16) + static_cast<uint32_t>(acc * p.acc_stride);
+      for (int c0 = 0; c0 < p.tokens; c0 += 32) {
+        uint32_t r[32];
+        tmem_ld_32x32(t_row + c0, r);
+        tmem_ld_wait(r);
+        if (c0 + 32 >= p.tokens) {  // the last columns sit in registers
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&tmem_empty[acc]);
+        }
 #pragma unroll
-          for (int j = 0; j < 32; ++j) {
-            const int t = c0 + j;
-            if (t < p.tokens) {
-              const float v = __uint_as_float(r[j]);
-              if (u.kind != 2) __stcg(part + static_cast<size_t>(t) * kTile, v);
-              else if (mine) out[t * p.out_m + n * p.out_n] = cast16<T>(v + bias);
-            }
+        for (int j = 0; j < 32; ++j) {
+          const int t = c0 + j;
+          if (t < p.tokens) {
+            const float v = __uint_as_float(r[j]);
+            if (u.kind != 2) __stcg(part + static_cast<size_t>(t) * kTile, v);
+            else if (mine) out[t * p.out_m + n * p.out_n] = cast16<T>(v + bias);
           }
         }
-        parity ^= 1u << acc;
-        acc ^= 1;
       }
+      parity ^= 1u << acc;
+      acc ^= 1;
       if (u.kind == 2) continue;
       // count this warp's quarter in; the last of its tile's parts adds them up
       const int dealt = u.tile - p.full_tiles;
       const int c_first = deal.cta_of(dealt * p.nkb), c_last = deal.cta_of((dealt + 1) * p.nkb - 1);
+      griddep_wait();  // the counters are clear
       __syncwarp();
       unsigned old = 0;
       if (lane == 0) old = add_acq_rel(p.arrived + dealt * 4 + warp, 1u);
       old = __shfl_sync(0xffffffffu, old, 0);
-      if (old != static_cast<unsigned>(c_last - c_first + 1)) continue;  // as many parts, and the update's unit
+      if (old != static_cast<unsigned>(c_last - c_first)) continue;
       __syncwarp();
-      // Four features per lane, four tokens per load instruction, four of those and four parts at a time: sixteen 16-byte loads
-      // are in flight before the first sum, since each round is a round trip to L2.
+      // Four features per lane, four tokens per load instruction; four of those and four parts at a time, or two and eight where
+      // there are no more tokens: sixteen 16-byte loads are in flight before the first sum, since each round is a round trip to L2.
       const int n4 = u.tile * kTile + warp * 32 + (lane & 7) * 4;
       const float* lane_parts = p.parts + warp * 32 + (lane & 7) * 4;
       const size_t slot_stride = static_cast<size_t>(p.tokens) * kTile;
       // only the first of the tile's CTAs can have begun inside an earlier tile
       const size_t first_slot = 2 * c_first + dealt - deal.begin(c_first) / p.nkb;
-      const float* update = lane_parts + (2 * static_cast<size_t>(gridDim.x) + dealt) * slot_stride;
       float b[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
       for (int i = 0; i < 4; ++i)
         if (p.bias != nullptr && n4 + i < p.n) b[i] = bias_at(p.bias, (n4 + i) * p.bias_stride, p.bias_dtype);
-      for (int t0 = lane >> 3; t0 < p.tokens; t0 += 16) {
-        float4 sum[4];
+      auto add_up = [&](auto parts_at_once, auto tokens_at_once) {
+        constexpr int kQ = decltype(parts_at_once)::value, kT = decltype(tokens_at_once)::value;
+        for (int t0 = lane >> 3; t0 < p.tokens; t0 += 4 * kT) {
+          float4 sum[kT];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) sum[j] = make_float4(b[0], b[1], b[2], b[3]);
-        for (int q0 = 0; q0 <= c_last - c_first + 1; q0 += 4) {
-          float4 v[4][4];
+          for (int j = 0; j < kT; ++j) sum[j] = make_float4(b[0], b[1], b[2], b[3]);
+          for (int q0 = 0; q0 <= c_last - c_first; q0 += kQ) {
+            float4 v[kQ][kT];
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const int c = c_first + q0 + q;
-            const bool there = c <= c_last || (c == c_last + 1 && count > 0);
-            const float* src = c == c_first ? lane_parts + first_slot * slot_stride
-                                            : (c <= c_last ? lane_parts + 2 * static_cast<size_t>(c) * slot_stride : update);
+            for (int q = 0; q < kQ; ++q) {
+              const int c = c_first + q0 + q;
+              const float* src = lane_parts + (c == c_first ? first_slot : 2 * static_cast<size_t>(c)) * slot_stride;
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-              v[q][j] = there && t0 + 4 * j < p.tokens ? __ldcg(reinterpret_cast<const float4*>(src + static_cast<size_t>(t0 + 4 * j) * kTile))
-                                                       : make_float4(0.f, 0.f, 0.f, 0.f);
+              for (int j = 0; j < kT; ++j)
+                v[q][j] = c <= c_last && t0 + 4 * j < p.tokens
+                              ? __ldcg(reinterpret_cast<const float4*>(src + static_cast<size_t>(t0 + 4 * j) * kTile))
+                              : make_float4(0.f, 0.f, 0.f, 0.f);
+            }
+#pragma unroll
+            for (int q = 0; q < kQ; ++q)
+#pragma unroll
+              for (int j = 0; j < kT; ++j) {
+                sum[j].x += v[q][j].x;
+                sum[j].y += v[q][j].y;
+                sum[j].z += v[q][j].z;
+                sum[j].w += v[q][j].w;
+              }
           }
 #pragma unroll
-          for (int q = 0; q < 4; ++q)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              sum[j].x += v[q][j].x;
-              sum[j].y += v[q][j].y;
-              sum[j].z += v[q][j].z;
-              sum[j].w += v[q][j].w;
+          for (int j = 0; j < kT; ++j) {
+            const int t = t0 + 4 * j;
+            if (t >= p.tokens) break;
+            T* o = out + t * p.out_m + n4 * p.out_n;
+            if (p.out_vec && n4 + 3 < p.n) {
+              alignas(8) const T quad[4] = {cast16<T>(sum[j].x), cast16<T>(sum[j].y), cast16<T>(sum[j].z), cast16<T>(sum[j].w)};
+              *reinterpret_cast<uint2*>(o) = *reinterpret_cast<const uint2*>(quad);
+              continue;
             }
+            if (n4 < p.n) o[0] = cast16<T>(sum[j].x);
+            if (n4 + 1 < p.n) o[p.out_n] = cast16<T>(sum[j].y);
+            if (n4 + 2 < p.n) o[2 * p.out_n] = cast16<T>(sum[j].z);
+            if (n4 + 3 < p.n) o[3 * p.out_n] = cast16<T>(sum[j].w);
+          }
         }
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int t = t0 + 4 * j;
-          if (t >= p.tokens) break;
-          T* o = out + t * p.out_m + n4 * p.out_n;
-          if (n4 < p.n) o[0] = cast16<T>(sum[j].x);
-          if (n4 + 1 < p.n) o[p.out_n] = cast16<T>(sum[j].y);
-          if (n4 + 2 < p.n) o[2 * p.out_n] = cast16<T>(sum[j].z);
-          if (n4 + 3 < p.n) o[3 * p.out_n] = cast16<T>(sum[j].w);
-        }
-      }
+      };
+      if (p.tokens <= 8) add_up(std::integral_constant<int, 8>{}, std::integral_constant<int, 2>{});
+      else add_up(std::integral_constant<int, 4>{}, std::integral_constant<int, 4>{});
       __syncwarp();
     }
   }
@@ -526,7 +535,7 @@ LoraDecodeShape lora_decode_shape(int tokens, int n, int grid) {
   const int tiles = (n + kTile - 1) / kTile;
   s.full_tiles = tiles / grid * grid;
   s.dealt_tiles = tiles - s.full_tiles;
-  s.part_bytes = 4ll * (2ll * grid + s.dealt_tiles) * tokens * kTile;
+  s.part_bytes = s.dealt_tiles > 0 ? 4ll * 2 * grid * tokens * kTile : 0;
   return s;
 }
 
@@ -558,6 +567,7 @@ int lora_decode(const tb_lora_args& a, const LoraDecodeShape& s, const LowRank& 
   p.out = a.out;
   p.out_m = a.out_stride_m;
   p.out_n = a.out_stride_n;
+  p.out_vec = a.out_stride_n == 1 && reinterpret_cast<uintptr_t>(a.out) % 8 == 0 && (a.m == 1 || a.out_stride_m % 4 == 0) ? 1 : 0;
   p.status = status;
   p.timeout_ns = a.wait_timeout_ms > 0 ? static_cast<unsigned long long>(a.wait_timeout_ms) * 1000000ull : 2000000000ull;
   const uint32_t fmt = a.dtype == TB_DTYPE_BF16 ? 1u : 0u;
