@@ -220,9 +220,9 @@ __device__ __forceinline__ void cluster_or_block_sync(int splits) {
 }
 
 // ------------------------------------------------------------------------------------------------------ decode batches
-// One cluster (of `splits` CTAs along K) per run of 16 rows; blockIdx.y deals the adapters of the run. Every warp takes K slices
-// and loads both operands straight into the fragments of mma.sync (16 bytes per lane and row; the order of K inside a slice is
-// the same for both, so it need not be the instruction's). NT: n-tiles of 8 ranks held in registers.
+// One cluster (of `splits` CTAs along K) per run of 16 rows; blockIdx.y deals the adapters of the run, 8 NT ranks at a time. Every
+// warp takes K slices and loads both operands straight into the fragments of mma.sync (16 bytes per lane and row; the order of K
+// inside a slice is the same for both, so it need not be the instruction's).
 template <typename T, int NT>
 __global__ void __launch_bounds__(kThreads, 2) lora_project_kernel(const ProjectParams p) {
   constexpr int kRows = 16, kCols = 8 * NT;
@@ -248,22 +248,25 @@ __global__ void __launch_bounds__(kThreads, 2) lora_project_kernel(const Project
   const T* x = static_cast<const T*>(p.x);
   const int g = lane >> 2, q = lane & 3;
   const int k_begin = rank * p.k_chunk, k_end = min(p.k, k_begin + p.k_chunk);
-  for (int turn = blockIdx.y; turn < found.y; turn += gridDim.y) {
+  const int slices = (p.rank + kCols - 1) / kCols;
+  for (int item = blockIdx.y; item < found.y * slices; item += gridDim.y) {
+    const int turn = item / slices, c0 = (item - turn * slices) * kCols;  // first rank of the slice
+    const int ranks = p.rank - c0;
     const int adapter = lists.run_ids[turn];
-    T* block = tile_blocks + lists.run_slots[turn] * static_cast<long long>(p.tile_rows) * p.v_cols;
+    T* block = tile_blocks + lists.run_slots[turn] * static_cast<long long>(p.tile_rows) * p.v_cols + c0;
     const float scale = p.scales != nullptr ? __ldg(p.scales + adapter) : 1.0f;
     // only rows with this adapter are read; the others enter the product as zeros
     bool live[2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) live[h] = run_ids[h * 8 + g] == adapter;
     const T* x_lane = x + (row0 + g) * p.x_stride + q * 8;
-    const T* a_lane = static_cast<const T*>(p.a) + adapter * p.a_adapter_stride + g * p.a_row_stride + q * 8;
+    const T* a_lane = static_cast<const T*>(p.a) + adapter * p.a_adapter_stride + (c0 + g) * p.a_row_stride + q * 8;
     float acc[NT][4];
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int i = 0; i < 4; ++i) acc[n][i] = 0.0f;
-    constexpr int kUnroll = NT <= 4 ? 4 : (NT <= 8 ? 2 : 1);
+    constexpr int kUnroll = 4;
     const uint4 zero = make_uint4(0, 0, 0, 0);
     // K in steps of 32 per warp: four lanes cover 64 contiguous bytes of a row
     for (int k0 = k_begin + warp * 32; k0 < k_end; k0 += kWarps * 32 * kUnroll) {
@@ -274,7 +277,7 @@ __global__ void __launch_bounds__(kThreads, 2) lora_project_kernel(const Project
         const bool in_k = k + q * 8 < k_end;
 #pragma unroll
         for (int n = 0; n < NT; ++n)
-          bb[s][n] = in_k && n * 8 < p.rank ? __ldg(reinterpret_cast<const uint4*>(a_lane + n * 8 * p.a_row_stride + k)) : zero;
+          bb[s][n] = in_k && n * 8 < ranks ? __ldg(reinterpret_cast<const uint4*>(a_lane + n * 8 * p.a_row_stride + k)) : zero;
 #pragma unroll
         for (int h = 0; h < 2; ++h)
           xa[s][h] = in_k && live[h] ? __ldg(reinterpret_cast<const uint4*>(x_lane + h * 8 * p.x_stride + k)) : zero;
@@ -305,12 +308,12 @@ __global__ void __launch_bounds__(kThreads, 2) lora_project_kernel(const Project
     }
     cluster_or_block_sync(p.splits);
     // the CTAs of a cluster write a share of the block each
-    for (int i = tid + rank * kThreads; i < kRows * p.v_cols; i += kThreads * p.splits) {
-      const int r = i / p.v_cols, c = i - r * p.v_cols;
+    for (int i = tid + rank * kThreads; i < kRows * kCols; i += kThreads * p.splits) {
+      const int r = i / kCols, c = i % kCols;
       float v = 0.0f;
-      if (c < p.rank && run_ids[r] == adapter)
+      if (c < ranks && run_ids[r] == adapter)
         v = scale * (p.splits > 1 ? cluster_sum(&s_part[r][c], p.splits) : s_part[r][c]);
-      block[i] = cast16<T>(v);
+      block[r * p.v_cols + c] = cast16<T>(v);
     }
     cluster_or_block_sync(p.splits);  // nobody overwrites or leaves its sums while another CTA still reads them
   }
@@ -518,9 +521,7 @@ int project_decode_nt(const ProjectParams& p, int runs, int stripes, int device,
 template <typename T>
 int project_decode(const ProjectParams& p, int runs, int stripes, int device, cudaStream_t stream) {
   if (p.rank <= 16) return project_decode_nt<T, 2>(p, runs, stripes, device, stream);
-  if (p.rank <= 32) return project_decode_nt<T, 4>(p, runs, stripes, device, stream);
-  if (p.rank <= 64) return project_decode_nt<T, 8>(p, runs, stripes, device, stream);
-  return project_decode_nt<T, 16>(p, runs, stripes, device, stream);
+  return project_decode_nt<T, 4>(p, runs, stripes, device, stream);
 }
 
 template <typename T>
@@ -578,7 +579,7 @@ int lora_plan(const tb_lora_args& a, int num_sms, tb_gemm_args* g, LoraPlan* l) 
   g->wait_timeout_ms = a.wait_timeout_ms;
   l->decode = a.m <= 64;
   if (l->decode) {
-    l->shape = lora_decode_shape(a.m, a.n, num_sms);
+    l->shape = lora_decode_shape(a.m, a.n, a.k, num_sms);
     l->tile_rows = l->shape.cols;
   } else {
     const int rc = low_rank_config(*g, &l->cfg);
@@ -667,8 +668,10 @@ int lora_impl(const tb_lora_args& a, cudaStream_t stream) {
   int stripes = 1;
   p.splits = 1;
   if (decode) {
-    stripes = most < a.m ? most : a.m;
-    const int by_blocks = num_sms * 7 / 8 / (live_runs * stripes), by_k = a.k / 256;
+    const int blocks = num_sms * 7 / 8;
+    stripes = (most < a.m ? most : a.m) * ((a.rank + 31) / 32);
+    if (live_runs * stripes > blocks) stripes = blocks / live_runs;
+    const int by_blocks = blocks / (live_runs * stripes), by_k = a.k / 256;
     p.splits = by_blocks < by_k ? by_blocks : by_k;
     p.splits = p.splits < 1 ? 1 : (p.splits > 8 ? 8 : p.splits);
   } else {

@@ -44,7 +44,7 @@ struct DecodeParams {
   int acc_stride, tmem_cols;
   int nkb;              // stages per tile
   int w_mn;             // 1: W is stored with its output features contiguous
-  int full_tiles, dealt_tiles;
+  int full_tiles, dealt_tiles, deal_ctas;
   // low-rank update
   const int* list;      // number of adapters, then their indices
   int max_slots, pack, kblocks, rank;
@@ -61,15 +61,15 @@ struct DecodeParams {
   unsigned long long timeout_ns;
 };
 
-// The dealt tiles' stages [0, dealt_tiles * nkb) in equal runs, one per CTA.
+// The dealt tiles' stages [0, dealt_tiles * nkb) in equal runs, one for each of the first deal_ctas CTAs.
 struct Deal {
-  int base, rem;
-  __device__ Deal(const DecodeParams& p) {
+  int base, rem, ctas;
+  __device__ Deal(const DecodeParams& p) : ctas(p.deal_ctas) {
     const int total = p.dealt_tiles * p.nkb;
-    base = total / static_cast<int>(gridDim.x);
-    rem = total - base * static_cast<int>(gridDim.x);
+    base = total / max(ctas, 1);
+    rem = total - base * ctas;
   }
-  __device__ int begin(int cta) const { return cta * base + min(cta, rem); }
+  __device__ int begin(int cta) const { return min(cta, ctas) * base + min(cta, rem); }
   __device__ int cta_of(int stage) const {
     const int wide = rem * (base + 1);
     return stage < wide ? stage / (base + 1) : rem + (stage - wide) / max(base, 1);
@@ -528,13 +528,19 @@ int decode_launch(const CUtensorMap& w, const CUtensorMap& x, const CUtensorMap&
 
 // Whole rounds of tiles go to one CTA each, the rest is dealt. (64-row tiles measured 1 us better up to eight tokens at 8192 x
 // 28672 and 4-15 % worse everywhere else, so there are none.)
-LoraDecodeShape lora_decode_shape(int tokens, int n, int grid) {
+// A dealt tile has at most as many parts as make its reading and the sum over them about equally long: a stage takes a quarter of a
+// microsecond, as does a part of up to 16 tokens in the sum, or two parts of up to 8.
+LoraDecodeShape lora_decode_shape(int tokens, int n, int k, int grid) {
   LoraDecodeShape s;
   s.cols = (tokens + 15) / 16 * 16;
   s.grid = grid;
   const int tiles = (n + kTile - 1) / kTile;
   s.full_tiles = tiles / grid * grid;
   s.dealt_tiles = tiles - s.full_tiles;
+  const int ratio = (k + kStageK - 1) / kStageK * (tokens <= 8 ? 2 : 1) / ((tokens + 15) / 16);
+  int parts = 1;
+  while ((parts + 1) * (parts + 1) <= ratio && parts < grid) ++parts;
+  s.deal_ctas = s.dealt_tiles * parts < grid ? s.dealt_tiles * parts : grid;
   s.part_bytes = s.dealt_tiles > 0 ? 4ll * 2 * grid * tokens * kTile : 0;
   return s;
 }
@@ -554,6 +560,7 @@ int lora_decode(const tb_lora_args& a, const LoraDecodeShape& s, const LowRank& 
   p.nkb = (a.k + kStageK - 1) / kStageK;
   p.full_tiles = s.full_tiles;
   p.dealt_tiles = s.dealt_tiles;
+  p.deal_ctas = s.deal_ctas;
   p.list = lr.list;
   p.max_slots = lr.list_stride - 1;
   p.pack = lr.pack;
