@@ -192,6 +192,19 @@ def test_more_than_32_adapters_in_every_tile_of_a_block(T, N, R):
     check(tb.lora_matmul(x, w, a, b, ids, s), x, w, a, b, ids, scales=s)
 
 
+@pytest.mark.parametrize("T,N,R", [(64, 256, 128), (64, 1000, 64), (40, 8192, 72), (64, 4096, 16), (17, 136, 40), (8, 640, 128), (48, 28672, 32)])
+def test_long_updates_in_pieces(T, N, R):
+    """Lists that are as long as the batch, shorter than the pieces they could have, a single entry, or empty."""
+    x, w, a, b, _, s = make(T, 192, N, R, T, torch.bfloat16)
+    t = torch.arange(T, device="cuda")
+    bias = torch.randn(N, device="cuda")
+    for ids in ((t * 7) % T, t % 9 - 1, t * 0 + T - 1, t * 0 - 1, torch.where(t == T - 1, 3, -1), t // 2):
+        ids = ids.int()
+        got = tb.lora_matmul(x, w, a, b, ids, s, bias=bias)
+        check(got, x, w, a, b, ids, scales=s, bias=bias, what=str(ids.unique().numel()))
+        assert torch.equal(got, tb.lora_matmul(x, w, a, b, ids, s, bias=bias))
+
+
 def test_grad_is_refused():
     x, w, a, b, ids, s = make(4, 64, 64, 8, 2, torch.bfloat16)
     with pytest.raises(RuntimeError, match="inference only"):

@@ -46,10 +46,10 @@ int gemm_low_rank(const tb_gemm_args& a, const tb_config& cfg, const LowRank& lr
 // Decode form of the same product (lora_decode.cu), up to 64 rows: how it is cut, and its launch.
 // `parts` holds part_bytes, `arrived` 4 * dealt_tiles zeroed words.
 struct LoraDecodeShape {
-  int cols, grid, full_tiles, dealt_tiles, deal_ctas;
+  int cols, grid, full_tiles, dealt_tiles, deal_ctas, pieces;
   long long part_bytes;
 };
-LoraDecodeShape lora_decode_shape(int tokens, int n, int k, int grid);
+LoraDecodeShape lora_decode_shape(int tokens, int n, int k, int update_stages, int grid);
 int lora_decode(const tb_lora_args& a, const LoraDecodeShape& s, const LowRank& lr, void* parts, void* arrived, int device,
                 int smem_optin, int* status, cudaStream_t stream);
 

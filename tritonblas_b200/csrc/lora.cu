@@ -223,8 +223,9 @@ __device__ __forceinline__ void cluster_or_block_sync(int splits) {
 // One cluster (of `splits` CTAs along K) per run of 16 rows; blockIdx.y deals the adapters of the run, 8 NT ranks at a time. Every
 // warp takes K slices and loads both operands straight into the fragments of mma.sync (16 bytes per lane and row; the order of K
 // inside a slice is the same for both, so it need not be the instruction's).
+// 120 registers: see lora_decode_kernel, whose block is to join this one's on its SM.
 template <typename T, int NT>
-__global__ void __launch_bounds__(kThreads, 2) lora_project_kernel(const ProjectParams p) {
+__global__ void __maxnreg__(120) lora_project_kernel(const ProjectParams p) {
   constexpr int kRows = 16, kCols = 8 * NT;
   __shared__ RunLists<kRows> lists;
   __shared__ float s_red[kWarps][kRows][8];
@@ -579,8 +580,7 @@ int lora_plan(const tb_lora_args& a, int num_sms, tb_gemm_args* g, LoraPlan* l) 
   g->wait_timeout_ms = a.wait_timeout_ms;
   l->decode = a.m <= 64;
   if (l->decode) {
-    l->shape = lora_decode_shape(a.m, a.n, a.k, num_sms);
-    l->tile_rows = l->shape.cols;
+    l->tile_rows = (a.m + 15) / 16 * 16;
   } else {
     const int rc = low_rank_config(*g, &l->cfg);
     if (rc != TB_OK) return rc;
@@ -591,6 +591,10 @@ int lora_plan(const tb_lora_args& a, int num_sms, tb_gemm_args* g, LoraPlan* l) 
   // small ranks share a stage of the GEMM: see GemmParams::lr_pack
   l->pack = a.rank <= 16 ? 4 : (a.rank <= 32 ? 2 : 1);
   l->v_cols = l->pack > 1 ? 64 / l->pack : (a.rank + 63) / 64 * 64;
+  if (l->decode) {
+    const int most = a.m < l->max_slots ? a.m : l->max_slots;
+    l->shape = lora_decode_shape(a.m, a.n, a.k, (most + l->pack - 1) / l->pack * ((a.rank + 63) / 64), num_sms);
+  }
   l->v_rows = static_cast<long long>(l->tiles) * l->max_slots * l->tile_rows;
   if (l->v_rows > 0x7fffffffll) return TB_ERR_UNSUPPORTED;  // a row coordinate of a copy has 32 bits; shorter batches fit
   auto up = [](long long v) { return (v + 255) & ~255ll; };

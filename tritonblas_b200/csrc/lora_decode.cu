@@ -35,6 +35,8 @@ constexpr int kMaxStages = 10;    // 160 KB of weights ahead
 constexpr int kRowBytes = 128;
 constexpr int kStageK = 64;       // K of a stage: one 128-byte row of 16-bit elements
 constexpr int kTile = 128;        // features of a tile
+constexpr int kMaxTokens = 64;
+constexpr int kPieceStages = 4;   // of an update, at least
 constexpr uint32_t kWeightBytes = kTile * kRowBytes;  // of a stage
 
 struct DecodeParams {
@@ -48,7 +50,8 @@ struct DecodeParams {
   // low-rank update
   const int* list;      // number of adapters, then their indices
   int max_slots, pack, kblocks, rank;
-  float* parts;         // [2 * grid][tokens][kTile]
+  int pieces;           // a dealt tile's update is cut into at most this many
+  float* parts;         // [2 * grid][tokens][kTile], and [grid] more when there are pieces
   unsigned* arrived;    // [dealt_tiles][4], cleared by the first launch
   const void* bias;
   long long bias_stride;
@@ -78,12 +81,17 @@ struct Deal {
 
 // What a CTA works on, in order; every role walks the same sequence. Its run of dealt stages is at most one tile long, so it has
 // at most two parts: the end of a tile's K range, or a piece of it, and the beginning of the next one's. The beginning comes
-// first: the part that holds a tile's last stage also takes the tile's update, which needs the first launch to be through.
+// first: the part that holds a tile's last stage also takes the tile's update, which needs the first launch to be through. Of a
+// long update it takes the first piece, the others go to one CTA each, from the last one down.
 struct Unit {
-  int kind;       // 0 none, 1 part of a dealt tile, 2 whole tile with its update, 3 last part of a dealt tile with its update
+  // 0 none, 1 part of a dealt tile, 2 whole tile with its update, 3 last part of a dealt tile with its update or the first piece of
+  // it, 4 another piece
+  int kind;
   int tile, kb0, kb1;
   int slot;       // of the part in the workspace
+  int piece;
 };
+template <bool PIECES>
 struct Units {
   const DecodeParams& p;
   int at, split, end, first_tile, next_full, turn;
@@ -97,18 +105,24 @@ struct Units {
     const int tile = p.full_tiles + first_tile, k0 = first_tile * p.nkb, slot = 2 * static_cast<int>(blockIdx.x);
     if (turn == 0) {
       turn = 1;
-      if (split < end) return Unit{1, tile + 1, 0, end - split, slot + 1};
+      if (split < end) return Unit{1, tile + 1, 0, end - split, slot + 1, 0};
     }
     if (turn == 1) {
       turn = 2;
-      if (at < split) return Unit{split - k0 == p.nkb ? 3 : 1, tile, at - k0, split - k0, slot};
+      if (at < split) return Unit{split - k0 == p.nkb ? 3 : 1, tile, at - k0, split - k0, slot, 0};
+    }
+    if (PIECES && turn == 2) {
+      turn = 3;
+      const int j = static_cast<int>(gridDim.x - 1 - blockIdx.x);
+      if (j < (p.pieces - 1) * p.dealt_tiles)
+        return Unit{4, p.full_tiles + j % p.dealt_tiles, 0, 0, static_cast<int>(2 * gridDim.x + blockIdx.x), 1 + j / p.dealt_tiles};
     }
     if (next_full < p.full_tiles) {
-      const Unit u = {2, next_full, 0, p.nkb, 0};
+      const Unit u = {2, next_full, 0, p.nkb, 0, 0};
       next_full += gridDim.x;
       return u;
     }
-    return Unit{0, 0, 0, 0, 0};
+    return Unit{0, 0, 0, 0, 0, 0};
   }
 };
 
@@ -149,8 +163,11 @@ __device__ __forceinline__ __nv_bfloat16 cast16<__nv_bfloat16>(float v) { return
 template <>
 __device__ __forceinline__ __half cast16<__half>(float v) { return __float2half_rn(v); }
 
-template <typename T>
-__global__ void __launch_bounds__(kThreads, 1)
+// PIECES: with dealt updates (the form without them is half a microsecond shorter). A quarter of an SM's registers belongs to each of
+// its four warp schedulers: 136 for the two of these seven warps that meet there are what leaves room for two of the first launch's
+// at 120. With 144 and 128 the kernels run one after the other (1 row of 4096 x 4096: 14.9 us, not 12.9).
+template <typename T, bool PIECES>
+__global__ void __maxnreg__(136)
 lora_decode_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_x,
                    const __grid_constant__ CUtensorMap tmap_b, const __grid_constant__ CUtensorMap tmap_v, const DecodeParams p) {
   extern __shared__ uint8_t smem_raw[];
@@ -187,7 +204,7 @@ lora_decode_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
   // writes itself (list, v, cleared counters) is waited for by each role before its first use.
   griddep_launch_dependents();
   const Deal deal(p);
-  Units units(p, deal);
+  Units<PIECES> units(p, deal);
   // The adapter list, at most 64 entries for as many rows; every lane of the warp calls it. Whole tiles ask for it a few stages ahead
   // of their update; the part of a dealt tile only when all of its weights are on their way, since asking means waiting for the
   // first launch.
@@ -197,6 +214,18 @@ lora_decode_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
     count = __ldcg(p.list);
     entries = lane < p.max_slots ? __ldcg(p.list + 1 + lane) : 0;
     more_entries = 32 + lane < p.max_slots ? __ldcg(p.list + 33 + lane) : 0;
+  };
+  // Adapters per piece of a dealt tile's update: whole stages, at least four of them; the list's length says how many pieces there are.
+  auto piece_length = [&]() {
+    if (!PIECES) return kMaxTokens;
+    const int groups = (count + p.pack - 1) / p.pack;
+    return max((groups + p.pieces - 1) / p.pieces, (kPieceStages + p.kblocks - 1) / p.kblocks) * p.pack;
+  };
+  // The adapters [x, y) of the list that a unit's update takes.
+  auto update_range = [&](const Unit& u) {
+    if (!PIECES || u.kind == 2) return make_int2(0, count);
+    const int length = piece_length();
+    return make_int2(min(u.piece * length, count), min((u.piece + 1) * length, count));
   };
   const int part_w = kWeightBytes / p.pack, part_v = p.cols * kRowBytes / p.pack;  // bytes of one adapter's share of a stage
 
@@ -230,7 +259,8 @@ lora_decode_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
       }
       if (!ok || u.kind == 1) continue;
       if (count < 0) read_list();
-      for (int i = 0; i < count && ok; i += p.pack) {
+      const int2 range = update_range(u);
+      for (int i = range.x; i < range.y && ok; i += p.pack) {
         const int filled = min(p.pack, count - i);
         int adapter[4];
 #pragma unroll
@@ -278,7 +308,8 @@ lora_decode_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
       }
       if (!ok || u.kind == 1) continue;
       if (count < 0) read_list();
-      for (int i = 0; i < count && ok; i += p.pack) {
+      const int2 range = update_range(u);
+      for (int i = range.x; i < range.y && ok; i += p.pack) {
         const int filled = min(p.pack, count - i);
         for (int kb = 0; kb < p.kblocks; ++kb) {
           ok = wait_warp(&empty_bar[s], ph ^ 1, wctx, TB_DEV_TIMEOUT_SMEM_EMPTY);
@@ -313,6 +344,11 @@ lora_decode_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
     const uint64_t xa0 = make_smem_desc(ring_addr, 16, row_group, swizzle);
     const uint64_t xb0 = make_smem_desc(ring_addr + kWeightBytes, 16, row_group, swizzle);
     for (Unit u = units.next(); u.kind != 0 && ok; u = units.next()) {
+      if (PIECES && u.kind == 4) {
+        if (count < 0) read_list();
+        const int2 range = update_range(u);
+        if (range.x >= range.y) continue;  // a shorter list: the other roles know it too
+      }
       const uint32_t d = tmem_base + static_cast<uint32_t>(acc * p.acc_stride);
       ok = wait_warp(&tmem_empty[acc], ((acc_parity >> acc) & 1u) ^ 1u, wctx, TB_DEV_TIMEOUT_TMEM_EMPTY);
       if (!ok) break;
@@ -338,7 +374,8 @@ lora_decode_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
       if (!ok) break;
       if (u.kind != 1) {
         if (count < 0) read_list();
-        for (int i = 0, kb = 0; i < count;) {
+        const int2 range = update_range(u);
+        for (int i = range.x, kb = 0; i < range.y;) {
           ok = wait_warp(&full_bar[s], ph, wctx, TB_DEV_TIMEOUT_SMEM_FULL);
           if (!ok) break;
           if (elect_one()) {
@@ -347,7 +384,8 @@ lora_decode_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
             const int steps = min(4 / p.pack, (p.rank - kb * kStageK + 15) >> 4);  // columns behind the rank are zeros
             for (int j = 0; j < filled; ++j)
               for (int k = 0; k < steps; ++k)
-                umma<0, 1>(d, xa0 + soff + ((j * part_w) >> 4) + 2 * k, xb0 + soff + ((j * part_v) >> 4) + 2 * k, p.idesc, 1u);
+                umma<0, 1>(d, xa0 + soff + ((j * part_w) >> 4) + 2 * k, xb0 + soff + ((j * part_v) >> 4) + 2 * k, p.idesc,
+                           (PIECES && u.kind == 4 && i == range.x && kb == 0 && j == 0 && k == 0) ? 0u : 1u);
             umma_commit(&empty_bar[s]);
           }
           __syncwarp();
@@ -377,6 +415,11 @@ lora_decode_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
       const int n = u.tile * kTile + warp * 32 + lane;  // this lane's feature
       const bool mine = n < p.n;
       const float bias = u.kind == 2 && mine && p.bias != nullptr ? bias_at(p.bias, n * p.bias_stride, p.bias_dtype) : 0.0f;
+      if (PIECES && u.kind == 4) {
+        if (count < 0) read_list();
+        const int2 range = update_range(u);
+        if (range.x >= range.y) continue;
+      }
       float* part = p.parts + static_cast<size_t>(u.slot) * p.tokens * kTile + warp * 32 + lane;
       ok = __all_sync(0xffffffffu, mbar_wait(&tmem_full[acc], (parity >> acc) & 1u, wctx, TB_DEV_TIMEOUT_TMEM_FULL));
       if (!ok) break;
@@ -408,11 +451,17 @@ lora_decode_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
       const int dealt = u.tile - p.full_tiles;
       const int c_first = deal.cta_of(dealt * p.nkb), c_last = deal.cta_of((dealt + 1) * p.nkb - 1);
       griddep_wait();  // the counters are clear
+      int extra = 0;  // pieces behind the first one
+      if (PIECES) {
+        if (count < 0) read_list();
+        const int length = piece_length();
+        extra = max((count + length - 1) / length, 1) - 1;
+      }
       __syncwarp();
       unsigned old = 0;
       if (lane == 0) old = add_acq_rel(p.arrived + dealt * 4 + warp, 1u);
       old = __shfl_sync(0xffffffffu, old, 0);
-      if (old != static_cast<unsigned>(c_last - c_first)) continue;
+      if (old != static_cast<unsigned>(c_last - c_first + extra)) continue;
       __syncwarp();
       // Four features per lane, four tokens per load instruction; four of those and four parts at a time, or two and eight where
       // there are no more tokens: sixteen 16-byte loads are in flight before the first sum, since each round is a round trip to L2.
@@ -431,28 +480,31 @@ lora_decode_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
           float4 sum[kT];
 #pragma unroll
           for (int j = 0; j < kT; ++j) sum[j] = make_float4(b[0], b[1], b[2], b[3]);
-          for (int q0 = 0; q0 <= c_last - c_first; q0 += kQ) {
-            float4 v[kQ][kT];
+          auto add = [&](int n, auto slot_of) {
+            for (int q0 = 0; q0 < n; q0 += kQ) {
+              float4 v[kQ][kT];
 #pragma unroll
-            for (int q = 0; q < kQ; ++q) {
-              const int c = c_first + q0 + q;
-              const float* src = lane_parts + (c == c_first ? first_slot : 2 * static_cast<size_t>(c)) * slot_stride;
+              for (int q = 0; q < kQ; ++q) {
+                const float* src = lane_parts + slot_of(q0 + q) * slot_stride;
 #pragma unroll
-              for (int j = 0; j < kT; ++j)
-                v[q][j] = c <= c_last && t0 + 4 * j < p.tokens
-                              ? __ldcg(reinterpret_cast<const float4*>(src + static_cast<size_t>(t0 + 4 * j) * kTile))
-                              : make_float4(0.f, 0.f, 0.f, 0.f);
-            }
-#pragma unroll
-            for (int q = 0; q < kQ; ++q)
-#pragma unroll
-              for (int j = 0; j < kT; ++j) {
-                sum[j].x += v[q][j].x;
-                sum[j].y += v[q][j].y;
-                sum[j].z += v[q][j].z;
-                sum[j].w += v[q][j].w;
+                for (int j = 0; j < kT; ++j)
+                  v[q][j] = q0 + q < n && t0 + 4 * j < p.tokens
+                                ? __ldcg(reinterpret_cast<const float4*>(src + static_cast<size_t>(t0 + 4 * j) * kTile))
+                                : make_float4(0.f, 0.f, 0.f, 0.f);
               }
-          }
+#pragma unroll
+              for (int q = 0; q < kQ; ++q)
+#pragma unroll
+                for (int j = 0; j < kT; ++j) {
+                  sum[j].x += v[q][j].x;
+                  sum[j].y += v[q][j].y;
+                  sum[j].z += v[q][j].z;
+                  sum[j].w += v[q][j].w;
+                }
+            }
+          };
+          add(c_last - c_first + 1, [&](int q) { return q == 0 ? first_slot : 2 * static_cast<size_t>(c_first + q); });
+          if (PIECES && extra > 0) add(extra, [&](int q) { return static_cast<size_t>(3 * gridDim.x - 1 - (q * p.dealt_tiles + dealt)); });
 #pragma unroll
           for (int j = 0; j < kT; ++j) {
             const int t = t0 + 4 * j;
@@ -490,10 +542,10 @@ lora_decode_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
   }
 }
 
-template <typename T>
+template <typename T, bool PIECES>
 int decode_launch(const CUtensorMap& w, const CUtensorMap& x, const CUtensorMap& b, const CUtensorMap& v, const DecodeParams& p, int grid,
                   int smem_bytes, int device, cudaStream_t stream) {
-  auto kernel = lora_decode_kernel<T>;
+  auto kernel = lora_decode_kernel<T, PIECES>;
   // the opt-in shared-memory size is set once per instantiation and device, and again if a launch needs more
   static int configured[64] = {};
   static std::mutex mu;
@@ -530,7 +582,10 @@ int decode_launch(const CUtensorMap& w, const CUtensorMap& x, const CUtensorMap&
 // 28672 and 4-15 % worse everywhere else, so there are none.)
 // A dealt tile has at most as many parts as make its reading and the sum over them about equally long: a stage takes a quarter of a
 // microsecond, as does a part of up to 16 tokens in the sum, or two parts of up to 8.
-LoraDecodeShape lora_decode_shape(int tokens, int n, int k, int grid) {
+// Its update, up to update_stages long, is cut into pieces of four stages or more as long as every CTA gets at most one of them, and
+// where a quarter of the CTAs' number of tiles or fewer is dealt (64 rows of 1024 x 256, 64 adapters of rank 128: 69 -> 38 us; of
+// 4096 x 8192, rank 16, with two pieces for each of 64 tiles: 35 -> 42, so not there).
+LoraDecodeShape lora_decode_shape(int tokens, int n, int k, int update_stages, int grid) {
   LoraDecodeShape s;
   s.cols = (tokens + 15) / 16 * 16;
   s.grid = grid;
@@ -541,7 +596,12 @@ LoraDecodeShape lora_decode_shape(int tokens, int n, int k, int grid) {
   int parts = 1;
   while ((parts + 1) * (parts + 1) <= ratio && parts < grid) ++parts;
   s.deal_ctas = s.dealt_tiles * parts < grid ? s.dealt_tiles * parts : grid;
-  s.part_bytes = s.dealt_tiles > 0 ? 4ll * 2 * grid * tokens * kTile : 0;
+  s.pieces = 1;
+  if (s.dealt_tiles > 0) {
+    const int by_grid = grid / s.dealt_tiles, by_stages = (update_stages - 1) / kPieceStages;
+    if (by_grid >= 4) s.pieces += by_grid < by_stages ? by_grid : by_stages;
+  }
+  s.part_bytes = s.dealt_tiles > 0 ? 4ll * (s.pieces > 1 ? 3 : 2) * grid * tokens * kTile : 0;
   return s;
 }
 
@@ -561,6 +621,7 @@ int lora_decode(const tb_lora_args& a, const LoraDecodeShape& s, const LowRank& 
   p.full_tiles = s.full_tiles;
   p.dealt_tiles = s.dealt_tiles;
   p.deal_ctas = s.deal_ctas;
+  p.pieces = s.pieces;
   p.list = lr.list;
   p.max_slots = lr.list_stride - 1;
   p.pack = lr.pack;
@@ -598,7 +659,8 @@ int lora_decode(const tb_lora_args& a, const LoraDecodeShape& s, const LowRank& 
   const uint32_t box[3] = {inner, kTile, 1};
   if ((rc = encode_nd(&tb_, a.dtype, lr.b, 3, dims, strides, box)) != TB_OK) return rc;
   const int smem_bytes = p.stages * p.stage_bytes + 1024;
-  auto launch = fmt ? decode_launch<__nv_bfloat16> : decode_launch<__half>;
+  auto launch = p.pieces > 1 ? (fmt ? decode_launch<__nv_bfloat16, true> : decode_launch<__half, true>)
+                             : (fmt ? decode_launch<__nv_bfloat16, false> : decode_launch<__half, false>);
   return launch(tw, tx, tb_, tv, p, s.grid, smem_bytes, device, stream);
 }
 
