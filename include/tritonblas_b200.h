@@ -293,10 +293,10 @@ int tb_moe_mlp(const tb_moe_mlp_args* args, void* stream);
  *   out[t, :] = x[t, :] W + bias + s_a (x[t, :] A_a^T) B_a^T,  a = adapter_ids[t]; no adapter when a is outside [0, num_adapters).
  * x (m, k) rows contiguous, w (k, n) with one unit stride, lora_a (num_adapters, rank, k), lora_b (num_adapters, n, rank), out
  * (m, n) any strides, all of `dtype` (f16 or bf16); adapter_ids (m) int32 or int64, scales (num_adapters) fp32 or NULL (1), bias
- * (n) or NULL. k and rank multiples of 8, rank <= 128; x, w, lora_a, lora_b with 16-byte aligned bases and pitches. One fp32
- * sum and one rounding; the rank-sized products are rounded to `dtype` in between (they are a tensor-core operand). The
- * workspace (tb_lora_workspace_bytes of the same arguments, 256-byte aligned) needs no initialisation and must not be shared
- * by calls that can overlap. */
+ * (n) or NULL. k and rank multiples of 8, rank <= 128, k <= 2^28, m and n <= 2^30; rows (columns) of w must not overlap; x, w,
+ * lora_a, lora_b with 16-byte aligned bases and pitches. One fp32 sum and one rounding; the rank-sized products are rounded to
+ * `dtype` in between (they are a tensor-core operand). The workspace (tb_lora_workspace_bytes of the same arguments, 256-byte
+ * aligned) needs no initialisation and must not be shared by calls that can overlap. */
 typedef struct tb_lora_args {
   int32_t m, n, k, rank, num_adapters, dtype;
   const void* x; int64_t x_row_stride;
