@@ -203,7 +203,8 @@ int tb_grouped_gemm(const tb_gemm_args* args, const tb_config* cfg, void* stream
 /* Memory-bound steps around the grouped MoE GEMMs (the reference has no MoE path, so no counterpart):
  *   tb_swiglu:      out[r, j] = silu(h[r, j]) * h[r, ffn + j] for h = [gate | up] (rows, 2*ffn); fp32 math, one cast.
  *   tb_moe_combine: out[t, :] = sum_k weights[t, k] * y[pos[t, k], :]; pos = row of y that holds the k-th expert output
- *                   of token t (int64, tokens x topk), weights fp32 (tokens x topk); fp32 accumulate in k order.
+ *                   of token t (int64, tokens x topk; negative: none, adds nothing), weights fp32 (tokens x topk); fp32
+ *                   accumulate in k order.
  * f16 / bf16 data, 16-byte aligned rows, ffn and hidden multiples of 8. */
 int tb_swiglu(const void* h, int64_t h_row_stride, void* out, int64_t out_row_stride, int64_t rows, int32_t ffn,
               int32_t dtype, void* stream);

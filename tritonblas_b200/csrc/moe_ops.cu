@@ -89,6 +89,7 @@ __global__ void __launch_bounds__(256) combine_kernel(const T* __restrict__ y, l
     float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
     for (int k = 0; k < topk; ++k) {
       const long long src = pos[static_cast<long long>(t) * topk + k];
+      if (src < 0) continue;  // no expert
       const float wk = w[static_cast<long long>(t) * topk + k];
       float v[8];
       Vec8<T>::load(y + src * y_stride + c, v);

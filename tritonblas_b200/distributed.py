@@ -188,7 +188,7 @@ class ColumnShardedGemm:
 @dataclass
 class DispatchPlan:
     """Everything the combine step needs to undo a dispatch."""
-    sort_idx: torch.Tensor          # (T*topk,) positions of the flattened (token, k) pairs in expert order
+    sort_idx: torch.Tensor          # positions of the routed ones of the T*topk flattened (token, k) pairs in expert order
     send_counts: torch.Tensor       # (world, experts_per_rank) rows this rank sends, per destination expert
     recv_counts: torch.Tensor       # (world, experts_per_rank) rows this rank receives, per source rank and local expert
     send_splits: List[int]
@@ -196,7 +196,7 @@ class DispatchPlan:
     regroup_idx: Optional[torch.Tensor]   # received rows (source-major) -> expert-major order
     group_offsets: torch.Tensor     # int32 (experts_per_rank + 1,) row offsets of the expert-major buffer
     regroup_inv: Optional[torch.Tensor] = None   # expert-major -> source-major (inverse of regroup_idx)
-    pos: Optional[torch.Tensor] = None           # position of every (token, k) pair in expert order (inverse of sort_idx)
+    pos: Optional[torch.Tensor] = None           # (T*topk,) position of every pair in expert order (inverse of sort_idx), -1 = none
 
 
 def balanced_expert_placement(expert_load, world: int) -> torch.Tensor:
@@ -221,17 +221,25 @@ def balanced_expert_placement(expert_load, world: int) -> torch.Tensor:
     return place
 
 
+def _routed_experts(topk_ids: torch.Tensor, num_experts: int):
+    """The flattened ids in 64 bits with ``num_experts`` in the place of every id outside [0, num_experts), and which are inside."""
+    flat = topk_ids.reshape(-1).to(torch.int64)
+    routed = (flat >= 0) & (flat < num_experts)
+    return torch.where(routed, flat, num_experts), routed
+
+
 def plan_dispatch(topk_ids: torch.Tensor, num_experts: int, group=None, expert_place: Optional[torch.Tensor] = None) -> DispatchPlan:
     """Sort the (token, k) pairs of this rank by expert and exchange per-expert row counts with the other ranks.
-    ``expert_place`` maps expert ids to their position in the layout order (see balanced_expert_placement)."""
+    ``expert_place`` maps expert ids to their position in the layout order (see balanced_expert_placement). A pair whose id is
+    outside [0, num_experts) (-1: no expert) is not sent anywhere."""
     world = dist.get_world_size(group) if dist.is_initialized() else 1
     assert num_experts % world == 0, "experts must divide evenly over the ranks"
     epr = num_experts // world
-    flat = topk_ids.reshape(-1).to(torch.int64)
+    flat, routed = _routed_experts(topk_ids, num_experts)
     if expert_place is not None:
-        flat = expert_place.to(flat.device).to(torch.int64)[flat]
-    sort_idx = torch.argsort(flat, stable=True)
-    send_counts = torch.bincount(flat, minlength=num_experts).reshape(world, epr)
+        place = expert_place.to(flat.device).to(torch.int64)
+        flat = torch.where(routed, place[flat.clamp(max=num_experts - 1)], flat)
+    send_counts = torch.bincount(flat, minlength=num_experts + 1)[:num_experts].reshape(world, epr)
     if world > 1:
         recv_counts = torch.empty_like(send_counts)
         dist.all_to_all_single(recv_counts, send_counts, group=group)
@@ -239,12 +247,13 @@ def plan_dispatch(topk_ids: torch.Tensor, num_experts: int, group=None, expert_p
         recv_counts = send_counts.clone()
     send_splits = send_counts.sum(1).tolist()
     recv_splits = recv_counts.sum(1).tolist()
+    sort_idx = torch.argsort(flat, stable=True)[:sum(send_splits)]          # pairs without an expert sort behind the others
     # received rows arrive source-major, each source's rows expert-sorted; regroup them expert-major
     per_expert = recv_counts.sum(0)
     group_offsets = torch.zeros(epr + 1, dtype=torch.int32, device=topk_ids.device)
     group_offsets[1:] = per_expert.cumsum(0).to(torch.int32)
     regroup_idx = regroup_inv = None
-    pos = torch.empty_like(sort_idx)
+    pos = torch.full_like(flat, -1)
     pos[sort_idx] = torch.arange(sort_idx.numel(), device=sort_idx.device)
     if world > 1:
         total = int(sum(recv_splits))
@@ -271,6 +280,8 @@ def _gather_rows(x: torch.Tensor, index: torch.Tensor) -> torch.Tensor:
     from . import _lib
     index = index.to(torch.int64).contiguous()
     out = x.new_empty(index.numel(), x.shape[1])
+    if out.numel() == 0:
+        return out
     with torch.cuda.device(x.device):
         rc = _lib.lib.tb_moe_gather_rows(ctypes.c_void_p(x.data_ptr()), x.stride(0), ctypes.c_void_p(index.data_ptr()),
                                          ctypes.c_void_p(out.data_ptr()), out.stride(0), index.numel(), x.shape[1],
@@ -292,7 +303,7 @@ def dispatch(x: torch.Tensor, topk: int, plan: DispatchPlan, group=None) -> torc
 
 def combine(y: torch.Tensor, topk_weights: torch.Tensor, plan: DispatchPlan, group=None) -> torch.Tensor:
     """Inverse of dispatch for the experts' outputs y (expert-major), followed by the top-k weighted sum per token
-    (fp32 accumulate in k order, one cast)."""
+    (fp32 accumulate in k order, one cast). A pair that went to no expert adds nothing, whatever its weight."""
     tokens, topk = topk_weights.shape
     if plan.regroup_idx is not None:
         src_major = _gather_rows(y, plan.regroup_inv)            # a gather; the scatter form is several times slower
@@ -301,9 +312,12 @@ def combine(y: torch.Tensor, topk_weights: torch.Tensor, plan: DispatchPlan, gro
     else:
         back = y
     pos = plan.pos
+    if back.shape[0] == 0:
+        return back.new_zeros(tokens, back.shape[1])
     if back.is_cuda:
         return _combine_cuda(back, pos, topk_weights, tokens, topk)
-    return (back[pos].reshape(tokens, topk, -1).float() * topk_weights.unsqueeze(-1).float()).sum(1).to(y.dtype)
+    rows = back[pos.clamp(min=0)].reshape(tokens, topk, -1).float() * topk_weights.unsqueeze(-1).float()
+    return rows.masked_fill((pos < 0).reshape(tokens, topk, 1), 0.0).sum(1).to(y.dtype)
 
 
 def _combine_cuda(back, pos, topk_weights, tokens, topk):
@@ -332,6 +346,8 @@ def swiglu(h: torch.Tensor) -> torch.Tensor:
     h = h if h.stride(1) == 1 else h.contiguous()
     ffn = h.shape[1] // 2
     out = h.new_empty(h.shape[0], ffn)
+    if out.numel() == 0:
+        return out
     with torch.cuda.device(h.device):
         rc = _lib.lib.tb_swiglu(ctypes.c_void_p(h.data_ptr()), h.stride(0), ctypes.c_void_p(out.data_ptr()), out.stride(0),
                                 h.shape[0], ffn, _lib.DTYPE_CODE[h.dtype], _lib.current_stream_ptr(h.device))
@@ -401,14 +417,16 @@ def plan_peer_dispatch(topk_ids: torch.Tensor, counts_all: torch.Tensor, rank: i
     counts_all: int64 (world, num_experts), counts_all[r, e] = pairs of rank r routed to expert e (every rank holds the
     same matrix after an all-gather of its own bincount). Expert e lives on rank e // experts_per_rank; inside that
     rank's receive buffer the experts follow each other, and inside an expert the source ranks follow each other, each
-    source's rows in its own stable expert-sorted order.
+    source's rows in its own stable expert-sorted order. A pair whose id is outside [0, num_experts) goes nowhere: it stands
+    behind the others in the sorted list, with row -1 and rank 0, and the counts do not hold it.
     """
     world, num_experts = counts_all.shape
     epr = num_experts // world
-    flat = topk_ids.reshape(-1).to(torch.int64)
+    flat, _ = _routed_experts(topk_ids, num_experts)
     n = flat.numel()
     sort_idx = torch.argsort(flat, stable=True)
-    e_sorted = flat[sort_idx]
+    routed = flat[sort_idx] < num_experts
+    e_sorted = flat[sort_idx].clamp(max=num_experts - 1)
     totals = counts_all.sum(0)                                              # rows per expert over all sources
     per_owner = totals.view(world, epr)
     owner_off = (per_owner.cumsum(1) - per_owner).reshape(-1)               # start of expert e inside its owner's buffer
@@ -416,8 +434,8 @@ def plan_peer_dispatch(topk_ids: torch.Tensor, counts_all: torch.Tensor, rank: i
     mine = counts_all[rank]
     my_start = mine.cumsum(0) - mine                                        # start of expert e in my sorted list
     i = torch.arange(n, device=flat.device)
-    dest_row = dest_base[e_sorted] + (i - my_start[e_sorted])
-    dest_rank = (e_sorted // epr).to(torch.int32)
+    dest_row = torch.where(routed, dest_base[e_sorted] + (i - my_start[e_sorted]), -1)
+    dest_rank = torch.where(routed, e_sorted // epr, 0).to(torch.int32)
     pair_row = torch.empty_like(dest_row)
     pair_row[sort_idx] = dest_row
     pair_rank = torch.empty_like(dest_rank)
