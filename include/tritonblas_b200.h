@@ -218,8 +218,8 @@ int tb_moe_gather_rows(const void* x, int64_t x_row_stride, const int64_t* src_r
 /* Expert-parallel dispatch and combine over peer-mapped memory (each rank's receive / output buffer mapped into every
  * process, e.g. by CUDA IPC or torch symmetric memory), in place of all-to-all collectives. Ordinary loads and stores.
  *   tb_moe_dispatch_peers: for i < n, row src_token[i] of x is copied to row dest_row[i] of peer_bufs[dest_rank[i]];
- *                          rows outside [0, capacity_rows) are dropped and counted in *overflow_count (device int, may
- *                          be NULL).
+ *                          rows at capacity_rows or behind are dropped and counted in *overflow_count (device int, may
+ *                          be NULL); a negative row (a pair without an expert) is skipped.
  *   tb_moe_combine_peers:  out[t, :] = sum_k weights[t,k] * y_peers[pair_rank[t,k]][pair_row[t,k], :] (fp32, k order);
  *                          pairs whose row lies outside [0, capacity_rows), i.e. rows the dispatch dropped, add nothing.
  * peer_bufs / y_peers are HOST arrays of up to 8 device pointers; index arrays are device memory. The caller orders the

@@ -50,3 +50,17 @@ def test_expert_parallel_layer(T, K):
     out, _ = tbd.ExpertParallelMoE(w1, w2, E).forward(x, ids * 0 - 1, weights)
     assert out.shape == x.shape and (out == 0).all()
     assert tb.device_status() == 0
+
+
+@pytest.mark.parametrize("T,K", [(200, 2), (33, 5)])
+def test_peer_memory_layer_counts_no_overflow(T, K):
+    """The overflow counter tells a receive buffer that is too small; pairs without an expert need no row."""
+    x, w1, w2, weights, ids = _case(T, K)
+    live = int((ids >= 0).sum())
+    moe = tbd.PeerMemoryMoE(w1, w2, E, live)
+    out, _ = moe.forward(x, ids, weights)
+    _check(out, _reference(x, w1, w2, weights, ids), K)
+    assert int(moe.overflow) == 0
+    small = tbd.PeerMemoryMoE(w1, w2, E, live - 7)
+    small.forward(x, ids, weights)
+    assert int(small.overflow) == 7 and tb.device_status() == 0

@@ -187,7 +187,8 @@ __global__ void __launch_bounds__(256) moe_dispatch_kernel(const uint4* __restri
   const long long warps = (static_cast<long long>(gridDim.x) * blockDim.x) >> 5;
   for (long long r = (blockIdx.x * static_cast<long long>(blockDim.x) + threadIdx.x) >> 5; r < n; r += warps) {
     const long long row = dest_row[r];
-    if (row < 0 || row >= capacity_rows) {  // a receive buffer too small for this routing: drop the row, tell the host
+    if (row < 0) continue;  // a pair without an expert
+    if (row >= capacity_rows) {  // a receive buffer too small for this routing: drop the row, tell the host
       if (lane == 0 && overflow != nullptr) atomicAdd(overflow, 1);
       continue;
     }

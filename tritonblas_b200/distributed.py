@@ -458,7 +458,8 @@ class PeerMemoryMoE:
     combine is ONE kernel that reads the experts' outputs from the owners' buffers and forms the top-k weighted sum. Two
     symmetric-memory barriers per call order the phases; the only collective is an all-gather of the per-expert counts
     (world x experts integers), and nothing synchronises with the host. Rows routed beyond ``capacity`` are dropped and
-    counted in ``overflow``; the tokens they belong to lose that expert's contribution.
+    counted in ``overflow``; the tokens they belong to lose that expert's contribution. A pair without an expert (an id
+    outside [0, num_experts)) goes nowhere, adds nothing and is not counted.
 
     With one rank (no process group) the same kernels run on ordinary device buffers, without barriers or collectives.
     """
