@@ -1,0 +1,94 @@
+"""Router weights and gradients element by element, relative to what each element is made of.
+
+Bounds, in half units u = 2^-24 of fp32 arithmetic. An exponential exp(l - m) is off by its argument's rounding (computed exactly
+below: zero where both are short) and 4 u; a row's sum by the largest of those, 37 u of additions (32 in a lane at most, five
+exchanges) and a quotient by u: (argument + 64 u) relative covers a softmax score. A sigmoid 1 / (1 + exp(-l)) or its complement
+is off by 8 u, a sum of topk of them by topk u more. A gradient term g w - p dot or w (g - dot) is off by what its factors are,
+dot by the sum of what |g w| are off and (topk + 2) u, and the result by half a step of its type."""
+import pytest
+import torch
+
+import tritonblas_b200 as tb
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0 ** -24
+MODES = [("softmax", True), ("softmax", False), ("sigmoid", True), ("sigmoid", False)]
+
+
+def expected(logits, topk, scoring, renormalize, grad):
+    """(ids, weights, their bound, gradient, its bound) in 64 bits."""
+    l32 = logits.detach().float().cpu()
+    l32 = torch.where(torch.isnan(l32), torch.full_like(l32, float("-inf")), l32)
+    l = l32.double()
+    order = torch.argsort(-l, dim=1, stable=True)[:, :topk]
+    dead = torch.gather(l, 1, order) == float("-inf")
+    g = grad.double().cpu().masked_fill(dead, 0.0)
+    pick = lambda t: torch.gather(t, 1, order).masked_fill(dead, 0.0)
+    if scoring == "softmax":
+        top = l32.max(1, keepdim=True).values
+        top = torch.where(top > float("-inf"), top, torch.zeros_like(top))
+        off = torch.nan_to_num(((l32 - top).double() - (l - top.double())).abs())        # the argument's rounding
+        p = torch.exp(l - top.double())
+        if renormalize:
+            s, so = pick(p), pick(off)
+            w = s / s.sum(1, keepdim=True).clamp(min=1e-300)
+            rel = so + so.max(1, keepdim=True).values + (topk + 32) * U
+        else:
+            p = p / p.sum(1, keepdim=True).clamp(min=1e-300)
+            rel_p = off + (p * off).sum(1, keepdim=True) + 64 * U
+            w, rel = pick(p), pick(rel_p)
+    else:
+        s = torch.sigmoid(l)
+        comp = pick(torch.sigmoid(-l))
+        w, rel = pick(s), torch.full_like(g, 8 * U)
+        if renormalize:
+            # the scores' common factor cancels: the quotient stays good where the scores themselves are too small for fp32
+            t = pick(torch.nn.functional.logsigmoid(l))
+            t = torch.exp(t - t.masked_fill(dead, float("-inf")).max(1, keepdim=True).values.nan_to_num(neginf=0.0)).masked_fill(dead, 0.0)
+            w = t / t.sum(1, keepdim=True).clamp(min=1e-300)
+            m32 = torch.gather(l32, 1, order[:, :1])
+            args = ((m32 - torch.gather(l32, 1, order)).double() - (m32.double() - torch.gather(l, 1, order))).abs().nan_to_num(0.0, 0.0, 0.0)
+            rel = torch.where(m32 < 0, args + args.max(1, keepdim=True).values, torch.zeros_like(args)) + (topk + 40) * U
+    dot = (g * w).sum(1, keepdim=True)
+    ddot = (g * w).abs().mul(rel + (topk + 2) * U).sum(1, keepdim=True)
+    if scoring == "softmax" and not renormalize:
+        term, dterm = g * w, (g * w).abs() * (rel + 2 * U)
+        d = (torch.zeros_like(l).scatter_(1, order, term) - p * dot)
+        b = torch.zeros_like(l).scatter_(1, order, dterm) + p * ((rel_p + 3 * U) * dot.abs() + ddot)
+    else:
+        c = comp if scoring == "sigmoid" else torch.ones_like(w)
+        inner, dinner = (g - dot, ddot + 2 * U * (g.abs() + dot.abs())) if renormalize else (g, torch.zeros_like(g))
+        term = w * c * inner
+        d = torch.zeros_like(l).scatter_(1, order, term.masked_fill(dead, 0.0))
+        b = torch.zeros_like(l).scatter_(1, order, (w * c * dinner + term.abs() * (rel + 12 * U)).masked_fill(dead, 0.0))
+    f = torch.finfo(logits.dtype)
+    small = 2.0 ** -125         # exponentials below fp32's normal numbers
+    b = b + f.eps / 2 * d.abs() + f.smallest_normal * f.eps / 2 + small * g.abs().sum(1, keepdim=True)
+    return order.masked_fill(dead, -1).to(torch.int32), w, rel * w + small, d, b
+
+
+def check(logits, topk, scoring, renormalize, seed=0):
+    grad = torch.randn(logits.shape[0], topk, generator=torch.Generator().manual_seed(seed)).cuda()
+    x = logits.detach().requires_grad_(True)
+    w, ids = tb.moe_route(x, topk, scoring=scoring, renormalize=renormalize)
+    (dl,) = torch.autograd.grad(w, x, grad)
+    rids, rw, bw, rd, bd = expected(x, topk, scoring, renormalize, grad)
+    assert torch.equal(ids.cpu(), rids)
+    err = (w.detach().cpu().double() - rw).abs()
+    assert (err <= bw).all(), f"weights: worst err / bound {float((err / bw).max()):.3g}"
+    err = (dl.cpu().double() - rd).abs()
+    assert (err <= bd).all(), f"gradient: worst err / bound {float((err / bd).max()):.3g} at {divmod(int((err / bd).argmax()), rd.shape[1])}"
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("renormalize", [True, False])
+def test_saturated_sigmoid_scores_keep_their_gradient(dtype, renormalize):
+    """1 - s of a score next to 1 is exp(-l): it has no bits left in a rounded s."""
+    g = torch.Generator().manual_seed(3)
+    logits = (torch.rand(50, 40, generator=g) * 10 + 10).to(dtype).cuda()
+    logits[:, ::2] -= 16
+    check(logits, 6, "sigmoid", renormalize)
+    x = torch.full((1, 4), 18.0, device="cuda", requires_grad=True)
+    (d,) = torch.autograd.grad(tb.moe_route(x, 1, scoring="sigmoid", renormalize=False)[0].sum(), x)
+    assert 1.4e-8 < float(d[0, 0]) < 1.6e-8         # e^-18

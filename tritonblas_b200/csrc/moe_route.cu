@@ -5,7 +5,9 @@
 //   w_j     = p_{S_j}, or p_{S_j} / sum_S p when renormalised (softmax: the sum over all experts cancels and is not formed)
 //   d l     softmax, renormalised:  w_j (g_j - sum_S g w) on S, 0 elsewhere
 //           softmax:                p_i (g~_i - sum_S g p), g~ = g on S, 0 elsewhere
-//           sigmoid:                g_j p_j (1 - p_j) on S;  renormalised: g_j replaced by (g_j - sum_S g w) / sum_S p
+//           sigmoid:                g_j w_j (1 - p_j) on S;  renormalised: g_j replaced by g_j - sum_S g w
+//             (w_j = p_j, or p_j / sum_S p, is what the forward pass returned; 1 - p_j = 1 / (1 + exp(l_j)) is formed from the
+//             logit, since a rounded p_j next to 1 has none of its bits)
 //
 // A row is held in the registers of 4 to 32 lanes, eight logits each (16 or 32 above 256 experts), so a warp works on up to
 // eight rows at once; one pass over the logits in either direction, statistics in fp32. The choice is made on the logits
@@ -265,31 +267,20 @@ route_bwd_kernel(const T* __restrict__ logits, long long stride, long long token
     }
     return c;
   };
-  auto sigmoid_of = [&](int e) { return 1.0f / (1.0f + expf(-to_float(row[e]))); };
+  auto complement_of = [&](int e) { return 1.0f / (1.0f + expf(to_float(row[e]))); };
   const Choice mine = chosen(sub);
-  float dot = 0.0f, total = 0.0f;  // sum of g w, and of the scores where they are needed
+  float dot = 0.0f;  // sum of g w
   for (int j = sub; j < topk; j += LANES) {
     const Choice c = j == sub ? mine : chosen(j);
     dot += c.g * c.w;
-    if (sigmoid && renorm && c.e >= 0) total += sigmoid_of(c.e);
   }
   dot = lanes_sum<LANES>(dot);
-  if (sigmoid && renorm) total = lanes_sum<LANES>(total);
   __syncwarp();
   for (int j = sub; j < topk; j += LANES) {
     const Choice c = j == sub ? mine : chosen(j);
     if (c.e < 0) continue;
-    float d;
-    if (sigmoid) {
-      float s = c.w, g = c.g;
-      if (renorm) {
-        s = sigmoid_of(c.e);
-        g = total > 0.0f ? (g - dot) / total : 0.0f;
-      }
-      d = g * s * (1.0f - s);
-    } else {
-      d = renorm ? c.w * (c.g - dot) : c.g * c.w;
-    }
+    float d = c.w * (renorm ? c.g - dot : c.g);
+    if (sigmoid) d *= complement_of(c.e);
     buf[c.e] = d;
   }
   float first = 0.0f, inv = 0.0f;
