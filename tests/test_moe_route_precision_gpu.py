@@ -92,3 +92,21 @@ def test_saturated_sigmoid_scores_keep_their_gradient(dtype, renormalize):
     x = torch.full((1, 4), 18.0, device="cuda", requires_grad=True)
     (d,) = torch.autograd.grad(tb.moe_route(x, 1, scoring="sigmoid", renormalize=False)[0].sum(), x)
     assert 1.4e-8 < float(d[0, 0]) < 1.6e-8         # e^-18
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("low", [-60.0, -95.0, -3e4])
+def test_renormalised_sigmoid_of_very_negative_logits(dtype, low):
+    """The scores of such a row are too small for fp32, their quotients are exponentials of differences."""
+    g = torch.Generator().manual_seed(7)
+    logits = torch.randn(30, 24, generator=g) * 3 + low
+    logits[::3, 5] = 2.0                                    # rows with one large score among them
+    logits[4] = float("-inf")
+    logits[6, 3:] = float("-inf")
+    logits[8] = torch.finfo(dtype).min                      # a row of the type's lowest value: all alike
+    logits = logits.to(dtype).cuda()
+    check(logits, 6, "sigmoid", True)
+    w, ids = tb.moe_route(logits, 6, scoring="sigmoid")
+    live = (ids >= 0).any(1)
+    # six quotients, each within (topk + 40) u plus its arguments' roundings, at most 2^-8 where logits are near 3e4 and fp32
+    assert ((w.sum(1) - 1).abs()[live] <= 1e-2).all() and torch.allclose(w[8], torch.full((6,), 1 / 6, device="cuda"))

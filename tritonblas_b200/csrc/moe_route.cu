@@ -201,17 +201,20 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_kernel(const T* __rest
   }
   __syncwarp();
   const float top = choice[0] != 0 ? Key<T>::value(choice[0]) : 0.0f;
+  // Renormalised sigmoid scores are formed over exp(m), m = min(top, 0), which cancels in the quotient: below -88 the scores
+  // themselves leave fp32's range, their quotients do not. With m = 0 this is the plain 1 / (1 + exp(-l)).
+  const float m = renorm ? fminf(top, 0.0f) : 0.0f, unit = expf(m);
   float sum = 0.0f;
   for (int j = sub; j < topk; j += LANES) {
     const K k = choice[j];
     float s = 0.0f;
-    if (k != 0) s = sigmoid ? 1.0f / (1.0f + expf(-Key<T>::value(k))) : expf(Key<T>::value(k) - top);
+    if (k != 0) s = sigmoid ? 1.0f / (unit + expf(m - Key<T>::value(k))) : expf(Key<T>::value(k) - top);
     score[j] = s;
     sum += s;
   }
   if (renorm) {
     sum = lanes_sum<LANES>(sum);
-    if (sum == 0.0f) sum = 1.0f;  // sigmoid scores that all underflow, or nothing to choose
+    if (sum == 0.0f) sum = 1.0f;  // nothing to choose
   } else if (sigmoid) {
     sum = 1.0f;
   } else {
