@@ -1,8 +1,8 @@
 """Router weights and gradients element by element, relative to what each element is made of.
 
 Bounds, in half units u = 2^-24 of fp32 arithmetic. An exponential exp(l - m) is off by its argument's rounding (computed exactly
-below: zero where both are short) and 4 u; a row's sum by the largest of those, 37 u of additions (32 in a lane at most, five
-exchanges) and a quotient by u: (argument + 64 u) relative covers a softmax score. A sigmoid 1 / (1 + exp(-l)) or its complement
+below: zero where both are short) and 4 u; a row's sum by the mean of those and a half unit per addition (as many as a lane holds
+logits, 8 to 32, and five exchanges), a quotient by u and a product by u: argument + (11 + additions) u covers a softmax score. A sigmoid 1 / (1 + exp(-l)) or its complement
 is off by 8 u, a sum of topk of them by topk u more. A gradient term g w - p dot or w (g - dot) is off by what its factors are,
 dot by the sum of what |g w| are off and (topk + 2) u, and the result by half a step of its type."""
 import pytest
@@ -36,7 +36,8 @@ def expected(logits, topk, scoring, renormalize, grad):
             rel = so + so.max(1, keepdim=True).values + (topk + 32) * U
         else:
             p = p / p.sum(1, keepdim=True).clamp(min=1e-300)
-            rel_p = off + (p * off).sum(1, keepdim=True) + 64 * U
+            adds = (8 if logits.shape[1] <= 256 else 16 if logits.shape[1] <= 512 else 32) + 5
+            rel_p = off + (p * off).sum(1, keepdim=True) + (11 + adds) * U
             w, rel = pick(p), pick(rel_p)
     else:
         s = torch.sigmoid(l)
@@ -110,3 +111,26 @@ def test_renormalised_sigmoid_of_very_negative_logits(dtype, low):
     live = (ids >= 0).any(1)
     # six quotients, each within (topk + 40) u plus its arguments' roundings, at most 2^-8 where logits are near 3e4 and fp32
     assert ((w.sum(1) - 1).abs()[live] <= 1e-2).all() and torch.allclose(w[8], torch.full((6,), 1 / 6, device="cuda"))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("experts", [24, 64, 200])
+def test_small_softmax_scores(dtype, experts):
+    """Scores down to exp(-80) of the largest: the error of an exponential does not grow with its distance from the maximum. The
+    logits are multiples of 1/4, so their differences are exact."""
+    g = torch.Generator().manual_seed(experts)
+    logits = (torch.rand(40, experts, generator=g) * 320).round() / 4 - 40
+    check(logits.to(dtype).cuda(), 7, "softmax", False)
+
+
+def test_the_error_of_a_small_score_does_not_grow_with_its_distance():
+    """One score of 1 and a tail that vanishes beside it: weight and sum are exactly 1, and d_i = -exp(l_i - l_0) is an exponential
+    of an exact argument, good to 4 u, times two factors of 1."""
+    logits = (-torch.arange(0, 84 * 64, 1).double() / 64).view(84, 64)[25:80].float().cuda()        # 25 to 80, in steps of 1/64
+    logits[:, 0] = 0.0
+    x = logits.requires_grad_(True)
+    w, ids = tb.moe_route(x, 1, renormalize=False)
+    assert (w == 1).all() and (ids == 0).all()
+    (d,) = torch.autograd.grad(w.sum(), x)
+    want = -torch.exp(logits.detach().double())[:, 1:]
+    assert ((d.double()[:, 1:] - want).abs() <= 4 * U * want.abs()).all()

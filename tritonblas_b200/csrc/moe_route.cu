@@ -220,7 +220,7 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_kernel(const T* __rest
   } else {
     sum = 0.0f;
 #pragma unroll
-    for (int i = 0; i < VPT; ++i) sum += __expf(l[i] - top);  // 2 units in the last place more: terms below the first, which is 1
+    for (int i = 0; i < VPT; ++i) sum += expf(l[i] - top);
     sum = lanes_sum<LANES>(sum);
   }
   if (live) {
@@ -311,7 +311,7 @@ route_bwd_kernel(const T* __restrict__ logits, long long stride, long long token
 #pragma unroll
       for (int j = 0; j < VEC; ++j) {
         float d = v[j];
-        if (dense) d -= __expf(p[i + j] - first) * inv;
+        if (dense) d -= expf(p[i + j] - first) * inv;
         from_float(d, o.v[j]);
       }
       *reinterpret_cast<Pack<T, VEC>*>(drow + c) = o;
