@@ -134,3 +134,56 @@ def test_the_error_of_a_small_score_does_not_grow_with_its_distance():
     (d,) = torch.autograd.grad(w.sum(), x)
     want = -torch.exp(logits.detach().double())[:, 1:]
     assert ((d.double()[:, 1:] - want).abs() <= 4 * U * want.abs()).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("scoring,renormalize", MODES)
+@pytest.mark.parametrize("tokens,experts,topk,offset", [(5, 24, 3, 0), (70, 100, 8, 1), (9, 256, 32, 0), (3, 257, 8, 0), (40, 300, 10, 0), (7, 304, 32, 0),
+                                                        (33, 304, 4, 1), (6, 512, 8, 0), (4, 512, 1, 3), (5, 520, 9, 0), (3, 1000, 10, 0), (2, 1024, 32, 0),
+                                                        (9, 1024, 2, 1)])
+def test_every_width(tokens, experts, topk, offset, dtype, scoring, renormalize):
+    """All lane counts, 8, 16 and 32 logits a lane, runs of eight and single elements (odd sizes, or a base that is `offset`
+    elements behind a 16-byte boundary)."""
+    g = torch.Generator().manual_seed(experts + topk)
+    logits = torch.randn(tokens, experts, generator=g) * 2
+    logits[torch.rand(tokens, experts, generator=g) < 0.05] = float("-inf")
+    logits[-1] = 0.5
+    logits[tokens // 2, 1:] = float("nan")
+    buf = torch.empty(tokens * experts + offset, dtype=dtype, device="cuda")
+    view = buf[offset:].view(tokens, experts)
+    view.copy_(logits.to(dtype))
+    check(view, topk, scoring, renormalize, seed=experts)
+    if scoring == "softmax" and not renormalize:
+        # the bound sees the gradient of the experts that were not chosen: without it the expectation itself is outside
+        _, _, _, d, b = expected(view, topk, scoring, renormalize, torch.randn(tokens, topk, generator=torch.Generator().manual_seed(experts)))
+        ids = tb.moe_route(view, topk)[1].cpu().long()
+        kept = torch.zeros_like(d).scatter_(1, ids.clamp(min=0), 1.0)
+        missing = (d.abs() > b) & (kept == 0)
+        assert missing.sum() > 0.5 * ((kept == 0) & (view.cpu().float() > float("-inf"))).sum()
+
+
+@pytest.mark.parametrize("scoring,renormalize", MODES)
+@pytest.mark.parametrize("experts", [300, 1000])
+def test_wide_rows_against_differences(experts, scoring, renormalize):
+    """Central differences in 64 bits at fixed choices. Step 1e-4: truncation h^2 / 6 times a third derivative of at most 1, and
+    cancellation 2^-53 / h; the kernel's own error is a few hundred u of sums of |g| times weights."""
+    g = torch.Generator().manual_seed(experts)
+    x = (torch.randn(2, experts, generator=g) * 1.5).cuda().requires_grad_(True)
+    grad = torch.randn(2, 6, generator=g).cuda()
+    w, ids = tb.moe_route(x, 6, scoring=scoring, renormalize=renormalize)
+    (dl,) = torch.autograd.grad(w, x, grad)
+
+    def value(l):
+        p = torch.softmax(l, -1) if scoring == "softmax" else torch.sigmoid(l)
+        s = torch.gather(p, -1, ids.long().expand(l.shape[0], 2, 6))
+        if renormalize:
+            s = s / s.sum(-1, keepdim=True)
+        return (s * grad.double()).sum(-1)
+
+    h = 1e-4
+    step = torch.eye(experts, dtype=torch.float64, device="cuda").unsqueeze(1) * h
+    l = x.detach().double().unsqueeze(0)
+    d = ((value(l + step) - value(l - step)) / (2 * h)).T
+    scale = (grad.double() * w.detach().double()).abs().sum(1, keepdim=True)
+    assert ((dl.double() - d).abs() <= 3e-8 + 300 * U * scale).all()
+    assert (d.abs() > 3e-8 + 300 * U * scale).sum() > (experts if scoring == "softmax" and not renormalize else 8)
