@@ -271,8 +271,10 @@ int tb_moe_route_backward(const void* logits, int32_t dtype, int64_t row_stride,
  *   out[t, :] = sum_j topk_weights[t, j] * W2_e ( silu(G_e x_t) * (U_e x_t) ),  e = topk_ids[t, j],  W1_e = [G_e ; U_e].
  * x (tokens, hidden), w1 (num_experts, 2*ffn, hidden), w2 (num_experts, hidden, ffn), out (tokens, hidden), all of `dtype`
  * (f16 or bf16), rows contiguous, x, w1 and w2 with 16-byte aligned rows and bases; topk_ids (tokens, topk) int32 or int64,
- * topk_weights (tokens, topk) fp32, both contiguous. Sums, activation and weights are fp32, one cast at the end. An id outside
- * [0, num_experts) adds nothing (a token with no other id gets zeros); the same id twice in a row counts twice.
+ * topk_weights (tokens, topk) fp32, both contiguous. Sums, activation and weights are fp32, one cast at the end; the activation's
+ * result is kept in two 16-bit halves in between (bf16: 2^-16 relative; f16: 2^-22 relative or 2^-28 absolute, whichever is more,
+ * infinite above 65504 * 256). An id outside [0, num_experts) adds nothing (a token with no other id gets zeros); the same id
+ * twice in a row counts twice.
  * tokens <= 128, topk <= 32, num_experts <= 1024, hidden and ffn multiples of 8. The workspace
  * (tb_moe_mlp_workspace_bytes, 256-byte aligned) needs no initialisation and must not be shared by calls that can overlap.
  * Device-side waits are bounded (wait_timeout_ms, 0 = 2 s) and report through tb_device_status. */

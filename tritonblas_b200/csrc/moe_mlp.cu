@@ -20,6 +20,11 @@
 // Rounding: sums, activation, routing weights and the sum over experts are fp32. The tensor core takes h in 16 bits, so h is
 // kept as two 16-bit halves, h = hi + lo with lo = round(h - hi), and multiplied by both: the MMAs double, the bytes do not,
 // and the result stays as close to the formula as its own rounding allows (a single 16-bit h would double the squared error).
+// fp16 has neither the range nor the small numbers for that, so there the halves stand in units of their own, 2^8 and 2^-3,
+// which the second epilogue multiplies back in (each half has its own columns of the product): h is held to 2^-22 relative or
+// 2^-28 absolute, whichever is more, up to 65504 * 2^8; above that it is infinite. The floor is chosen against the output's own
+// smallest step, 2^-24: rows of W2 with a norm of up to about 10 add less than half of it. (Without the units the floor was
+// 2^-25, 3e-3 of an h of 1e-5, and the limit 65504.) bf16 has fp32's range: its units are 1.
 // No reference counterpart (the reference has no MoE path).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -370,6 +375,16 @@ template <>
 __device__ __forceinline__ float from_bits<__half>(unsigned short v) {
   return __half2float(__ushort_as_half(v));
 }
+
+// Units of the two halves of h: hi * kHi + lo * kLo.
+template <typename T>
+struct HalfUnits {
+  static constexpr float kHi = 1.0f, kLo = 1.0f;
+};
+template <>
+struct HalfUnits<__half> {
+  static constexpr float kHi = 256.0f, kLo = 0.125f;  // kHi / kLo = 2^11: the rest of the largest hi still fits lo
+};
 
 __device__ __forceinline__ float4 add4(float4 a, float4 b) { return make_float4(a.x + b.x, a.y + b.y, a.z + b.z, a.w + b.w); }
 // Four consecutive outputs; `vec`: the address is a multiple of 8.
@@ -754,10 +769,11 @@ moe_mlp_kernel(const __grid_constant__ CUtensorMap tmap_w1, const __grid_constan
               const float g = __uint_as_float(r[j]);
               const float up = __shfl_xor_sync(0xffffffffu, g, 8);
               const float h = g / (1.0f + expf(-g)) * up;
-              const unsigned short hi = to_bits<T>(h);
+              const unsigned short hi = to_bits<T>(h * (1.0f / HalfUnits<T>::kHi));
               // an infinite h has no low half (inf - inf)
-              const float rest = h - from_bits<T>(hi);
-              const unsigned short lo = fabsf(rest) < __builtin_huge_valf() ? to_bits<T>(rest) : static_cast<unsigned short>(0);
+              const float rest = h - from_bits<T>(hi) * HalfUnits<T>::kHi;
+              const unsigned short lo =
+                  fabsf(rest) < __builtin_huge_valf() ? to_bits<T>(rest * (1.0f / HalfUnits<T>::kLo)) : static_cast<unsigned short>(0);
               if (mine) {
                 unsigned short* dst = reinterpret_cast<unsigned short*>(p.h) + static_cast<long long>(row) * 2 * p.ffn + f;
                 dst[0] = hi;
@@ -773,7 +789,8 @@ moe_mlp_kernel(const __grid_constant__ CUtensorMap tmap_w1, const __grid_constan
             const int row = (c0 + j) >> 1;
             if (row < u.rows && mine)
               __stcg(p.y + static_cast<long long>(u.off + row) * p.hidden + hcol,
-                     __ldcg(row_weight + u.off + row) * (__uint_as_float(r[j]) + __uint_as_float(r[j + 1])));
+                     __ldcg(row_weight + u.off + row) *
+                         (__uint_as_float(r[j]) * HalfUnits<T>::kHi + __uint_as_float(r[j + 1]) * HalfUnits<T>::kLo));
           }
         }
       }

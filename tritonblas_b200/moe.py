@@ -152,8 +152,10 @@ def moe_mlp(x, w1, w2, topk_ids, topk_weights, out: Optional[torch.Tensor] = Non
     x: (tokens, hidden); w1: (experts, 2*ffn, hidden) and w2: (experts, hidden, ffn), the layout ``PeerMemoryMoE`` takes; all
     float16 or all bfloat16, hidden and ffn multiples of 8. topk_ids: (tokens, topk) int32 or int64, topk_weights: (tokens, topk),
     as ``moe_route`` returns them. An id outside [0, experts) adds nothing; the same id twice counts twice. Sums, activation and
-    weighting are float32 with one cast at the end; silu(gate) * up itself has the operands' range (float16: infinite above 65504). ``out`` may be given: (tokens, hidden), contiguous rows, no overlap with the
-    weights. Inference only. More tokens: ``distributed.PeerMemoryMoE``.
+    weighting are float32 with one cast at the end. silu(gate) * up is an operand of a tensor-core product and kept in two 16-bit
+    halves: to 2^-16 relative in bfloat16; in float16 to 2^-22 relative or 2^-28 absolute, and infinite above 65504 * 256.
+    ``out`` may be given: (tokens, hidden), contiguous rows, no overlap with the weights. Inference only. More tokens:
+    ``distributed.PeerMemoryMoE``.
     """
     if x.ndim != 2 or w1.ndim != 3 or w2.ndim != 3 or topk_ids.ndim != 2:
         refuse("x must be (tokens, hidden), w1 and w2 3-D, topk_ids 2-D")
