@@ -90,15 +90,16 @@ def lora_matmul(x, w, lora_a, lora_b, adapter_ids, scales=None, bias=None, out: 
                          None if bias is None else bias.data_ptr(), 0 if bias is None else bias.stride(0), out.data_ptr(), o_m, o_n,
                          None, 0, 0 if bias is None else _lib.DTYPE_CODE[bias.dtype], int(ids.dtype is torch.int64), 0)
     ref = ctypes.byref(args)
-    need = _lib.lib.tb_lora_workspace_bytes(ref)
-    rows = tokens
-    while (need > _MAX_WORKSPACE or need == 0) and rows > 256:     # 0: more rows than one launch pair can number
-        args.m = rows = max(256, (rows // 2 + 255) // 256 * 256)
-        need = _lib.lib.tb_lora_workspace_bytes(ref)
-    # per call, from torch's allocator: calls on other streams and captured graphs never share it
-    ws = torch.empty(need, dtype=torch.uint8, device=device)
-    args.workspace, args.workspace_bytes = ws.data_ptr(), need
+    # the plan behind both calls goes by the current device's SMs
     with on_device(device):
+        need = _lib.lib.tb_lora_workspace_bytes(ref)
+        rows = tokens
+        while (need > _MAX_WORKSPACE or need == 0) and rows > 256:     # 0: more rows than one launch pair can number
+            args.m = rows = max(256, (rows // 2 + 255) // 256 * 256)
+            need = _lib.lib.tb_lora_workspace_bytes(ref)
+        # per call, from torch's allocator: calls on other streams and captured graphs never share it
+        ws = torch.empty(need, dtype=torch.uint8, device=device)
+        args.workspace, args.workspace_bytes = ws.data_ptr(), need
         stream = _lib.current_stream_ptr(device)
         first = 0
         while True:
