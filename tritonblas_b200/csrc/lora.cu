@@ -212,6 +212,7 @@ __device__ __forceinline__ void clear_absent(const ProjectParams& p, const RunLi
 
 __device__ __forceinline__ void cluster_or_block_sync(int splits) {
   if (splits > 1) {
+    __syncwarp();  // the cluster barrier's instructions are .aligned, and what comes before them here branches per lane
     cluster_arrive();
     cluster_wait();
   } else {
