@@ -22,3 +22,10 @@ def test_cluster_barriers_are_reached_by_whole_warps():
                 before = [q for q in st[:i] if not q.startswith("if ")][-1]
                 assert before in ("__syncwarp()", "__syncthreads()"), (os.path.basename(path), before)
     assert found >= 3
+
+
+def test_the_adapters_projection_takes_tensor_memory_between_wait_and_launch():
+    """A block that holds tensor memory while it waits for another kernel could keep a block of that kernel from getting its own."""
+    text = open(os.path.join(CSRC, "lora.cu")).read()
+    body = text[text.index("lora_project_tc_kernel("):]
+    assert body.index("griddep_wait()") < body.index("tmem_alloc<1>") < body.index("griddep_launch_dependents()")
