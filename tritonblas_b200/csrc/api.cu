@@ -574,10 +574,10 @@ static int gemm_impl(const tb_gemm_args& a_in, const tb_config* user_cfg, cudaSt
     p.lr_tile_rows = lr->tile_rows;
     CUtensorMap tv, tlb;
     p.lr_pack = lr->pack;
-    const uint32_t inner = bk / lr->pack;
-    const uint64_t v_cols = static_cast<uint64_t>(lr->kblocks) * inner;
+    const uint32_t inner = 32u / lr->pack, v_inner = 2 * inner;  // of v both halves
+    const uint64_t v_cols = static_cast<uint64_t>(lr->kblocks) * v_inner;
     const uint64_t v_dims[2] = {v_cols, static_cast<uint64_t>(lr->v_rows)}, v_strides[1] = {v_cols * es};
-    const uint32_t v_box[2] = {inner, 128};
+    const uint32_t v_box[2] = {v_inner, 128};
     if ((rc = encode_nd(&tv, a.a_dtype, lr->v, 2, v_dims, v_strides, v_box)) != TB_OK) return rc;
     const uint64_t dims[3] = {static_cast<uint64_t>(lr->rank), static_cast<uint64_t>(lr->n), static_cast<uint64_t>(lr->num_adapters)};
     const uint64_t strides[2] = {static_cast<uint64_t>(lr->b_row_stride) * es,

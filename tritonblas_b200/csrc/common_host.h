@@ -26,8 +26,9 @@ int encode_2d(CUtensorMap* map, int dtype, const void* base, uint64_t inner, uin
 int encode_nd(CUtensorMap* map, int dtype, const void* base, int rank, const uint64_t* dims, const uint64_t* strides,
               const uint32_t* box);
 
-// Low-rank update of a dense launch (see GemmParams::lr_list): the tokens' masked projections v, one block of tile_rows rows of
-// kblocks * 64 / pack elements per token tile and listed adapter, and lora_b (num_adapters, n, rank).
+// Low-rank update of a dense launch (see GemmParams::lr_list): the tokens' masked projections v, one block of tile_rows rows per
+// token tile and listed adapter, and lora_b (num_adapters, n, rank). A row is `kblocks` times as many high 16-bit halves as a stage
+// has ranks of one adapter (32 / pack, in the decode form 64 / pack) and as many low ones.
 struct LowRank {
   const void* v;
   int64_t v_rows;

@@ -102,15 +102,16 @@ struct GemmParams {
   // schedules, plain 2-D / 3-D operand copies).
   int early_operand;
   // Low-rank update beside the product (LOWRANK instantiation: data-parallel, narrow tiles, K-major 16-bit extension operands):
-  // after a tile's own K range come further stages for the adapters that occur among the tile's rows: `lr_kblocks` per adapter,
-  // or one for `lr_pack` adapters whose ranks fit side by side in a stage (each with rows of 128 / lr_pack bytes). On A's side
-  // they hold the rows' rank-sized projections, zero in rows of other adapters (tensor map `sfa`, one block of lr_tile_rows rows
-  // per tile of rows and listed adapter), on B's side that adapter's rows of lora_b (`sfb`). All of it adds up in the same
-  // accumulator, so the sum is rounded once.
+  // after a tile's own K range come further stages for the adapters that occur among the tile's rows: `lr_kblocks` of 32 ranks per
+  // adapter, or one for two adapters of up to 16 (lr_pack = 2). On A's side they hold the rows' rank-sized projections, zero in
+  // rows of other adapters, as 32 / lr_pack high 16-bit halves and the low ones behind them (rows of 128 / lr_pack bytes; tensor
+  // map `sfa`, one block of lr_tile_rows rows per tile of rows and listed adapter), on B's side that adapter's rows of lora_b
+  // (rows of 64 / lr_pack bytes; `sfb`), which either half is multiplied by. All of it adds up in the same accumulator, so the sum
+  // is rounded once.
   const int* lr_list;   // per tile of rows: number of adapters, then their indices; written by the kernel launched before
   int lr_list_stride;   // words per tile of rows
   int lr_kblocks;       // stages per adapter (1 when lr_pack > 1)
-  int lr_pack;          // adapters per stage: 1 (128-byte swizzle), 2 (64-byte) or 4 (32-byte)
+  int lr_pack;          // adapters per stage: 1 or 2
   int lr_rank;
   int lr_tile_rows;     // rows of a tile of this launch
   // failure reporting
@@ -926,33 +927,34 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ 
         if constexpr (LOWRANK) {
           if (!ok) break;
           const int block_row0 = tg.m0 / p.lr_tile_rows * (p.lr_list_stride - 1) * p.lr_tile_rows;
-          const int a_part = kATileBytes / p.lr_pack, b_part = b_tile_bytes / p.lr_pack;
+          const int width = 32 / p.lr_pack;
+          const int a_part = kATileBytes / p.lr_pack, b_part = b_tile_bytes / (2 * p.lr_pack);
           for (int i = 0; i < lr_count && ok; i += p.lr_pack) {
             if (i > 0 && (i & 31) == 0) lr_mine = i + lane + 1 < p.lr_list_stride ? __ldcg(lr_entries + 1 + i + lane) : 0;
             const int filled = min(p.lr_pack, lr_count - i);
-            int adapter[4];  // lr_pack divides 32: a group's entries stand in one run of the warp's lanes
+            int adapter[2];  // lr_pack divides 32: a group's entries stand in one run of the warp's lanes
 #pragma unroll
-            for (int j = 0; j < 4; ++j) adapter[j] = __shfl_sync(0xffffffffu, lr_mine, (i + j) & 31);
+            for (int j = 0; j < 2; ++j) adapter[j] = __shfl_sync(0xffffffffu, lr_mine, (i + j) & 31);
             for (int kb = 0; kb < p.lr_kblocks; ++kb) {
               ok = mbar_wait_warp(&empty_bar[s], ph ^ 1, wctx, TB_DEV_TIMEOUT_SMEM_EMPTY);
               if (!ok) break;
               uint8_t* sa = ring + static_cast<size_t>(s) * stage_bytes;
               uint8_t* sb = sa + kATileBytes;
-              const int k0 = kb * p.k_per_stage;
+              const int k0 = kb * width;
               if (elect_one()) {
                 const uint32_t bytes = static_cast<uint32_t>(filled * (a_part + b_part)) * CTAS;
                 const uint32_t bar = (CTAS == 2) ? mapa_cluster(smem_u32(&full_bar[s]), 0) : 0u;
                 if (CTAS == 1 || cta_rank == 0) mbar_arrive_expect_tx(&full_bar[s], bytes);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
+                for (int j = 0; j < 2; ++j) {
                   if (j >= filled) break;
                   const int block_row = block_row0 + (i + j) * p.lr_tile_rows;
                   uint8_t *da = sa + j * a_part, *db = sb + j * b_part;
                   if constexpr (CTAS == 1) {
-                    tma_load_2d(da, &tmap_sfa, &full_bar[s], k0, block_row);
+                    tma_load_2d(da, &tmap_sfa, &full_bar[s], 2 * k0, block_row);
                     tma_load_3d(db, &tmap_sfb, &full_bar[s], k0, n0, adapter[j]);
                   } else {
-                    tma_load_2d_pair(da, &tmap_sfa, bar, k0, block_row + static_cast<int>(cta_rank) * kTileM);
+                    tma_load_2d_pair(da, &tmap_sfa, bar, 2 * k0, block_row + static_cast<int>(cta_rank) * kTileM);
                     tma_load_3d_pair(db, &tmap_sfb, bar, k0, n0, adapter[j]);
                   }
                 }
@@ -1097,11 +1099,12 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ 
           }
           if (!ok) break;
           if constexpr (LOWRANK) {
-            // both extension operands are K-major whatever the product's own layouts are; rows of 128 / lr_pack bytes
-            const uint32_t swizzle = p.lr_pack == 1 ? 2u : (p.lr_pack == 2 ? 4u : 6u), row_group = 1024u / p.lr_pack;
-            const uint64_t xa0 = make_smem_desc(ring_addr, 16u, row_group, swizzle);
-            const uint64_t xb0 = make_smem_desc(ring_addr + kATileBytes, 16u, row_group, swizzle);
-            const uint64_t a_part = (kATileBytes / p.lr_pack) >> 4, b_part = (b_tile_bytes / p.lr_pack) >> 4;
+            // both extension operands are K-major whatever the product's own layouts are
+            const int width = 32 / p.lr_pack;
+            const uint64_t xa0 = make_smem_desc(ring_addr, 16u, 1024u / p.lr_pack, p.lr_pack == 1 ? 2u : 4u);
+            const uint64_t xb0 = make_smem_desc(ring_addr + kATileBytes, 16u, 512u / p.lr_pack, p.lr_pack == 1 ? 4u : 6u);
+            const uint64_t a_low = static_cast<uint64_t>(width) * 2 >> 4;
+            const uint64_t a_part = (kATileBytes / p.lr_pack) >> 4, b_part = (b_tile_bytes / (2 * p.lr_pack)) >> 4;
             const uint32_t x_idesc = idesc & ~(3u << 15);
             for (int i = 0, kb = 0; i < lr_count;) {
               ok = mbar_wait_warp(&full_bar[s], ph, wctx, TB_DEV_TIMEOUT_SMEM_FULL);
@@ -1109,10 +1112,10 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ 
               if (elect_one()) {
                 const uint64_t soff = static_cast<uint64_t>(s * stage_step);
                 const int filled = min(p.lr_pack, lr_count - i);
-                const int steps = min(4 / p.lr_pack, (p.lr_rank - kb * p.k_per_stage + 15) >> 4);  // behind the rank: zeros
+                const int steps = min(2 / p.lr_pack, (p.lr_rank - kb * width + 15) >> 4);  // behind the rank: zeros
                 for (int j = 0; j < filled; ++j)
-                  for (int k = 0; k < steps; ++k)
-                    umma<KIND, CTAS>(d0, xa0 + soff + j * a_part + 2 * k, xb0 + soff + j * b_part + 2 * k, x_idesc, 1u);
+                  for (int k = 0; k < 2 * steps; ++k)  // high and low half in turn
+                    umma<KIND, CTAS>(d0, xa0 + soff + j * a_part + (k & 1) * a_low + (k & ~1), xb0 + soff + j * b_part + (k & ~1), x_idesc, 1u);
                 commit(&empty_bar[s]);
               }
               __syncwarp();

@@ -9,8 +9,12 @@
 // either waits for one outside its own cluster, so calls on several streams cannot block each other.
 //
 // The projection is bound by reading x and the used adapters' A once; it has a form for decode batches (mostly one adapter per
-// row) and one for longer ones. v is rounded to the operands' 16-bit type once, after the scale: it is an operand of a tensor-core
-// product. Its error is eps / 2 of each of `rank` terms of the update, next to the one rounding of the output.
+// row) and one for longer ones.
+//
+// Rounding: all sums are fp32. v is an operand of a tensor-core product, so it is kept as two 16-bit halves, v = hi + lo with
+// lo = round(v - hi), which stand side by side in a row of its block, 16 to 64 ranks at a time, and are both multiplied by the same rows of B: 2^-16 of v
+// (bf16), or 2^-22 or 2^-25 absolute, whichever is more (fp16, whose v is infinite above 65504: the update adds up in the
+// product's own accumulator, so it can have no unit of its own).
 // No reference counterpart (the reference has no adapters).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -46,7 +50,8 @@ struct ProjectParams {
   int tokens, k, rank, num_adapters;
   int tile_rows;        // rows of a GEMM tile
   int max_slots;        // list entries per tile
-  int v_cols;           // columns of a block (rank rounded up to 16, 32 or a multiple of 64)
+  int v_width;          // ranks of a stage of the product: a block's row is their high halves, then the low ones, for v_cols ranks
+  int v_cols;           // rank rounded up to a multiple of v_width
   int splits;           // CTAs of a cluster that share K
   int k_chunk;          // K per CTA, a multiple of 32
   void* v;
@@ -83,6 +88,13 @@ template <>
 __device__ __forceinline__ __nv_bfloat16 cast16<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 template <>
 __device__ __forceinline__ __half cast16<__half>(float v) { return __float2half_rn(v); }
+
+// The two halves of v; an infinite v has no low half (inf - inf).
+template <typename T>
+__device__ __forceinline__ T low_half(float v, T hi) {
+  const float rest = v - static_cast<float>(hi);
+  return cast16<T>(fabsf(rest) < __builtin_huge_valf() ? rest : 0.0f);
+}
 
 // Sum of one float per CTA of the cluster (at most 8) at the same shared-memory offset, in rank order.
 __device__ __forceinline__ float cluster_sum(const float* mine, int splits) {
@@ -202,11 +214,11 @@ __device__ __forceinline__ int2 find_adapters(const ProjectParams& p, RunLists<k
 // The run's rows in the blocks of the tile's other adapters are zeros; dealt over the blocks of the grid's y axis.
 template <int kRows, typename T>
 __device__ __forceinline__ void clear_absent(const ProjectParams& p, const RunLists<kRows>& l, T* tile_blocks, int count, int rank) {
-  const long long block_stride = static_cast<long long>(p.tile_rows) * p.v_cols;
+  const long long block_stride = static_cast<long long>(p.tile_rows) * 2 * p.v_cols;
   for (int slot = blockIdx.y; slot < count; slot += gridDim.y) {
     if (l.present[slot]) continue;
     uint4* block = reinterpret_cast<uint4*>(tile_blocks + slot * block_stride);
-    for (int i = threadIdx.x + rank * kThreads; i < kRows * p.v_cols / 8; i += kThreads * p.splits) block[i] = make_uint4(0, 0, 0, 0);
+    for (int i = threadIdx.x + rank * kThreads; i < kRows * 2 * p.v_cols / 8; i += kThreads * p.splits) block[i] = make_uint4(0, 0, 0, 0);
   }
 }
 
@@ -243,8 +255,9 @@ __global__ void __maxnreg__(120) lora_project_kernel(const ProjectParams p) {
     for (int i = tid; i < p.counter_words; i += kThreads) p.counters[i] = 0u;
   const int2 found = find_adapters<kRows>(p, lists, row0, row0 == tile_row0 && blockIdx.y == 0 && rank == 0);
   const int* run_ids = lists.ids + (row0 - tile_row0);
-  T* tile_blocks = static_cast<T*>(p.v) + static_cast<long long>(tile) * p.max_slots * p.tile_rows * p.v_cols +
-                   static_cast<long long>(row0 - tile_row0) * p.v_cols;
+  const int v_row = 2 * p.v_cols;
+  T* tile_blocks = static_cast<T*>(p.v) + static_cast<long long>(tile) * p.max_slots * p.tile_rows * v_row +
+                   static_cast<long long>(row0 - tile_row0) * v_row;
   clear_absent<kRows>(p, lists, tile_blocks, found.x, rank);
 
   const T* x = static_cast<const T*>(p.x);
@@ -255,7 +268,8 @@ __global__ void __maxnreg__(120) lora_project_kernel(const ProjectParams p) {
     const int turn = item / slices, c0 = (item - turn * slices) * kCols;  // first rank of the slice
     const int ranks = p.rank - c0;
     const int adapter = lists.run_ids[turn];
-    T* block = tile_blocks + lists.run_slots[turn] * static_cast<long long>(p.tile_rows) * p.v_cols + c0;
+    T* block = tile_blocks + lists.run_slots[turn] * static_cast<long long>(p.tile_rows) * v_row +
+               2 * (c0 & ~(p.v_width - 1)) + (c0 & (p.v_width - 1));  // kCols divides v_width
     const float scale = p.scales != nullptr ? __ldg(p.scales + adapter) : 1.0f;
     // only rows with this adapter are read; the others enter the product as zeros
     bool live[2];
@@ -315,7 +329,9 @@ __global__ void __maxnreg__(120) lora_project_kernel(const ProjectParams p) {
       float v = 0.0f;
       if (c < ranks && run_ids[r] == adapter)
         v = scale * (p.splits > 1 ? cluster_sum(&s_part[r][c], p.splits) : s_part[r][c]);
-      block[r * p.v_cols + c] = cast16<T>(v);
+      const T hi = cast16<T>(v);
+      block[r * v_row + c] = hi;
+      block[r * v_row + p.v_width + c] = low_half<T>(v, hi);
     }
     cluster_or_block_sync(p.splits);  // nobody overwrites or leaves its sums while another CTA still reads them
   }
@@ -366,8 +382,9 @@ lora_project_tc_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_
   tc_fence_after();
   const uint32_t tmem_base = tmem_slot;
   const int* run_ids = lists.ids + (row0 - tile_row0);
-  T* tile_blocks = static_cast<T*>(p.v) + static_cast<long long>(tile) * p.max_slots * p.tile_rows * p.v_cols +
-                   static_cast<long long>(row0 - tile_row0) * p.v_cols;
+  const int v_row = 2 * p.v_cols, width = p.v_width;
+  T* tile_blocks = static_cast<T*>(p.v) + static_cast<long long>(tile) * p.max_slots * p.tile_rows * v_row +
+                   static_cast<long long>(row0 - tile_row0) * v_row;
   clear_absent<kRows>(p, lists, tile_blocks, found.x, cta);
 
   const int kb_begin = cta * p.k_chunk / 64;
@@ -376,7 +393,7 @@ lora_project_tc_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_
   uint32_t ph = 0, acc_ph = 0;
   for (int turn = blockIdx.y; turn < found.y; turn += gridDim.y) {
     const int adapter = lists.run_ids[turn];
-    T* block = tile_blocks + lists.run_slots[turn] * static_cast<long long>(p.tile_rows) * p.v_cols;
+    T* block = tile_blocks + lists.run_slots[turn] * static_cast<long long>(p.tile_rows) * v_row;
     const float scale = p.scales != nullptr ? __ldg(p.scales + adapter) : 1.0f;
     if (abort_word) {
       // an earlier turn's wait ran out: nothing more is loaded or multiplied
@@ -453,10 +470,15 @@ lora_project_tc_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[j] *= scale;
       }
-      alignas(16) T o[8];
+      alignas(16) T hi[8], lo[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) o[j] = cast16<T>(v[j]);
-      *reinterpret_cast<uint4*>(block + static_cast<long long>(r) * p.v_cols + c) = *reinterpret_cast<const uint4*>(o);
+      for (int j = 0; j < 8; ++j) {
+        hi[j] = cast16<T>(v[j]);
+        lo[j] = low_half<T>(v[j], hi[j]);
+      }
+      T* o = block + static_cast<long long>(r) * v_row + 2 * (c & ~(width - 1)) + (c & (width - 1));
+      *reinterpret_cast<uint4*>(o) = *reinterpret_cast<const uint4*>(hi);
+      *reinterpret_cast<uint4*>(o + width) = *reinterpret_cast<const uint4*>(lo);
     }
     cluster_or_block_sync(p.splits);  // nobody overwrites or leaves its sums while another CTA still reads them
   }
@@ -566,7 +588,7 @@ struct LoraPlan {
   bool decode;
   LoraDecodeShape shape;  // decode
   tb_config cfg;          // otherwise
-  int tile_rows, tiles, max_slots, v_cols, pack;
+  int tile_rows, tiles, max_slots, v_cols, v_width, pack, kblocks;
   long long v_offset, v_rows, list_offset, gemm_offset, gemm_bytes, bytes;
 };
 
@@ -589,12 +611,15 @@ int lora_plan(const tb_lora_args& a, int num_sms, tb_gemm_args* g, LoraPlan* l) 
   }
   l->tiles = (a.m + l->tile_rows - 1) / l->tile_rows;
   l->max_slots = l->tile_rows < a.num_adapters ? l->tile_rows : a.num_adapters;
-  // small ranks share a stage of the GEMM: see GemmParams::lr_pack
-  l->pack = a.rank <= 16 ? 4 : (a.rank <= 32 ? 2 : 1);
-  l->v_cols = l->pack > 1 ? 64 / l->pack : (a.rank + 63) / 64 * 64;
+  // small ranks share a stage of the product, which has room for 64 ranks up to 64 rows and for 32 above: see GemmParams::lr_pack
+  const int stage_ranks = l->decode ? 64 : 32;
+  l->pack = a.rank <= 16 ? stage_ranks / 16 : (a.rank <= 32 ? stage_ranks / 32 : 1);
+  l->v_width = stage_ranks / l->pack;
+  l->kblocks = (a.rank + l->v_width - 1) / l->v_width;
+  l->v_cols = l->kblocks * l->v_width;
   if (l->decode) {
     const int most = a.m < l->max_slots ? a.m : l->max_slots;
-    l->shape = lora_decode_shape(a.m, a.n, a.k, (most + l->pack - 1) / l->pack * ((a.rank + 63) / 64), num_sms);
+    l->shape = lora_decode_shape(a.m, a.n, a.k, (most + l->pack - 1) / l->pack * l->kblocks, num_sms);
   }
   l->v_rows = static_cast<long long>(l->tiles) * l->max_slots * l->tile_rows;
   if (l->v_rows > 0x7fffffffll) return TB_ERR_UNSUPPORTED;  // a row coordinate of a copy has 32 bits; shorter batches fit
@@ -604,7 +629,7 @@ int lora_plan(const tb_lora_args& a, int num_sms, tb_gemm_args* g, LoraPlan* l) 
   l->gemm_bytes = l->decode ? kCounterBytes + up(l->shape.part_bytes) : 0;
   l->list_offset = l->gemm_bytes;
   l->v_offset = l->list_offset + up(4ll * l->tiles * (1 + l->max_slots));
-  l->bytes = l->v_offset + up(l->v_rows * l->v_cols * 2);
+  l->bytes = l->v_offset + up(l->v_rows * 2 * l->v_cols * 2);
   return TB_OK;
 }
 
@@ -653,7 +678,7 @@ int lora_impl(const tb_lora_args& a, cudaStream_t stream) {
   p.ids = a.adapter_ids; p.is64 = a.ids_are_int64 != 0;
   p.scales = a.scales;
   p.tokens = a.m; p.k = a.k; p.rank = a.rank; p.num_adapters = a.num_adapters;
-  p.tile_rows = l.tile_rows; p.max_slots = l.max_slots; p.v_cols = l.v_cols;
+  p.tile_rows = l.tile_rows; p.max_slots = l.max_slots; p.v_cols = l.v_cols; p.v_width = l.v_width;
   p.v = ws + l.v_offset;
   p.list = reinterpret_cast<int*>(ws + l.list_offset);
   p.counters = reinterpret_cast<unsigned*>(ws + l.gemm_offset);
@@ -697,7 +722,7 @@ int lora_impl(const tb_lora_args& a, cudaStream_t stream) {
   lr.v = p.v;
   lr.v_rows = l.v_rows;
   lr.pack = l.pack;
-  lr.kblocks = l.pack > 1 ? 1 : l.v_cols / 64;
+  lr.kblocks = l.kblocks;
   lr.rank = a.rank;
   lr.tile_rows = l.tile_rows;
   lr.b = a.lora_b;

@@ -1,6 +1,6 @@
 // The shared projection of a decode batch (up to 64 rows) with its rows' low-rank updates: the second launch of lora.cu.
 //     out[t, n] = sum_k x[t, k] W[k, n] + bias[n] + sum over the listed adapters a of sum_r v_a[t, r] B_a[n, r]
-// v_a is what the first launch wrote: the rows' scaled rank-sized products, zero in rows of other adapters.
+// v_a is what the first launch wrote: the rows' scaled rank-sized products in two 16-bit halves, zero in rows of other adapters.
 //
 // Bound by reading W and the used B once. W's rows (output features) stand on the 128-row side of the tensor-core tile and the
 // tokens on its narrow side, a stage of the ring is 16 KB of weights and the tokens' share. Tiles that fill whole
@@ -227,7 +227,11 @@ lora_decode_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
     const int length = piece_length();
     return make_int2(min(u.piece * length, count), min((u.piece + 1) * length, count));
   };
-  const int part_w = kWeightBytes / p.pack, part_v = p.cols * kRowBytes / p.pack;  // bytes of one adapter's share of a stage
+  // An update's stage: the rows of B of `pack` adapters (`width` ranks of each) fill the weights' part, both halves of v for them the
+  // tokens' part, which has room for two columns' worth for that. (A stage of half as many ranks, within the room that the product
+  // itself needs, halves the bytes of B in flight, and with them the rate: 64 rows of 4096 x 8192, 64 adapters of rank 128: 152 us.)
+  const int width = kStageK / p.pack;
+  const int part_w = kWeightBytes / p.pack, part_v = 2 * p.cols * kRowBytes / p.pack;  // bytes of one adapter's share of a stage
 
   if (warp == kWarpWeights) {
     // -------------------------------------------------------------- weights and lora_b
@@ -319,7 +323,9 @@ lora_decode_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
             mbar_arrive_expect_tx(&full_bar[s], static_cast<uint32_t>(filled * part_v));
 #pragma unroll
             for (int j = 0; j < 4; ++j)
-              if (j < filled) tma_load_2d(dst + j * part_v, &tmap_v, &full_bar[s], kb * kStageK, (i + j) * p.cols);
+              if (j < filled) tma_load_2d(dst + j * part_v, &tmap_v, &full_bar[s], kb * 2 * width, (i + j) * p.cols);
+            // rows of 2 * width elements, or 128 bytes of them at a time
+            if (p.pack == 1) tma_load_2d(dst + part_v / 2, &tmap_v, &full_bar[s], (2 * kb + 1) * width, i * p.cols);
           }
           __syncwarp();
           if (++s == p.stages) {
@@ -340,9 +346,10 @@ lora_decode_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
     const uint64_t x0 = make_smem_desc(ring_addr + kWeightBytes, 16, 1024);
     const uint64_t w_step = p.w_mn ? 16 * kRowBytes >> 4 : 2;
     const uint32_t idesc = p.idesc | (p.w_mn ? 1u << 15 : 0u);
-    const uint32_t swizzle = p.pack == 1 ? 2u : (p.pack == 2 ? 4u : 6u), row_group = 1024u / p.pack;
-    const uint64_t xa0 = make_smem_desc(ring_addr, 16, row_group, swizzle);
-    const uint64_t xb0 = make_smem_desc(ring_addr + kWeightBytes, 16, row_group, swizzle);
+    // an update's operands: rows of 128, 64 or 32 bytes of B, twice that of v but no more than 128
+    const uint64_t xa0 = make_smem_desc(ring_addr, 16, 1024u / p.pack, p.pack == 1 ? 2u : (p.pack == 2 ? 4u : 6u));
+    const uint64_t xb0 = make_smem_desc(ring_addr + kWeightBytes, 16, p.pack == 4 ? 512u : 1024u, p.pack == 4 ? 4u : 2u);
+    const uint64_t v_low = static_cast<uint64_t>(p.pack == 1 ? part_v / 2 : width * 2) >> 4;
     for (Unit u = units.next(); u.kind != 0 && ok; u = units.next()) {
       if (PIECES && u.kind == 4) {
         if (count < 0) read_list();
@@ -383,8 +390,8 @@ lora_decode_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
             const int filled = min(p.pack, count - i);
             const int steps = min(4 / p.pack, (p.rank - kb * kStageK + 15) >> 4);  // columns behind the rank are zeros
             for (int j = 0; j < filled; ++j)
-              for (int k = 0; k < steps; ++k)
-                umma<0, 1>(d, xa0 + soff + ((j * part_w) >> 4) + 2 * k, xb0 + soff + ((j * part_v) >> 4) + 2 * k, p.idesc,
+              for (int k = 0; k < 2 * steps; ++k)  // high and low half in turn
+                umma<0, 1>(d, xa0 + soff + ((j * part_w) >> 4) + (k & ~1), xb0 + soff + ((j * part_v) >> 4) + (k & 1) * v_low + (k & ~1), p.idesc,
                            (PIECES && u.kind == 4 && i == range.x && kb == 0 && j == 0 && k == 0) ? 0u : 1u);
             umma_commit(&empty_bar[s]);
           }
@@ -611,7 +618,7 @@ int lora_decode(const tb_lora_args& a, const LoraDecodeShape& s, const LowRank& 
   p.tokens = a.m;
   p.n = a.n;
   p.cols = s.cols;
-  p.stage_bytes = static_cast<int>(kWeightBytes) + s.cols * kRowBytes;
+  p.stage_bytes = static_cast<int>(kWeightBytes) + 2 * s.cols * kRowBytes;  // twice the tokens' part: both halves of an update's v
   // beside the ring: the barriers, the ring's alignment, and a block of the first launch, which runs at the same time
   p.stages = (smem_optin - 28 * 1024) / p.stage_bytes;
   if (p.stages > kMaxStages) p.stages = kMaxStages;
@@ -649,9 +656,9 @@ int lora_decode(const tb_lora_args& a, const LoraDecodeShape& s, const LowRank& 
   rc = encode_2d(&tx, a.dtype, a.x, a.k, a.m, static_cast<uint64_t>(a.m > 1 ? a.x_row_stride : a.k) * 2, kStageK, a.m, 1);
   if (rc != TB_OK) return rc;
   const uint32_t inner = static_cast<uint32_t>(kStageK / lr.pack);
-  const uint64_t v_cols = static_cast<uint64_t>(lr.kblocks) * inner;
+  const uint64_t v_cols = 2ull * lr.kblocks * inner;  // both halves
   const uint64_t v_dims[2] = {v_cols, static_cast<uint64_t>(lr.v_rows)}, v_strides[1] = {v_cols * 2};
-  const uint32_t v_box[2] = {inner, static_cast<uint32_t>(s.cols)};
+  const uint32_t v_box[2] = {lr.pack == 1 ? inner : 2 * inner, static_cast<uint32_t>(s.cols)};
   if ((rc = encode_nd(&tv, a.dtype, lr.v, 2, v_dims, v_strides, v_box)) != TB_OK) return rc;
   const uint64_t dims[3] = {static_cast<uint64_t>(lr.rank), static_cast<uint64_t>(lr.n), static_cast<uint64_t>(lr.num_adapters)};
   const uint64_t row = static_cast<uint64_t>(lr.b_row_stride) * 2;

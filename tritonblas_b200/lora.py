@@ -22,9 +22,10 @@ def lora_matmul(x, w, lora_a, lora_b, adapter_ids, scales=None, bias=None, out: 
     x: (tokens, k); w: (k, n) in any of ``matmul``'s layouts (k contiguous, i.e. stored (n, k), is the fast one); lora_a:
     (adapters, rank, k); lora_b: (adapters, n, rank); all float16 or all bfloat16. adapter_ids: (tokens,) int32 or int64 on the
     GPU, in any order; an id outside [0, adapters), -1 for instance, leaves the row to the shared projection. scales: (adapters,)
-    or None for 1; bias: (n,). k and rank multiples of 8, rank up to 128. The sum is float32 and rounded once; the rank-sized
-    products ``scales[a] * x[t] @ lora_a[a].T`` are rounded to the operands' type on the way. ``out`` may be given: (tokens, n),
-    any strides, no overlap with the inputs. Inference only.
+    or None for 1; bias: (n,). k and rank multiples of 8, rank up to 128. The sum is float32 and rounded once. The rank-sized
+    products ``scales[a] * x[t] @ lora_a[a].T`` are operands of a tensor-core product and kept in two 16-bit halves: to 2^-16
+    relative in bfloat16; in float16 to 2^-22 relative or 2^-25 absolute, and infinite above 65504. ``out`` may be given:
+    (tokens, n), any strides, no overlap with the inputs. Inference only.
 
     Values in x, lora_a and scales stay with their rows. An infinity or NaN in ``lora_b[a]`` does not: it also makes NaN of the
     rows without that adapter that stand in the same tile (up to 256 neighbours) as a row with it, because the update is one
