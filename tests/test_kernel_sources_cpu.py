@@ -24,8 +24,14 @@ def test_cluster_barriers_are_reached_by_whole_warps():
     assert found >= 3
 
 
-def test_the_adapters_projection_takes_tensor_memory_between_wait_and_launch():
-    """A block that holds tensor memory while it waits for another kernel could keep a block of that kernel from getting its own."""
-    text = open(os.path.join(CSRC, "lora.cu")).read()
-    body = text[text.index("lora_project_tc_kernel("):]
-    assert body.index("griddep_wait()") < body.index("tmem_alloc<1>") < body.index("griddep_launch_dependents()")
+def test_the_next_kernel_starts_after_tensor_memory_is_taken():
+    """Kernels of this library take tensor memory while they wait for the kernel before them. One that let the next kernel start
+    ahead of its own request could find the columns it needs held by blocks that wait for it."""
+    found = 0
+    for path in sorted(glob.glob(os.path.join(CSRC, "*.cu")) + glob.glob(os.path.join(CSRC, "*.cuh"))):
+        text = re.sub(r"//[^\n]*", "", open(path).read())
+        for body in text.split("__global__")[1:]:
+            if "tmem_alloc<" in body and "griddep_launch_dependents()" in body:
+                found += 1
+                assert body.index("tmem_alloc<") < body.index("griddep_launch_dependents()"), os.path.basename(path)
+    assert found >= 4

@@ -676,7 +676,6 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ 
     // Everything above touched only shared memory. From here on global memory is read, which has to wait for the
     // previous kernel of the stream when this launch was allowed to start before that one finished; only an operand the
     // caller declared untouched by earlier work may be requested before that.
-    griddep_launch_dependents();
     if constexpr (CTAS == 1 && !GATHER && KIND != 3) {
       if (p.early_operand != 0 && p.group_offsets == nullptr && p.tile_counter == nullptr) {
         prefetch_tmap(p.early_operand == 1 ? &tmap_a : &tmap_b);
@@ -720,6 +719,9 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ 
   if (warp == 1) {
     tmem_alloc<CTAS>(tmem_ptr_slot, p.tmem_cols);
     tmem_relinquish<CTAS>();
+    // The next kernel may start once every block holds its tensor memory: blocks of that kernel take theirs while they wait for
+    // this one, and could keep a block of this one, on the same SM with its own request still open, from ever finishing.
+    griddep_launch_dependents();
   }
   tc_fence_before();
   __syncthreads();

@@ -369,18 +369,18 @@ lora_project_tc_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_
     prefetch_tmap(&tmap_x);
     prefetch_tmap(&tmap_a);
   }
-  griddep_wait();
-  // Tensor memory is taken after the wait for the kernel before and ahead of letting the next one start: a block that held some
-  // while it waits could keep a block it waits for, on the same SM and with its own request still open, from ever finishing.
   if (warp == 1) {
     tmem_alloc<1>(&tmem_slot, static_cast<uint32_t>(p.tmem_cols));
     tmem_relinquish<1>();
-    griddep_launch_dependents();
   }
   tc_fence_before();
-  const int2 found = find_adapters<kRows>(p, lists, row0, row0 == tile_row0 && blockIdx.y == 0 && cta == 0);  // ends with a barrier
+  __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = tmem_slot;
+  griddep_wait();
+  griddep_launch_dependents();
+
+  const int2 found = find_adapters<kRows>(p, lists, row0, row0 == tile_row0 && blockIdx.y == 0 && cta == 0);
   const int* run_ids = lists.ids + (row0 - tile_row0);
   const int v_row = 2 * p.v_cols, width = p.v_width;
   T* tile_blocks = static_cast<T*>(p.v) + static_cast<long long>(tile) * p.max_slots * p.tile_rows * v_row +
