@@ -299,8 +299,9 @@ int tb_moe_mlp(const tb_moe_mlp_args* args, void* stream);
  * (n) or NULL. k and rank multiples of 8, rank <= 128, k <= 2^28, m and n <= 2^30; rows (columns) of w must not overlap; x, w,
  * lora_a, lora_b with 16-byte aligned bases and pitches. One fp32 sum and one rounding; the rank-sized products are kept in two
  * 16-bit halves in between (they are a tensor-core operand; bf16: 2^-16 relative; f16: 2^-22 relative or 2^-25 absolute, whichever
- * is more, infinite above 65504). The workspace (tb_lora_workspace_bytes of the same arguments, 256-byte
- * aligned) needs no initialisation and must not be shared by calls that can overlap. */
+ * is more, infinite above 65504). Infinities and NaN in an adapter reach only the rows that use it. The workspace
+ * (tb_lora_workspace_bytes of the same arguments, 256-byte aligned) needs no initialisation and must not be shared by calls that
+ * can overlap. */
 typedef struct tb_lora_args {
   int32_t m, n, k, rank, num_adapters, dtype;
   const void* x; int64_t x_row_stride;

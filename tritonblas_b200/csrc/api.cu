@@ -572,6 +572,7 @@ static int gemm_impl(const tb_gemm_args& a_in, const tb_config* user_cfg, cudaSt
     p.lr_kblocks = lr->kblocks;
     p.lr_rank = lr->rank;
     p.lr_tile_rows = lr->tile_rows;
+    p.lr_rows = lr->rows;
     CUtensorMap tv, tlb;
     p.lr_pack = lr->pack;
     const uint32_t inner = 32u / lr->pack, v_inner = 2 * inner;  // of v both halves

@@ -29,6 +29,7 @@ int encode_nd(CUtensorMap* map, int dtype, const void* base, int rank, const uin
 // Low-rank update of a dense launch (see GemmParams::lr_list): the tokens' masked projections v, one block of tile_rows rows per
 // token tile and listed adapter, and lora_b (num_adapters, n, rank). A row is `kblocks` times as many high 16-bit halves as a stage
 // has ranks of one adapter (32 / pack, in the decode form 64 / pack) and as many low ones.
+struct LowRankRows;  // low_rank.cuh
 struct LowRank {
   const void* v;
   int64_t v_rows;
@@ -38,6 +39,7 @@ struct LowRank {
   int num_adapters, n;
   const int* list;
   int list_stride;
+  const LowRankRows* rows;
 };
 // Configuration the library would pick for `a` (more than 64 rows): data-parallel, narrow tiles; and the launch of `a` with that
 // configuration and the update.

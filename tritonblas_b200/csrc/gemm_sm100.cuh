@@ -22,6 +22,7 @@
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
 
+#include "low_rank.cuh"
 #include "ptx.cuh"
 
 namespace tb {
@@ -114,6 +115,7 @@ struct GemmParams {
   int lr_pack;          // adapters per stage: 1 or 2
   int lr_rank;
   int lr_tile_rows;     // rows of a tile of this launch
+  const LowRankRows* lr_rows;  // for elements that another row's adapter made non-finite
   // failure reporting
   int* status;
   unsigned long long timeout_ns;
@@ -1261,6 +1263,18 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ 
       // staged stores need whole 32-column chunks inside N and 16-byte aligned rows in every destination (host-checked)
       const bool staged = owner && p.staged_store && (n0 + p.block_n <= p.N);
       const uint32_t t_row = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + static_cast<uint32_t>(acc_i * acc_stride);
+      bool odd_sums = false;  // LOWRANK: a sum that is not finite, see low_rank.cuh
+      if constexpr (LOWRANK) {
+        float zero = 0.0f;
+        for (int c = 0; c < nchunks; ++c) {
+          uint32_t r[32];
+          tmem_ld_32x32(t_row + c * 32, r);
+          tmem_ld_wait(r);
+#pragma unroll
+          for (int j = 0; j < 32; ++j) zero = fmaf(__uint_as_float(r[j]), 0.0f, zero);
+        }
+        odd_sums = __any_sync(0xffffffffu, !(zero == 0.0f));
+      }
       // Hand the accumulator back to the MMA issuer: called once the last chunk sits in registers, before it is stored.
       auto release_accumulator = [&]() {
         tc_fence_before();
@@ -1447,6 +1461,9 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ 
           // debug bit 2 (value 4) withholds the flag: the failure-path test uses it to make the owner's bounded wait run out
           if (mbar_wait(publish_bar, 0, wctx, TB_DEV_TIMEOUT_STORE) && !(p.debug_flags & 4)) flag_release(&p.flags[slot], p.epoch);
         }
+      }
+      if constexpr (LOWRANK) {
+        if (odd_sums) low_rank::redo(p.lr_rows, m0 + q * 32, min(m0 + q * 32 + 32, row_end), n0, min(n0 + p.block_n, p.N));
       }
       epi_parity ^= 1u << acc_i;
       }  // halves

@@ -15,6 +15,7 @@
 // lo = round(v - hi), which stand side by side in a row of its block, 16 to 64 ranks at a time, and are both multiplied by the same rows of B: 2^-16 of v
 // (bf16), or 2^-22 or 2^-25 absolute, whichever is more (fp16, whose v is infinite above 65504: the update adds up in the
 // product's own accumulator, so it can have no unit of its own).
+// An infinity or NaN in one adapter's B would reach the tile's other rows, whose blocks hold zeros: see low_rank.cuh.
 // No reference counterpart (the reference has no adapters).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -22,6 +23,7 @@
 #include <mutex>
 
 #include "common_host.h"
+#include "low_rank.cuh"
 #include "selector.h"  // the SM count when there is no device
 #include "ptx.cuh"
 
@@ -56,6 +58,8 @@ struct ProjectParams {
   int k_chunk;          // K per CTA, a multiple of 32
   void* v;
   int* list;            // [tiles][1 + max_slots]
+  LowRankRows rows;     // left in the workspace for the second launch
+  LowRankRows* rows_out;
   unsigned* counters;   // of the decode kernel, to clear
   int counter_words;
   // tensor-core form
@@ -251,8 +255,10 @@ __global__ void __maxnreg__(120) lora_project_kernel(const ProjectParams p) {
   griddep_wait();
   griddep_launch_dependents();
 
-  if (blockIdx.x == 0 && blockIdx.y == 0)
+  if (blockIdx.x == 0 && blockIdx.y == 0) {
     for (int i = tid; i < p.counter_words; i += kThreads) p.counters[i] = 0u;
+    if (tid == 0) *p.rows_out = p.rows;
+  }
   const int2 found = find_adapters<kRows>(p, lists, row0, row0 == tile_row0 && blockIdx.y == 0 && rank == 0);
   const int* run_ids = lists.ids + (row0 - tile_row0);
   const int v_row = 2 * p.v_cols;
@@ -380,6 +386,7 @@ lora_project_tc_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_
   griddep_wait();
   griddep_launch_dependents();
 
+  if (blockIdx.x == 0 && blockIdx.y == 0 && tid == 0) *p.rows_out = p.rows;
   const int2 found = find_adapters<kRows>(p, lists, row0, row0 == tile_row0 && blockIdx.y == 0 && cta == 0);
   const int* run_ids = lists.ids + (row0 - tile_row0);
   const int v_row = 2 * p.v_cols, width = p.v_width;
@@ -589,7 +596,7 @@ struct LoraPlan {
   LoraDecodeShape shape;  // decode
   tb_config cfg;          // otherwise
   int tile_rows, tiles, max_slots, v_cols, v_width, pack, kblocks;
-  long long v_offset, v_rows, list_offset, gemm_offset, gemm_bytes, bytes;
+  long long v_offset, v_rows, list_offset, rows_offset, gemm_offset, gemm_bytes, bytes;
 };
 
 int lora_plan(const tb_lora_args& a, int num_sms, tb_gemm_args* g, LoraPlan* l) {
@@ -627,7 +634,8 @@ int lora_plan(const tb_lora_args& a, int num_sms, tb_gemm_args* g, LoraPlan* l) 
   l->gemm_offset = 0;
   // decode: counters (cleared by the projection) at the front, then partial tiles
   l->gemm_bytes = l->decode ? kCounterBytes + up(l->shape.part_bytes) : 0;
-  l->list_offset = l->gemm_bytes;
+  l->rows_offset = l->gemm_bytes;
+  l->list_offset = l->rows_offset + up(sizeof(LowRankRows));
   l->v_offset = l->list_offset + up(4ll * l->tiles * (1 + l->max_slots));
   l->bytes = l->v_offset + up(l->v_rows * 2 * l->v_cols * 2);
   return TB_OK;
@@ -681,6 +689,10 @@ int lora_impl(const tb_lora_args& a, cudaStream_t stream) {
   p.tile_rows = l.tile_rows; p.max_slots = l.max_slots; p.v_cols = l.v_cols; p.v_width = l.v_width;
   p.v = ws + l.v_offset;
   p.list = reinterpret_cast<int*>(ws + l.list_offset);
+  p.rows = {a.x, g.a_stride_m, a.w, a.w_stride_k, a.w_stride_n, a.lora_b, a.lora_b_adapter_stride, a.lora_b_row_stride, a.adapter_ids,
+            p.list, p.v, a.bias, a.bias_stride, a.out, a.out_stride_m, a.out_stride_n, p.is64, a.num_adapters, 1 + l.max_slots,
+            2 * l.v_cols, l.v_width, l.tile_rows, a.k, a.rank, a.bias_dtype, a.dtype == TB_DTYPE_BF16 ? 1 : 0};
+  p.rows_out = reinterpret_cast<LowRankRows*>(ws + l.rows_offset);
   p.counters = reinterpret_cast<unsigned*>(ws + l.gemm_offset);
   p.counter_words = l.decode ? 4 * l.shape.dealt_tiles : 0;
   p.status = status;
@@ -730,6 +742,7 @@ int lora_impl(const tb_lora_args& a, cudaStream_t stream) {
   lr.b_row_stride = a.lora_b_row_stride;
   lr.num_adapters = a.num_adapters;
   lr.n = a.n;
+  lr.rows = p.rows_out;
   lr.list = p.list;
   lr.list_stride = 1 + l.max_slots;
   if (l.decode)

@@ -21,6 +21,7 @@
 #include <type_traits>
 
 #include "common_host.h"
+#include "low_rank.cuh"
 #include "ptx.cuh"
 
 namespace tb {
@@ -50,6 +51,7 @@ struct DecodeParams {
   // low-rank update
   const int* list;      // number of adapters, then their indices
   int max_slots, pack, kblocks, rank;
+  const LowRankRows* rows;
   int pieces;           // a dealt tile's update is cut into at most this many
   float* parts;         // [2 * grid][tokens][kTile], and [grid] more when there are pieces
   unsigned* arrived;    // [dealt_tiles][4], cleared by the first launch
@@ -432,6 +434,7 @@ lora_decode_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
       if (!ok) break;
       tc_fence_after();
       const uint32_t t_row = tmem_base + (static_cast<uint32_t>(warp * 32) << 16) + static_cast<uint32_t>(acc * p.acc_stride);
+      float zero = 0.0f;  // stays so as long as every sum is finite
       for (int c0 = 0; c0 < p.tokens; c0 += 32) {
         uint32_t r[32];
         tmem_ld_32x32(t_row + c0, r);
@@ -448,12 +451,17 @@ lora_decode_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
             const float v = __uint_as_float(r[j]);
             if (u.kind != 2) __stcg(part + static_cast<size_t>(t) * kTile, v);
             else if (mine) out[t * p.out_m + n * p.out_n] = cast16<T>(v + bias);
+            zero = fmaf(v, 0.0f, zero);
           }
         }
       }
       parity ^= 1u << acc;
       acc ^= 1;
-      if (u.kind == 2) continue;
+      const int n_first = u.tile * kTile + warp * 32, n_last = min(n_first + 32, p.n);
+      if (u.kind == 2) {
+        if (__any_sync(0xffffffffu, !(zero == 0.0f))) low_rank::redo(p.rows, 0, p.tokens, n_first, n_last);
+        continue;
+      }
       // count this warp's quarter in; the last of its tile's parts adds them up
       const int dealt = u.tile - p.full_tiles;
       const int c_first = deal.cta_of(dealt * p.nkb), c_last = deal.cta_of((dealt + 1) * p.nkb - 1);
@@ -481,6 +489,7 @@ lora_decode_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
 #pragma unroll
       for (int i = 0; i < 4; ++i)
         if (p.bias != nullptr && n4 + i < p.n) b[i] = bias_at(p.bias, (n4 + i) * p.bias_stride, p.bias_dtype);
+      zero = 0.0f;
       auto add_up = [&](auto parts_at_once, auto tokens_at_once) {
         constexpr int kQ = decltype(parts_at_once)::value, kT = decltype(tokens_at_once)::value;
         for (int t0 = lane >> 3; t0 < p.tokens; t0 += 4 * kT) {
@@ -516,6 +525,7 @@ lora_decode_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
           for (int j = 0; j < kT; ++j) {
             const int t = t0 + 4 * j;
             if (t >= p.tokens) break;
+            zero = fmaf(sum[j].x, 0.0f, fmaf(sum[j].y, 0.0f, fmaf(sum[j].z, 0.0f, fmaf(sum[j].w, 0.0f, zero))));
             T* o = out + t * p.out_m + n4 * p.out_n;
             if (p.out_vec && n4 + 3 < p.n) {
               alignas(8) const T quad[4] = {cast16<T>(sum[j].x), cast16<T>(sum[j].y), cast16<T>(sum[j].z), cast16<T>(sum[j].w)};
@@ -532,6 +542,7 @@ lora_decode_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
       if (p.tokens <= 8) add_up(std::integral_constant<int, 8>{}, std::integral_constant<int, 2>{});
       else add_up(std::integral_constant<int, 4>{}, std::integral_constant<int, 4>{});
       __syncwarp();
+      if (__any_sync(0xffffffffu, !(zero == 0.0f))) low_rank::redo(p.rows, 0, p.tokens, n_first, n_last);
     }
   }
 
@@ -634,6 +645,7 @@ int lora_decode(const tb_lora_args& a, const LoraDecodeShape& s, const LowRank& 
   p.pack = lr.pack;
   p.kblocks = lr.kblocks;
   p.rank = a.rank;
+  p.rows = lr.rows;
   p.parts = static_cast<float*>(parts);
   p.arrived = static_cast<unsigned*>(arrived);
   p.bias = a.bias;

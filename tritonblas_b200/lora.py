@@ -27,9 +27,7 @@ def lora_matmul(x, w, lora_a, lora_b, adapter_ids, scales=None, bias=None, out: 
     relative in bfloat16; in float16 to 2^-22 relative or 2^-25 absolute, and infinite above 65504. ``out`` may be given:
     (tokens, n), any strides, no overlap with the inputs. Inference only.
 
-    Values in x, lora_a and scales stay with their rows. An infinity or NaN in ``lora_b[a]`` does not: it also makes NaN of the
-    rows without that adapter that stand in the same tile (up to 256 neighbours) as a row with it, because the update is one
-    matrix product per tile in which those rows hold zeros.
+    Infinities and NaN in x, lora_a, lora_b and scales stay with the rows that use them; calls that meet some are slower.
     """
     if x.ndim != 2 or w.ndim != 2 or lora_a.ndim != 3 or lora_b.ndim != 3:
         refuse("x and w must be 2-D, lora_a and lora_b 3-D")
