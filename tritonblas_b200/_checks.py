@@ -7,6 +7,7 @@ import contextlib
 import torch
 
 _nullcontext = contextlib.nullcontext()
+_PLAIN = (torch.Tensor, torch.nn.Parameter)
 
 
 def refuse(message):
@@ -40,3 +41,11 @@ def rows16(t):
         if n != 1 and (s < row or s % per16):
             return False
     return True
+
+
+def traced(t):
+    """True where a call has to go through its registered operator because something looks at it or rewrites it: torch.compile, fake
+    tensors and other subclasses, a dispatch mode (torch.export, make_fx, ...), a torch.func transform. Plain eager calls skip the
+    dispatcher, which costs more than the operators run."""
+    return (torch.compiler.is_compiling() or type(t) not in _PLAIN or torch._C._len_torch_dispatch_stack() > 0
+            or torch._C._functorch.peek_interpreter_stack() is not None)

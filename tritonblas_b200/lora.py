@@ -8,7 +8,7 @@ from typing import Optional
 import torch
 
 from . import _lib
-from ._checks import on_device, refuse, refuse_devices, rows16
+from ._checks import on_device, refuse, refuse_devices, rows16, traced
 from .matmul import _repitch, _strides, _tma_loadable, _unit_stride_2d
 
 _MAX_RANK = 128
@@ -16,19 +16,7 @@ _MAX_RANK = 128
 _MAX_WORKSPACE = 256 << 20
 
 
-def lora_matmul(x, w, lora_a, lora_b, adapter_ids, scales=None, bias=None, out: Optional[torch.Tensor] = None):
-    """``out[t] = x[t] @ w + scales[a] * (x[t] @ lora_a[a].T) @ lora_b[a].T (+ bias)`` with ``a = adapter_ids[t]``.
-
-    x: (tokens, k); w: (k, n) in any of ``matmul``'s layouts (k contiguous, i.e. stored (n, k), is the fast one); lora_a:
-    (adapters, rank, k); lora_b: (adapters, n, rank); all float16 or all bfloat16. adapter_ids: (tokens,) int32 or int64 on the
-    GPU, in any order; an id outside [0, adapters), -1 for instance, leaves the row to the shared projection. scales: (adapters,)
-    or None for 1; bias: (n,). k and rank multiples of 8, rank up to 128. The sum is float32 and rounded once. The rank-sized
-    products ``scales[a] * x[t] @ lora_a[a].T`` are operands of a tensor-core product and kept in two 16-bit halves: to 2^-16
-    relative in bfloat16; in float16 to 2^-22 relative or 2^-25 absolute, and infinite above 65504. ``out`` may be given:
-    (tokens, n), any strides, no overlap with the inputs. Inference only.
-
-    Infinities and NaN in x, lora_a, lora_b and scales stay with the rows that use them; calls that meet some are slower.
-    """
+def _check(x, w, lora_a, lora_b, adapter_ids, scales, bias, out):
     if x.ndim != 2 or w.ndim != 2 or lora_a.ndim != 3 or lora_b.ndim != 3:
         refuse("x and w must be 2-D, lora_a and lora_b 3-D")
     tokens, k = x.shape
@@ -54,17 +42,24 @@ def lora_matmul(x, w, lora_a, lora_b, adapter_ids, scales=None, bias=None, out: 
         refuse("bias must be (n,) in float16, bfloat16 or float32")
     if out is not None and (out.shape != (tokens, n) or out.dtype is not dtype):
         refuse(f"out must be {(tokens, n)} of {dtype}")
-    if out is not None and tokens and n and out.data_ptr() == x.data_ptr():
-        refuse("out must not be x: other columns of its rows are still read while the first ones are written")
     if not x.is_cuda or not device == w.device == lora_a.device == lora_b.device == adapter_ids.device \
             or any(t is not None and t.device != device for t in (scales, bias, out)):
         refuse_devices(x, w, lora_a, lora_b, adapter_ids, scales, bias, out)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, w, lora_a, lora_b, scales, bias, out)):
         raise RuntimeError("tritonblas.lora_matmul(): inference only, but one of the arguments requires grad.")
+
+
+def _run(x, w, lora_a, lora_b, adapter_ids, scales, bias, out):
+    tokens, k = x.shape
+    n = w.shape[1]
+    adapters, rank, _ = lora_a.shape
+    dtype, device = x.dtype, x.device
     if out is None:
         out = torch.empty(tokens, n, dtype=x.dtype, device=x.device)
     if tokens == 0 or n == 0:
         return out
+    if out.data_ptr() == x.data_ptr():
+        refuse("out must not be x: other columns of its rows are still read while the first ones are written")
     if not rows16(x):
         x = x.clone(memory_format=torch.contiguous_format)
     if not rows16(lora_a):
@@ -115,3 +110,44 @@ def lora_matmul(x, w, lora_a, lora_b, adapter_ids, scales=None, bias=None, out: 
             if need > ws.numel():       # the shorter last piece may be cut differently
                 ws = torch.empty(need, dtype=torch.uint8, device=device)
                 args.workspace, args.workspace_bytes = ws.data_ptr(), need
+
+
+@torch.library.custom_op("tritonblas::_lora_matmul", mutates_args=())
+def _lora_matmul(x: torch.Tensor, w: torch.Tensor, lora_a: torch.Tensor, lora_b: torch.Tensor, adapter_ids: torch.Tensor,
+                 scales: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None) -> torch.Tensor:
+    _check(x, w, lora_a, lora_b, adapter_ids, scales, bias, None)
+    return _run(x, w, lora_a, lora_b, adapter_ids, scales, bias, None)
+
+
+@_lora_matmul.register_fake
+def _(x, w, lora_a, lora_b, adapter_ids, scales=None, bias=None):
+    return x.new_empty(x.shape[0], w.shape[1])
+
+
+@torch.library.custom_op("tritonblas::_lora_matmul_out", mutates_args={"out"})
+def _lora_matmul_out(x: torch.Tensor, w: torch.Tensor, lora_a: torch.Tensor, lora_b: torch.Tensor, adapter_ids: torch.Tensor,
+                     out: torch.Tensor, scales: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None) -> None:
+    _check(x, w, lora_a, lora_b, adapter_ids, scales, bias, out)
+    _run(x, w, lora_a, lora_b, adapter_ids, scales, bias, out)
+
+
+def lora_matmul(x, w, lora_a, lora_b, adapter_ids, scales=None, bias=None, out: Optional[torch.Tensor] = None):
+    """``out[t] = x[t] @ w + scales[a] * (x[t] @ lora_a[a].T) @ lora_b[a].T (+ bias)`` with ``a = adapter_ids[t]``.
+
+    x: (tokens, k); w: (k, n) in any of ``matmul``'s layouts (k contiguous, i.e. stored (n, k), is the fast one); lora_a:
+    (adapters, rank, k); lora_b: (adapters, n, rank); all float16 or all bfloat16. adapter_ids: (tokens,) int32 or int64 on the
+    GPU, in any order; an id outside [0, adapters), -1 for instance, leaves the row to the shared projection. scales: (adapters,)
+    or None for 1; bias: (n,). k and rank multiples of 8, rank up to 128. The sum is float32 and rounded once. The rank-sized
+    products ``scales[a] * x[t] @ lora_a[a].T`` are operands of a tensor-core product and kept in two 16-bit halves: to 2^-16
+    relative in bfloat16; in float16 to 2^-22 relative or 2^-25 absolute, and infinite above 65504. ``out`` may be given:
+    (tokens, n), any strides, no overlap with the inputs. Inference only.
+
+    Infinities and NaN in x, lora_a, lora_b and scales stay with the rows that use them; calls that meet some are slower.
+    """
+    _check(x, w, lora_a, lora_b, adapter_ids, scales, bias, out)
+    if traced(x):
+        if out is None:
+            return _lora_matmul(x, w, lora_a, lora_b, adapter_ids, scales, bias)
+        _lora_matmul_out(x, w, lora_a, lora_b, adapter_ids, out, scales, bias)
+        return out
+    return _run(x, w, lora_a, lora_b, adapter_ids, scales, bias, out)

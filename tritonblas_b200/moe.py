@@ -10,7 +10,7 @@ from typing import Optional, Tuple
 import torch
 
 from . import _lib
-from ._checks import on_device, refuse, refuse_devices, rows16
+from ._checks import on_device, refuse, refuse_devices, rows16, traced
 
 MOE_MLP_MAX_TOKENS = 128
 _MAX_EXPERTS, _MAX_TOPK = 1024, 32
@@ -136,7 +136,7 @@ def moe_route(logits, topk, scoring="softmax", renormalize=True):
     if not 1 <= topk <= min(_MAX_TOPK, experts):
         refuse(f"topk must be between 1 and min({_MAX_TOPK}, experts), got {topk}")
     sigmoid, renormalize = _SCORING[scoring], 1 if renormalize else 0
-    if torch.compiler.is_compiling():
+    if traced(logits):
         return _moe_route(logits, topk, bool(sigmoid), bool(renormalize))
     if logits.requires_grad and torch.is_grad_enabled():
         return _Route.apply(logits, topk, sigmoid, renormalize)
@@ -144,19 +144,7 @@ def moe_route(logits, topk, scoring="softmax", renormalize=True):
 
 
 # -------------------------------------------------------------------------------------------------------- expert layer
-def moe_mlp(x, w1, w2, topk_ids, topk_weights, out: Optional[torch.Tensor] = None):
-    """Expert feed-forward of up to 128 tokens in two launches:
-    ``out[t] = sum_j topk_weights[t, j] * (silu(x[t] @ gate.T) * (x[t] @ up.T)) @ w2[e].T`` with ``e = topk_ids[t, j]`` and
-    ``w1[e] = [gate; up]``.
-
-    x: (tokens, hidden); w1: (experts, 2*ffn, hidden) and w2: (experts, hidden, ffn), the layout ``PeerMemoryMoE`` takes; all
-    float16 or all bfloat16, hidden and ffn multiples of 8. topk_ids: (tokens, topk) int32 or int64, topk_weights: (tokens, topk),
-    as ``moe_route`` returns them. An id outside [0, experts) adds nothing; the same id twice counts twice. Sums, activation and
-    weighting are float32 with one cast at the end. silu(gate) * up is an operand of a tensor-core product and kept in two 16-bit
-    halves: to 2^-16 relative in bfloat16; in float16 to 2^-22 relative or 2^-28 absolute, and infinite above 65504 * 256.
-    ``out`` may be given: (tokens, hidden), contiguous rows, no overlap with the weights. Inference only. More tokens:
-    ``distributed.PeerMemoryMoE``.
-    """
+def _check_mlp(x, w1, w2, topk_ids, topk_weights, out):
     if x.ndim != 2 or w1.ndim != 3 or w2.ndim != 3 or topk_ids.ndim != 2:
         refuse("x must be (tokens, hidden), w1 and w2 3-D, topk_ids 2-D")
     tokens, hidden = x.shape
@@ -186,15 +174,21 @@ def moe_mlp(x, w1, w2, topk_ids, topk_weights, out: Optional[torch.Tensor] = Non
     if torch.is_grad_enabled() and (x.requires_grad or w1.requires_grad or w2.requires_grad or topk_weights.requires_grad
                                     or (out is not None and out.requires_grad)):
         raise RuntimeError("tritonblas.moe_mlp(): inference only, but one of the arguments requires grad.")
-    if out is None:
-        out = torch.empty(tokens, hidden, dtype=dtype, device=device)
-    else:
+    if out is not None:
         if out.shape != (tokens, hidden) or out.dtype is not dtype:
             refuse(f"out must be {(tokens, hidden)} of {dtype}")
         if out.device != device:
             refuse_devices(x, out)
         if out.stride(1) != 1 or (tokens > 1 and out.stride(0) < hidden):
             refuse("out must have contiguous, non-overlapping rows")
+
+
+def _run_mlp(x, w1, w2, topk_ids, topk_weights, out):
+    tokens, hidden = x.shape
+    experts, _, ffn = w2.shape
+    topk, dtype, device = topk_ids.shape[1], x.dtype, x.device
+    if out is None:
+        out = torch.empty(tokens, hidden, dtype=dtype, device=device)
     if tokens == 0:
         return out
     if not rows16(x):
@@ -216,3 +210,43 @@ def moe_mlp(x, w1, w2, topk_ids, topk_weights, out: Optional[torch.Tensor] = Non
         rc = _lib.lib.tb_moe_mlp(ctypes.byref(args), _lib.current_stream_ptr(device))
     _lib.check(rc, "tb_moe_mlp")
     return out
+
+
+@torch.library.custom_op("tritonblas::_moe_mlp", mutates_args=())
+def _moe_mlp(x: torch.Tensor, w1: torch.Tensor, w2: torch.Tensor, topk_ids: torch.Tensor, topk_weights: torch.Tensor) -> torch.Tensor:
+    _check_mlp(x, w1, w2, topk_ids, topk_weights, None)
+    return _run_mlp(x, w1, w2, topk_ids, topk_weights, None)
+
+
+@_moe_mlp.register_fake
+def _(x, w1, w2, topk_ids, topk_weights):
+    return x.new_empty(x.shape)
+
+
+@torch.library.custom_op("tritonblas::_moe_mlp_out", mutates_args={"out"})
+def _moe_mlp_out(x: torch.Tensor, w1: torch.Tensor, w2: torch.Tensor, topk_ids: torch.Tensor, topk_weights: torch.Tensor,
+                 out: torch.Tensor) -> None:
+    _check_mlp(x, w1, w2, topk_ids, topk_weights, out)
+    _run_mlp(x, w1, w2, topk_ids, topk_weights, out)
+
+
+def moe_mlp(x, w1, w2, topk_ids, topk_weights, out: Optional[torch.Tensor] = None):
+    """Expert feed-forward of up to 128 tokens in two launches:
+    ``out[t] = sum_j topk_weights[t, j] * (silu(x[t] @ gate.T) * (x[t] @ up.T)) @ w2[e].T`` with ``e = topk_ids[t, j]`` and
+    ``w1[e] = [gate; up]``.
+
+    x: (tokens, hidden); w1: (experts, 2*ffn, hidden) and w2: (experts, hidden, ffn), the layout ``PeerMemoryMoE`` takes; all
+    float16 or all bfloat16, hidden and ffn multiples of 8. topk_ids: (tokens, topk) int32 or int64, topk_weights: (tokens, topk),
+    as ``moe_route`` returns them. An id outside [0, experts) adds nothing; the same id twice counts twice. Sums, activation and
+    weighting are float32 with one cast at the end. silu(gate) * up is an operand of a tensor-core product and kept in two 16-bit
+    halves: to 2^-16 relative in bfloat16; in float16 to 2^-22 relative or 2^-28 absolute, and infinite above 65504 * 256.
+    ``out`` may be given: (tokens, hidden), contiguous rows, no overlap with the weights. Inference only. More tokens:
+    ``distributed.PeerMemoryMoE``.
+    """
+    _check_mlp(x, w1, w2, topk_ids, topk_weights, out)
+    if traced(x):
+        if out is None:
+            return _moe_mlp(x, w1, w2, topk_ids, topk_weights)
+        _moe_mlp_out(x, w1, w2, topk_ids, topk_weights, out)
+        return out
+    return _run_mlp(x, w1, w2, topk_ids, topk_weights, out)
