@@ -80,6 +80,20 @@ def test_a_traced_decode_step_holds_the_operators():
                                                                   "tritonblas._moe_mlp.default"]
 
 
+def test_tangents_are_refused():
+    """Forward-mode differentiation: none of the operators has a rule, and a result without its tangent would be a wrong one. The
+    refusal comes before any call into the library, so fake device checks suffice."""
+    from torch.autograd import forward_ad
+    from tritonblas_b200._checks import refuse_tangents
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(torch.zeros(3), torch.ones(3))
+        refuse_tangents("f", torch.zeros(3), None, torch.zeros(2, dtype=torch.int32))
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            refuse_tangents("f", None, dual)
+    with pytest.raises(RuntimeError, match="forward-mode"):
+        torch.func.jvp(lambda t: refuse_tangents("f", t) or t, (torch.zeros(3),), (torch.ones(3),))
+
+
 def test_operators_check_what_the_functions_check():
     """Called by name, with host tensors."""
     z = torch.zeros

@@ -1,7 +1,8 @@
-"""The per-token operators through torch.compile, torch.export and torch.func on the GPU."""
+"""The per-token operators through torch.compile, torch.export, torch.func and forward-mode differentiation on the GPU."""
 import pytest
 import torch
 from torch._subclasses.fake_tensor import FakeTensorMode
+from torch.autograd import forward_ad
 
 import tritonblas_b200 as tb
 from tests.test_lora_gpu import make as make_lora
@@ -67,7 +68,7 @@ def test_registrations():
     check(torch.ops.tritonblas._moe_route.default, (torch.randn(6, 16, device="cuda", requires_grad=True), 4, False, True))
 
 
-def test_transforms():
+def test_transforms_and_tangents():
     l = torch.randn(6, 16, device="cuda")
     with FakeTensorMode() as mode:
         fake = mode.from_tensor(l).requires_grad_(True)
@@ -75,3 +76,13 @@ def test_transforms():
         assert d.shape == l.shape
     with pytest.raises(RuntimeError):           # registered operators have no torch.func rule (matmul's neither): said, not dropped
         torch.func.grad(lambda t: tb.moe_route(t, 4)[0][:, 0].sum())(l)
+    case, experts = make_lora(6, 64, 40, 8, 3, torch.bfloat16), make_experts(6, 8, 2, 64, 64, torch.bfloat16)
+    calls = (lambda t: tb.moe_route(t.float(), 4)[0], lambda t: tb.lora_matmul(t, *case[1:]), lambda t: tb.moe_mlp(t, *experts[1:]))
+    for f in calls:
+        t = torch.randn(6, 64, device="cuda").bfloat16()
+        with forward_ad.dual_level():
+            with pytest.raises((RuntimeError, NotImplementedError)):
+                f(forward_ad.make_dual(t, torch.ones_like(t)))
+        with pytest.raises((RuntimeError, NotImplementedError)):
+            torch.func.jvp(f, (t,), (torch.ones_like(t),))
+        f(t)

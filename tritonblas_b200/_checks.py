@@ -5,6 +5,7 @@ formatted unless a call is refused."""
 import contextlib
 
 import torch
+from torch.autograd import forward_ad
 
 _nullcontext = contextlib.nullcontext()
 _PLAIN = (torch.Tensor, torch.nn.Parameter)
@@ -49,3 +50,10 @@ def traced(t):
     dispatcher, which costs more than the operators run."""
     return (torch.compiler.is_compiling() or type(t) not in _PLAIN or torch._C._len_torch_dispatch_stack() > 0
             or torch._C._functorch.peek_interpreter_stack() is not None)
+
+
+def refuse_tangents(name, *tensors):
+    """Error for dual tensors of forward-mode differentiation: their tangents would be lost."""
+    if forward_ad._current_level >= 0 and any(t is not None and t.is_floating_point() and forward_ad.unpack_dual(t).tangent is not None
+                                              for t in tensors):
+        raise RuntimeError(f"tritonblas.{name}(): no forward-mode derivative.")

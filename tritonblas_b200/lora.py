@@ -8,7 +8,7 @@ from typing import Optional
 import torch
 
 from . import _lib
-from ._checks import on_device, refuse, refuse_devices, rows16, traced
+from ._checks import on_device, refuse, refuse_devices, refuse_tangents, rows16, traced
 from .matmul import _repitch, _strides, _tma_loadable, _unit_stride_2d
 
 _MAX_RANK = 128
@@ -145,6 +145,7 @@ def lora_matmul(x, w, lora_a, lora_b, adapter_ids, scales=None, bias=None, out: 
     Infinities and NaN in x, lora_a, lora_b and scales stay with the rows that use them; calls that meet some are slower.
     """
     _check(x, w, lora_a, lora_b, adapter_ids, scales, bias, out)
+    refuse_tangents("lora_matmul", x, w, lora_a, lora_b, scales, bias)
     if traced(x):
         if out is None:
             return _lora_matmul(x, w, lora_a, lora_b, adapter_ids, scales, bias)

@@ -10,7 +10,7 @@ from typing import Optional, Tuple
 import torch
 
 from . import _lib
-from ._checks import on_device, refuse, refuse_devices, rows16, traced
+from ._checks import on_device, refuse, refuse_devices, refuse_tangents, rows16, traced
 
 MOE_MLP_MAX_TOKENS = 128
 _MAX_EXPERTS, _MAX_TOPK = 1024, 32
@@ -136,6 +136,7 @@ def moe_route(logits, topk, scoring="softmax", renormalize=True):
     if not 1 <= topk <= min(_MAX_TOPK, experts):
         refuse(f"topk must be between 1 and min({_MAX_TOPK}, experts), got {topk}")
     sigmoid, renormalize = _SCORING[scoring], 1 if renormalize else 0
+    refuse_tangents("moe_route", logits)
     if traced(logits):
         return _moe_route(logits, topk, bool(sigmoid), bool(renormalize))
     if logits.requires_grad and torch.is_grad_enabled():
@@ -244,6 +245,7 @@ def moe_mlp(x, w1, w2, topk_ids, topk_weights, out: Optional[torch.Tensor] = Non
     ``distributed.PeerMemoryMoE``.
     """
     _check_mlp(x, w1, w2, topk_ids, topk_weights, out)
+    refuse_tangents("moe_mlp", x, w1, w2, topk_weights)
     if traced(x):
         if out is None:
             return _moe_mlp(x, w1, w2, topk_ids, topk_weights)
