@@ -5,6 +5,7 @@ expert layer of a decode batch in two launches. Batches of more than 128 tokens 
 ``distributed.ExpertParallelMoE``, whose grouped GEMMs work on 128-row tiles. The reference has no MoE path.
 """
 import ctypes
+import operator
 from typing import Optional, Tuple
 
 import torch
@@ -132,7 +133,7 @@ def moe_route(logits, topk, scoring="softmax", renormalize=True):
     experts = logits.shape[1]
     if not 1 <= experts <= _MAX_EXPERTS:
         refuse(f"between 1 and {_MAX_EXPERTS} experts, got {experts}")
-    topk = int(topk)
+    topk = operator.index(topk)     # a whole number: 2.5 is not 2
     if not 1 <= topk <= min(_MAX_TOPK, experts):
         refuse(f"topk must be between 1 and min({_MAX_TOPK}, experts), got {topk}")
     sigmoid, renormalize = _SCORING[scoring], 1 if renormalize else 0
