@@ -3,6 +3,7 @@
 These operators run in microseconds, so their argument checks are plain ``if not ...: refuse(...)`` statements: nothing is
 formatted unless a call is refused."""
 import contextlib
+import math
 
 import torch
 from torch.autograd import forward_ad
@@ -42,6 +43,17 @@ def rows16(t):
         if n != 1 and (s < row or s % per16):
             return False
     return True
+
+
+def overlaps_itself(t):
+    """True when two elements of a 2-D tensor share memory: an expanded tensor, or a pitch shorter than a row."""
+    if t.is_contiguous():
+        return False
+    (n0, n1), (s0, s1) = t.shape, t.stride()
+    if (n0 > 1 and s0 == 0) or (n1 > 1 and s1 == 0):
+        return True
+    step = math.gcd(s0, s1)     # i s0 = j s1 for the first time at i = s1 / step, j = s0 / step
+    return s1 // step < n0 and s0 // step < n1
 
 
 def traced(t):

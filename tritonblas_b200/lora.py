@@ -8,7 +8,7 @@ from typing import Optional
 import torch
 
 from . import _lib
-from ._checks import on_device, refuse, refuse_devices, refuse_tangents, rows16, traced
+from ._checks import on_device, overlaps_itself, refuse, refuse_devices, refuse_tangents, rows16, traced
 from .matmul import _repitch, _strides, _tma_loadable, _unit_stride_2d
 
 _MAX_RANK = 128
@@ -42,6 +42,8 @@ def _check(x, w, lora_a, lora_b, adapter_ids, scales, bias, out):
         refuse("bias must be (n,) in float16, bfloat16 or float32")
     if out is not None and (out.shape != (tokens, n) or out.dtype is not dtype):
         refuse(f"out must be {(tokens, n)} of {dtype}")
+    if out is not None and tokens and n and overlaps_itself(out):
+        refuse("out must not overlap itself")
     if not x.is_cuda or not device == w.device == lora_a.device == lora_b.device == adapter_ids.device \
             or any(t is not None and t.device != device for t in (scales, bias, out)):
         refuse_devices(x, w, lora_a, lora_b, adapter_ids, scales, bias, out)
@@ -140,7 +142,7 @@ def lora_matmul(x, w, lora_a, lora_b, adapter_ids, scales=None, bias=None, out: 
     or None for 1; bias: (n,). k and rank multiples of 8, rank up to 128. The sum is float32 and rounded once. The rank-sized
     products ``scales[a] * x[t] @ lora_a[a].T`` are operands of a tensor-core product and kept in two 16-bit halves: to 2^-16
     relative in bfloat16; in float16 to 2^-22 relative or 2^-25 absolute, and infinite above 65504. ``out`` may be given:
-    (tokens, n), any strides, no overlap with the inputs. Inference only.
+    (tokens, n), any strides, no overlap with itself or the inputs. Inference only.
 
     Infinities and NaN in x, lora_a, lora_b and scales stay with the rows that use them; calls that meet some are slower.
     """
