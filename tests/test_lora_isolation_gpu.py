@@ -71,3 +71,23 @@ def test_rows_of_nan_with_several_adapters():
         x, w, a, b, ids, s = make(T, 512, 1024, 16, 5, torch.bfloat16)
         got = tb.lora_matmul(x * float("nan"), w, a, b, ids, s)
         assert torch.isnan(got).all() and tb.device_status() == 0
+
+
+@pytest.mark.parametrize("T", [40, 300])
+def test_what_is_not_finite_by_the_formula_stays_what_it_is(T):
+    """Rows of x with a NaN or an infinity, infinite entries of an adapter that cancel or not, all beside a broken adapter: NaN where
+    the formula in 64 bits has NaN, infinities of its sign where it has those."""
+    x, w, a, b, ids, s = make(T, 128, 264, 16, 5, torch.bfloat16)
+    s = s.abs() + 0.25
+    ids[:6] = torch.tensor([0, 1, 2, 3, 4, -1], device="cuda")
+    b[0] = float("nan")
+    b[1, 7, 3], b[1, 9, 2], b[1, 9, 5] = float("inf"), float("inf"), float("-inf")
+    x[T // 2, 5], x[T // 3, 9], x[T // 4, 0] = float("nan"), float("inf"), float("-inf")
+    got = tb.lora_matmul(x, w, a, b, ids, s).double()
+    want = x.double() @ w.double()
+    for i in range(5):
+        rows = ids == i
+        want[rows] += float(s[i]) * (x[rows].double() @ a[i].double().T) @ b[i].double().T
+    assert torch.equal(torch.isnan(got), torch.isnan(want))
+    sure = torch.isfinite(want) & (want.abs() < 1e30)
+    assert torch.isfinite(got[sure]).all() and torch.equal(got[torch.isinf(want)], want[torch.isinf(want)])

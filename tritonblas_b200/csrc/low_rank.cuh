@@ -5,7 +5,7 @@
 // (one multiply-add per element, nothing else as long as all are) and have those elements formed again from the definition:
 //     out[t, n] = sum_k x[t, k] W[k, n] + bias[n] + sum_r v[t, r] B_a[n, r],   a = adapter_ids[t],  no other adapter.
 // An element that is not finite by this formula stays so. Only batches with such values pay for it: a warp takes one element at a
-// time.
+// time, and goes by the row's own update and by the row of x first, either of which may hold the NaN itself.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -51,6 +51,8 @@ static __device__ __noinline__ void redo(const LowRankRows* rows, int t0, int t1
   const unsigned short *bs = static_cast<const unsigned short*>(a.b), *vs = static_cast<const unsigned short*>(a.v);
   unsigned short* out = static_cast<unsigned short*>(a.out);
   const int count = max(t1 - t0, 0) * max(width, 0);
+  int seen_t = -1;        // the row that was looked at last,
+  bool nan_row = false;   // and whether its x holds a NaN: then so does every element
   for (int base = 0; base < count; base += 32) {
     const int e = base + lane, my_t = t0 + e / width, my_n = n0 + e % width;
     bool odd = false;
@@ -71,8 +73,24 @@ static __device__ __noinline__ void redo(const LowRankRows* rows, int t0, int t1
       place = static_cast<int>(__reduce_max_sync(0xffffffffu, static_cast<unsigned>(place)));
       if (!__any_sync(0xffffffffu, others)) continue;
       const unsigned short* x = xs + t * a.x_stride;
+      if (t != seen_t) {
+        bool nan = false;
+        for (int k = lane; k < a.k; k += 32) nan = nan || isnan(from16(x[k], a.bf16));
+        nan_row = __any_sync(0xffffffffu, nan);
+        seen_t = t;
+      }
+      if (nan_row) continue;
       const unsigned short* w = ws + n * a.w_n;
       float s = 0.0f;
+      if (place > 0) {
+        const unsigned short* v = vs + ((static_cast<long long>(tile) * (a.list_stride - 1) + place - 1) * a.tile_rows + t % a.tile_rows) * a.v_row;
+        const unsigned short* b = bs + id * a.b_adapter + n * a.b_row;
+        for (int r = lane; r < a.rank; r += 32) {
+          const int at = 2 * (r & ~(a.v_width - 1)) + (r & (a.v_width - 1));
+          s = fmaf(from16(__ldcg(v + at), a.bf16) + from16(__ldcg(v + at + a.v_width), a.bf16), from16(b[r], a.bf16), s);
+        }
+        if (__any_sync(0xffffffffu, isnan(s))) continue;
+      }
       if (a.w_k == 1) {  // rows of x and columns of w start on 16-byte boundaries, k is a multiple of 8
         for (int k = lane * 8; k < a.k; k += 256) {
           const uint4 xq = *reinterpret_cast<const uint4*>(x + k), wq = *reinterpret_cast<const uint4*>(w + k);
@@ -85,14 +103,6 @@ static __device__ __noinline__ void redo(const LowRankRows* rows, int t0, int t1
         }
       } else {
         for (int k = lane; k < a.k; k += 32) s = fmaf(from16(x[k], a.bf16), from16(w[k * a.w_k], a.bf16), s);
-      }
-      if (place > 0) {
-        const unsigned short* v = vs + ((static_cast<long long>(tile) * (a.list_stride - 1) + place - 1) * a.tile_rows + t % a.tile_rows) * a.v_row;
-        const unsigned short* b = bs + id * a.b_adapter + n * a.b_row;
-        for (int r = lane; r < a.rank; r += 32) {
-          const int at = 2 * (r & ~(a.v_width - 1)) + (r & (a.v_width - 1));
-          s = fmaf(from16(__ldcg(v + at), a.bf16) + from16(__ldcg(v + at + a.v_width), a.bf16), from16(b[r], a.bf16), s);
-        }
       }
 #pragma unroll
       for (int d = 16; d > 0; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
