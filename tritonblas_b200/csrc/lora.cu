@@ -26,10 +26,9 @@
 #include "low_rank.cuh"
 #include "selector.h"  // the SM count when there is no device
 #include "ptx.cuh"
+#include "token_ops.cuh"
 
 namespace tb {
-
-bool pdl_enabled();  // api.cu
 
 namespace {
 
@@ -86,13 +85,6 @@ __device__ __forceinline__ void mma_16816<__half>(float (&d)[4], uint32_t a0, ui
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-template <typename T>
-__device__ __forceinline__ T cast16(float v);
-template <>
-__device__ __forceinline__ __nv_bfloat16 cast16<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
-template <>
-__device__ __forceinline__ __half cast16<__half>(float v) { return __float2half_rn(v); }
-
 // The two halves of v; an infinite v has no low half (inf - inf).
 template <typename T>
 __device__ __forceinline__ T low_half(float v, T hi) {
@@ -501,7 +493,6 @@ lora_project_tc_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_
   }
 }
 
-// One launch of either kernel: clusters of p.splits CTAs, programmatic dependent launch as the GEMM kernels use it.
 // The carve-out is asked for at its largest: an SM keeps the division between L1 and shared memory while blocks run on it, and the
 // second launch's blocks are to join these (1 row of 4096 x 4096: 15.0 -> 14.5 us at the time).
 template <typename K>
@@ -519,27 +510,8 @@ int prefer_shared(K kernel, int device, bool (&done)[64]) {
 template <typename... Params, typename... Args>
 int project_launch(void (*kernel)(Params...), int runs, const ProjectParams& p, int stripes, int smem_bytes, cudaStream_t stream,
                    Args... args) {
-  cudaLaunchConfig_t lc = {};
-  lc.gridDim = dim3(static_cast<unsigned>(runs * p.splits), static_cast<unsigned>(stripes), 1);
-  lc.blockDim = dim3(kThreads, 1, 1);
-  lc.dynamicSmemBytes = static_cast<size_t>(smem_bytes);
-  lc.stream = stream;
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = static_cast<unsigned>(p.splits);
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  lc.attrs = attr;
-  lc.numAttrs = 1;
-  if (pdl_enabled()) {
-    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[1].val.programmaticStreamSerializationAllowed = 1;
-    lc.numAttrs = 2;
-  }
-  cudaError_t e = cudaLaunchKernelEx(&lc, kernel, args..., p);
-  if (e != cudaSuccess) return cuda_fail(e, "lora_project_kernel launch");
-  g_launches.fetch_add(1, std::memory_order_relaxed);
-  return TB_OK;
+  return launch_token_kernel(kernel, dim3(static_cast<unsigned>(runs * p.splits), static_cast<unsigned>(stripes), 1), kThreads, smem_bytes, p.splits,
+                             stream, "lora_project_kernel launch", args..., p);
 }
 
 template <typename T, int NT>
@@ -577,16 +549,8 @@ int project_tc(const tb_lora_args& a, ProjectParams& p, int runs, int stripes, i
   const uint32_t box[3] = {64, static_cast<uint32_t>(p.rank_pad), 1};
   if ((rc = encode_nd(&ta, a.dtype, a.lora_a, 3, dims, strides, box)) != TB_OK) return rc;
   auto kernel = lora_project_tc_kernel<T>;
-  static int configured[64] = {};
-  static std::mutex mu;
-  {
-    std::lock_guard<std::mutex> lk(mu);
-    if (smem_bytes > configured[device & 63]) {
-      cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes);
-      if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(lora_project_tc)");
-      configured[device & 63] = smem_bytes;
-    }
-  }
+  static SmemOptIn configured;
+  if ((rc = opt_in_smem(kernel, smem_bytes, device, configured, "cudaFuncSetAttribute(lora_project_tc)")) != TB_OK) return rc;
   return project_launch(kernel, runs, p, stripes, smem_bytes, stream, tx, ta);
 }
 

@@ -17,16 +17,14 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
-#include <mutex>
 #include <type_traits>
 
 #include "common_host.h"
 #include "low_rank.cuh"
 #include "ptx.cuh"
+#include "token_ops.cuh"
 
 namespace tb {
-
-bool pdl_enabled();  // api.cu
 
 namespace {
 
@@ -128,19 +126,6 @@ struct Units {
   }
 };
 
-__device__ __noinline__ bool wait_slow(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* status,
-                                       unsigned long long timeout_ns, int code) {
-  return mbar_wait_warp(bar, parity, WaitCtx{abort_flag, status, timeout_ns}, code);
-}
-__device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity, const WaitCtx& w, int code) {
-  if (__builtin_expect(__all_sync(0xffffffffu, mbar_try_wait(bar, parity)), 1)) return true;
-  return wait_slow(bar, parity, w.abort_flag, w.status, w.timeout_ns, code);
-}
-__device__ __forceinline__ uint64_t evict_first_policy() {
-  uint64_t policy;
-  asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(policy));
-  return policy;
-}
 __device__ __forceinline__ void tma_load_2d_hint(void* smem_dst, const CUtensorMap* tmap, uint64_t* bar, int x, int y, uint64_t policy) {
   asm volatile(
       "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1, {%3, %4}], [%2], %5;" ::"r"(
@@ -158,13 +143,6 @@ __device__ __forceinline__ float bias_at(const void* bias, long long i, int dtyp
   if (dtype == TB_DTYPE_BF16) return __bfloat162float(static_cast<const __nv_bfloat16*>(bias)[i]);
   return __half2float(static_cast<const __half*>(bias)[i]);
 }
-template <typename T>
-__device__ __forceinline__ T cast16(float v);
-template <>
-__device__ __forceinline__ __nv_bfloat16 cast16<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
-template <>
-__device__ __forceinline__ __half cast16<__half>(float v) { return __float2half_rn(v); }
-
 // PIECES: with dealt updates (the form without them is half a microsecond shorter). A quarter of an SM's registers belongs to each of
 // its four warp schedulers: 136 for the two of these seven warps that meet there are what leaves room for two of the first launch's
 // at 120. With 144 and 128 the kernels run one after the other (1 row of 4096 x 4096: 14.9 us, not 12.9).
@@ -564,34 +542,10 @@ template <typename T, bool PIECES>
 int decode_launch(const CUtensorMap& w, const CUtensorMap& x, const CUtensorMap& b, const CUtensorMap& v, const DecodeParams& p, int grid,
                   int smem_bytes, int device, cudaStream_t stream) {
   auto kernel = lora_decode_kernel<T, PIECES>;
-  // the opt-in shared-memory size is set once per instantiation and device, and again if a launch needs more
-  static int configured[64] = {};
-  static std::mutex mu;
-  {
-    std::lock_guard<std::mutex> lk(mu);
-    if (smem_bytes > configured[device & 63]) {
-      cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes);
-      if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(lora_decode)");
-      configured[device & 63] = smem_bytes;
-    }
-  }
-  cudaLaunchConfig_t lc = {};
-  lc.gridDim = dim3(static_cast<unsigned>(grid), 1, 1);
-  lc.blockDim = dim3(kThreads, 1, 1);
-  lc.dynamicSmemBytes = static_cast<size_t>(smem_bytes);
-  lc.stream = stream;
-  cudaLaunchAttribute attr[1];
-  lc.attrs = attr;
-  lc.numAttrs = 0;
-  if (pdl_enabled()) {
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    lc.numAttrs = 1;
-  }
-  cudaError_t e = cudaLaunchKernelEx(&lc, kernel, w, x, b, v, p);
-  if (e != cudaSuccess) return cuda_fail(e, "lora_decode_kernel launch");
-  g_launches.fetch_add(1, std::memory_order_relaxed);
-  return TB_OK;
+  static SmemOptIn configured;
+  const int rc = opt_in_smem(kernel, smem_bytes, device, configured, "cudaFuncSetAttribute(lora_decode)");
+  if (rc != TB_OK) return rc;
+  return launch_token_kernel(kernel, dim3(static_cast<unsigned>(grid)), kThreads, smem_bytes, 0, stream, "lora_decode_kernel launch", w, x, b, v, p);
 }
 
 }  // namespace

@@ -29,14 +29,11 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
-#include <mutex>
-
 #include "common_host.h"
 #include "ptx.cuh"
+#include "token_ops.cuh"
 
 namespace tb {
-
-bool pdl_enabled();  // api.cu
 
 namespace {
 
@@ -60,7 +57,6 @@ __host__ __device__ constexpr int mlp_slabs(int m) { return m == 64 ? 2 : 1; }
 struct MlpLayout {
   // word offsets
   static constexpr int kNumExperts = 0;   // distinct experts
-  static constexpr int kNumRows = 1;      // distinct (expert, token) rows
   static constexpr int kNumGroups = 2;    // row groups: at most group_cap rows of one expert
   static constexpr int kNextUnit = 4;     // counters
   static constexpr int kRowsDone = 5;     // units of the second kind that are complete, times the four epilogue warps
@@ -182,7 +178,6 @@ moe_mlp_plan_kernel(const void* __restrict__ ids, int is64, const float* __restr
   for (int i = tid; i < lay.experts; i += kPlanThreads) ws[lay.expert_done() + i] = 0;
   if (tid == 0) {
     ws[MlpLayout::kNumExperts] = s_scan[0][31];
-    ws[MlpLayout::kNumRows] = s_scan[1][31];
     ws[MlpLayout::kNumGroups] = s_scan[2][31];
     ws[lay.expert_off() + s_scan[0][31]] = s_scan[1][31];
     ws[MlpLayout::kNextUnit] = 0;
@@ -266,7 +261,6 @@ moe_mlp_plan_warp_kernel(const void* __restrict__ ids, int is64, const float* __
   if (lane < lay.experts) ws[lay.expert_done() + lane] = 0;
   if (lane == 0) {
     ws[MlpLayout::kNumExperts] = num;
-    ws[MlpLayout::kNumRows] = total;
     ws[MlpLayout::kNumGroups] = num;
     ws[lay.expert_off() + num] = total;
     ws[MlpLayout::kNextUnit] = 0;
@@ -278,11 +272,6 @@ moe_mlp_plan_warp_kernel(const void* __restrict__ ids, int is64, const float* __
 // Weights are read once per call (or once per row group, soon after each other): their lines leave L2 first, so that h, the
 // weighted rows and x are still there when they are read. Measured at 128 tokens, 64 experts of 4096 x 1536: 404 us
 // without the hint, 392 with it.
-__device__ __forceinline__ uint64_t evict_first_policy() {
-  uint64_t policy;
-  asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(policy));
-  return policy;
-}
 __device__ __forceinline__ void tma_load_5d_hint(void* smem_dst, const CUtensorMap* tmap, uint64_t* bar, int x, int y, int z, int w,
                                                  int v, uint64_t policy) {
   asm volatile(
@@ -332,16 +321,6 @@ __device__ __forceinline__ bool counter_wait_warp(const int* counter, int want, 
   ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
   if (ok) load_acquire(counter);  // each lane's own acquire
   return ok;
-}
-
-// mbar_wait_warp with its slow part out of line: the roles' loops are one warp each, so every taken branch in them is exposed.
-__device__ __noinline__ bool wait_slow(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* status,
-                                       unsigned long long timeout_ns, int code) {
-  return mbar_wait_warp(bar, parity, WaitCtx{abort_flag, status, timeout_ns}, code);
-}
-__device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity, const WaitCtx& w, int code) {
-  if (__builtin_expect(__all_sync(0xffffffffu, mbar_try_wait(bar, parity)), 1)) return true;
-  return wait_slow(bar, parity, w.abort_flag, w.status, w.timeout_ns, code);
 }
 
 // One unit as the weight loader hands it to the other roles.
@@ -870,34 +849,11 @@ template <typename T, int M1, int M2>
 int mlp_launch(const CUtensorMap& w1, const CUtensorMap& w2, const CUtensorMap& x, const CUtensorMap (&h)[3], const MlpParams& p,
                int grid, int smem_bytes, int device, cudaStream_t stream) {
   auto kernel = moe_mlp_kernel<T, M1, M2>;
-  // the opt-in shared-memory size is set once per instantiation and device, and again if a launch needs more
-  static int configured[64] = {};
-  static std::mutex mu;
-  {
-    std::lock_guard<std::mutex> lk(mu);
-    if (smem_bytes > configured[device & 63]) {
-      cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes);
-      if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(moe_mlp)");
-      configured[device & 63] = smem_bytes;
-    }
-  }
-  cudaLaunchConfig_t lc = {};
-  lc.gridDim = dim3(static_cast<unsigned>(grid), 1, 1);
-  lc.blockDim = dim3(kMlpThreads, 1, 1);
-  lc.dynamicSmemBytes = static_cast<size_t>(smem_bytes);
-  lc.stream = stream;
-  cudaLaunchAttribute attr[1];
-  lc.attrs = attr;
-  lc.numAttrs = 0;
-  if (pdl_enabled()) {
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    lc.numAttrs = 1;
-  }
-  cudaError_t e = cudaLaunchKernelEx(&lc, kernel, w1, w2, x, h[0], h[1], h[2], p);
-  if (e != cudaSuccess) return cuda_fail(e, "moe_mlp_kernel launch");
-  g_launches.fetch_add(1, std::memory_order_relaxed);
-  return TB_OK;
+  static SmemOptIn configured;
+  const int rc = opt_in_smem(kernel, smem_bytes, device, configured, "cudaFuncSetAttribute(moe_mlp)");
+  if (rc != TB_OK) return rc;
+  return launch_token_kernel(kernel, dim3(static_cast<unsigned>(grid)), kMlpThreads, smem_bytes, 0, stream, "moe_mlp_kernel launch", w1, w2, x, h[0],
+                             h[1], h[2], p);
 }
 
 template <typename T>
@@ -993,25 +949,12 @@ int mlp_impl(const tb_moe_mlp_args& a, cudaStream_t stream) {
   for (int i = 0; i < 3; ++i)
     if ((rc = encode_2d(&th[i], a.dtype, p.h, a.ffn, 2ull * s.lay.pairs, a.ffn * es, kStageK, h_box[i], 1)) != TB_OK) return rc;
 
-  cudaLaunchConfig_t lc = {};
-  lc.gridDim = dim3(1, 1, 1);
   const bool one_warp = s.lay.pairs <= 32 && a.tokens <= s.group_cap, narrow = a.num_experts <= 256;
-  lc.blockDim = dim3(one_warp ? 32 : (narrow ? 256 : kMlpMaxExperts), 1, 1);
-  lc.stream = stream;
-  cudaLaunchAttribute attr[1];
-  lc.attrs = attr;
-  lc.numAttrs = 0;
-  if (pdl_enabled()) {
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    lc.numAttrs = 1;
-  }
   auto plan = one_warp ? moe_mlp_plan_warp_kernel : (narrow ? moe_mlp_plan_kernel<256> : moe_mlp_plan_kernel<kMlpMaxExperts>);
-  cudaError_t e = cudaLaunchKernelEx(&lc, plan, a.topk_ids, static_cast<int>(a.ids_are_int64 != 0), a.topk_weights,
-                                     static_cast<int>(a.tokens), static_cast<int>(a.topk), static_cast<int>(a.num_experts),
-                                     s.group_cap, s.lay, p.ws);
-  if (e != cudaSuccess) return cuda_fail(e, "moe_mlp_plan_kernel launch");
-  g_launches.fetch_add(1, std::memory_order_relaxed);
+  rc = launch_token_kernel(plan, dim3(1), one_warp ? 32 : (narrow ? 256 : kMlpMaxExperts), 0, 0, stream, "moe_mlp_plan_kernel launch", a.topk_ids,
+                           static_cast<int>(a.ids_are_int64 != 0), a.topk_weights, static_cast<int>(a.tokens), static_cast<int>(a.topk),
+                           static_cast<int>(a.num_experts), s.group_cap, s.lay, p.ws);
+  if (rc != TB_OK) return rc;
   auto launch = p.bf16 ? mlp_variant<__nv_bfloat16>(s.m1, s.m2) : mlp_variant<__half>(s.m1, s.m2);
   return launch(tw1, tw2, tx, th, p, num_sms, smem_bytes, device, stream);
 }

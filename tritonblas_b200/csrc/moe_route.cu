@@ -24,10 +24,9 @@
 
 #include "common_host.h"
 #include "ptx.cuh"
+#include "token_ops.cuh"
 
 namespace tb {
-
-bool pdl_enabled();  // api.cu
 
 namespace {
 
@@ -319,27 +318,6 @@ route_bwd_kernel(const T* __restrict__ logits, long long stride, long long token
   }
 }
 
-// Programmatic dependent launch as the GEMM kernels use it.
-template <typename K, typename... Args>
-int launch_rows(K kernel, long long blocks, cudaStream_t st, const char* what, Args... args) {
-  cudaLaunchConfig_t lc = {};
-  lc.gridDim = dim3(static_cast<unsigned>(blocks), 1, 1);
-  lc.blockDim = dim3(kRouteWarps * 32, 1, 1);
-  lc.stream = st;
-  cudaLaunchAttribute attr[1];
-  lc.attrs = attr;
-  lc.numAttrs = 0;
-  if (pdl_enabled()) {
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    lc.numAttrs = 1;
-  }
-  cudaError_t e = cudaLaunchKernelEx(&lc, kernel, args...);
-  if (e != cudaSuccess) return cuda_fail(e, what);
-  g_launches.fetch_add(1, std::memory_order_relaxed);
-  return TB_OK;
-}
-
 struct RouteCall {
   const void* logits;
   long long stride, tokens;
@@ -356,11 +334,13 @@ int route_launch(const RouteCall& c) {
   constexpr int kPerBlock = kRouteWarps * (32 / LANES);
   const long long blocks = (c.tokens + kPerBlock - 1) / kPerBlock;
   if (c.grad == nullptr)
-    return launch_rows(route_kernel<T, LANES, VPT, VEC>, blocks, c.stream, "route_kernel launch", static_cast<const T*>(c.logits),
-                       c.stride, c.tokens, c.experts, c.topk, c.sigmoid, c.renorm, c.weights, c.ids);
-  return launch_rows(route_bwd_kernel<T, LANES, VPT, VEC>, blocks, c.stream, "route_bwd_kernel launch",
-                     static_cast<const T*>(c.logits), c.stride, c.tokens, c.experts, c.topk, c.sigmoid, c.renorm,
-                     static_cast<const float*>(c.weights), static_cast<const int*>(c.ids), c.grad, static_cast<T*>(c.dlogits));
+    return launch_token_kernel(route_kernel<T, LANES, VPT, VEC>, dim3(static_cast<unsigned>(blocks)), kRouteWarps * 32, 0, 0, c.stream,
+                               "route_kernel launch", static_cast<const T*>(c.logits), c.stride, c.tokens, c.experts, c.topk, c.sigmoid,
+                               c.renorm, c.weights, c.ids);
+  return launch_token_kernel(route_bwd_kernel<T, LANES, VPT, VEC>, dim3(static_cast<unsigned>(blocks)), kRouteWarps * 32, 0, 0, c.stream,
+                             "route_bwd_kernel launch", static_cast<const T*>(c.logits), c.stride, c.tokens, c.experts, c.topk, c.sigmoid,
+                             c.renorm, static_cast<const float*>(c.weights), static_cast<const int*>(c.ids), c.grad,
+                             static_cast<T*>(c.dlogits));
 }
 
 // Loads are eight elements wide where every row starts on a 16-byte boundary and holds whole runs of eight, single elements
