@@ -10,6 +10,9 @@ from torch.autograd import forward_ad
 
 _nullcontext = contextlib.nullcontext()
 _PLAIN = (torch.Tensor, torch.nn.Parameter)
+_is_compiling = torch.compiler.is_compiling
+_dispatch_modes = torch._C._len_torch_dispatch_stack
+_transform = torch._C._functorch.peek_interpreter_stack
 
 
 def refuse(message):
@@ -60,8 +63,7 @@ def traced(t):
     """True where a call has to go through its registered operator because something looks at it or rewrites it: torch.compile, fake
     tensors and other subclasses, a dispatch mode (torch.export, make_fx, ...), a torch.func transform. Plain eager calls skip the
     dispatcher, which costs more than the operators run."""
-    return (torch.compiler.is_compiling() or type(t) not in _PLAIN or torch._C._len_torch_dispatch_stack() > 0
-            or torch._C._functorch.peek_interpreter_stack() is not None)
+    return _is_compiling() or type(t) not in _PLAIN or _dispatch_modes() > 0 or _transform() is not None
 
 
 def refuse_tangents(name, *tensors):

@@ -6,6 +6,7 @@ import ctypes
 from typing import Optional
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from ._checks import on_device, overlaps_itself, refuse, refuse_devices, refuse_tangents, rows16, traced
@@ -45,19 +46,20 @@ def _check(x, w, lora_a, lora_b, adapter_ids, scales, bias, out):
     if out is not None and tokens and n and overlaps_itself(out):
         refuse("out must not overlap itself")
     if not x.is_cuda or not device == w.device == lora_a.device == lora_b.device == adapter_ids.device \
-            or any(t is not None and t.device != device for t in (scales, bias, out)):
+            or (scales is not None and scales.device != device) or (bias is not None and bias.device != device) \
+            or (out is not None and out.device != device):
         refuse_devices(x, w, lora_a, lora_b, adapter_ids, scales, bias, out)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, w, lora_a, lora_b, scales, bias, out)):
+    if torch.is_grad_enabled() and (x.requires_grad or w.requires_grad or lora_a.requires_grad or lora_b.requires_grad
+                                    or (scales is not None and scales.requires_grad) or (bias is not None and bias.requires_grad)
+                                    or (out is not None and out.requires_grad)):
         raise RuntimeError("tritonblas.lora_matmul(): inference only, but one of the arguments requires grad.")
+    return tokens, k, n, adapters, rank, dtype, device
 
 
-def _run(x, w, lora_a, lora_b, adapter_ids, scales, bias, out):
-    tokens, k = x.shape
-    n = w.shape[1]
-    adapters, rank, _ = lora_a.shape
-    dtype, device = x.dtype, x.device
+def _run(checked, x, w, lora_a, lora_b, adapter_ids, scales, bias, out):
+    tokens, k, n, adapters, rank, dtype, device = checked
     if out is None:
-        out = torch.empty(tokens, n, dtype=x.dtype, device=x.device)
+        out = torch.empty(tokens, n, dtype=dtype, device=device)
     if tokens == 0 or n == 0:
         return out
     if out.data_ptr() == x.data_ptr():
@@ -117,8 +119,7 @@ def _run(x, w, lora_a, lora_b, adapter_ids, scales, bias, out):
 @torch.library.custom_op("tritonblas::_lora_matmul", mutates_args=())
 def _lora_matmul(x: torch.Tensor, w: torch.Tensor, lora_a: torch.Tensor, lora_b: torch.Tensor, adapter_ids: torch.Tensor,
                  scales: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None) -> torch.Tensor:
-    _check(x, w, lora_a, lora_b, adapter_ids, scales, bias, None)
-    return _run(x, w, lora_a, lora_b, adapter_ids, scales, bias, None)
+    return _run(_check(x, w, lora_a, lora_b, adapter_ids, scales, bias, None), x, w, lora_a, lora_b, adapter_ids, scales, bias, None)
 
 
 @_lora_matmul.register_fake
@@ -129,8 +130,7 @@ def _(x, w, lora_a, lora_b, adapter_ids, scales=None, bias=None):
 @torch.library.custom_op("tritonblas::_lora_matmul_out", mutates_args={"out"})
 def _lora_matmul_out(x: torch.Tensor, w: torch.Tensor, lora_a: torch.Tensor, lora_b: torch.Tensor, adapter_ids: torch.Tensor,
                      out: torch.Tensor, scales: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None) -> None:
-    _check(x, w, lora_a, lora_b, adapter_ids, scales, bias, out)
-    _run(x, w, lora_a, lora_b, adapter_ids, scales, bias, out)
+    _run(_check(x, w, lora_a, lora_b, adapter_ids, scales, bias, out), x, w, lora_a, lora_b, adapter_ids, scales, bias, out)
 
 
 def lora_matmul(x, w, lora_a, lora_b, adapter_ids, scales=None, bias=None, out: Optional[torch.Tensor] = None):
@@ -146,11 +146,12 @@ def lora_matmul(x, w, lora_a, lora_b, adapter_ids, scales=None, bias=None, out: 
 
     Infinities and NaN in x, lora_a, lora_b and scales stay with the rows that use them; calls that meet some are slower.
     """
-    _check(x, w, lora_a, lora_b, adapter_ids, scales, bias, out)
-    refuse_tangents("lora_matmul", x, w, lora_a, lora_b, scales, bias)
+    checked = _check(x, w, lora_a, lora_b, adapter_ids, scales, bias, out)
+    if forward_ad._current_level >= 0:
+        refuse_tangents("lora_matmul", x, w, lora_a, lora_b, scales, bias)
     if traced(x):
         if out is None:
             return _lora_matmul(x, w, lora_a, lora_b, adapter_ids, scales, bias)
         _lora_matmul_out(x, w, lora_a, lora_b, adapter_ids, out, scales, bias)
         return out
-    return _run(x, w, lora_a, lora_b, adapter_ids, scales, bias, out)
+    return _run(checked, x, w, lora_a, lora_b, adapter_ids, scales, bias, out)

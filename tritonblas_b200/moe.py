@@ -9,6 +9,7 @@ import operator
 from typing import Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from ._checks import on_device, refuse, refuse_devices, refuse_tangents, rows16, traced
@@ -137,7 +138,8 @@ def moe_route(logits, topk, scoring="softmax", renormalize=True):
     if not 1 <= topk <= min(_MAX_TOPK, experts):
         refuse(f"topk must be between 1 and min({_MAX_TOPK}, experts), got {topk}")
     sigmoid, renormalize = _SCORING[scoring], 1 if renormalize else 0
-    refuse_tangents("moe_route", logits)
+    if forward_ad._current_level >= 0:
+        refuse_tangents("moe_route", logits)
     if traced(logits):
         return _moe_route(logits, topk, bool(sigmoid), bool(renormalize))
     if logits.requires_grad and torch.is_grad_enabled():
@@ -183,12 +185,11 @@ def _check_mlp(x, w1, w2, topk_ids, topk_weights, out):
             refuse_devices(x, out)
         if out.stride(1) != 1 or (tokens > 1 and out.stride(0) < hidden):
             refuse("out must have contiguous, non-overlapping rows")
+    return tokens, topk, experts, hidden, ffn, dtype, device
 
 
-def _run_mlp(x, w1, w2, topk_ids, topk_weights, out):
-    tokens, hidden = x.shape
-    experts, _, ffn = w2.shape
-    topk, dtype, device = topk_ids.shape[1], x.dtype, x.device
+def _run_mlp(checked, x, w1, w2, topk_ids, topk_weights, out):
+    tokens, topk, experts, hidden, ffn, dtype, device = checked
     if out is None:
         out = torch.empty(tokens, hidden, dtype=dtype, device=device)
     if tokens == 0:
@@ -216,8 +217,7 @@ def _run_mlp(x, w1, w2, topk_ids, topk_weights, out):
 
 @torch.library.custom_op("tritonblas::_moe_mlp", mutates_args=())
 def _moe_mlp(x: torch.Tensor, w1: torch.Tensor, w2: torch.Tensor, topk_ids: torch.Tensor, topk_weights: torch.Tensor) -> torch.Tensor:
-    _check_mlp(x, w1, w2, topk_ids, topk_weights, None)
-    return _run_mlp(x, w1, w2, topk_ids, topk_weights, None)
+    return _run_mlp(_check_mlp(x, w1, w2, topk_ids, topk_weights, None), x, w1, w2, topk_ids, topk_weights, None)
 
 
 @_moe_mlp.register_fake
@@ -228,8 +228,7 @@ def _(x, w1, w2, topk_ids, topk_weights):
 @torch.library.custom_op("tritonblas::_moe_mlp_out", mutates_args={"out"})
 def _moe_mlp_out(x: torch.Tensor, w1: torch.Tensor, w2: torch.Tensor, topk_ids: torch.Tensor, topk_weights: torch.Tensor,
                  out: torch.Tensor) -> None:
-    _check_mlp(x, w1, w2, topk_ids, topk_weights, out)
-    _run_mlp(x, w1, w2, topk_ids, topk_weights, out)
+    _run_mlp(_check_mlp(x, w1, w2, topk_ids, topk_weights, out), x, w1, w2, topk_ids, topk_weights, out)
 
 
 def moe_mlp(x, w1, w2, topk_ids, topk_weights, out: Optional[torch.Tensor] = None):
@@ -245,11 +244,12 @@ def moe_mlp(x, w1, w2, topk_ids, topk_weights, out: Optional[torch.Tensor] = Non
     ``out`` may be given: (tokens, hidden), contiguous rows, no overlap with the weights. Inference only. More tokens:
     ``distributed.PeerMemoryMoE``.
     """
-    _check_mlp(x, w1, w2, topk_ids, topk_weights, out)
-    refuse_tangents("moe_mlp", x, w1, w2, topk_weights)
+    checked = _check_mlp(x, w1, w2, topk_ids, topk_weights, out)
+    if forward_ad._current_level >= 0:
+        refuse_tangents("moe_mlp", x, w1, w2, topk_weights)
     if traced(x):
         if out is None:
             return _moe_mlp(x, w1, w2, topk_ids, topk_weights)
         _moe_mlp_out(x, w1, w2, topk_ids, topk_weights, out)
         return out
-    return _run_mlp(x, w1, w2, topk_ids, topk_weights, out)
+    return _run_mlp(checked, x, w1, w2, topk_ids, topk_weights, out)
