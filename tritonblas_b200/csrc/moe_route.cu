@@ -15,7 +15,10 @@
 // integer that orders like it, with the complement of its index below (16-bit logits leave 13 bits of a 32-bit word for that,
 // fp32 ones take 64 bits), so a maximum is the next choice and ties go to the lowest index by themselves. Every lane sorts its
 // eight keys once; a round is a maximum over the lanes' first keys and a shift in the lane that held it.
-// What bounds it is the number of instructions per row, then the latency of a launch: see the figures at route_kernel.
+// What bounds it is the number of instructions per row, then the latency of a launch: 32771 rows of 256 bf16 logits, top-8, softmax
+// over all experts, 36 us forward and gradient (592 and 420 warp instructions a row, 86 and 79 % of the issue slots; the bytes alone:
+// 5.6 us); 16384 x 64: 5.0 us; a launch of three rows: 2.6 us. The exponentials are expf: the fast form took 33 us instead of 36, but
+// its error grows with the distance from the row's maximum.
 // No reference counterpart (the reference has no MoE path).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -202,7 +205,11 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_kernel(const T* __rest
   const float top = choice[0] != 0 ? Key<T>::value(choice[0]) : 0.0f;
   // Renormalised sigmoid scores are formed over exp(m), m = min(top, 0), which cancels in the quotient: below -88 the scores
   // themselves leave fp32's range, their quotients do not. With m = 0 this is the plain 1 / (1 + exp(-l)).
-  const float m = renorm ? fminf(top, 0.0f) : 0.0f, unit = expf(m);
+  float m = 0.0f, unit = 1.0f;
+  if (sigmoid && renorm) {
+    m = fminf(top, 0.0f);
+    unit = expf(m);
+  }
   float sum = 0.0f;
   for (int j = sub; j < topk; j += LANES) {
     const K k = choice[j];
