@@ -10,9 +10,9 @@
 // The parts come first, the ones that take a dealt tile's update last among them, then the whole tiles: the sums over parts are
 // hidden behind the whole tiles where there are any.
 //
-// Measured back to back: 1 row of 4096 x 4096, rank 16: 12.9 us (19.5 with the general GEMM and the same update); 48 rows of 8192
-// x 28672, 30 adapters of rank 16: 89 us, 5.7 TB/s (101); 1 row of 8192 x 28672: 73-77 us, 0.95 of the copy rate; n-contiguous
-// weights within 2 %. A unit of its own for the updates instead of the last parts, and parts written only once the first launch
+// Measured back to back: 1 row of 4096 x 4096, rank 16: 13.2 us (19.5 with the general GEMM and the same update); 48 rows of 8192
+// x 28672, 30 adapters of rank 16: 91 us, 5.6 TB/s (101); 1 row of 8192 x 28672: 75 us, 0.96 of the copy rate; n-contiguous
+// weights within 4 %. A unit of its own for the updates instead of the last parts, and parts written only once the first launch
 // is through, took 15.0 us for 1 row of 4096 x 4096 and 37 instead of 33 for 64 rows of 4096 x 8192 with 64 adapters.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -145,7 +145,7 @@ __device__ __forceinline__ float bias_at(const void* bias, long long i, int dtyp
 }
 // PIECES: with dealt updates (the form without them is half a microsecond shorter). A quarter of an SM's registers belongs to each of
 // its four warp schedulers: 136 for the two of these seven warps that meet there are what leaves room for two of the first launch's
-// at 120. With 144 and 128 the kernels run one after the other (1 row of 4096 x 4096: 14.9 us, not 12.9).
+// at 120. With 144 and 128 the kernels run one after the other (1 row of 4096 x 4096: 14.9 us, not 12.9 at the time).
 template <typename T, bool PIECES>
 __global__ void __maxnreg__(136)
 lora_decode_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_x,
