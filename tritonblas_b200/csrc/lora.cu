@@ -12,9 +12,9 @@
 // row) and one for longer ones.
 //
 // Rounding: all sums are fp32. v is an operand of a tensor-core product, so it is kept as two 16-bit halves, v = hi + lo with
-// lo = round(v - hi), which stand side by side in a row of its block, 16 to 64 ranks at a time, and are both multiplied by the same rows of B: 2^-16 of v
-// (bf16), or 2^-22 or 2^-25 absolute, whichever is more (fp16, whose v is infinite above 65504: the update adds up in the
-// product's own accumulator, so it can have no unit of its own).
+// lo = round(v - hi), which stand side by side in a row of its block, 16 to 64 ranks at a time, and are both multiplied by the same
+// rows of B. That holds v to 2^-16 (bf16), or to 2^-22 or 2^-25 absolute, whichever is more (fp16, whose v is infinite above 65504:
+// the update adds up in the product's own accumulator, so it can have no unit of its own).
 // An infinity or NaN in one adapter's B would reach the tile's other rows, whose blocks hold zeros: see low_rank.cuh.
 // No reference counterpart (the reference has no adapters).
 #include <cuda_bf16.h>

@@ -45,7 +45,11 @@ __device__ __forceinline__ bool finite(float f) { return fabsf(f) < __builtin_hu
 static __device__ __noinline__ void redo(const LowRankRows* rows, int t0, int t1, int n0, int n1) {
   griddep_wait();  // of the first launch
   __syncwarp();
-  const LowRankRows a = *rows;
+  LowRankRows a;  // from L2, as all that the first launch wrote
+  static_assert(sizeof(LowRankRows) % 8 == 0, "copied in words of eight bytes");
+#pragma unroll
+  for (int i = 0; i < static_cast<int>(sizeof(LowRankRows) / 8); ++i)
+    reinterpret_cast<unsigned long long*>(&a)[i] = __ldcg(reinterpret_cast<const unsigned long long*>(rows) + i);
   const int lane = threadIdx.x & 31, width = n1 - n0;
   const unsigned short *xs = static_cast<const unsigned short*>(a.x), *ws = static_cast<const unsigned short*>(a.w);
   const unsigned short *bs = static_cast<const unsigned short*>(a.b), *vs = static_cast<const unsigned short*>(a.v);
